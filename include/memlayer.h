@@ -584,6 +584,14 @@ int32_t memlayer_model_forward(const memlayer_model_config* cfg, const memlayer_
                                const int32_t* tokens, int64_t batch, int64_t seq, float* logits, void* workspace,
                                size_t workspace_bytes, void* stream);
 
+/* The residual stream [batch, seq, d_model] (float32) after the last block,
+ * before ln_final: what the final norm, the tied logits and their loss
+ * (memlayer_layer_norm, memlayer_cross_entropy) are applied to, and where
+ * their gradients come back. */
+int32_t memlayer_model_hidden(const memlayer_model_config* cfg, const memlayer_model_params* params,
+                              const int32_t* tokens, int64_t batch, int64_t seq, float* hidden, void* workspace,
+                              size_t workspace_bytes, void* stream);
+
 /* Bytes of the key / value cache of `batch` rows: [n_layers][2][batch][max_len][d_model] float32. */
 int32_t memlayer_model_cache_size(const memlayer_model_config* cfg, int64_t batch, size_t* bytes);
 
@@ -595,6 +603,126 @@ int32_t memlayer_model_cache_size(const memlayer_model_config* cfg, int64_t batc
 int32_t memlayer_model_decode_step(const memlayer_model_config* cfg, const memlayer_model_params* params,
                                    const int32_t* tokens, int64_t batch, const int32_t* pos, void* cache,
                                    float* logits, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- Operators of the training step around the memory layer -------------
+ * What a training step of the language model needs beside the memory layer's
+ * own backward and row update: the layer norm with its gradient, the
+ * vocabulary's cross entropy with its gradient (the two ends of the backward
+ * pass), and an orthogonalised update for the Dense kernels.  Activations
+ * are float32, float16 or bfloat16 (`dtype`), statistics and sums float32.
+ * Input rows may be strided (elements between rows, at least the width);
+ * outputs are contiguous.  Outputs overlap no input.  Addresses are aligned
+ * to the element; 16-byte aligned rows run faster.  Results do not depend on
+ * timing: equal calls give equal bits. */
+
+typedef struct {
+  int64_t rows;                  /* product of the leading dimensions */
+  int32_t d_model;               /* 1 .. 16384 */
+  int32_t dtype;                 /* memlayer_dtype of x, residual, y, sum and of their gradients */
+  float epsilon;                 /* > 0; flax's LayerNorm has 1e-6 */
+} memlayer_norm_config;
+
+typedef struct {
+  const void* x;                 /* [rows, d_model] */
+  int64_t x_stride;
+  const void* residual;          /* added to x first; may be NULL */
+  int64_t residual_stride;
+  const float *scale, *bias;     /* [d_model] */
+  void* y;                       /* [rows, d_model] */
+  void* sum;                     /* [rows, d_model] x + residual, rounded to dtype: what the norm reads
+                                    (may be NULL; unused without residual) */
+} memlayer_norm_args;
+
+typedef struct {
+  const void* dy;                /* [rows, d_model] */
+  int64_t dy_stride;
+  const void* x;                 /* [rows, d_model] the forward's normalised input (its sum) */
+  int64_t x_stride;
+  const void* dresidual;         /* gradient reaching the input beside the norm, added to dx; may be NULL */
+  int64_t dresidual_stride;
+  const float* scale;            /* [d_model] */
+  void* dx;                      /* [rows, d_model] */
+  float *dscale, *dbias;         /* [d_model] */
+} memlayer_norm_grads;
+
+/* y = (s - mean) / sqrt(var + epsilon) * scale + bias with s = x + residual,
+ * over the rows' d_model entries (var: the centred, biased variance).
+ * model.py:87,96,124's LayerNorm with the residual add before it. */
+int32_t memlayer_layer_norm(const memlayer_norm_config* cfg, const memlayer_norm_args* args, void* stream);
+
+int32_t memlayer_layer_norm_backward_workspace_size(const memlayer_norm_config* cfg, size_t* bytes);
+
+/* Gradients of sum(dy * y) (+ dresidual) in the input, and of scale and bias
+ * (zeros when rows is 0).  mean and variance are taken from x again. */
+int32_t memlayer_layer_norm_backward(const memlayer_norm_config* cfg, const memlayer_norm_grads* grads,
+                                     void* workspace, size_t workspace_bytes, void* stream);
+
+typedef struct {
+  int64_t tokens;                /* T */
+  int32_t d_model;               /* 1 .. 65536 */
+  int32_t vocab_size;            /* V */
+  int32_t dtype;                 /* memlayer_dtype of h, weight, dh, dweight */
+  int32_t ignore_index;          /* a target of this value carries no loss */
+} memlayer_loss_config;
+
+typedef struct {
+  const void* h;                 /* [T, d_model] hidden states (the output of the last norm) */
+  int64_t h_stride;
+  const void* weight;            /* [V, d_model] output projection; the tied embedding in this model */
+  int64_t weight_stride;
+  const int32_t* targets;        /* [T] */
+  float* loss;                   /* [T] log sum exp(z) - z[target], z = h weight^T; 0 when ignored (forward) */
+  float* lse;                    /* [T] log sum exp(z) (forward) */
+} memlayer_loss_args;
+
+typedef struct {
+  const float* lse;              /* [T] the forward's */
+  const float* dloss;            /* [T] gradient of loss; not read at ignored tokens */
+  const float* dlse;             /* [T] gradient of lse (a log-partition penalty, say); may be NULL */
+  void* dh;                      /* [T, d_model] */
+  void* dweight;                 /* [V, d_model] */
+} memlayer_loss_grads;
+
+int32_t memlayer_cross_entropy_workspace_size(const memlayer_loss_config* cfg, int32_t backward, size_t* bytes);
+
+/* The integer-label softmax cross entropy of the tied logits
+ * (model.py:125 under the trainer's loss) without the [T, V] logits.  A
+ * target outside [0, V) that is not ignore_index gives a NaN loss and, in the
+ * backward, no gradient; it records status 27, read with
+ * memlayer_cross_entropy_status.  float32 products keep 22 bits of each
+ * operand (relative to its matrix's largest entry). */
+int32_t memlayer_cross_entropy(const memlayer_loss_config* cfg, const memlayer_loss_args* args, void* workspace,
+                               size_t workspace_bytes, void* stream);
+
+/* dh and dweight of sum(dloss * loss) + sum(dlse * lse); args as in the
+ * forward (loss and lse there are not used).  h must be finite at ignored
+ * tokens too: their zero gradient multiplies it in dweight. */
+int32_t memlayer_cross_entropy_backward(const memlayer_loss_config* cfg, const memlayer_loss_args* args,
+                                        const memlayer_loss_grads* grads, void* workspace, size_t workspace_bytes,
+                                        void* stream);
+
+/* The device status word of the last cross entropy call on this workspace (synchronises the stream). */
+int32_t memlayer_cross_entropy_status(const void* workspace, int32_t* code, void* stream);
+
+typedef struct {
+  int64_t batch;                 /* matrices */
+  int32_t rows, cols;            /* of each, 1 .. 32768 */
+  int32_t dtype;                 /* memlayer_dtype of update and out */
+  int32_t steps;                 /* 1 .. 64 */
+  float a, b, c;                 /* x <- x (a + b x^2 + c x^4) on the singular values */
+  float epsilon;                 /* >= 0, added to the Frobenius norm */
+} memlayer_orth_config;
+
+int32_t memlayer_orthogonalize_workspace_size(const memlayer_orth_config* cfg, size_t* bytes);
+
+/* out [batch, rows, cols] = update / (|update|_F + epsilon) after `steps`
+ * Newton-Schulz products that bring its singular values near 1: the update of
+ * a Dense kernel with its scale per direction removed.  Products keep 22 bits
+ * of their operands and add in float32, whatever dtype.  Coefficients whose
+ * iteration leaves the range of those operands (a matrix above 12, a singular
+ * value above 2.7) are MEMLAYER_ERR_UNSUPPORTED. */
+int32_t memlayer_orthogonalize(const memlayer_orth_config* cfg, const void* update, void* out, void* workspace,
+                               size_t workspace_bytes, void* stream);
 
 /* Size of the library's built-in scratch array used by
  * memlayer_pool_forward_noalloc (64 MiB).  A device holds it from the moment

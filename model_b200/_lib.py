@@ -185,11 +185,95 @@ class MemlayerLayerGrads(C.Structure):
     ]
 
 
+class MemlayerNormConfig(C.Structure):
+    _fields_ = [
+        ("rows", C.c_int64),
+        ("d_model", C.c_int32),
+        ("dtype", C.c_int32),
+        ("epsilon", C.c_float),
+    ]
+
+
+class MemlayerNormArgs(C.Structure):
+    _fields_ = [
+        ("x", C.c_void_p),
+        ("x_stride", C.c_int64),
+        ("residual", C.c_void_p),
+        ("residual_stride", C.c_int64),
+        ("scale", C.c_void_p),
+        ("bias", C.c_void_p),
+        ("y", C.c_void_p),
+        ("sum", C.c_void_p),
+    ]
+
+
+class MemlayerNormGrads(C.Structure):
+    _fields_ = [
+        ("dy", C.c_void_p),
+        ("dy_stride", C.c_int64),
+        ("x", C.c_void_p),
+        ("x_stride", C.c_int64),
+        ("dresidual", C.c_void_p),
+        ("dresidual_stride", C.c_int64),
+        ("scale", C.c_void_p),
+        ("dx", C.c_void_p),
+        ("dscale", C.c_void_p),
+        ("dbias", C.c_void_p),
+    ]
+
+
+class MemlayerLossConfig(C.Structure):
+    _fields_ = [
+        ("tokens", C.c_int64),
+        ("d_model", C.c_int32),
+        ("vocab_size", C.c_int32),
+        ("dtype", C.c_int32),
+        ("ignore_index", C.c_int32),
+    ]
+
+
+class MemlayerLossArgs(C.Structure):
+    _fields_ = [
+        ("h", C.c_void_p),
+        ("h_stride", C.c_int64),
+        ("weight", C.c_void_p),
+        ("weight_stride", C.c_int64),
+        ("targets", C.c_void_p),
+        ("loss", C.c_void_p),
+        ("lse", C.c_void_p),
+    ]
+
+
+class MemlayerLossGrads(C.Structure):
+    _fields_ = [
+        ("lse", C.c_void_p),
+        ("dloss", C.c_void_p),
+        ("dlse", C.c_void_p),
+        ("dh", C.c_void_p),
+        ("dweight", C.c_void_p),
+    ]
+
+
+class MemlayerOrthConfig(C.Structure):
+    _fields_ = [
+        ("batch", C.c_int64),
+        ("rows", C.c_int32),
+        ("cols", C.c_int32),
+        ("dtype", C.c_int32),
+        ("steps", C.c_int32),
+        ("a", C.c_float),
+        ("b", C.c_float),
+        ("c", C.c_float),
+        ("epsilon", C.c_float),
+    ]
+
+
 DEVICE_ERRORS = {11: "producer wait timed out", 12: "MMA wait timed out", 13: "MMA wait timed out",
                  14: "epilogue wait timed out", 15: "epilogue pair wait timed out",
                  21: "sub-key id out of range", 22: "sharded row id out of range",
                  23: "fetched slot id out of range", 24: "row push beyond inbox capacity",
                  25: "host-table row id out of range", 26: "token id or position out of range",
+                 27: "target id out of range",
                  31: "peer inbox wait timed out", 32: "peer partial-sum wait timed out",
                  33: "row-gradient inbox wait timed out", 34: "norm partial wait timed out",
                  35: "peer probe-row wait timed out", 36: "peer dot wait timed out"}
@@ -258,6 +342,8 @@ def lib() -> C.CDLL:
         L.memlayer_model_forward.argtypes = [C.POINTER(MemlayerModelConfig), C.POINTER(MemlayerModelParams),
                                              C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p, C.c_size_t,
                                              C.c_void_p]
+        L.memlayer_model_hidden.restype = C.c_int32
+        L.memlayer_model_hidden.argtypes = L.memlayer_model_forward.argtypes
         L.memlayer_model_decode_step.restype = C.c_int32
         L.memlayer_model_decode_step.argtypes = [C.POINTER(MemlayerModelConfig), C.POINTER(MemlayerModelParams),
                                                  C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p,
@@ -321,6 +407,31 @@ def lib() -> C.CDLL:
         L.memlayer_layer_backward_sharded.argtypes = [C.POINTER(MemlayerConfig), C.POINTER(MemlayerLayerArgs),
                                                       C.POINTER(MemlayerLayerGrads), C.c_void_p, C.c_int32,
                                                       C.c_void_p, C.c_size_t, C.c_void_p]
+        L.memlayer_layer_norm.restype = C.c_int32
+        L.memlayer_layer_norm.argtypes = [C.POINTER(MemlayerNormConfig), C.POINTER(MemlayerNormArgs), C.c_void_p]
+        L.memlayer_layer_norm_backward_workspace_size.restype = C.c_int32
+        L.memlayer_layer_norm_backward_workspace_size.argtypes = [C.POINTER(MemlayerNormConfig),
+                                                                  C.POINTER(C.c_size_t)]
+        L.memlayer_layer_norm_backward.restype = C.c_int32
+        L.memlayer_layer_norm_backward.argtypes = [C.POINTER(MemlayerNormConfig), C.POINTER(MemlayerNormGrads),
+                                                   C.c_void_p, C.c_size_t, C.c_void_p]
+        L.memlayer_cross_entropy_workspace_size.restype = C.c_int32
+        L.memlayer_cross_entropy_workspace_size.argtypes = [C.POINTER(MemlayerLossConfig), C.c_int32,
+                                                            C.POINTER(C.c_size_t)]
+        L.memlayer_cross_entropy.restype = C.c_int32
+        L.memlayer_cross_entropy.argtypes = [C.POINTER(MemlayerLossConfig), C.POINTER(MemlayerLossArgs), C.c_void_p,
+                                             C.c_size_t, C.c_void_p]
+        L.memlayer_cross_entropy_backward.restype = C.c_int32
+        L.memlayer_cross_entropy_backward.argtypes = [C.POINTER(MemlayerLossConfig), C.POINTER(MemlayerLossArgs),
+                                                      C.POINTER(MemlayerLossGrads), C.c_void_p, C.c_size_t,
+                                                      C.c_void_p]
+        L.memlayer_cross_entropy_status.restype = C.c_int32
+        L.memlayer_cross_entropy_status.argtypes = [C.c_void_p, C.POINTER(C.c_int32), C.c_void_p]
+        L.memlayer_orthogonalize_workspace_size.restype = C.c_int32
+        L.memlayer_orthogonalize_workspace_size.argtypes = [C.POINTER(MemlayerOrthConfig), C.POINTER(C.c_size_t)]
+        L.memlayer_orthogonalize.restype = C.c_int32
+        L.memlayer_orthogonalize.argtypes = [C.POINTER(MemlayerOrthConfig), C.c_void_p, C.c_void_p, C.c_void_p,
+                                             C.c_size_t, C.c_void_p]
         if L.memlayer_abi_version() != 1:
             raise ImportError("libmemlayer.so ABI version mismatch; rebuild")
         _lib = L

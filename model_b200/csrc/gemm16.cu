@@ -1,0 +1,230 @@
+// Host side of the 16-bit tensor-core GEMM (gemm16.cuh) and the kernels that
+// put its operands into 16-bit form: the largest magnitude of float32
+// matrices, their split into f16 pieces, and the copy of 16-bit matrices
+// whose rows TMA cannot address.
+#include <cudaTypedefs.h>
+
+#include <mutex>
+
+#include "gemm16.cuh"
+
+#include "pieces16.cuh"
+
+namespace ml {
+
+namespace {
+
+constexpr int NTH = 256;
+
+// Bits of the largest finite |x| (order of non-negative floats = order of bits).
+__global__ void __launch_bounds__(NTH) amax_kernel(AmaxArgs A) {
+  __shared__ unsigned red[NTH / 32];
+  int i = 0, b = blockIdx.x;
+  while (b >= A.m[i].blocks) b -= A.m[i++].blocks;
+  const AmaxMat M = A.m[i];
+  unsigned mx = 0;
+  auto take = [&](float x) {
+    const unsigned u = __float_as_uint(x) & 0x7FFFFFFFu;
+    if (u < 0x7F800000u && u > mx) mx = u;
+  };
+  const int64_t step = (int64_t)M.blocks * NTH, at = (int64_t)b * NTH + threadIdx.x;
+  if (M.pitch == M.cols && (reinterpret_cast<uintptr_t>(M.x) & 15) == 0) {
+    const int64_t n = M.rows * M.cols, n4 = n >> 2;
+    const float4* x4 = reinterpret_cast<const float4*>(M.x);
+    int64_t e = at;
+    for (; e + 3 * step < n4; e += 4 * step) {     // four loads in flight
+      float4 v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = x4[e + j * step];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        take(v[j].x);
+        take(v[j].y);
+        take(v[j].z);
+        take(v[j].w);
+      }
+    }
+    for (; e < n4; e += step) {
+      const float4 v = x4[e];
+      take(v.x);
+      take(v.y);
+      take(v.z);
+      take(v.w);
+    }
+    if (at < (n & 3)) take(M.x[(n4 << 2) + at]);
+  } else {
+    const int64_t n = M.rows * M.cols;
+    for (int64_t e = at; e < n; e += step) take(M.x[(e / M.cols) * M.pitch + e % M.cols]);
+  }
+  mx = __reduce_max_sync(FULL, mx);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = mx;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < NTH / 32; ++w) mx = max(mx, red[w]);
+    if (mx) atomicMax(M.out, mx);                  // a maximum: the order does not matter
+  }
+}
+
+// 8 columns a thread: hi / lo pieces of x s (float32 source) or a plain copy
+// (16-bit source), zeros in the padding columns.
+template <typename E>
+__global__ void __launch_bounds__(NTH) pieces_kernel(PiecesArgs A) {
+  int i = 0, b = blockIdx.x;
+  while (b >= A.m[i].blocks) b -= A.m[i++].blocks;
+  const PiecesMat M = A.m[i];
+  const int c8 = (int)(M.ld >> 3);
+  const int64_t n = M.rows * c8;
+  const E* src = reinterpret_cast<const E*>(M.x);
+  const float sc = sizeof(E) == 4 ? g16::scale_of(M.amax) : 1.f;
+  const bool vec = sizeof(E) == 4 && M.pitch % 4 == 0 && (reinterpret_cast<uintptr_t>(M.x) & 15) == 0;
+  for (int64_t e = (int64_t)b * NTH + threadIdx.x; e < n; e += (int64_t)M.blocks * NTH) {
+    const int64_t r = e / c8;
+    const int c = (int)(e - r * c8) * 8;
+    const E* p = src + r * M.pitch + c;
+    if constexpr (sizeof(E) == 4) {
+      float v[8];
+      if (vec && c + 8 <= M.cols) {
+        const float4 a = *reinterpret_cast<const float4*>(p), q = *reinterpret_cast<const float4*>(p + 4);
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+        v[4] = q.x; v[5] = q.y; v[6] = q.z; v[7] = q.w;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = c + j < M.cols ? p[j] : 0.f;
+      }
+      __half2 h[4], l[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) g16::split2(v[2 * j] * sc, v[2 * j + 1] * sc, h[j], l[j]);
+      *reinterpret_cast<uint4*>(reinterpret_cast<__half*>(M.hi) + r * M.ld + c) = *reinterpret_cast<uint4*>(h);
+      *reinterpret_cast<uint4*>(reinterpret_cast<__half*>(M.lo) + r * M.ld + c) = *reinterpret_cast<uint4*>(l);
+    } else {
+      alignas(16) E v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = c + j < M.cols ? p[j] : E(0);
+      *reinterpret_cast<uint4*>(reinterpret_cast<E*>(M.hi) + r * M.ld + c) = *reinterpret_cast<uint4*>(v);
+    }
+  }
+}
+
+int blocks_for(int64_t items, int per_thread) {
+  const int64_t b = (items + (int64_t)NTH * per_thread - 1) / ((int64_t)NTH * per_thread), cap = 8 * g16::device_sms();
+  return (int)(b < 1 ? 1 : b < cap ? b : cap);
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encode16_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  });
+  return fn;
+}
+
+}  // namespace
+
+namespace g16 {
+
+int device_sms() {
+  int dev = 0, sms = 148;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return sms;
+}
+
+cudaError_t make_operand(CUtensorMap* map, const void* base, int64_t rows, int64_t k, int64_t pitch, bool mn,
+                         int box_rows, int bf16, int batch, int64_t bstride) {
+  auto enc = encode16_fn();
+  if (!enc) return cudaErrorNotSupported;
+  const cuuint64_t dims[3] = {(cuuint64_t)(mn ? rows : k), (cuuint64_t)(mn ? k : rows), (cuuint64_t)batch};
+  const cuuint64_t strides[2] = {(cuuint64_t)pitch * 2, (cuuint64_t)(batch > 1 ? bstride : pitch * dims[1]) * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)(mn ? 64 : box_rows), 1}, one[3] = {1, 1, 1};
+  const CUresult r = enc(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                         const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+cudaError_t make_store(CUtensorMap* map, void* base, int64_t rows, int64_t cols, int64_t pitch, int dtype, int64_t z,
+                       int64_t zstride) {
+  auto enc = encode16_fn();
+  if (!enc) return cudaErrorNotSupported;
+  const bool f32 = dtype == MEMLAYER_F32;
+  const cuuint64_t es = f32 ? 4 : 2;
+  const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)z};
+  const cuuint64_t strides[2] = {pitch * es, (cuuint64_t)(z > 1 ? zstride : pitch * rows) * es};
+  const cuuint32_t box[3] = {32, 32, 1}, one[3] = {1, 1, 1};
+  const CUresult r =
+      enc(map,
+          f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+              : dtype == MEMLAYER_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+          3, base, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+          f32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+double distribute(Sched* S, int most, double over) {
+  const int n0 = S->prod[0].total(), n1 = S->prod[1].total();
+  int C = n0 + n1 < most ? n0 + n1 : most;
+  if (C < 1) C = 1;
+  S->clusters = C;
+  S->q = n0 / C;
+  S->r = n0 % C;
+  S->x[0] = S->x[1] = S->e[0] = S->e[1] = 0;
+  const double c0 = S->prod[0].kq + over, c1 = S->prod[1].kq + over;
+  double load[2] = {(S->q + 1) * c0, S->q * c0};
+  const int size[2] = {S->r, C - S->r};
+  int left = n1;
+  while (left > 0) {                       // a round of the less loaded group at a time
+    const int g = size[0] > 0 && load[0] < load[1] ? 0 : 1;
+    load[g] += c1;
+    if (left >= size[g]) {
+      S->x[g]++;
+      left -= size[g];
+    } else {
+      S->e[g] = left;
+      left = 0;
+    }
+  }
+  return size[0] > 0 && load[0] > load[1] ? load[0] : load[1];
+}
+
+}  // namespace g16
+
+cudaError_t launch_amax(AmaxArgs A, cudaStream_t s) {
+  int total = 0;
+  for (int i = 0; i < 4; ++i) {
+    if (A.m[i].rows * A.m[i].cols == 0) {
+      A.m[i].blocks = 0;
+      continue;
+    }
+    A.m[i].blocks = blocks_for(A.m[i].rows * A.m[i].cols, 16);
+    total += A.m[i].blocks;
+  }
+  if (!total) return cudaSuccess;
+  amax_kernel<<<total, NTH, 0, s>>>(A);
+  count_launch();
+  return cudaGetLastError();
+}
+
+cudaError_t launch_pieces(PiecesArgs A, int dtype, cudaStream_t s) {
+  int total = 0;
+  for (int i = 0; i < 2; ++i) {
+    const int64_t n = A.m[i].rows * (A.m[i].ld >> 3);
+    A.m[i].blocks = n ? blocks_for(n, 2) : 0;
+    total += A.m[i].blocks;
+  }
+  if (!total) return cudaSuccess;
+  if (dtype == MEMLAYER_F32)
+    pieces_kernel<float><<<total, NTH, 0, s>>>(A);
+  else
+    pieces_kernel<unsigned short><<<total, NTH, 0, s>>>(A);   // 16 bits as they are
+  count_launch();
+  return cudaGetLastError();
+}
+
+}  // namespace ml

@@ -1,0 +1,671 @@
+// Persistent 16-bit tensor-core GEMM with exchangeable epilogues: the products
+// of the vocabulary cross entropy (loss.cu) and of the orthogonalised update
+// (orth.cu).
+//
+//   acc[i, j] = sum_k A(i, k) B(j, k)   in float32 TMEM accumulators
+//
+// An operand is one 16-bit matrix, or two (PA, PB = 2): the float32 matrix
+// x s (s a power of two) as hi = f16(x s), lo = f16(x s - hi), 22 bits of it;
+// then the product is hi.hi + hi.lo + lo.hi -- the dropped lo.lo is below
+// 2^-22 -- at three 16-bit products, half the tensor time of the 3xTF32
+// split (kind::tf32 runs at half the 16-bit rate).  The f16 range does for
+// float32 data because s puts the largest entry at 2^14..2^15: entries down
+// to 2^-18 of it keep all 22 bits, smaller ones an absolute error of 2^-40
+// of it.
+//
+// The tensor cores add into TMEM by truncation: an entry loses up to one unit
+// of its last place per 16-k step, always towards zero.  Over a k of
+// thousands that is 1e-5 (measured: dh of a 9,000-entry vocabulary 2.4e-5
+// off), too much for a float32 result.  So of a stage's two-piece products
+// the small ones go first, while the accumulator is small, and epilogues that
+// ask for it (kSum) get k in segments of S.seg stages, which they add in
+// registers, rounding to nearest.
+//
+// Each operand is read as stored, by TMA with the 128-byte swizzle: K-major
+// (k contiguous) or MN-major (the row index contiguous).  Rows past the end
+// and the tail of k read as zeros.  z: independent products (batch).
+//
+// CTA = 12 warps: warps 0-7 epilogue (TMEM lane = output row; the two warps
+// of a lane quarter take half of the columns each), warp 8 TMA producer, warp
+// 9 MMA issuer, two idle ones that complete its warpgroup.  CG = 2 pairs two SMs on a 256-row tile: each CTA stages
+// its own 128 rows of A and half of the rows of B, the leader issues for
+// both, and each CTA drains its own 128 rows.  Accumulators are
+// double-buffered in TMEM, so an epilogue runs beside the next tile's MMAs.
+// Every mbarrier wait is bounded.
+#pragma once
+
+#include "tc_common.cuh"
+
+namespace ml {
+namespace g16 {
+
+constexpr int THREADS = 384;
+constexpr int EPI_WARPS = 8;
+constexpr int BK = 64;                    // k elements per stage: 128-byte rows
+constexpr int MAX_STAGES = 8;
+constexpr uint32_t STAGING = 4096;        // an epilogue warp's 32 rows x 128 bytes
+constexpr uint32_t CTL_BYTES = 1024;
+constexpr uint32_t SMEM_LIMIT = 227 * 1024;
+
+struct Ctl {
+  uint64_t full[MAX_STAGES], empty[MAX_STAGES], tfull[2], tempty[2];
+  uint32_t tmem_base;
+  int abort;
+};
+
+struct Maps {
+  CUtensorMap a[2][2], b[2][2];           // [product of the launch][hi / lo]
+};
+
+struct Tile {
+  int q, z, mt, nt, ks;                   // q: product of the launch
+};
+
+// One product: its tiles, cut into `splits` slices of kq BK-element stages.
+struct Prod {
+  int m_tiles, n_tiles, splits, batch;
+  int kq, kq_total;
+  uint32_t amn, bmn;                      // operand is MN-major
+  __host__ __device__ int total() const { return m_tiles * n_tiles * splits * batch; }
+};
+
+// The tiles of one launch, over `clusters` clusters (CTAs or pairs).
+// contiguous (one product, one slice): cluster c takes an equal run of the
+// tiles, column tile fastest -- for an epilogue that keeps state along a row
+// block.  Otherwise the first product's tiles go round the clusters, row
+// tile fastest (neighbouring clusters share B), and the second product's,
+// which are no longer than the first's, fill the clusters up to a common
+// level in runs: the first `r` clusters, which have one long tile more, take
+// x[0] each, the others x[1], and the first e[g] of a group one more.
+struct Sched {
+  Prod prod[2];
+  int clusters, contiguous;
+  int q, r, x[2], e[2];
+  int BN;                                 // columns per tile (MMA N)
+  int seg;                                // stages per segment (kSum)
+  int stages;
+  uint32_t bf16;                          // operand type
+  // Where the contiguous run of cluster c begins.
+  __host__ __device__ int first(int c) const { return (int)((int64_t)prod[0].total() * c / clusters); }
+  // The cluster whose contiguous run holds tile `lin`.
+  __host__ __device__ int owner(int lin) const {
+    const int64_t n = prod[0].total();
+    return (int)((((int64_t)lin + 1) * clusters + n - 1) / n) - 1;
+  }
+  __device__ __forceinline__ int count(int c) const {
+    if (contiguous) return first(c + 1) - first(c);
+    const int g = c < r ? 0 : 1, i = g ? c - r : c;
+    return q + (c < r) + x[g] + (i < e[g]);
+  }
+  __device__ __forceinline__ Tile tile(int c, int i) const {
+    Tile t;
+    if (contiguous) {
+      const int lin = first(c) + i;
+      t.mt = lin / prod[0].n_tiles;
+      t.nt = lin - t.mt * prod[0].n_tiles;
+      t.q = t.ks = t.z = 0;
+      return t;
+    }
+    const int own = q + (c < r);
+    int lin = c + i * clusters;
+    t.q = 0;
+    if (i >= own) {
+      const int g = c < r ? 0 : 1, j = g ? c - r : c;
+      lin = (g ? r * x[0] + e[0] : 0) + j * x[g] + min(j, e[g]) + (i - own);
+      t.q = 1;
+    }
+    const Prod& p = prod[t.q];
+    t.mt = lin % p.m_tiles;
+    lin /= p.m_tiles;
+    t.nt = lin % p.n_tiles;
+    lin /= p.n_tiles;
+    t.ks = lin % p.splits;
+    t.z = lin / p.splits;
+    return t;
+  }
+  __device__ __forceinline__ int stages_of(const Tile& t) const {
+    const int rem = prod[t.q].kq_total - t.ks * prod[t.q].kq;
+    return rem < prod[t.q].kq ? rem : prod[t.q].kq;
+  }
+};
+
+// Fills in the distribution over at most `most` clusters; the cost of a tile
+// is its stages plus `over`.  Returns the largest cluster's cost.
+double distribute(Sched* S, int most, double over);
+
+// ---- PTX pieces ----------------------------------------------------------------
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t map_to_cta(uint32_t saddr, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
+  return r;
+}
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// bar: a shared::cluster address (CG = 2: the leader's barrier).
+template <int CG>
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y, int z) {
+  if constexpr (CG == 2)
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, "
+        "%4, %5}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], "
+        "[%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+
+template <int CG>
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  if constexpr (CG == 2)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// Arrives on the barrier (of both CTAs of a pair) once the MMAs issued so far are done.
+template <int CG>
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  if constexpr (CG == 2)
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            tc::smem_u32(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+  else
+    tc::mma_commit(bar);
+}
+
+template <int CG>
+__device__ __forceinline__ void tmem_alloc(uint32_t* dst, uint32_t cols) {
+  if constexpr (CG == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(dst)),
+                 "r"(cols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  } else {
+    tc::tmem_alloc(dst, cols);
+  }
+}
+
+template <int CG>
+__device__ __forceinline__ void tmem_dealloc(uint32_t addr, uint32_t cols) {
+  if constexpr (CG == 2)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols) : "memory");
+  else
+    tc::tmem_dealloc(addr, cols);
+}
+
+// Descriptor of an MN-major tile: 64 rows (128 bytes) x 64 k per block, each
+// block 8 KB of 128-byte k rows in 1024-byte swizzle atoms of 8 k.  Leading
+// byte offset: block to block along the row index; stride byte offset: atom
+// to atom along k.
+__device__ __forceinline__ uint64_t sdesc_mn_sw128(uint32_t saddr) {
+  return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)(8192 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+// Instruction descriptor of kind::f16: D float32, A and B both f16 or both
+// bf16, each K-major or MN-major.
+__device__ __forceinline__ uint32_t idesc_16(int M, int N, uint32_t bf16, uint32_t amn, uint32_t bmn) {
+  return (1u << 4) | (bf16 << 7) | (bf16 << 10) | (amn << 15) | (bmn << 16) |
+         ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
+// 2^x (ex2.approx: 2 ulp).
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// ---- staged stores ---------------------------------------------------------------
+// An epilogue thread holds a row; a warp's stores straight from registers
+// would touch 32 rows each.  Instead a warp writes 32 rows x 32 columns into
+// its staging buffer (swizzled as the tensor map says) and one thread hands
+// the block to a bulk tensor store, which clips it at the matrix's edges.
+template <int N, bool READ>
+__device__ __forceinline__ void bulk_wait() {
+  if constexpr (READ)
+    asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+  else
+    asm volatile("cp.async.bulk.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void bulk_store(const CUtensorMap* map, uint32_t src, int x, int y, int z, bool add) {
+  if (add)
+    asm volatile(
+        "cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+            reinterpret_cast<uint64_t>(map)),
+        "r"(src), "r"(x), "r"(y), "r"(z)
+        : "memory");
+  else
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+                     reinterpret_cast<uint64_t>(map)),
+                 "r"(src), "r"(x), "r"(y), "r"(z)
+                 : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+
+__device__ __forceinline__ void st_shared(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+// The calling lane's row of 32 16-bit values (64 bytes, 64-byte swizzle) /
+// of 32 floats (128 bytes, 128-byte swizzle).
+__device__ __forceinline__ void stage16(uint32_t buf, int lane, const uint32_t (&h)[16]) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    st_shared(buf + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4), h[4 * c], h[4 * c + 1], h[4 * c + 2], h[4 * c + 3]);
+}
+__device__ __forceinline__ void stage32(uint32_t buf, int lane, const uint32_t (&v)[32]) {
+#pragma unroll
+  for (int c = 0; c < 8; ++c)
+    st_shared(buf + lane * 128 + ((c ^ (lane & 7)) << 4), v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+}
+// Entry (row, column) of a staged block.
+__device__ __forceinline__ uint32_t at16(uint32_t buf, int r, int c) {
+  return buf + r * 64 + (((c >> 3) ^ ((r >> 1) & 3)) << 4) + (c & 7) * 2;
+}
+__device__ __forceinline__ uint32_t at32(uint32_t buf, int r, int c) {
+  return buf + r * 128 + (((c >> 2) ^ (r & 7)) << 4) + (c & 3) * 4;
+}
+
+// The calling lane's row of 32 float32 values staged in the output's type.
+__device__ __forceinline__ void stage_as(int dtype, uint32_t buf, int lane, const uint32_t (&v)[32]) {
+  if (dtype == MEMLAYER_F32) {
+    stage32(buf, lane, v);
+    return;
+  }
+  uint32_t h[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const float x = __uint_as_float(v[2 * j]), y = __uint_as_float(v[2 * j + 1]);
+    if (dtype == MEMLAYER_BF16) {
+      const __nv_bfloat162 u = __floats2bfloat162_rn(x, y);
+      h[j] = *reinterpret_cast<const uint32_t*>(&u);
+    } else {
+      const __half2 u = __floats2half2_rn(x, y);
+      h[j] = *reinterpret_cast<const uint32_t*>(&u);
+    }
+  }
+  stage16(buf, lane, h);
+}
+
+// A staged block to rows that TMA cannot address: a row per pass, a column
+// per lane; `at`: the block's first entry, `rows` x `cols` of it inside.
+__device__ __forceinline__ void copy_rows(int dtype, uint32_t buf, void* out, int64_t at, int64_t ld, int rows,
+                                          int cols, bool add) {
+  const int lane = threadIdx.x & 31;
+  if (lane >= cols) return;
+  for (int r0 = 0; r0 < rows; r0 += 8) {   // eight loads in flight
+    if (dtype == MEMLAYER_F32) {
+      float* p = reinterpret_cast<float*>(out) + at + r0 * ld + lane;
+      float old[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r) old[r] = add && r0 + r < rows ? p[r * ld] : 0.f;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        float x;
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(at32(buf, r0 + r, lane)) : "memory");
+        if (r0 + r < rows) p[r * ld] = old[r] + x;
+      }
+    } else {
+      uint16_t* p = reinterpret_cast<uint16_t*>(out) + at + r0 * ld + lane;
+#pragma unroll
+      for (int r = 0; r < 8; ++r) {
+        uint16_t x;
+        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(x) : "r"(at16(buf, r0 + r, lane)) : "memory");
+        if (r0 + r < rows) p[r * ld] = x;
+      }
+    }
+  }
+}
+
+// A segment's columns (64 or 128) added to a thread's sums.  They have to
+// stay in registers (hence the redistribution of the CTA's): spilled, a
+// segment's drain took 4,000 to 6,000 cycles instead of 700.
+__device__ __forceinline__ void add_segment(uint32_t taddr, float (&sum)[128], int cols, int sg) {
+#pragma unroll
+  for (int c = 0; c < 128; c += 64) {
+    if (c >= cols) break;
+    uint32_t v[32], w[32];
+    tc::tmem_ld32(taddr + c, v);
+    tc::tmem_ld32(taddr + c + 32, w);
+    tc::tmem_wait_ld();
+    if (sg == 0) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        sum[c + j] = __uint_as_float(v[j]);
+        sum[c + 32 + j] = __uint_as_float(w[j]);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        sum[c + j] += __uint_as_float(v[j]);
+        sum[c + 32 + j] += __uint_as_float(w[j]);
+      }
+    }
+  }
+}
+
+// ---- power-of-two scales ---------------------------------------------------------
+// amax: the float bits of the largest finite magnitude (0: no entry or all
+// zero).  scale_of puts it in [2^14, 2^15); the exponent is clamped so that
+// both the scale and its inverse are normal floats.
+__device__ __forceinline__ int scale_exp(unsigned amax) {
+  if (amax == 0) return 0;
+  const int e = (int)(amax >> 23) - 127;   // a subnormal maximum counts as 2^-127
+  const int s = 14 - e;
+  return s > 126 ? 126 : s;
+}
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
+__device__ __forceinline__ float scale_of(const unsigned* amax) { return amax ? pow2(scale_exp(*amax)) : 1.0f; }
+
+// x 2^e of a product's accumulator, e beyond one float's exponent range too.
+struct Unscale {
+  float a, b;
+  __device__ __forceinline__ explicit Unscale(int e) {
+    const int e1 = max(-126, min(127, e));
+    a = pow2(e1);
+    b = pow2(max(-126, min(127, e - e1)));
+  }
+  __device__ __forceinline__ float operator()(float x) const { return x * a * b; }
+};
+
+// ---- the kernel --------------------------------------------------------------------
+__host__ __device__ inline uint32_t a_bytes() { return 128 * 128; }                  // one piece, one stage, one CTA
+__host__ __device__ inline uint32_t b_bytes(int BN, int cg) { return (uint32_t)(BN / cg) * 128; }
+
+template <class EPI, int CG, int PA, int PB>
+__global__ void __launch_bounds__(THREADS, 1)
+    gemm16_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Sched S,
+                  const __grid_constant__ typename EPI::Args ea, int* err) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  Ctl* ctl = reinterpret_cast<Ctl*>(smem);
+  uint8_t* ring = smem + CTL_BYTES;
+  volatile int* abort = &ctl->abort;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = CG == 2 ? cluster_rank() : 0;
+  const int cluster = blockIdx.x / CG;
+  const uint32_t ab = a_bytes(), bb = b_bytes(S.BN, CG), stage_bytes = PA * ab + PB * bb;
+  constexpr bool SUM = EPI::kSum;
+  const int cnt = S.count(cluster);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S.stages; ++s) {
+      tc::mbar_init(&ctl->full[s], 1);
+      tc::mbar_init(&ctl->empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      tc::mbar_init(&ctl->tfull[b], 1);
+      tc::mbar_init(&ctl->tempty[b], CG * EPI_WARPS);
+    }
+    ctl->abort = 0;
+    tc::fence_mbar_init();
+  }
+  if (warp == 9) tmem_alloc<CG>(&ctl->tmem_base, 512);
+  tc::fence_before_sync();
+  if constexpr (CG == 2)
+    cluster_sync();
+  else
+    __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem_base = ctl->tmem_base;
+
+  if (warp < EPI_WARPS) {
+    // kSum keeps 128 sums a thread: 384 x 168 registers dealt out again, 256 x 224 + 128 x 56
+    if constexpr (SUM) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    const int quarter = warp & 3, half = warp >> 2;
+    EPI epi;
+    epi.begin(ea, S, cluster, ring + (size_t)S.stages * stage_bytes + warp * STAGING);
+    int acc = 0;
+    uint32_t aph = 0;
+    uint32_t tempty[2];
+    for (int b = 0; b < 2; ++b) {
+      tempty[b] = tc::smem_u32(&ctl->tempty[b]);
+      if constexpr (CG == 2) tempty[b] = map_to_cta(tempty[b], 0);
+    }
+    for (int i = 0; i < cnt; ++i) {
+      const Tile t = S.tile(cluster, i);
+      const int64_t row = (int64_t)t.mt * (128 * CG) + rank * 128 + quarter * 32 + lane;
+      const int nseg = SUM ? (S.stages_of(t) + S.seg - 1) / S.seg : 1;
+      bool ok = true;
+      for (int sg = 0; sg < nseg; ++sg) {
+        if (!__all_sync(FULL, tc::mbar_wait(&ctl->tfull[acc], aph, abort, err, 15))) {
+          ok = false;
+          break;
+        }
+        tc::fence_after_sync();
+        const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * 256);
+        if constexpr (SUM)
+          add_segment(taddr + half * (S.BN >> 1), epi.sum, S.BN >> 1, sg);
+        else
+          epi.tile(ea, S, t, row, half, taddr);
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (CG == 2)
+            arrive_cluster(tempty[acc]);
+          else
+            tc::mbar_arrive(&ctl->tempty[acc]);
+        }
+        if constexpr (SUM) {               // the accumulator is free before the stores
+          if (sg == nseg - 1) epi.store(ea, S, t, row, half);
+        }
+        acc ^= 1;
+        if (acc == 0) aph ^= 1;
+      }
+      if (!ok) break;
+    }
+    epi.end(ea, S, half);
+    if constexpr (EPI::kStore) {
+      if (lane == 0) bulk_wait<0, false>();   // the stores are done with the staging buffers
+    }
+  } else {
+    if constexpr (SUM) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 8) {
+      if (lane == 0) {
+        for (int q = 0; q < 2 && S.prod[q].m_tiles > 0; ++q)
+          for (int p = 0; p < 2; ++p) {
+            if (p < PA) tc::prefetch_tmap(&maps.a[q][p]);
+            if (p < PB) tc::prefetch_tmap(&maps.b[q][p]);
+          }
+        int s = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        for (int i = 0; i < cnt && ok; ++i) {
+          const Tile t = S.tile(cluster, i);
+          const int nk = S.stages_of(t);
+          const uint32_t amn = S.prod[t.q].amn, bmn = S.prod[t.q].bmn;
+          const int ar = t.mt * (128 * CG) + (int)rank * 128;
+          const int br = t.nt * S.BN + (int)rank * (S.BN / CG);
+          for (int kc = 0; kc < nk; ++kc) {
+            if (!tc::mbar_wait(&ctl->empty[s], ph ^ 1, abort, err, 11)) {
+              ok = false;
+              break;
+            }
+            const int k = (t.ks * S.prod[t.q].kq + kc) * BK;
+            const uint32_t st = tc::smem_u32(ring + (size_t)s * stage_bytes);
+            if (rank == 0) tc::mbar_expect_tx(&ctl->full[s], CG * stage_bytes);
+            uint32_t bar = tc::smem_u32(&ctl->full[s]);
+            if constexpr (CG == 2) bar = map_to_cta(bar, 0);
+  #pragma unroll
+            for (int p = 0; p < PA; ++p) {
+              const uint32_t da = st + p * ab;
+              const CUtensorMap* ma = &maps.a[t.q][p];
+              if (amn) {
+                tma_load_3d<CG>(da, ma, bar, ar, k, t.z);
+                tma_load_3d<CG>(da + 8192, ma, bar, ar + 64, k, t.z);
+              } else {
+                tma_load_3d<CG>(da, ma, bar, k, ar, t.z);
+              }
+            }
+  #pragma unroll
+            for (int p = 0; p < PB; ++p) {
+              const uint32_t db = st + PA * ab + p * bb;
+              const CUtensorMap* mb = &maps.b[t.q][p];
+              if (bmn) {
+                for (int c = 0; c < S.BN / CG; c += 64) tma_load_3d<CG>(db + (c >> 6) * 8192, mb, bar, br + c, k, t.z);
+              } else {
+                tma_load_3d<CG>(db, mb, bar, k, br, t.z);
+              }
+            }
+            if (++s == S.stages) {
+              s = 0;
+              ph ^= 1;
+            }
+          }
+        }
+        // every stage read (in a pair: the leader's arrivals on this CTA's barriers are in)
+        for (int j = 0; j < S.stages && ok; ++j) {
+          ok = tc::mbar_wait(&ctl->empty[s], ph ^ 1, abort, err, 11);
+          if (++s == S.stages) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+      }
+    } else if (warp == 9) {
+      if (lane == 0 && rank == 0) {
+        int s = 0, acc = 0;
+        uint32_t ph = 0, aph = 0;
+        bool ok = true;
+        for (int i = 0; i < cnt && ok; ++i) {
+          const Tile t = S.tile(cluster, i);
+          const int nk = S.stages_of(t);
+          const uint32_t amn = S.prod[t.q].amn, bmn = S.prod[t.q].bmn;
+          const uint32_t idesc = idesc_16(128 * CG, S.BN, S.bf16, amn, bmn);
+          // 16 k: 32 bytes along a K-major row, 16 rows of 128 bytes of an MN-major block
+          const uint32_t astep = amn ? 2048 : 32, bstep = bmn ? 2048 : 32;
+          const uint64_t adesc = amn ? sdesc_mn_sw128(0) : tc::sdesc_k_sw128(0);
+          const uint64_t bdesc = bmn ? sdesc_mn_sw128(0) : tc::sdesc_k_sw128(0);
+          const int nseg = SUM ? (nk + S.seg - 1) / S.seg : 1;
+          for (int sg = 0; sg < nseg && ok; ++sg) {
+            if (!tc::mbar_wait(&ctl->tempty[acc], aph ^ 1, abort, err, 12)) {
+              ok = false;
+              break;
+            }
+            tc::fence_after_sync();
+            const uint32_t d = tmem_base + (uint32_t)(acc * 256);
+            const int kc0 = nk * sg / nseg, kc1 = nk * (sg + 1) / nseg;
+            for (int kc = kc0; kc < kc1; ++kc) {
+              if (!tc::mbar_wait(&ctl->full[s], ph, abort, err, 13)) {
+                ok = false;
+                break;
+              }
+              tc::fence_after_sync();
+              const uint32_t sa = tc::smem_u32(ring + (size_t)s * stage_bytes), sb = sa + PA * ab;
+              uint32_t more = kc > kc0;
+              auto step = [&](uint32_t a, uint32_t b) {
+                mma_f16<CG>(d, adesc | ((a >> 4) & 0x3FFF), bdesc | ((b >> 4) & 0x3FFF), idesc, more);
+                more = 1;
+              };
+              if constexpr (PA == 2) {
+#pragma unroll
+                for (int k16 = 0; k16 < BK / 16; ++k16) step(sa + ab + k16 * astep, sb + k16 * bstep);
+              }
+              if constexpr (PB == 2) {
+#pragma unroll
+                for (int k16 = 0; k16 < BK / 16; ++k16) step(sa + k16 * astep, sb + bb + k16 * bstep);
+              }
+#pragma unroll
+              for (int k16 = 0; k16 < BK / 16; ++k16) step(sa + k16 * astep, sb + k16 * bstep);
+              commit<CG>(&ctl->empty[s]);
+              if (++s == S.stages) {
+                s = 0;
+                ph ^= 1;
+              }
+            }
+            if (!ok) break;
+            commit<CG>(&ctl->tfull[acc]);
+            acc ^= 1;
+            if (acc == 0) aph ^= 1;
+          }
+        }
+      }
+    }
+  }
+  __syncwarp();
+  tc::fence_before_sync();
+  if constexpr (CG == 2)
+    cluster_sync();
+  else
+    __syncthreads();
+  if (warp == 9) {
+    tc::fence_after_sync();
+    tmem_dealloc<CG>(tmem_base, 512);
+  }
+}
+
+// ---- host side -------------------------------------------------------------------
+// One 16-bit operand: rows x k (per batch), K-major (row pitch `pitch`) or
+// MN-major (k rows of `pitch` elements).  pitch and bstride in elements,
+// multiples of 8; base 16-byte aligned.  box_rows: rows staged per CTA.
+cudaError_t make_operand(CUtensorMap* map, const void* base, int64_t rows, int64_t k, int64_t pitch, bool mn,
+                         int box_rows, int bf16, int batch = 1, int64_t bstride = 0);
+
+// A matrix written by staged stores: rows x cols of 16-bit or float32
+// entries, row pitch in elements (rows 16 bytes apart), z of them.
+cudaError_t make_store(CUtensorMap* map, void* base, int64_t rows, int64_t cols, int64_t pitch, int dtype,
+                       int64_t z = 1, int64_t zstride = 0);
+
+inline int smem_stages(int BN, int cg, int pa, int pb, bool store) {
+  const uint32_t st = pa * a_bytes() + pb * b_bytes(BN, cg);
+  const int n = (int)((SMEM_LIMIT - 1024 - CTL_BYTES - (store ? EPI_WARPS * STAGING : 0)) / st);
+  return n > MAX_STAGES ? MAX_STAGES : n;
+}
+
+int device_sms();
+
+template <class EPI, int CG, int PA, int PB>
+cudaError_t launch_one(const Maps& maps, Sched S, const typename EPI::Args& ea, int* err, cudaStream_t s) {
+  S.stages = smem_stages(S.BN, CG, PA, PB, EPI::kStore);
+  const size_t smem = 1024 + CTL_BYTES + (size_t)S.stages * (PA * a_bytes() + PB * b_bytes(S.BN, CG)) +
+                      (EPI::kStore ? EPI_WARPS * STAGING : 0);
+  auto kern = gemm16_kernel<EPI, CG, PA, PB>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(S.clusters * CG);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = CG;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, kern, maps, S, ea, err);
+  count_launch();
+  return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+}  // namespace g16
+}  // namespace ml

@@ -1,0 +1,805 @@
+// Softmax cross entropy over the vocabulary, fused with the output projection
+// (the tied logits of memory_pool_model/model.py:125 under the trainer's
+// integer-label cross entropy), and its gradient:
+//
+//   z = h W^T                       [T, V], never stored
+//   lse_t = log sum_v exp z_tv,  loss_t = lse_t - z_t,target (0 when ignored)
+//   dz_tv = p_tv (dloss_t + dlse_t) - [v == target] dloss_t,  p = exp(z - lse)
+//   dh = dz W,  dW = dz^T h
+//
+// Forward: one pass of 16-bit tensor-core tiles (gemm16.cuh) over the
+// vocabulary; the epilogue thread of a row keeps the running maximum and sum
+// of its columns in registers along its cluster's run of tiles, so a row
+// block leaves one (maximum, sum) pair per run and column half; a second
+// kernel joins them.  Backward: the vocabulary in pieces; for each piece the
+// logits are computed again, the epilogue turns them into dz (16 bits, the
+// piece's [T, piece] matrix in the workspace), and one launch multiplies it
+// both ways, dW of the piece and its part of dh.
+//
+// float32 operands run as two f16 pieces each (22 bits, see gemm16.cuh), dz
+// too; 16-bit operands as they are, dz rounded once to their type (its
+// relative error, 2^-9 or 2^-12, averages out over the sums it enters).  f16
+// dz carries a power-of-two scale from the largest |dloss|.  Statistics,
+// exponentials and sums are float32.
+#include "loss.cuh"
+
+#include <float.h>
+
+#include "gemm16.cuh"
+#include "pieces16.cuh"
+
+namespace ml {
+
+namespace {
+
+using g16::Maps;
+using g16::Prod;
+using g16::Sched;
+using g16::Tile;
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr int STATUS_TARGET = 27;
+// Stages per segment of k in the float32 gradient products: 192 k, 12 steps.
+// dW of 1,000 tokens is 0.8e-6 off with 4, 0.58e-6 with 3, 0.45e-6 with 2
+// (a float32 GEMM 0.56e-6); at 8192 x 256 x 16384 they take 296, 304, 367 us.
+constexpr int SEG = 3;
+// Stages per segment of the float32 logits, beyond a k of as many: there the
+// loss is up to 0.6e-6 off, without segments 1.3e-6 at a k of 1024.
+constexpr int LOGIT_SEG = 8;
+
+__device__ __forceinline__ int exp_of(const unsigned* amax) { return amax ? g16::scale_exp(*amax) : 0; }
+
+// Factor that turns an accumulator of the logits back: a normal float (beyond
+// that range logits are zero or infinite for every purpose).
+__device__ __forceinline__ float logit_unscale(const unsigned* amax_h, const unsigned* amax_w) {
+  return g16::pow2(max(-100, min(126, -exp_of(amax_h) - exp_of(amax_w))));
+}
+
+// The 32 columns from cc on of an epilogue thread's row: from its accumulator,
+// or from the sums of its segments.
+struct FromTmem {
+  uint32_t taddr;
+  __device__ __forceinline__ void operator()(int cc, uint32_t (&v)[32]) const {
+    tc::tmem_ld32(taddr + cc, v);
+    tc::tmem_wait_ld();
+  }
+};
+struct FromSums {
+  const float (&sum)[128];
+  __device__ __forceinline__ void operator()(int cc, uint32_t (&v)[32]) const {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(sum[cc + j]);
+  }
+};
+
+// ---- forward epilogue ------------------------------------------------------------
+struct StatsArgs {
+  int64_t T;
+  int V;
+  const unsigned *amax_h, *amax_w;   // float32 operands: scale maxima (else null)
+  const int* targets;
+  float2* part;                      // [slot][half][T] (maximum in log2 units, sum)
+  float* zt;                         // [T] target logit
+};
+
+template <bool SUM>
+struct EpiStats {
+  static constexpr bool kSum = SUM, kStore = false;
+  float sum[128];
+  using Args = StatsArgs;
+  float m, s, c, un;
+  int mt, slot, target;
+  int64_t row;
+  bool any;
+
+  __device__ __forceinline__ void begin(const Args& A, const Sched&, int cluster, uint8_t*) {
+    un = logit_unscale(A.amax_h, A.amax_w);
+    c = un * LOG2E;
+    mt = -1;
+    slot = cluster;
+    any = false;
+  }
+  __device__ __forceinline__ void flush(const Args& A, const Sched& S, int half) {
+    if (!any || row >= A.T) return;
+    // clusters before this one that hold tiles of the row block
+    const int first = S.owner(mt * S.prod[0].n_tiles);
+    A.part[((int64_t)(slot - first) * 2 + half) * A.T + row] = make_float2(m * c, s);
+  }
+  template <class Get>
+  __device__ __forceinline__ void blocks(const Args& A, const Sched& S, const Tile& t, int64_t r, int half, Get get) {
+    if (t.mt != mt) {
+      flush(A, S, half);
+      mt = t.mt;
+      row = r;
+      m = -INFINITY;
+      s = 0.f;
+      any = true;
+      target = row < A.T ? A.targets[row] : -1;
+    }
+    const int hw = S.BN >> 1;
+    const int col0 = t.nt * S.BN + half * hw;
+#pragma unroll
+    for (int cc = 0; cc < 128; cc += 32) {
+      if (cc >= hw || col0 + cc >= A.V) break;   // the same for the whole warp
+      uint32_t v[32];
+      __syncwarp();
+      get(cc, v);
+      const int left = A.V - (col0 + cc);
+      if (left < 32) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (j >= left) v[j] = 0xFF800000u;   // -inf
+      }
+      float mx = __uint_as_float(v[0]);
+#pragma unroll
+      for (int j = 1; j < 32; ++j) mx = fmaxf(mx, __uint_as_float(v[j]));
+      const float mn = fmaxf(m, mx);
+      const float ref = mn == -INFINITY ? 0.f : mn * c;
+      float a[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < 32; ++j) a[j & 3] += g16::exp2_fast(fmaf(__uint_as_float(v[j]), c, -ref));
+      s = fmaf(s, g16::exp2_fast(fmaf(m, c, -ref)), (a[0] + a[1]) + (a[2] + a[3]));
+      m = mn;
+      const unsigned at = (unsigned)(target - (col0 + cc));
+      if (at < 32u && (int)at < left) {
+        float z = 0.f;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) z = at == j ? __uint_as_float(v[j]) : z;
+        A.zt[row] = z * un;
+      }
+    }
+  }
+  __device__ __forceinline__ void tile(const Args& A, const Sched& S, const Tile& t, int64_t row, int half,
+                                       uint32_t taddr) {
+    blocks(A, S, t, row, half, FromTmem{taddr + half * (S.BN >> 1)});
+  }
+  __device__ __forceinline__ void store(const Args& A, const Sched& S, const Tile& t, int64_t row, int half) {
+    blocks(A, S, t, row, half, FromSums{sum});
+  }
+  __device__ __forceinline__ void end(const Args& A, const Sched& S, int half) { flush(A, S, half); }
+};
+
+// Joins the partial (maximum, sum) pairs of a row, in slot order per lane and
+// a fixed tree over the lanes.  One warp per row.
+__global__ void __launch_bounds__(256) loss_join_kernel(const float2* __restrict__ part, const float* __restrict__ zt,
+                                                        const int* __restrict__ targets, int64_t T, int V, Sched S,
+                                                        int rows_per_tile, int ignore,
+                                                        float* __restrict__ loss, float* __restrict__ lse,
+                                                        int* __restrict__ err) {
+  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (row >= T) return;
+  const int mt = (int)(row / rows_per_tile), nt = S.prod[0].n_tiles;
+  const int c0 = S.owner(mt * nt), c1 = S.owner(mt * nt + nt - 1);
+  const int n = (c1 - c0 + 1) * 2;
+  float m = -INFINITY, s = 0.f;
+  for (int i = lane; i < n; i += 32) {
+    const float2 p = part[(int64_t)i * T + row];
+    const float mn = fmaxf(m, p.x);
+    const float ref = mn == -INFINITY ? 0.f : mn;
+    s = s * exp2f(m - ref) + p.y * exp2f(p.x - ref);
+    m = mn;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float m2 = __shfl_xor_sync(FULL, m, o), s2 = __shfl_xor_sync(FULL, s, o);
+    const float mn = fmaxf(m, m2);
+    const float ref = mn == -INFINITY ? 0.f : mn;
+    s = s * exp2f(m - ref) + s2 * exp2f(m2 - ref);
+    m = mn;
+  }
+  if (lane == 0) {
+    const float l = (m + log2f(s)) * LN2;
+    lse[row] = l;
+    const int t = targets[row];
+    const bool in = t >= 0 && t < V;
+    float x = 0.f;
+    if (t != ignore) {
+      x = in ? l - zt[row] : __int_as_float(0x7FC00000);
+      if (!in) atomicCAS(err, 0, STATUS_TARGET);
+    }
+    loss[row] = x;
+  }
+}
+
+// ---- backward ---------------------------------------------------------------------
+// Per token: the factor of p, the factor of the one-hot target and the target
+// (-1: none); the largest of the factors' magnitudes for the scale of dz.
+__global__ void __launch_bounds__(256) loss_rows_kernel(const int* __restrict__ targets,
+                                                        const float* __restrict__ dloss,
+                                                        const float* __restrict__ dlse, int64_t T, int V, int ignore,
+                                                        float2* __restrict__ coef, int* __restrict__ tgt,
+                                                        unsigned* __restrict__ amax, int* __restrict__ err) {
+  unsigned mx = 0;
+  for (int64_t t = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; t < T; t += (int64_t)gridDim.x * blockDim.x) {
+    const int v = targets[t];
+    const bool in = v >= 0 && v < V && v != ignore;
+    if (!in && v != ignore) atomicCAS(err, 0, STATUS_TARGET);
+    const float g = in ? dloss[t] : 0.f, q = g + (dlse ? dlse[t] : 0.f);
+    coef[t] = make_float2(q, g);
+    tgt[t] = in ? v : -1;
+    const unsigned a = __float_as_uint(g) & 0x7FFFFFFFu, b = __float_as_uint(q) & 0x7FFFFFFFu;
+    if (a < 0x7F800000u) mx = max(mx, a);
+    if (b < 0x7F800000u) mx = max(mx, b);
+  }
+  mx = __reduce_max_sync(FULL, mx);
+  if ((threadIdx.x & 31) == 0 && mx) atomicMax(amax, mx);
+}
+
+// Scale of dz: |p q - [target] g| <= 2 max(|q|, |g|) < 2^15.
+__device__ __forceinline__ int dz_exp(const unsigned* amax) { return amax ? g16::scale_exp(*amax) - 1 : 0; }
+
+struct GradArgs {
+  int64_t T;
+  int v0, vc;                          // the piece: columns [v0, v0 + vc)
+  const unsigned *amax_h, *amax_w, *amax_g;
+  const float* lse;
+  const float2* coef;
+  const int* tgt;
+  CUtensorMap out[2];                  // dz: hi, lo
+};
+
+// dz as PIECES 16-bit matrices (hi, lo).
+template <bool BF16, int PIECES, bool SUM>
+struct EpiGrad {
+  static constexpr bool kSum = SUM, kStore = true;
+  float sum[128];
+  using Args = GradArgs;
+  float un, sg;
+  uint32_t buf;
+  int turn;
+  __device__ __forceinline__ void begin(const Args& A, const Sched&, int, uint8_t* staging) {
+    buf = tc::smem_u32(staging);
+    turn = 0;
+    un = logit_unscale(A.amax_h, A.amax_w);
+    sg = g16::pow2(dz_exp(A.amax_g));
+  }
+  template <class Get>
+  __device__ __forceinline__ void blocks(const Args& A, const Sched& S, const Tile& t, int64_t row, int half,
+                                         Get get) {
+    const bool on = row < A.T;
+    float l = 0.f, q = 0.f, g = 0.f;
+    int tg = -1;
+    if (on) {
+      const float2 c = A.coef[row];
+      l = A.lse[row];
+      q = c.x * sg;
+      g = c.y * sg;
+      tg = A.tgt[row] - A.v0;
+    }
+    const int hw = S.BN >> 1;
+    const int col0 = t.nt * S.BN + half * hw;
+#pragma unroll
+    for (int cc = 0; cc < 128; cc += 32) {
+      if (cc >= hw || col0 + cc >= A.vc) break;
+      uint32_t v[32];
+      __syncwarp();
+      get(cc, v);
+      float x[32];
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        x[j] = g16::exp2_fast(fmaf(__uint_as_float(v[j]), un, -l) * LOG2E) * q;
+      const unsigned at = (unsigned)(tg - (col0 + cc));
+      if (at < 32u) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) x[j] = at == j ? x[j] - g : x[j];
+      }
+      if (q == 0.f && g == 0.f) {      // an ignored token: nothing, whatever its logits are
+#pragma unroll
+        for (int j = 0; j < 32; ++j) x[j] = 0.f;
+      }
+      uint32_t h[16], o[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float a = x[2 * j], b = x[2 * j + 1];
+        if constexpr (BF16) {
+          const __nv_bfloat162 u = __floats2bfloat162_rn(a, b);
+          h[j] = *reinterpret_cast<const uint32_t*>(&u);
+          if constexpr (PIECES == 2) {
+            const float2 f = __bfloat1622float2(u);
+            const __nv_bfloat162 w = __floats2bfloat162_rn(a - f.x, b - f.y);
+            o[j] = *reinterpret_cast<const uint32_t*>(&w);
+          }
+        } else if constexpr (PIECES == 2) {
+          __half2 u, w;
+          g16::split2(a, b, u, w);
+          h[j] = *reinterpret_cast<const uint32_t*>(&u);
+          o[j] = *reinterpret_cast<const uint32_t*>(&w);
+        } else {
+          const __half2 u = __floats2half2_rn(a, b);
+          h[j] = *reinterpret_cast<const uint32_t*>(&u);
+        }
+      }
+      // the halves of the staging buffer: hi and lo, or this block and the one before
+      const int lane = threadIdx.x & 31;
+      const uint32_t b0 = buf + (PIECES == 2 ? 0 : turn * 2048);
+      turn ^= 1;
+      if (lane == 0) g16::bulk_wait<PIECES == 2 ? 0 : 1, true>();
+      __syncwarp();
+      g16::stage16(b0, lane, h);
+      if constexpr (PIECES == 2) g16::stage16(b0 + 2048, lane, o);
+      tc::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0 && on) {           // lane 0 has the block's first row
+        g16::bulk_store(&A.out[0], b0, col0 + cc, (int)row, 0, false);
+        if constexpr (PIECES == 2) g16::bulk_store(&A.out[1], b0 + 2048, col0 + cc, (int)row, 0, false);
+      }
+    }
+  }
+  __device__ __forceinline__ void tile(const Args& A, const Sched& S, const Tile& t, int64_t row, int half,
+                                       uint32_t taddr) {
+    blocks(A, S, t, row, half, FromTmem{taddr + half * (S.BN >> 1)});
+  }
+  __device__ __forceinline__ void store(const Args& A, const Sched& S, const Tile& t, int64_t row, int half) {
+    blocks(A, S, t, row, half, FromSums{sum});
+  }
+  __device__ __forceinline__ void end(const Args&, const Sched&, int) {}
+};
+
+struct OutOne {
+  CUtensorMap map;                     // out as staged stores write it (tma)
+  int64_t M;
+  int N;
+  int64_t ld, slice;                   // slice: elements between the slices' partials
+  void* out;
+  int type;                            // memlayer_dtype of out
+  int add;                             // float32 only: added to what is there
+  int tma;                             // rows are 16 bytes apart
+  const unsigned *amax_a, *amax_b;     // scale maxima of the operands (null: unscaled); amax_a is dz's
+};
+struct OutArgs { OutOne o[2]; };
+
+// Plain outputs: out[row, col] = acc unscaled (+ what is there), float32 or
+// the 16-bit type; slices write float32 partials.
+template <bool SUM>
+struct EpiOut {
+  static constexpr bool kSum = SUM, kStore = true;
+  using Args = OutArgs;
+  float sum[128];                      // the thread's columns over the segments of k
+  uint32_t buf;
+  int turn;
+  __device__ __forceinline__ void begin(const Args&, const Sched&, int, uint8_t* staging) {
+    buf = tc::smem_u32(staging);
+    turn = 0;
+  }
+  // The warp's 32 rows x 32 columns.
+  __device__ __forceinline__ void block(const OutOne& O, uint32_t (&v)[32], const g16::Unscale& un, int64_t row0,
+                                        int col, int ks) {
+    const int lane = threadIdx.x & 31;
+    const bool f32 = O.type == MEMLAYER_F32;
+    const uint32_t b = buf + (f32 ? 0 : turn * 2048);
+    turn ^= 1;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(un(__uint_as_float(v[j])));
+    if (lane == 0) {
+      if (f32)
+        g16::bulk_wait<0, true>();
+      else
+        g16::bulk_wait<1, true>();
+    }
+    __syncwarp();
+    g16::stage_as(O.type, b, lane, v);
+    if (O.tma) {
+      tc::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) g16::bulk_store(&O.map, b, col, (int)row0, ks, O.add);
+    } else {
+      __syncwarp();
+      g16::copy_rows(O.type, b, O.out, ks * O.slice + row0 * O.ld + col, O.ld,
+                     (int)(O.M - row0 < 32 ? O.M - row0 : 32), O.N - col, O.add);
+      __syncwarp();
+    }
+  }
+  template <class Get>
+  __device__ __forceinline__ void blocks(const Args& A, const Sched& S, const Tile& t, int64_t row, int half,
+                                         Get get) {
+    const OutOne& O = A.o[t.q];
+    const g16::Unscale un(-dz_exp(O.amax_a) - exp_of(O.amax_b));
+    const int64_t row0 = row - (threadIdx.x & 31);
+    const int hw = S.BN >> 1;
+    const int col0 = t.nt * S.BN + half * hw;
+#pragma unroll
+    for (int cc = 0; cc < 128; cc += 32) {
+      if (cc >= hw || col0 + cc >= O.N) break;
+      uint32_t v[32];
+      __syncwarp();
+      get(cc, v);
+      if (row0 < O.M) block(O, v, un, row0, col0 + cc, t.ks);
+    }
+  }
+  __device__ __forceinline__ void tile(const Args& A, const Sched& S, const Tile& t, int64_t row, int half,
+                                       uint32_t taddr) {
+    blocks(A, S, t, row, half, FromTmem{taddr + half * (S.BN >> 1)});
+  }
+  __device__ __forceinline__ void store(const Args& A, const Sched& S, const Tile& t, int64_t row, int half) {
+    blocks(A, S, t, row, half, FromSums{sum});
+  }
+  __device__ __forceinline__ void end(const Args&, const Sched&, int) {}
+};
+
+// out = the slices' partials added in slice order, in the storage type; four
+// entries a thread (both buffers come 256-byte aligned or are written one by one).
+__global__ void __launch_bounds__(256) loss_slices_kernel(const float* __restrict__ P, int S, int64_t n, void* out,
+                                                          int type, int vec) {
+  auto put = [&](int64_t e, float x) {
+    if (type == MEMLAYER_F32)
+      reinterpret_cast<float*>(out)[e] = x;
+    else if (type == MEMLAYER_F16)
+      reinterpret_cast<__half*>(out)[e] = __float2half_rn(x);
+    else
+      reinterpret_cast<__nv_bfloat16*>(out)[e] = __float2bfloat16_rn(x);
+  };
+  const int64_t at = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, step = (int64_t)gridDim.x * blockDim.x;
+  if (vec) {
+    for (int64_t e = at * 4; e < n; e += step * 4) {
+      float4 x = *reinterpret_cast<const float4*>(P + e);
+      for (int s = 1; s < S; ++s) {
+        const float4 y = *reinterpret_cast<const float4*>(P + s * n + e);
+        x = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
+      }
+      if (type == MEMLAYER_F32) {
+        *reinterpret_cast<float4*>(reinterpret_cast<float*>(out) + e) = x;
+      } else {
+        uint2 o;
+        if (type == MEMLAYER_F16) {
+          const __half2 a = __floats2half2_rn(x.x, x.y), b = __floats2half2_rn(x.z, x.w);
+          o = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+        } else {
+          const __nv_bfloat162 a = __floats2bfloat162_rn(x.x, x.y), b = __floats2bfloat162_rn(x.z, x.w);
+          o = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+        }
+        *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(out) + e) = o;
+      }
+    }
+  } else {
+    for (int64_t e = at; e < n; e += step) {
+      float x = P[e];
+      for (int s = 1; s < S; ++s) x += P[s * n + e];
+      put(e, x);
+    }
+  }
+}
+
+cudaError_t launch_slices(const float* P, int S, int64_t n, void* out, int type, cudaStream_t s) {
+  const int vec = n % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+  const int64_t items = vec ? n / 4 : n;
+  int64_t blocks = (items + 255) / 256;
+  const int64_t cap = 8 * g16::device_sms();
+  if (blocks > cap) blocks = cap;
+  loss_slices_kernel<<<(unsigned)blocks, 256, 0, s>>>(P, S, n, out, type, vec);
+  count_launch();
+  return cudaGetLastError();
+}
+
+// ---- plan -----------------------------------------------------------------------
+int64_t up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
+
+struct Plan {
+  int P, PZ;                           // pieces of h and W, of dz
+  int cg, BN;                          // CTAs per tile; columns per tile of the logits
+  int m_tiles, n_tiles;
+  int slots;                           // partial pairs per row and column half
+  int64_t ld;                          // row pitch of the 16-bit forms
+  int vc;                              // columns of a vocabulary piece = row pitch of its dz
+  int oBN;                             // columns per tile of the gradient products
+  int s_h, s_w;                        // k slices of dh and of dW
+  size_t o_hh, o_hl, o_wh, o_wl, o_part, o_zt, o_coef, o_tgt, o_g, o_g2, o_dh, o_dw, bytes;
+};
+
+constexpr size_t O_ERR = 256, O_AMAX = 512, HEAD = 1024;   // amax words: h, W, dz
+
+// 16-bit matrices TMA can address: rows 16 bytes apart, 16-byte base.
+bool tma_rows(const void* p, int64_t stride) { return stride % 8 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+constexpr int64_t kPieceBytes = 256ll << 20;   // dz of one vocabulary piece
+
+Prod product(int64_t m_tiles, int64_t n_tiles, int splits, int64_t k, bool amn, bool bmn) {
+  Prod p{};
+  p.m_tiles = (int)m_tiles;
+  p.n_tiles = (int)n_tiles;
+  p.batch = 1;
+  p.kq_total = (int)(up(k, g16::BK) / g16::BK);
+  p.kq = (p.kq_total + splits - 1) / splits;
+  p.splits = (p.kq_total + p.kq - 1) / p.kq;   // no empty slice
+  p.amn = amn;
+  p.bmn = bmn;
+  return p;
+}
+
+// The two products of a piece of vc columns, the one with the longer tiles
+// first; returns which place dh has.
+int out_products(const Plan& p, int64_t T, int64_t vc, int64_t d, Sched* S) {
+  const int rt = 128 * p.cg;
+  const int64_t nd = up(d, p.oBN) / p.oBN;
+  const Prod w = product(up(vc, rt) / rt, nd, p.s_w, T, true, true);
+  const Prod h = product(up(T, rt) / rt, nd, p.s_h, vc, false, true);
+  const int at = h.kq > w.kq ? 0 : 1;
+  S->prod[at] = h;
+  S->prod[1 - at] = w;
+  S->BN = p.oBN;
+  S->seg = SEG;
+  return at;
+}
+
+// Columns per piece and slices of k.
+void piece_plan(int64_t T, int64_t V, int64_t d, int sms, Plan* p) {
+  int64_t most = kPieceBytes / (2 * p->PZ) / (T ? T : 1);
+  if (most < 256) most = 256;
+  const int64_t n = (V + most - 1) / most;
+  p->vc = (int)up((V + n - 1) / n, 256);
+  const int rt = 128 * p->cg;
+  const int64_t nd = up(d, p->oBN) / p->oBN, kh = up(p->vc, 64) / 64, kw = up(T, 64) / 64;
+  const double ideal = (double)(up(T, rt) / rt * nd * kh + up(p->vc, rt) / rt * nd * kw) / (sms / p->cg);
+  const double cap = ideal * 1.25 < 16 ? 16 : ideal * 1.25;
+  p->s_h = kh > cap ? (int)(kh / cap + 0.999) : 1;
+  p->s_w = kw > cap ? (int)(kw / cap + 0.999) : 1;
+}
+
+bool plan(const memlayer_loss_config& c, bool backward, Plan* out) {
+  Plan p{};
+  const int64_t T = c.tokens, V = c.vocab_size, d = c.d_model;
+  const bool f32 = c.dtype == MEMLAYER_F32;
+  const int sms = g16::device_sms();
+  p.P = f32 ? 2 : 1;
+  // 16-bit dz rounds once more than the results; up to 128 tokens, where the
+  // products wait for memory, a second piece makes it exact enough for free
+  p.PZ = f32 || T <= 128 ? 2 : 1;
+  p.cg = T > 128 ? 2 : 1;
+  p.BN = p.cg == 2 ? 256 : 128;
+  const int64_t mt = up(T, 128 * p.cg) / (128 * p.cg), nt = up(V, p.BN) / p.BN;
+  if (mt * nt >= (1ll << 31)) return false;
+  p.m_tiles = (int)mt;
+  p.n_tiles = (int)nt;
+  const int64_t total = mt * nt, cl = total < sms / p.cg ? total : sms / p.cg;
+  const int64_t per = cl ? total / cl : 1;
+  p.slots = (int)((nt + per - 1) / (per ? per : 1) + 1);
+  p.ld = up(d, 8);
+  size_t off = HEAD;
+  auto take = [&](int64_t bytes) {
+    const size_t o = off;
+    off += (size_t)up(bytes, 256);
+    return o;
+  };
+  // room for the 16-bit forms whether or not this call's strides need them
+  p.o_hh = take(T * p.ld * 2);
+  p.o_wh = take(V * p.ld * 2);
+  if (f32) {
+    p.o_hl = take(T * p.ld * 2);
+    p.o_wl = take(V * p.ld * 2);
+  }
+  if (!backward) {
+    p.o_part = take((int64_t)p.slots * 2 * T * 8);
+    p.o_zt = take(T * 4);
+  } else {
+    p.o_coef = take(T * 8);
+    p.o_tgt = take(T * 4);
+    p.oBN = d > 128 ? 256 : 128;
+    piece_plan(T, V, d, sms, &p);
+    p.o_g = take(T * p.vc * 2);
+    if (p.PZ == 2) p.o_g2 = take(T * p.vc * 2);
+    p.o_dh = take((int64_t)p.s_h * T * d * 4);
+    p.o_dw = p.s_w > 1 ? take((int64_t)p.s_w * p.vc * d * 4) : 0;
+  }
+  p.bytes = off;
+  *out = p;
+  return true;
+}
+
+struct Operands {
+  const void *h[2], *w[2];
+  int64_t ldh, ldw;
+};
+
+// Operands in 16-bit form: the caller's where TMA can address them, else the workspace's.
+cudaError_t prepare(const memlayer_loss_config& c, const memlayer_loss_args& a, const Plan& p, char* ws, Operands* o,
+                    cudaStream_t s) {
+  unsigned* amax = reinterpret_cast<unsigned*>(ws + O_AMAX);
+  const bool f32 = c.dtype == MEMLAYER_F32;
+  o->h[0] = a.h;
+  o->w[0] = a.weight;
+  o->ldh = a.h_stride;
+  o->ldw = a.weight_stride;
+  const bool ch = f32 || !tma_rows(a.h, a.h_stride), cw = f32 || !tma_rows(a.weight, a.weight_stride);
+  cudaError_t e;
+  if (f32) {
+    AmaxArgs A{};
+    A.m[0] = {(const float*)a.h, c.tokens, c.d_model, a.h_stride, amax, 0};
+    A.m[1] = {(const float*)a.weight, c.vocab_size, c.d_model, a.weight_stride, amax + 1, 0};
+    if ((e = launch_amax(A, s)) != cudaSuccess) return e;
+  }
+  if (!ch && !cw) return cudaSuccess;
+  PiecesArgs B{};
+  if (ch) {
+    o->h[0] = ws + p.o_hh;
+    o->h[1] = ws + p.o_hl;
+    o->ldh = p.ld;
+    B.m[0] = {a.h, c.tokens, c.d_model, a.h_stride, ws + p.o_hh, ws + p.o_hl, p.ld, amax, 0};
+  }
+  if (cw) {
+    o->w[0] = ws + p.o_wh;
+    o->w[1] = ws + p.o_wl;
+    o->ldw = p.ld;
+    B.m[1] = {a.weight, c.vocab_size, c.d_model, a.weight_stride, ws + p.o_wh, ws + p.o_wl, p.ld, amax + 1, 0};
+  }
+  return launch_pieces(B, c.dtype, s);
+}
+
+#define LS_TRY(x)                             \
+  do {                                        \
+    const cudaError_t e_ = (x);               \
+    if (e_ != cudaSuccess) return e_;         \
+  } while (0)
+
+template <class EPI, int PA, int PB>
+cudaError_t launch(int cg, const Maps& m, const Sched& S, const typename EPI::Args& ea, int* err, cudaStream_t s) {
+  return cg == 2 ? g16::launch_one<EPI, 2, PA, PB>(m, S, ea, err, s)
+                 : g16::launch_one<EPI, 1, PA, PB>(m, S, ea, err, s);
+}
+
+}  // namespace
+
+bool loss_workspace(const memlayer_loss_config& c, bool backward, size_t* bytes) {
+  Plan p;
+  if (!plan(c, backward, &p)) return false;
+  *bytes = p.bytes;
+  return true;
+}
+
+cudaError_t launch_loss_forward(const memlayer_loss_config& c, const memlayer_loss_args& a, char* ws, cudaStream_t s) {
+  Plan p;
+  if (!plan(c, false, &p)) return cudaErrorInvalidValue;
+  int* err = reinterpret_cast<int*>(ws + O_ERR);
+  LS_TRY(cudaMemsetAsync(ws + O_ERR, 0, HEAD - O_ERR, s));
+  if (c.tokens == 0) return cudaSuccess;
+  Operands o{};
+  LS_TRY(prepare(c, a, p, ws, &o, s));
+  const int bf16 = c.dtype == MEMLAYER_BF16;
+  Maps m{};
+  for (int i = 0; i < p.P; ++i) {
+    LS_TRY(g16::make_operand(&m.a[0][i], o.h[i], c.tokens, c.d_model, o.ldh, false, 128, bf16));
+    LS_TRY(g16::make_operand(&m.b[0][i], o.w[i], c.vocab_size, c.d_model, o.ldw, false, p.BN / p.cg, bf16));
+  }
+  Sched S{};
+  const int sms = g16::device_sms() / p.cg;
+  S.prod[0] = product(p.m_tiles, p.n_tiles, 1, c.d_model, false, false);
+  S.contiguous = 1;
+  S.clusters = sms < S.prod[0].total() ? sms : S.prod[0].total();
+  S.BN = p.BN;
+  S.bf16 = bf16;
+  const unsigned* amax = p.P == 2 ? reinterpret_cast<unsigned*>(ws + O_AMAX) : nullptr;
+  StatsArgs ea{};
+  ea.T = c.tokens;
+  ea.V = c.vocab_size;
+  ea.amax_h = amax;
+  ea.amax_w = amax ? amax + 1 : nullptr;
+  ea.targets = a.targets;
+  ea.part = reinterpret_cast<float2*>(ws + p.o_part);
+  ea.zt = reinterpret_cast<float*>(ws + p.o_zt);
+  S.seg = LOGIT_SEG;
+  const bool sum = S.prod[0].kq > LOGIT_SEG;
+  if (p.P == 1)
+    LS_TRY((launch<EpiStats<false>, 1, 1>(p.cg, m, S, ea, err, s)));
+  else if (sum)
+    LS_TRY((launch<EpiStats<true>, 2, 2>(p.cg, m, S, ea, err, s)));
+  else
+    LS_TRY((launch<EpiStats<false>, 2, 2>(p.cg, m, S, ea, err, s)));
+  loss_join_kernel<<<(unsigned)((c.tokens + 7) / 8), 256, 0, s>>>(ea.part, ea.zt, a.targets, c.tokens, c.vocab_size,
+                                                                  S, 128 * p.cg, c.ignore_index, a.loss,
+                                                                  a.lse, err);
+  count_launch();
+  return cudaGetLastError();
+}
+
+cudaError_t launch_loss_backward(const memlayer_loss_config& c, const memlayer_loss_args& a,
+                                 const memlayer_loss_grads& g, char* ws, cudaStream_t s) {
+  Plan p;
+  if (!plan(c, true, &p)) return cudaErrorInvalidValue;
+  int* err = reinterpret_cast<int*>(ws + O_ERR);
+  const int64_t T = c.tokens, V = c.vocab_size, d = c.d_model;
+  LS_TRY(cudaMemsetAsync(ws + O_ERR, 0, HEAD - O_ERR, s));
+  const size_t esize = c.dtype == MEMLAYER_F32 ? 4 : 2;
+  if (T == 0) return cudaMemsetAsync(g.dweight, 0, (size_t)V * d * esize, s);
+  Operands o{};
+  LS_TRY(prepare(c, a, p, ws, &o, s));
+  unsigned* words = reinterpret_cast<unsigned*>(ws + O_AMAX);
+  const bool f32 = c.dtype == MEMLAYER_F32;
+  const int bf16 = c.dtype == MEMLAYER_BF16;
+  const unsigned *ah = f32 ? words : nullptr, *aw = f32 ? words + 1 : nullptr, *ag = bf16 ? nullptr : words + 2;
+  float2* coef = reinterpret_cast<float2*>(ws + p.o_coef);
+  int* tgt = reinterpret_cast<int*>(ws + p.o_tgt);
+  {
+    const int64_t b = (T + 255) / 256;
+    loss_rows_kernel<<<(unsigned)(b < 592 ? b : 592), 256, 0, s>>>(a.targets, g.dloss, g.dlse, T, c.vocab_size,
+                                                                   c.ignore_index, coef, tgt, words + 2, err);
+    count_launch();
+    LS_TRY(cudaGetLastError());
+  }
+  uint16_t *gh = reinterpret_cast<uint16_t*>(ws + p.o_g), *gl = reinterpret_cast<uint16_t*>(ws + p.o_g2);
+  float* acc_h = reinterpret_cast<float*>(ws + p.o_dh);
+  const int sms = g16::device_sms() / p.cg;
+  const int pieces = (int)((V + p.vc - 1) / p.vc);
+  // dh in place when it needs no joining: one slice, and float32 or one piece
+  const bool direct_h = p.s_h == 1 && (f32 || pieces == 1);
+  auto al16 = [](const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; };
+  for (int i = 0; i < pieces; ++i) {
+    const int v0 = i * p.vc;
+    const int vc = (int)(V - v0 < p.vc ? V - v0 : p.vc);
+    const int64_t woff = (int64_t)v0 * o.ldw * 2;
+    // dz of the piece
+    Maps m{};
+    for (int q = 0; q < p.P; ++q) {
+      LS_TRY(g16::make_operand(&m.a[0][q], o.h[q], T, d, o.ldh, false, 128, bf16));
+      LS_TRY(g16::make_operand(&m.b[0][q], (const char*)o.w[q] + woff, vc, d, o.ldw, false, p.BN / p.cg, bf16));
+    }
+    Sched S{};
+    S.prod[0] = product(p.m_tiles, (vc + p.BN - 1) / p.BN, 1, d, false, false);
+    S.BN = p.BN;
+    S.bf16 = bf16;
+    g16::distribute(&S, sms, 0);
+    GradArgs ga{T, v0, vc, ah, aw, ag, g.lse, coef, tgt, {}};
+    LS_TRY(g16::make_store(&ga.out[0], gh, T, p.vc, p.vc, f32 ? MEMLAYER_F16 : c.dtype));
+    if (p.PZ == 2) LS_TRY(g16::make_store(&ga.out[1], gl, T, p.vc, p.vc, f32 ? MEMLAYER_F16 : c.dtype));
+    S.seg = LOGIT_SEG;
+    if (f32 && S.prod[0].kq > LOGIT_SEG)
+      LS_TRY((launch<EpiGrad<false, 2, true>, 2, 2>(p.cg, m, S, ga, err, s)));
+    else if (f32)
+      LS_TRY((launch<EpiGrad<false, 2, false>, 2, 2>(p.cg, m, S, ga, err, s)));
+    else if (bf16)
+      LS_TRY(p.PZ == 2 ? (g16::launch_one<EpiGrad<true, 2, false>, 1, 1, 1>(m, S, ga, err, s))
+                       : (g16::launch_one<EpiGrad<true, 1, false>, 2, 1, 1>(m, S, ga, err, s)));
+    else
+      LS_TRY(p.PZ == 2 ? (g16::launch_one<EpiGrad<false, 2, false>, 1, 1, 1>(m, S, ga, err, s))
+                       : (g16::launch_one<EpiGrad<false, 1, false>, 2, 1, 1>(m, S, ga, err, s)));
+    // dW of the piece = dz^T h; dh (+)= dz W of the piece
+    Sched S2{};
+    const int qh = out_products(p, T, vc, d, &S2), qw = 1 - qh;
+    S2.bf16 = bf16;
+    g16::distribute(&S2, sms, 2);
+    Maps m2{};
+    const uint16_t* gz[2] = {gh, gl};
+    for (int q = 0; q < p.PZ; ++q) {
+      LS_TRY(g16::make_operand(&m2.a[qw][q], gz[q], vc, T, p.vc, true, 0, bf16));
+      LS_TRY(g16::make_operand(&m2.a[qh][q], gz[q], T, vc, p.vc, false, 128, bf16));
+    }
+    for (int q = 0; q < p.P; ++q) {
+      LS_TRY(g16::make_operand(&m2.b[qw][q], o.h[q], d, T, o.ldh, true, 0, bf16));
+      LS_TRY(g16::make_operand(&m2.b[qh][q], (const char*)o.w[q] + woff, d, vc, o.ldw, true, 0, bf16));
+    }
+    const int sw = S2.prod[qw].splits, sh = S2.prod[qh].splits;
+    char* dwp = (char*)g.dweight + (size_t)v0 * d * esize;
+    OutArgs ea{};
+    auto out = [&](OutOne& O, int64_t M, void* q, int type, bool add, int slices, const unsigned* ub) {
+      O.M = M;
+      O.N = (int)d;
+      O.ld = d;
+      O.slice = M * d;
+      O.out = q;
+      O.type = type;
+      O.add = add;
+      O.tma = al16(q) && (d * (type == MEMLAYER_F32 ? 4 : 2)) % 16 == 0;
+      O.amax_a = ag;
+      O.amax_b = ub;
+      return O.tma ? g16::make_store(&O.map, q, M, d, d, type, slices, M * d) : cudaSuccess;
+    };
+    if (sw > 1)
+      LS_TRY(out(ea.o[qw], vc, ws + p.o_dw, MEMLAYER_F32, false, sw, ah));
+    else
+      LS_TRY(out(ea.o[qw], vc, dwp, c.dtype, false, 1, ah));
+    if (direct_h)
+      LS_TRY(out(ea.o[qh], T, g.dh, c.dtype, i > 0, 1, aw));
+    else   // a shorter last piece may have fewer slices: the others keep what they hold
+      LS_TRY(out(ea.o[qh], T, acc_h, MEMLAYER_F32, i > 0, sh, aw));
+    if (f32)
+      LS_TRY((launch<EpiOut<true>, 2, 2>(p.cg, m2, S2, ea, err, s)));
+    else
+      LS_TRY(p.PZ == 2 ? (g16::launch_one<EpiOut<false>, 1, 2, 1>(m2, S2, ea, err, s))
+                       : (g16::launch_one<EpiOut<false>, 2, 1, 1>(m2, S2, ea, err, s)));
+    if (sw > 1)
+      LS_TRY(launch_slices(reinterpret_cast<float*>(ws + p.o_dw), sw, (int64_t)vc * d, dwp, c.dtype, s));
+    if (i == 0) p.s_h = sh;            // slices of the first (largest) piece
+  }
+  if (!direct_h) LS_TRY(launch_slices(acc_h, p.s_h, T * d, g.dh, c.dtype, s));
+  return cudaSuccess;
+}
+
+}  // namespace ml

@@ -196,6 +196,50 @@ int block_tail(const memlayer_model_config* c, const ModelDims& d, const memlaye
   return MEMLAYER_OK;
 }
 
+// One call's sizes and workspace after its blocks have run: the residual
+// stream in o_x, without the last block's update, which is in o_y.
+struct Run {
+  ModelDims d;
+  ModelWork W;
+  Ctx x;
+  int64_t M;
+};
+
+// Checks a whole-sequence call and runs the embedding and the blocks
+// (model.py:61-121); `out` is the call's output, checked only.
+int run_blocks(const memlayer_model_config* cfg, const memlayer_model_params* p, const int32_t* tokens, int64_t batch,
+               int64_t seq, const float* out, void* workspace, size_t workspace_bytes, void* stream, Run* r) {
+  ModelDims& d = r->d;
+  ModelWork& W = r->W;
+  int st = check_model(cfg, &d);
+  if (st) return st;
+  if (batch < 0 || seq < 0 || seq > d.max_len) return MEMLAYER_ERR_BAD_SHAPE;
+  const int64_t M = batch * seq;
+  r->M = M;
+  if ((st = check_params(cfg, d, p))) return st;
+  if (M > 0 && (!tokens || !out)) return MEMLAYER_ERR_BAD_POINTER;
+  if ((st = model_work(cfg, d, M, &W))) return st;
+  if (!workspace || workspace_bytes < W.bytes || (reinterpret_cast<uintptr_t>(workspace) % MALIGN))
+    return MEMLAYER_ERR_WORKSPACE;
+  const cudaStream_t s = (cudaStream_t)stream;
+  r->x = Ctx{(char*)workspace, &W, s, reinterpret_cast<int*>((char*)workspace + 256)};
+  const Ctx& x = r->x;
+  MM_TRY(cudaMemsetAsync(x.err, 0, sizeof(int), s));
+  if (M == 0) return MEMLAYER_OK;
+  float *X = x.f(W.o_x), *h = x.f(W.o_h), *y = x.f(W.o_y), *qkv = x.f(W.o_qkv), *att = x.f(W.o_att);
+  MM_TRY(launch_embed(tokens, M, (int)seq, nullptr, p->embedding, p->pos_embed, d.V, d.dm, d.max_len, X, x.err, s));
+  for (int i = 0; i < d.L; ++i) {
+    const memlayer_block_params& b = p->layers[i];
+    MM_TRY(launch_add_ln(X, i ? y : nullptr, b.ln_attn_scale, b.ln_attn_bias, h, M, d.dm, s));   // model.py:87
+    if ((st = dense(x, h, M, d.dm, b.w_qkv, false, b.b_qkv, 3 * d.dm, qkv, ACT_NONE))) return st;
+    MM_TRY(launch_attn_prefill(qkv, att, batch, (int)seq, d.H, d.dh, s));                      // model.py:88-94
+    if ((st = dense(x, att, M, d.dm, b.w_attn_out, false, b.b_attn_out, d.dm, y, ACT_NONE))) return st;
+    MM_TRY(launch_add_ln(X, y, b.ln_ffn_scale, b.ln_ffn_bias, h, M, d.dm, s));               // model.py:95-96
+    if ((st = block_tail(cfg, d, p, i, x, M))) return st;                                      // model.py:97-121
+  }
+  return MEMLAYER_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -225,34 +269,27 @@ int32_t memlayer_model_cache_size(const memlayer_model_config* cfg, int64_t batc
 int32_t memlayer_model_forward(const memlayer_model_config* cfg, const memlayer_model_params* p,
                                const int32_t* tokens, int64_t batch, int64_t seq, float* logits, void* workspace,
                                size_t workspace_bytes, void* stream) {
-  ModelDims d;
-  int st = check_model(cfg, &d);
-  if (st) return st;
-  if (batch < 0 || seq < 0 || seq > d.max_len) return MEMLAYER_ERR_BAD_SHAPE;
-  const int64_t M = batch * seq;
-  if ((st = check_params(cfg, d, p))) return st;
-  if (M > 0 && (!tokens || !logits)) return MEMLAYER_ERR_BAD_POINTER;
-  ModelWork W;
-  if ((st = model_work(cfg, d, M, &W))) return st;
-  if (!workspace || workspace_bytes < W.bytes || (reinterpret_cast<uintptr_t>(workspace) % MALIGN))
-    return MEMLAYER_ERR_WORKSPACE;
-  const cudaStream_t s = (cudaStream_t)stream;
-  Ctx x{(char*)workspace, &W, s, reinterpret_cast<int*>((char*)workspace + 256)};
-  MM_TRY(cudaMemsetAsync(x.err, 0, sizeof(int), s));
-  if (M == 0) return MEMLAYER_OK;
-  float *X = x.f(W.o_x), *h = x.f(W.o_h), *y = x.f(W.o_y), *qkv = x.f(W.o_qkv), *att = x.f(W.o_att);
-  MM_TRY(launch_embed(tokens, M, (int)seq, nullptr, p->embedding, p->pos_embed, d.V, d.dm, d.max_len, X, x.err, s));
-  for (int i = 0; i < d.L; ++i) {
-    const memlayer_block_params& b = p->layers[i];
-    MM_TRY(launch_add_ln(X, i ? y : nullptr, b.ln_attn_scale, b.ln_attn_bias, h, M, d.dm, s));   // model.py:87
-    if ((st = dense(x, h, M, d.dm, b.w_qkv, false, b.b_qkv, 3 * d.dm, qkv, ACT_NONE))) return st;
-    MM_TRY(launch_attn_prefill(qkv, att, batch, (int)seq, d.H, d.dh, s));                      // model.py:88-94
-    if ((st = dense(x, att, M, d.dm, b.w_attn_out, false, b.b_attn_out, d.dm, y, ACT_NONE))) return st;
-    MM_TRY(launch_add_ln(X, y, b.ln_ffn_scale, b.ln_ffn_bias, h, M, d.dm, s));               // model.py:95-96
-    if ((st = block_tail(cfg, d, p, i, x, M))) return st;                                      // model.py:97-121
-  }
-  MM_TRY(launch_add_ln(X, d.L ? y : nullptr, p->ln_final_scale, p->ln_final_bias, h, M, d.dm, s));  // model.py:124
-  return dense(x, h, M, d.dm, p->embedding, true, nullptr, d.V, logits, ACT_NONE);              // model.py:125
+  Run r;
+  const int st = run_blocks(cfg, p, tokens, batch, seq, logits, workspace, workspace_bytes, stream, &r);
+  if (st || r.M == 0) return st;
+  const Ctx& x = r.x;
+  float* h = x.f(r.W.o_h);
+  MM_TRY(launch_add_ln(x.f(r.W.o_x), r.d.L ? x.f(r.W.o_y) : nullptr, p->ln_final_scale, p->ln_final_bias, h, r.M,
+                       r.d.dm, x.s));                                                          // model.py:124
+  return dense(x, h, r.M, r.d.dm, p->embedding, true, nullptr, r.d.V, logits, ACT_NONE);        // model.py:125
+}
+
+int32_t memlayer_model_hidden(const memlayer_model_config* cfg, const memlayer_model_params* p, const int32_t* tokens,
+                              int64_t batch, int64_t seq, float* hidden, void* workspace, size_t workspace_bytes,
+                              void* stream) {
+  Run r;
+  const int st = run_blocks(cfg, p, tokens, batch, seq, hidden, workspace, workspace_bytes, stream, &r);
+  if (st || r.M == 0) return st;
+  const Ctx& x = r.x;
+  const int64_t n = r.M * r.d.dm;
+  if (r.d.L) MM_TRY(launch_add(x.f(r.W.o_x), x.f(r.W.o_y), n, x.s));                            // model.py:122
+  MM_TRY(cudaMemcpyAsync(hidden, x.f(r.W.o_x), sizeof(float) * n, cudaMemcpyDeviceToDevice, x.s));
+  return MEMLAYER_OK;
 }
 
 int32_t memlayer_model_decode_step(const memlayer_model_config* cfg, const memlayer_model_params* p,

@@ -1,0 +1,412 @@
+// Orthogonalised update of a batch of Dense kernels: the Newton-Schulz
+// iteration towards the polar factor of the update U [m, n],
+//
+//   X_0 = U / (|U|_F + eps)
+//   P = X X^T,  X <- (a I + b P + c P^2) X        (m <= n)
+//   P = X^T X,  X <- X (a I + b P + c P^2)        (m > n: the smaller side)
+//
+// Three products a step on the 16-bit tensor cores (gemm16.cuh), operands as
+// two f16 pieces (22 bits, like the float32 paths of loss.cu), accumulated
+// in float32 with segments of k.  The polynomial is written so that no
+// epilogue reads a matrix: the first product's epilogue writes P and
+// R = b I + c P, the second's a I + R P, the third's the next X (the output's
+// type in the last step).  Majors instead of transposes: the m > n products
+// read X along its other index.
+//
+// Entries of X, P, R and Q are bounded by their singular values, which the
+// host bounds for the given coefficients before it launches (the usual
+// (3.4445, -4.7750, 2.0315) keeps X below 1.21 and R, Q below 4.8), so the
+// pieces use one fixed scale, 2^12.
+#include "orth.cuh"
+
+#include <math.h>
+
+#include "gemm16.cuh"
+#include "pieces16.cuh"
+
+namespace ml {
+
+namespace {
+
+using g16::Maps;
+using g16::Prod;
+using g16::Sched;
+using g16::Tile;
+
+// Stages per segment of a product's k.  One (64 k, four steps) keeps the
+// error at a float32 GEMM's; its drains take 1.35 times a long product's
+// tensor time, so products of k > 512, whose float32 error is larger anyway,
+// take two.
+inline int seg_for(int64_t K) { return K > 512 ? 2 : 1; }
+constexpr float SCALE = 4096.f, BOUND = 15.f;   // 15 x 2^12 < 65504
+
+// ---- |U|_F and the pieces of X_0 -----------------------------------------------
+constexpr int NORM_CHUNKS = 256;
+
+template <typename E> __device__ __forceinline__ float up_f(E x);
+template <> __device__ __forceinline__ float up_f(float x) { return x; }
+template <> __device__ __forceinline__ float up_f(__half x) { return __half2float(x); }
+template <> __device__ __forceinline__ float up_f(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+// Partial sums of squares in float64 (squares of float32 values overflow and
+// underflow float32): chunk blockIdx.x of matrix blockIdx.y.
+template <typename E>
+__global__ void __launch_bounds__(256) orth_norm_kernel(const E* __restrict__ u, int64_t n, int chunks,
+                                                        double* __restrict__ part) {
+  __shared__ double red[8];
+  const int64_t per = ((n + chunks - 1) / chunks + 7) / 8 * 8;
+  const int64_t b = blockIdx.x * per, e = b + per < n ? b + per : n;
+  const E* x = u + blockIdx.y * n;
+  double s[4] = {0., 0., 0., 0.};
+  for (int64_t i = b + threadIdx.x; i < e; i += 1024) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (i + j * 256 < e) {
+        const double v = up_f(x[i + j * 256]);
+        s[j] = fma(v, v, s[j]);
+      }
+  }
+  double t = (s[0] + s[1]) + (s[2] + s[3]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(FULL, t, o);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = t;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 8; ++w) t += red[w];
+    part[blockIdx.y * chunks + blockIdx.x] = t;
+  }
+}
+
+// X_0's pieces, 8 columns a thread (zeros in the padding columns).
+template <typename E>
+__global__ void __launch_bounds__(256) orth_init_kernel(const E* __restrict__ u, int m, int n, int ld, double eps,
+                                                        const double* __restrict__ part, int chunks,
+                                                        __half* __restrict__ hi, __half* __restrict__ lo) {
+  __shared__ double inv_s;
+  if (threadIdx.x < 32) {
+    double t = 0.;
+    for (int i = threadIdx.x; i < chunks; i += 32) t += part[blockIdx.y * chunks + i];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(FULL, t, o);
+    if (threadIdx.x == 0) inv_s = (double)SCALE / (sqrt(t) + eps);
+  }
+  __syncthreads();
+  const double inv = inv_s;
+  const int c8 = ld >> 3;
+  const int64_t items = (int64_t)m * c8, z = (int64_t)blockIdx.y;
+  const E* x = u + z * m * n;
+  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < items; e += (int64_t)gridDim.x * 256) {
+    const int64_t r = e / c8;
+    const int c = (int)(e - r * c8) * 8;
+    const E* p = x + r * n + c;
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = c + j < n ? (float)((double)up_f(p[j]) * inv) : 0.f;
+    __half2 h[4], l[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) g16::split2(v[2 * j], v[2 * j + 1], h[j], l[j]);
+    const int64_t at = z * m * ld + r * ld + c;
+    *reinterpret_cast<uint4*>(hi + at) = *reinterpret_cast<uint4*>(h);
+    *reinterpret_cast<uint4*>(lo + at) = *reinterpret_cast<uint4*>(l);
+  }
+}
+
+// ---- epilogue ----------------------------------------------------------------------
+struct PolyArgs {
+  CUtensorMap out[2][2];               // [first, second output][hi, lo]; out[0][0]: the plain output when type >= 0
+  int64_t M;
+  int N;
+  int two;                             // a second output follows
+  float s[2], diag[2];                 // output q = s[q] acc + diag[q] I (in scaled units)
+  int type;                            // -1: pieces; else memlayer_dtype of the plain output
+  int tma;                             // the plain output's rows are 16 bytes apart
+  void* plain;                         // [batch][M][N]
+};
+
+struct EpiPoly {
+  static constexpr bool kSum = true, kStore = true;
+  using Args = PolyArgs;
+  float sum[128];
+  uint32_t buf;
+  int turn;
+  __device__ __forceinline__ void begin(const Args&, const Sched&, int, uint8_t* staging) {
+    buf = tc::smem_u32(staging);
+    turn = 0;
+  }
+  static __device__ __forceinline__ void pieces(const CUtensorMap* map, uint32_t buf, const uint32_t (&v)[32],
+                                                float s, float diag, int at, int col, int row0, int z) {
+    const int lane = threadIdx.x & 31;
+    uint32_t h[16], l[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      float x = __uint_as_float(v[2 * j]) * s, y = __uint_as_float(v[2 * j + 1]) * s;
+      if (at == 2 * j) x += diag;
+      if (at == 2 * j + 1) y += diag;
+      __half2 a, b;
+      g16::split2(x, y, a, b);
+      h[j] = *reinterpret_cast<const uint32_t*>(&a);
+      l[j] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+    if (lane == 0) g16::bulk_wait<0, true>();
+    __syncwarp();
+    g16::stage16(buf, lane, h);
+    g16::stage16(buf + 2048, lane, l);
+    tc::fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      g16::bulk_store(map, buf, col, row0, z, false);
+      g16::bulk_store(map + 1, buf + 2048, col, row0, z, false);
+    }
+  }
+  __device__ __forceinline__ void plain(const Args& A, uint32_t (&v)[32], int64_t row0, int col, int z) {
+    const int lane = threadIdx.x & 31;
+    const bool f32 = A.type == MEMLAYER_F32;
+    const uint32_t b = buf + (f32 ? 0 : turn * 2048);
+    turn ^= 1;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * A.s[0]);
+    if (lane == 0) {
+      if (f32)
+        g16::bulk_wait<0, true>();
+      else
+        g16::bulk_wait<1, true>();
+    }
+    __syncwarp();
+    g16::stage_as(A.type, b, lane, v);
+    if (A.tma) {
+      tc::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) g16::bulk_store(&A.out[0][0], b, col, (int)row0, z, false);
+    } else {
+      __syncwarp();
+      g16::copy_rows(A.type, b, A.plain, (z * A.M + row0) * A.N + col, A.N, (int)(A.M - row0 < 32 ? A.M - row0 : 32),
+                     A.N - col, false);
+      __syncwarp();
+    }
+  }
+  __device__ __forceinline__ void store(const Args& A, const Sched& S, const Tile& t, int64_t row, int half) {
+    const int64_t row0 = row - (threadIdx.x & 31);
+    const int hw = S.BN >> 1;
+    const int col0 = t.nt * S.BN + half * hw;
+    if (row0 >= A.M) return;
+#pragma unroll
+    for (int cc = 0; cc < 128; cc += 32) {
+      if (cc >= hw || col0 + cc >= A.N) break;
+      const int col = col0 + cc;
+      uint32_t v[32];
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(sum[cc + j]);
+      if (A.type >= 0) {
+        plain(A, v, row0, col, t.z);
+      } else {
+        const int64_t d = row - col;                         // the diagonal's column in this block
+        const int at = d >= 0 && d < 32 ? (int)d : -1;
+        pieces(A.out[0], buf, v, A.s[0], A.diag[0], at, col, (int)row0, t.z);
+        if (A.two) pieces(A.out[1], buf, v, A.s[1], A.diag[1], at, col, (int)row0, t.z);
+      }
+    }
+  }
+  __device__ __forceinline__ void end(const Args&, const Sched&, int) {}
+};
+
+// ---- plan -----------------------------------------------------------------------
+int64_t up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
+
+constexpr size_t O_ERR = 256, HEAD = 512;
+
+struct Plan {
+  int64_t B, m, n, s;                  // s: the smaller side
+  bool tall;
+  int64_t ldx, lds;
+  size_t o_part, o_x[2], o_p, o_r, o_q, bytes;   // hi then lo in each
+  int64_t xe, se;                      // entries of one piece of X, of an s x s matrix
+};
+
+bool make_plan(const memlayer_orth_config& c, Plan* out) {
+  Plan p{};
+  p.B = c.batch;
+  p.m = c.rows;
+  p.n = c.cols;
+  p.tall = c.rows > c.cols;
+  p.s = p.tall ? p.n : p.m;
+  p.ldx = up(p.n, 8);
+  p.lds = up(p.s, 8);
+  p.xe = p.B * p.m * p.ldx;
+  p.se = p.B * p.s * p.lds;
+  size_t off = HEAD;
+  auto take = [&](int64_t bytes) {
+    const size_t o = off;
+    off += (size_t)up(bytes, 256);
+    return o;
+  };
+  p.xe = up(p.xe, 128);                // the second piece starts 256-byte aligned
+  p.se = up(p.se, 128);
+  p.o_part = take(p.B * NORM_CHUNKS * 8);
+  p.o_x[0] = take(2 * p.xe * 2);
+  p.o_x[1] = take(2 * p.xe * 2);
+  p.o_p = take(2 * p.se * 2);
+  p.o_r = take(2 * p.se * 2);
+  p.o_q = take(2 * p.se * 2);
+  p.bytes = off;
+  *out = p;
+  return true;
+}
+
+struct Tiling {
+  int cg, BN;
+};
+
+// The largest tile that still gives every cluster one; the smallest where
+// none does (few products' tiles: more SMs share the work).
+Tiling tiling(int64_t M, int64_t N, int64_t batch) {
+  const int sms = g16::device_sms();
+  const Tiling all[3] = {{2, 256}, {2, 128}, {1, 128}};
+  for (const Tiling& t : all)
+    if (up(M, 128 * t.cg) / (128 * t.cg) * (up(N, t.BN) / t.BN) * batch >= sms / t.cg) return t;
+  return all[2];
+}
+
+#define OR_TRY(x)                             \
+  do {                                        \
+    const cudaError_t e_ = (x);               \
+    if (e_ != cudaSuccess) return e_;         \
+  } while (0)
+
+struct Mat {
+  const __half* p;                     // hi; lo is `lo` entries on
+  int64_t lo, ld, batch;               // batch: entries between matrices
+};
+
+// A(i, k): M rows; B(j, k): N rows; k of length K.
+cudaError_t product(const Plan& p, const Mat& a, bool amn, const Mat& b, bool bmn, int64_t M, int64_t N, int64_t K,
+                    PolyArgs& ea, int* err, cudaStream_t s) {
+  const Tiling t = tiling(M, N, p.B);
+  Maps m{};
+  for (int q = 0; q < 2; ++q) {
+    OR_TRY(g16::make_operand(&m.a[0][q], a.p + q * a.lo, M, K, a.ld, amn, 128, 0, (int)p.B, a.batch));
+    OR_TRY(g16::make_operand(&m.b[0][q], b.p + q * b.lo, N, K, b.ld, bmn, t.BN / t.cg, 0, (int)p.B, b.batch));
+  }
+  Sched S{};
+  Prod& r = S.prod[0];
+  r.m_tiles = (int)(up(M, 128 * t.cg) / (128 * t.cg));
+  r.n_tiles = (int)(up(N, t.BN) / t.BN);
+  r.splits = 1;
+  r.batch = (int)p.B;
+  r.kq = r.kq_total = (int)(up(K, g16::BK) / g16::BK);
+  r.amn = amn;
+  r.bmn = bmn;
+  S.BN = t.BN;
+  S.seg = seg_for(K);
+  g16::distribute(&S, g16::device_sms() / t.cg, 0);
+  ea.M = M;
+  ea.N = (int)N;
+  return t.cg == 2 ? g16::launch_one<EpiPoly, 2, 2, 2>(m, S, ea, err, s)
+                   : g16::launch_one<EpiPoly, 1, 2, 2>(m, S, ea, err, s);
+}
+
+template <typename E>
+cudaError_t start(const memlayer_orth_config& c, const Plan& p, const E* u, char* ws, cudaStream_t s) {
+  const int64_t n = p.m * p.n;
+  int64_t chunks = (n + 4095) / 4096;
+  if (chunks > NORM_CHUNKS) chunks = NORM_CHUNKS;
+  double* part = reinterpret_cast<double*>(ws + p.o_part);
+  orth_norm_kernel<E><<<dim3((unsigned)chunks, (unsigned)p.B), 256, 0, s>>>(u, n, (int)chunks, part);
+  count_launch();
+  OR_TRY(cudaGetLastError());
+  const int64_t items = p.m * (p.ldx / 8);
+  int64_t blocks = (items + 511) / 512;
+  const int64_t cap = up(8 * g16::device_sms(), p.B) / p.B;
+  if (blocks > cap) blocks = cap;
+  __half* x = reinterpret_cast<__half*>(ws + p.o_x[0]);
+  orth_init_kernel<E><<<dim3((unsigned)blocks, (unsigned)p.B), 256, 0, s>>>(
+      u, (int)p.m, (int)p.n, (int)p.ldx, (double)c.epsilon, part, (int)chunks, x, x + p.xe);
+  count_launch();
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+bool orth_workspace(const memlayer_orth_config& c, size_t* bytes) {
+  Plan p;
+  if (!make_plan(c, &p)) return false;
+  *bytes = p.bytes;
+  return true;
+}
+
+bool orth_coefficients_ok(const memlayer_orth_config& c) {
+  // singular values start in [0, 1] and go through x (a + b x^2 + c x^4);
+  // every matrix of a step is bounded by its largest singular value
+  const double a = c.a, b = c.b, d = c.c;
+  for (int i = 0; i <= 256; ++i) {
+    double x = i / 256.0;
+    for (int k = 0; k < c.steps; ++k) {
+      const double p = x * x, r = b + d * p, q = a + r * p;
+      if (!(p <= BOUND * 0.5) || !(fabs(r) <= BOUND * 0.8) || !(fabs(q) <= BOUND * 0.8)) return false;
+      x = fabs(x * q);
+    }
+    if (!(x <= BOUND * 0.2)) return false;
+  }
+  return true;
+}
+
+cudaError_t launch_orthogonalize(const memlayer_orth_config& c, const void* update, void* out, char* ws,
+                                 cudaStream_t s) {
+  Plan p;
+  if (!make_plan(c, &p)) return cudaErrorInvalidValue;
+  int* err = reinterpret_cast<int*>(ws + O_ERR);
+  OR_TRY(cudaMemsetAsync(err, 0, sizeof(int), s));
+  if (p.B == 0) return cudaSuccess;
+  switch (c.dtype) {
+    case MEMLAYER_F16: OR_TRY(start(c, p, (const __half*)update, ws, s)); break;
+    case MEMLAYER_BF16: OR_TRY(start(c, p, (const __nv_bfloat16*)update, ws, s)); break;
+    default: OR_TRY(start(c, p, (const float*)update, ws, s)); break;
+  }
+  __half *x[2] = {reinterpret_cast<__half*>(ws + p.o_x[0]), reinterpret_cast<__half*>(ws + p.o_x[1])};
+  __half *P = reinterpret_cast<__half*>(ws + p.o_p), *R = reinterpret_cast<__half*>(ws + p.o_r),
+         *Q = reinterpret_cast<__half*>(ws + p.o_q);
+  const Mat MP{P, p.se, p.lds, p.s * p.lds}, MR{R, p.se, p.lds, p.s * p.lds}, MQ{Q, p.se, p.lds, p.s * p.lds};
+  auto pieces = [&](CUtensorMap* map, __half* q, int64_t lo, int64_t rows, int64_t cols, int64_t ld) {
+    for (int i = 0; i < 2; ++i) {
+      const cudaError_t e = g16::make_store(map + i, q + i * lo, rows, cols, ld, MEMLAYER_F16, p.B, rows * ld);
+      if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
+  };
+  PolyArgs a1{}, a2{}, a3{};
+  OR_TRY(pieces(a1.out[0], P, p.se, p.s, p.s, p.lds));
+  OR_TRY(pieces(a1.out[1], R, p.se, p.s, p.s, p.lds));
+  OR_TRY(pieces(a2.out[0], Q, p.se, p.s, p.s, p.lds));
+  // accumulators carry SCALE^2, pieces SCALE
+  a1.type = a2.type = -1;
+  a1.two = 1;
+  a1.s[0] = 1.f / SCALE;
+  a1.s[1] = c.c / SCALE;
+  a1.diag[1] = c.b * SCALE;
+  a2.s[0] = 1.f / SCALE;
+  a2.diag[0] = c.a * SCALE;
+  const int64_t es = c.dtype == MEMLAYER_F32 ? 4 : 2;
+  for (int k = 0; k < c.steps; ++k) {
+    const Mat X{x[k & 1], p.xe, p.ldx, p.m * p.ldx};
+    __half* next = x[(k + 1) & 1];
+    OR_TRY(product(p, X, p.tall, X, p.tall, p.s, p.s, p.tall ? p.m : p.n, a1, err, s));
+    OR_TRY(product(p, MR, false, MP, false, p.s, p.s, p.s, a2, err, s));
+    if (k + 1 < c.steps) {
+      a3.type = -1;
+      a3.s[0] = 1.f / SCALE;
+      OR_TRY(pieces(a3.out[0], next, p.xe, p.m, p.n, p.ldx));
+    } else {
+      a3.type = c.dtype;
+      a3.s[0] = 1.f / (SCALE * SCALE);
+      a3.plain = out;
+      a3.tma = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && p.n * es % 16 == 0;
+      if (a3.tma) OR_TRY(g16::make_store(&a3.out[0][0], out, p.m, p.n, p.n, c.dtype, p.B, p.m * p.n));
+    }
+    if (p.tall)
+      OR_TRY(product(p, X, false, MQ, false, p.m, p.n, p.n, a3, err, s));
+    else
+      OR_TRY(product(p, MQ, false, X, true, p.m, p.n, p.m, a3, err, s));
+  }
+  return cudaSuccess;
+}
+
+}  // namespace ml

@@ -18,13 +18,15 @@ import ctypes as C
 import dataclasses
 import math
 import time
-from typing import Any, Dict, Tuple
+from typing import Any, Dict, Optional, Tuple
 
 import numpy as np
 import torch
 
 from . import _lib as L
-from .memory import MemoryPool, _cuda_f32, _raise_device_status, _workspace
+from .memory import MemoryPool, _cuda_f32, _raise_device_status, _workspace, on_stream
+from .train_ops import (layer_norm, layer_norm_backward, linear_cross_entropy,
+                        linear_cross_entropy_backward)
 
 
 @dataclasses.dataclass(frozen=True)
@@ -137,6 +139,27 @@ class MemoryPoolLM:
         prep = params if isinstance(params, PreparedModel) else self.prepare(params)
         return prep.forward(tokens, check=check, stream=stream), {}
 
+    def loss(self, params, tokens: torch.Tensor, targets: torch.Tensor, *, ignore_index: int = -100,
+             check: bool = False, stream=None):
+        """The cross entropy of every position's logits against ``targets [B, T]``
+        without the ``[B, T, V]`` logits: ``(loss, lse)``, float32 [B, T]; loss
+        is 0 where the target is ``ignore_index``."""
+        prep = params if isinstance(params, PreparedModel) else self.prepare(params)
+        return prep.loss(tokens, targets, ignore_index=ignore_index, check=check, stream=stream)
+
+    def loss_and_head_grads(self, params, tokens: torch.Tensor, targets: torch.Tensor, *,
+                            dloss: Optional[torch.Tensor] = None, ignore_index: int = -100, check: bool = False,
+                            stream=None):
+        """``(loss, grads)``: the loss as above and the gradients of
+        ``sum(dloss * loss)`` (default: the mean over the positions that count)
+        through the model's head, the final norm and the tied logits:
+        ``ln_final`` scale and bias, ``embed`` embedding (its part as the output
+        projection) and ``hidden``, the residual stream before the norm, from
+        which the blocks' backward goes on."""
+        prep = params if isinstance(params, PreparedModel) else self.prepare(params)
+        return prep.loss_and_head_grads(tokens, targets, dloss=dloss, ignore_index=ignore_index, check=check,
+                                        stream=stream)
+
 
 class PreparedModel:
     """Parameters of one MemoryPoolLM laid out for the C ABI."""
@@ -175,10 +198,11 @@ class PreparedModel:
                 b.w_gate, b.b_gate = (ptr(f(params[f"mem_gate_{i}"][k], k)) for k in ("kernel", "bias"))
                 b.w_out, b.b_out = (ptr(f(params[f"mem_out_{i}"][k], k)) for k in ("kernel", "bias"))
         self.values_dtype = torch.float32
+        self.ln_final = {k: f(params["ln_final"][k], "ln_final") for k in ("scale", "bias")}
         mp = L.MemlayerModelParams(embedding=self.embedding.data_ptr(), pos_embed=self.pos_embed.data_ptr(),
                                    layers=C.cast(blocks, C.POINTER(L.MemlayerBlockParams)),
-                                   ln_final_scale=ptr(f(params["ln_final"]["scale"], "ln_final")),
-                                   ln_final_bias=ptr(f(params["ln_final"]["bias"], "ln_final")))
+                                   ln_final_scale=ptr(self.ln_final["scale"]),
+                                   ln_final_bias=ptr(self.ln_final["bias"]))
         if model.memory_layers:
             pool = params["pool"]
             values = pool["values"]
@@ -201,19 +225,52 @@ class PreparedModel:
         return nb.value
 
     def forward(self, tokens: torch.Tensor, *, check: bool = False, stream=None) -> torch.Tensor:
+        return self._whole("memlayer_model_forward", tokens, self.model.cfg.vocab_size, check, stream)
+
+    @on_stream
+    def hidden(self, tokens: torch.Tensor, *, check: bool = False, stream=None) -> torch.Tensor:
+        """The residual stream [B, T, d_model] after the last block, before the
+        final norm (memlayer_model_hidden)."""
+        return self._whole("memlayer_model_hidden", tokens, self.model.cfg.d_model, check, stream)
+
+    def _whole(self, entry: str, tokens: torch.Tensor, width: int, check: bool, stream) -> torch.Tensor:
         if tokens.dim() != 2:
             raise ValueError("tokens must be [batch, seq]")
         B, T = tokens.shape
         tok = tokens.to(self.device, torch.int32).contiguous()
-        logits = torch.empty(B, T, self.model.cfg.vocab_size, dtype=torch.float32, device=self.device)
+        out = torch.empty(B, T, width, dtype=torch.float32, device=self.device)
         nb = self.workspace_bytes(B * T)
         ws = _workspace(nb, self.device)
         s = (stream or torch.cuda.current_stream(self.device)).cuda_stream
-        L.check(L.lib().memlayer_model_forward(C.byref(self.cfg), C.byref(self.params), tok.data_ptr(), B, T,
-                                               logits.data_ptr(), ws.data_ptr(), nb, s), "memlayer_model_forward")
+        L.check(getattr(L.lib(), entry)(C.byref(self.cfg), C.byref(self.params), tok.data_ptr(), B, T,
+                                        out.data_ptr(), ws.data_ptr(), nb, s), entry)
         if check:
             _raise_device_status(self.cfg.pool, ws, s)
-        return logits
+        return out
+
+    @on_stream
+    def loss(self, tokens: torch.Tensor, targets: torch.Tensor, *, ignore_index: int = -100, check: bool = False,
+             stream=None):
+        """``MemoryPoolLM.loss`` on these parameters."""
+        h = layer_norm(self.hidden(tokens, check=check), self.ln_final["scale"], self.ln_final["bias"])
+        return linear_cross_entropy(h, self.embedding, targets.to(self.device), ignore_index=ignore_index,
+                                    check=check)
+
+    @on_stream
+    def loss_and_head_grads(self, tokens: torch.Tensor, targets: torch.Tensor, *,
+                            dloss: Optional[torch.Tensor] = None, ignore_index: int = -100, check: bool = False,
+                            stream=None):
+        """``MemoryPoolLM.loss_and_head_grads`` on these parameters."""
+        targets = targets.to(self.device)
+        x = self.hidden(tokens, check=check)
+        h = layer_norm(x, self.ln_final["scale"], self.ln_final["bias"])
+        loss, lse = linear_cross_entropy(h, self.embedding, targets, ignore_index=ignore_index, check=check)
+        if dloss is None:
+            n = (targets != ignore_index).sum().clamp(min=1)
+            dloss = (1.0 / n).to(torch.float32).expand(targets.shape)
+        dh, dw = linear_cross_entropy_backward(h, self.embedding, targets, lse, dloss, ignore_index=ignore_index)
+        dx, dp = layer_norm_backward(dh, x, self.ln_final["scale"])
+        return loss, {"hidden": dx, "ln_final": dp, "embed": {"embedding": dw}}
 
 
 class Generator:
