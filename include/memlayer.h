@@ -615,6 +615,12 @@ int32_t memlayer_model_decode_step(const memlayer_model_config* cfg, const memla
  * to the element; 16-byte aligned rows run faster.  Results do not depend on
  * timing: equal calls give equal bits. */
 
+/* The device status word of the last memlayer_layer_norm_backward,
+ * memlayer_cross_entropy, memlayer_cross_entropy_backward or
+ * memlayer_orthogonalize on this workspace (0: fine; 27: a target out of range;
+ * 11-15: a bounded wait gave up).  Synchronises the stream. */
+int32_t memlayer_train_status(const void* workspace, int32_t* code, void* stream);
+
 typedef struct {
   int64_t rows;                  /* product of the leading dimensions */
   int32_t d_model;               /* 1 .. 16384 */
@@ -689,7 +695,7 @@ int32_t memlayer_cross_entropy_workspace_size(const memlayer_loss_config* cfg, i
  * (model.py:125 under the trainer's loss) without the [T, V] logits.  A
  * target outside [0, V) that is not ignore_index gives a NaN loss and, in the
  * backward, no gradient; it records status 27, read with
- * memlayer_cross_entropy_status.  float32 products keep 22 bits of each
+ * memlayer_train_status.  float32 products keep 22 bits of each
  * operand (relative to its matrix's largest entry). */
 int32_t memlayer_cross_entropy(const memlayer_loss_config* cfg, const memlayer_loss_args* args, void* workspace,
                                size_t workspace_bytes, void* stream);
@@ -700,9 +706,6 @@ int32_t memlayer_cross_entropy(const memlayer_loss_config* cfg, const memlayer_l
 int32_t memlayer_cross_entropy_backward(const memlayer_loss_config* cfg, const memlayer_loss_args* args,
                                         const memlayer_loss_grads* grads, void* workspace, size_t workspace_bytes,
                                         void* stream);
-
-/* The device status word of the last cross entropy call on this workspace (synchronises the stream). */
-int32_t memlayer_cross_entropy_status(const void* workspace, int32_t* code, void* stream);
 
 typedef struct {
   int64_t batch;                 /* matrices */

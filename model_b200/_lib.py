@@ -425,8 +425,8 @@ def lib() -> C.CDLL:
         L.memlayer_cross_entropy_backward.argtypes = [C.POINTER(MemlayerLossConfig), C.POINTER(MemlayerLossArgs),
                                                       C.POINTER(MemlayerLossGrads), C.c_void_p, C.c_size_t,
                                                       C.c_void_p]
-        L.memlayer_cross_entropy_status.restype = C.c_int32
-        L.memlayer_cross_entropy_status.argtypes = [C.c_void_p, C.POINTER(C.c_int32), C.c_void_p]
+        L.memlayer_train_status.restype = C.c_int32
+        L.memlayer_train_status.argtypes = [C.c_void_p, C.POINTER(C.c_int32), C.c_void_p]
         L.memlayer_orthogonalize_workspace_size.restype = C.c_int32
         L.memlayer_orthogonalize_workspace_size.argtypes = [C.POINTER(MemlayerOrthConfig), C.POINTER(C.c_size_t)]
         L.memlayer_orthogonalize.restype = C.c_int32

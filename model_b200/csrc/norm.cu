@@ -8,18 +8,29 @@
 //   dscale = sum over rows of dy xhat,  dbias = sum over rows of dy
 //
 // Both passes are bound by HBM: every tensor crosses it once.  A row is held
-// in the registers of `tpr` threads, 16 values each (16-byte accesses when
-// width, row strides and addresses allow, single elements otherwise), so the
-// variance is the centred one from registers -- E[x^2] - E[x]^2 loses the
-// variance of a row whose mean is large -- and the gradient recomputes mean
-// and rstd from the row it reads anyway instead of reading them back.
-// Statistics and sums are float32 whatever the storage type.
+// in registers, so the variance is the centred one -- E[x^2] - E[x]^2 loses
+// the variance of a row whose mean is large -- and the gradient recomputes
+// mean and rstd from the row it reads anyway instead of reading them back.
+// Statistics and sums are float32 whatever the storage type.  Two layouts:
 //
-// The parameter gradients: a block keeps dscale / dbias of its columns in
-// registers over all of its rows, adds its row groups in shared memory and
-// writes one partial row; a second kernel adds the partials in block order,
+//   group   a row in a power of two of threads, 16 values each; up to a warp
+//           (512 columns) its sums are shuffles.  Also every width whose rows
+//           16-byte accesses cannot reach, with single elements;
+//   warp    the forward up to 512 vectors, the gradient up to 2048 columns: a
+//           row in a warp, no barriers.  The gradient keeps its columns'
+//           parameter sums in registers (64 columns a lane), so few warps fit
+//           an SM; a ring of rows in shared memory, filled by bulk copies,
+//           keeps HBM busy beside them.  In a block per row its reductions
+//           took four times the instructions (16384 x 2048 bf16: 113 us);
+//   wide    beyond: a block per row.
+//
+// The parameter gradients: dscale / dbias of the columns stay in registers over
+// all of a block's rows; it adds its row groups in shared memory and writes one
+// partial row; a second kernel adds the partials in block order,
 // so the result does not depend on timing (no atomics).
 #include "norm.cuh"
+
+#include "tc_common.cuh"
 
 namespace ml {
 
@@ -98,10 +109,13 @@ struct NormArgs {
   const float *scale, *bias;
   void *y, *sum, *dx;
   float* part;
+  int* err;             // status word (gradient), cleared by the first block
 };
 
-template <typename E, int VEC, bool WIDE>
-__global__ void __launch_bounds__(WIDE ? 1024 : NT) layer_norm_kernel(NormArgs A) {
+// MAXT > 0: a row in the whole block (at most MAXT threads).
+template <typename E, int VEC, int MAXT>
+__global__ void __launch_bounds__(MAXT ? MAXT : NT, MAXT ? 1 : 2) layer_norm_kernel(NormArgs A) {
+  constexpr bool WIDE = MAXT > 0;
   __shared__ float red[32];
   using Part = RowPart<E, VEC>;
   const int tpr = A.tpr, d = A.d;
@@ -144,14 +158,16 @@ __global__ void __launch_bounds__(WIDE ? 1024 : NT) layer_norm_kernel(NormArgs A
   }
 }
 
-template <typename E, int VEC, bool WIDE>
-__global__ void __launch_bounds__(WIDE ? 1024 : NT) layer_norm_backward_kernel(NormArgs A) {
+template <typename E, int VEC, int MAXT>
+__global__ void __launch_bounds__(MAXT ? MAXT : NT, MAXT ? 1 : 2) layer_norm_backward_kernel(NormArgs A) {
+  constexpr bool WIDE = MAXT > 0;
   __shared__ float red[32];
   extern __shared__ float cols[];          // !WIDE: [groups][VALS * tpr]
   using Part = RowPart<E, VEC>;
   const int tpr = A.tpr, d = A.d;
   const int t = threadIdx.x & (tpr - 1), g = threadIdx.x / tpr, groups = blockDim.x / tpr;
   const int64_t step = (int64_t)gridDim.x * groups;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *A.err = 0;
   float ag[VALS], ab[VALS];
 #pragma unroll
   for (int k = 0; k < VALS; ++k) ag[k] = ab[k] = 0.f;
@@ -233,35 +249,597 @@ __global__ void __launch_bounds__(WIDE ? 1024 : NT) layer_norm_backward_kernel(N
   }
 }
 
-// dscale | dbias = the blocks' partial rows added in block order: 8 groups of
+// ---- wide rows ---------------------------------------------------------------------
+template <typename E, int V>
+struct alignas(V * sizeof(E)) Vec16 { E e[V]; };
+
+// Sums of N values over the block, the same in every thread: warp sums in
+// `red` (32 slots a value, those without a warp zero), added in warp order.
+// One barrier: callers alternate two buffers.
+template <int N>
+__device__ __forceinline__ void block_sums(float (&x)[N], float* red) {
+  const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int i = 0; i < N; ++i) x[i] = warp_sum(x[i]);
+  if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) red[i * 32 + warp] = x[i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float4* r4 = reinterpret_cast<const float4*>(red + i * 32);
+    float t = 0.f;
+    for (int w = 0; w < warps; w += 4) {
+      const float4 r = r4[w >> 2];
+      t += (r.x + r.y) + (r.z + r.w);
+    }
+    x[i] = t;
+  }
+}
+
+// Two float32 at once (the packed forms of add, multiply and fused
+// multiply-add: half the instructions, the same roundings).
+struct F2 {
+  unsigned long long v;
+};
+__device__ __forceinline__ F2 f2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ F2 f2(float a) { return f2(a, a); }
+__device__ __forceinline__ void split(F2 x, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v));
+}
+__device__ __forceinline__ F2 operator+(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ float sum(F2 x) {
+  float a, b;
+  split(x, a, b);
+  return a + b;
+}
+
+__device__ __forceinline__ void unpack2(const Vec16<float, 4>& v, F2 (&x)[2]) {
+  x[0] = f2(v.e[0], v.e[1]);
+  x[1] = f2(v.e[2], v.e[3]);
+}
+__device__ __forceinline__ void unpack2(const Vec16<__half, 8>& v, F2 (&x)[4]) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float2 t = __half22float2(*reinterpret_cast<const __half2*>(v.e + 2 * k));
+    x[k] = f2(t.x, t.y);
+  }
+}
+__device__ __forceinline__ void unpack2(const Vec16<__nv_bfloat16, 8>& v, F2 (&x)[4]) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const unsigned u = *reinterpret_cast<const unsigned*>(v.e + 2 * k);
+    x[k] = f2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
+  }
+}
+
+template <typename E, int V>
+__device__ __forceinline__ void unpack(const Vec16<E, V>& v, float (&x)[V]) {
+#pragma unroll
+  for (int k = 0; k < V; ++k) x[k] = Elem<E>::up(v.e[k]);
+}
+
+template <int V>
+__device__ __forceinline__ void load_f32(const float* p, float (&x)[V]) {
+  if constexpr (V == 1) x[0] = __ldg(p);
+#pragma unroll
+  for (int k = 0; k + 4 <= V; k += 4) {
+    const float4 t = __ldg(reinterpret_cast<const float4*>(p + k));
+    x[k] = t.x;
+    x[k + 1] = t.y;
+    x[k + 2] = t.z;
+    x[k + 3] = t.w;
+  }
+}
+
+template <typename E>
+__device__ __forceinline__ void pack(Vec16<E, 1>& v, const float (&x)[1]) {
+  v.e[0] = Elem<E>::down(x[0]);
+}
+__device__ __forceinline__ void pack(Vec16<float, 4>& v, const float (&x)[4]) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) v.e[k] = x[k];
+}
+__device__ __forceinline__ void pack(Vec16<__half, 8>& v, const float (&x)[8]) {
+#pragma unroll
+  for (int k = 0; k < 8; k += 2) *reinterpret_cast<__half2*>(v.e + k) = __floats2half2_rn(x[k], x[k + 1]);
+}
+__device__ __forceinline__ void pack(Vec16<__nv_bfloat16, 8>& v, const float (&x)[8]) {
+#pragma unroll
+  for (int k = 0; k < 8; k += 2) *reinterpret_cast<__nv_bfloat162*>(v.e + k) = __floats2bfloat162_rn(x[k], x[k + 1]);
+}
+
+// A row in a warp: vector i of lane t is columns (32 i + t) V .. + V.  No
+// barrier, and 12 to 24 warps an SM with 8 KB of loads in flight each.
+template <typename E, int V, int NV>
+__global__ void __launch_bounds__(128) layer_norm_warp_kernel(NormArgs A) {
+  using Vec = Vec16<E, V>;
+  const int d = A.d, lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (row >= A.rows) return;
+  Vec p[NV];
+  const E* x = reinterpret_cast<const E*>(A.x) + row * A.ldx;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int j = (i * 32 + lane) * V;
+    if (j < d) p[i] = *reinterpret_cast<const Vec*>(x + j);
+  }
+  if (A.r) {
+    Vec q[NV];
+    const E* r = reinterpret_cast<const E*>(A.r) + row * A.ldr;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int j = (i * 32 + lane) * V;
+      if (j < d) q[i] = *reinterpret_cast<const Vec*>(r + j);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int j = (i * 32 + lane) * V;
+      if (j >= d) continue;
+      float a[V], b[V];
+      unpack(p[i], a);
+      unpack(q[i], b);
+#pragma unroll
+      for (int k = 0; k < V; ++k) a[k] += b[k];
+      pack(p[i], a);
+      if (A.sum) *reinterpret_cast<Vec*>(reinterpret_cast<E*>(A.sum) + row * (int64_t)d + j) = p[i];
+    }
+  }
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if ((i * 32 + lane) * V < d) {
+      float a[V];
+      unpack(p[i], a);
+#pragma unroll
+      for (int k = 0; k < V; ++k) s += a[k];
+    }
+  const float mean = warp_sum(s) * A.inv_d;
+  float s2 = 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if ((i * 32 + lane) * V < d) {
+      float a[V];
+      unpack(p[i], a);
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        const float c = a[k] - mean;
+        s2 = fmaf(c, c, s2);
+      }
+    }
+  const float rstd = 1.0f / sqrtf(warp_sum(s2) * A.inv_d + A.eps);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int j = (i * 32 + lane) * V;
+    if (j >= d) continue;
+    float a[V], sc[V], bi[V];
+    unpack(p[i], a);
+    load_f32(A.scale + j, sc);
+    load_f32(A.bias + j, bi);
+#pragma unroll
+    for (int k = 0; k < V; ++k) a[k] = fmaf((a[k] - mean) * rstd, sc[k], bi[k]);
+    pack(p[i], a);
+    *reinterpret_cast<Vec*>(reinterpret_cast<E*>(A.y) + row * (int64_t)d + j) = p[i];
+  }
+}
+
+// A row in a block, for rows that a warp does not hold: thread t has columns
+// (i blockDim + t) V .. + V, i < NV.
+template <typename E, int NV, int MAXT>
+__global__ void __launch_bounds__(MAXT, 1) layer_norm_wide_kernel(NormArgs A) {
+  constexpr int V = 16 / sizeof(E);
+  using Vec = Vec16<E, V>;
+  __shared__ alignas(16) float red[2][32];
+  const int d = A.d, t = threadIdx.x, nt = blockDim.x;
+  if (t < 64) (&red[0][0])[t] = 0.f;     // slots without a warp
+  __syncthreads();
+  for (int64_t row = blockIdx.x; row < A.rows; row += gridDim.x) {
+    Vec p[NV];
+    float s[1] = {0.f}, s2[1] = {0.f};
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int j = (i * nt + t) * V;
+      if (j < d) p[i] = *reinterpret_cast<const Vec*>(reinterpret_cast<const E*>(A.x) + row * A.ldx + j);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int j = (i * nt + t) * V;
+      if (j >= d) continue;
+      float a[V];
+      unpack(p[i], a);
+      if (A.r) {
+        float b[V];
+        unpack(*reinterpret_cast<const Vec*>(reinterpret_cast<const E*>(A.r) + row * A.ldr + j), b);
+#pragma unroll
+        for (int k = 0; k < V; ++k) a[k] += b[k];
+        pack(p[i], a);
+        unpack(p[i], a);
+        if (A.sum) *reinterpret_cast<Vec*>(reinterpret_cast<E*>(A.sum) + row * (int64_t)d + j) = p[i];
+      }
+#pragma unroll
+      for (int k = 0; k < V; ++k) s[0] += a[k];
+    }
+    block_sums(s, red[0]);
+    const float mean = s[0] * A.inv_d;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if ((i * nt + t) * V < d) {
+        float a[V];
+        unpack(p[i], a);
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          const float c = a[k] - mean;
+          s2[0] = fmaf(c, c, s2[0]);
+        }
+      }
+    block_sums(s2, red[1]);
+    const float rstd = 1.0f / sqrtf(s2[0] * A.inv_d + A.eps);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int j = (i * nt + t) * V;
+      if (j >= d) continue;
+      float a[V], sc[V], bi[V];
+      unpack(p[i], a);
+      load_f32(A.scale + j, sc);
+      load_f32(A.bias + j, bi);
+#pragma unroll
+      for (int k = 0; k < V; ++k) a[k] = fmaf((a[k] - mean) * rstd, sc[k], bi[k]);
+      pack(p[i], a);
+      *reinterpret_cast<Vec*>(reinterpret_cast<E*>(A.y) + row * (int64_t)d + j) = p[i];
+    }
+  }
+}
+
+// R rows of a block's batch, as loaded.
+template <typename E, int R, int NV>
+struct Batch {
+  static constexpr int V = 16 / sizeof(E);
+  Vec16<E, V> p[R][NV], q[R][NV], e[R][NV];
+  __device__ __forceinline__ void load(const NormArgs& A, int64_t base) {
+    using Vec = Vec16<E, V>;
+    const int t = threadIdx.x, nt = blockDim.x;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (base + r >= A.rows) break;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int j = (i * nt + t) * V;
+        if (j >= A.d) continue;
+        p[r][i] = *reinterpret_cast<const Vec*>(reinterpret_cast<const E*>(A.x) + (base + r) * A.ldx + j);
+        q[r][i] = *reinterpret_cast<const Vec*>(reinterpret_cast<const E*>(A.dy) + (base + r) * A.lddy + j);
+        if (A.dr) e[r][i] = *reinterpret_cast<const Vec*>(reinterpret_cast<const E*>(A.dr) + (base + r) * A.lddr + j);
+      }
+    }
+  }
+};
+
+// AHEAD: the next batch's loads are issued before this one's sums, so HBM is
+// busy during the barriers (where the registers allow it).
+template <typename E, int R, int NV, int MAXT, bool AHEAD>
+__global__ void __launch_bounds__(MAXT, MAXT <= 256 ? 2 : 1) layer_norm_wide_backward_kernel(NormArgs A) {
+  constexpr int V = 16 / sizeof(E), H = V / 2;
+  using Vec = Vec16<E, V>;
+  __shared__ alignas(16) float red[2][3 * R * 32];
+  const int d = A.d, t = threadIdx.x, nt = blockDim.x;
+  for (int i = t; i < 2 * 3 * R * 32; i += nt) (&red[0][0])[i] = 0.f;   // slots without a warp
+  __syncthreads();
+  if (blockIdx.x == 0 && threadIdx.x == 0) *A.err = 0;
+  F2 ag[NV][H], ab[NV][H], sc[NV][H];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int j = (i * nt + t) * V;
+    float f[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) f[k] = 0.f;
+    if (j < d) load_f32(A.scale + j, f);
+#pragma unroll
+    for (int k = 0; k < H; ++k) {
+      ag[i][k] = ab[i][k] = f2(0.f);
+      sc[i][k] = f2(f[2 * k], f[2 * k + 1]);
+    }
+  }
+  const int64_t step = (int64_t)gridDim.x * R;
+  Batch<E, R, NV> next;
+  if constexpr (AHEAD) next.load(A, (int64_t)blockIdx.x * R);
+  for (int64_t base = (int64_t)blockIdx.x * R; base < A.rows; base += step) {
+    Batch<E, R, NV> b;
+    if constexpr (AHEAD) {
+      b = next;
+      next.load(A, base + step);
+    } else {
+      b.load(A, base);
+    }
+    float s[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      F2 acc = f2(0.f);
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if ((i * nt + t) * V < d) {
+          F2 a[H];
+          unpack2(b.p[r][i], a);
+#pragma unroll
+          for (int k = 0; k < H; ++k) acc = acc + a[k];
+        }
+      s[r] = sum(acc);
+    }
+    block_sums(s, red[0]);
+    // around the mean: sum c^2, sum gy, sum gy c (c2 = rstd times it)
+    float m[3 * R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const F2 mean = f2(-(s[r] * A.inv_d));
+      F2 s2 = f2(0.f), sg = f2(0.f), sgc = f2(0.f);
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if ((i * nt + t) * V < d) {
+          F2 a[H], g[H];
+          unpack2(b.p[r][i], a);
+          unpack2(b.q[r][i], g);
+#pragma unroll
+          for (int k = 0; k < H; ++k) {
+            const F2 c = a[k] + mean, gy = g[k] * sc[i][k];
+            s2 = fma2(c, c, s2);
+            sg = sg + gy;
+            sgc = fma2(gy, c, sgc);
+          }
+        }
+      m[3 * r] = sum(s2);
+      m[3 * r + 1] = sum(sg);
+      m[3 * r + 2] = sum(sgc);
+    }
+    block_sums(m, red[1]);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (base + r >= A.rows) break;
+      const float rstd_f = rsqrtf(m[3 * r] * A.inv_d + A.eps);
+      const F2 mean = f2(-(s[r] * A.inv_d)), rstd = f2(rstd_f), c1 = f2(-(m[3 * r + 1] * A.inv_d)),
+               c2 = f2(-(m[3 * r + 2] * rstd_f * A.inv_d));
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int j = (i * nt + t) * V;
+        if (j >= d) continue;
+        F2 a[H], g[H];
+        float x[V];
+        unpack2(b.p[r][i], a);
+        unpack2(b.q[r][i], g);
+#pragma unroll
+        for (int k = 0; k < H; ++k) {
+          const F2 xh = (a[k] + mean) * rstd;
+          ag[i][k] = fma2(g[k], xh, ag[i][k]);
+          ab[i][k] = ab[i][k] + g[k];
+          a[k] = rstd * fma2(xh, c2, g[k] * sc[i][k] + c1);
+        }
+        if (A.dr) {
+          unpack2(b.e[r][i], g);
+#pragma unroll
+          for (int k = 0; k < H; ++k) a[k] = a[k] + g[k];
+        }
+#pragma unroll
+        for (int k = 0; k < H; ++k) split(a[k], x[2 * k], x[2 * k + 1]);
+        Vec o;
+        pack(o, x);
+        *reinterpret_cast<Vec*>(reinterpret_cast<E*>(A.dx) + (base + r) * (int64_t)d + j) = o;
+      }
+    }
+  }
+  float* out = A.part + (int64_t)blockIdx.x * 2 * d;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int j = (i * nt + t) * V;
+    if (j >= d) continue;
+#pragma unroll
+    for (int k = 0; k < H; ++k) {
+      float a, c;
+      split(ag[i][k], a, c);
+      out[j + 2 * k] = a;
+      out[j + 2 * k + 1] = c;
+      split(ab[i][k], a, c);
+      out[d + j + 2 * k] = a;
+      out[d + j + 2 * k + 1] = c;
+    }
+  }
+}
+
+// The gradient of rows that a warp holds: a warp per row, without a barrier.
+// Each warp streams its rows of x and dy through a ring of its own in shared
+// memory (bulk copies, signalled by mbarriers) and reads them from there: the mean, the three sums around it, dx.  The columns' parameter sums
+// stay in its registers over all of its rows; the block adds its warps' at
+// the end.
+template <typename E, int NV, int MAXW>
+__global__ void __launch_bounds__(MAXW * 32, 1) layer_norm_ring_backward_kernel(NormArgs A, int stages) {
+  constexpr int V = 16 / sizeof(E), H = V / 2;
+  using Vec = Vec16<E, V>;
+  extern __shared__ uint8_t smem_raw[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const int d = A.d, rb = d * (int)sizeof(E);
+  constexpr int tensors = 2;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem) + warp * 4;              // 4 stages at most
+  volatile int* abort = reinterpret_cast<int*>(smem + 12 * 32);
+  float* scale_s = reinterpret_cast<float*>(smem + 512);
+  uint8_t* rings = smem + 512 + (((size_t)d * 4 + 127) & ~size_t(127));
+  const int rbp = (rb + 127) & ~127;                                           // a row's pitch in the ring
+  uint8_t* ring = rings + (size_t)warp * stages * tensors * rbp;
+  if (lane == 0)
+    for (int i = 0; i < stages; ++i) tc::mbar_init(&full[i], 1);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *A.err = 0;
+  if (threadIdx.x == 0) *abort = 0;
+  tc::fence_mbar_init();
+  for (int j = threadIdx.x; j < d; j += blockDim.x) scale_s[j] = A.scale[j];
+  __syncthreads();
+
+  const int64_t first = (int64_t)blockIdx.x * warps + warp, step = (int64_t)gridDim.x * warps;
+  auto fetch = [&](int64_t row, int st) {   // lane 0
+    tc::mbar_expect_tx(&full[st], (uint32_t)(tensors * rb));
+    uint8_t* at = ring + (size_t)st * tensors * rbp;
+    auto copy = [&](uint8_t* dst, const void* src) {
+      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                       tc::smem_u32(dst)),
+                   "l"(src), "r"(rb), "r"(tc::smem_u32(&full[st]))
+                   : "memory");
+    };
+    copy(at, reinterpret_cast<const E*>(A.x) + row * A.ldx);
+    copy(at + rbp, reinterpret_cast<const E*>(A.dy) + row * A.lddy);
+  };
+  F2 ag[NV][H], ab[NV][H];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int k = 0; k < H; ++k) ag[i][k] = ab[i][k] = f2(0.f);
+  if (lane == 0)
+    for (int i = 0; i < stages; ++i)
+      if (first + i * step < A.rows) fetch(first + i * step, i);
+  int st = 0;
+  uint32_t ph = 0;
+  for (int64_t row = first; row < A.rows; row += step) {
+    Vec e[NV];                               // used last: loaded straight into registers meanwhile
+    if (A.dr) {
+      const Vec* es = reinterpret_cast<const Vec*>(reinterpret_cast<const E*>(A.dr) + row * A.lddr);
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if ((i * 32 + lane) * V < d) e[i] = es[i * 32 + lane];
+    }
+    if (!__all_sync(FULL, tc::mbar_wait(&full[st], ph, abort, A.err, 11))) break;
+    const uint8_t* at = ring + (size_t)st * tensors * rbp;
+    const Vec* xs = reinterpret_cast<const Vec*>(at);
+    const Vec* gs = reinterpret_cast<const Vec*>(at + rbp);
+    F2 acc = f2(0.f);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if ((i * 32 + lane) * V < d) {
+        F2 a[H];
+        unpack2(xs[i * 32 + lane], a);
+#pragma unroll
+        for (int k = 0; k < H; ++k) acc = acc + a[k];
+      }
+    const F2 mean = f2(-(warp_sum(sum(acc)) * A.inv_d));
+    F2 s2 = f2(0.f), sg = f2(0.f), sgc = f2(0.f);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if ((i * 32 + lane) * V < d) {
+        F2 a[H], g[H];
+        unpack2(xs[i * 32 + lane], a);
+        unpack2(gs[i * 32 + lane], g);
+        const F2* sc = reinterpret_cast<const F2*>(scale_s + (i * 32 + lane) * V);
+#pragma unroll
+        for (int k = 0; k < H; ++k) {
+          const F2 c = a[k] + mean, gy = g[k] * sc[k];
+          s2 = fma2(c, c, s2);
+          sg = sg + gy;
+          sgc = fma2(gy, c, sgc);
+        }
+      }
+    const float rstd_f = rsqrtf(warp_sum(sum(s2)) * A.inv_d + A.eps);
+    const F2 rstd = f2(rstd_f), c1 = f2(-(warp_sum(sum(sg)) * A.inv_d)),
+             c2 = f2(-(warp_sum(sum(sgc)) * rstd_f * A.inv_d));
+    Vec* out = reinterpret_cast<Vec*>(reinterpret_cast<E*>(A.dx) + row * (int64_t)d);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if ((i * 32 + lane) * V < d) {
+        F2 a[H], g[H];
+        float x[V];
+        unpack2(xs[i * 32 + lane], a);
+        unpack2(gs[i * 32 + lane], g);
+        const F2* sc = reinterpret_cast<const F2*>(scale_s + (i * 32 + lane) * V);
+#pragma unroll
+        for (int k = 0; k < H; ++k) {
+          const F2 xh = (a[k] + mean) * rstd;
+          ag[i][k] = fma2(g[k], xh, ag[i][k]);
+          ab[i][k] = ab[i][k] + g[k];
+          a[k] = rstd * fma2(xh, c2, g[k] * sc[k] + c1);
+        }
+        if (A.dr) {
+          unpack2(e[i], g);
+#pragma unroll
+          for (int k = 0; k < H; ++k) a[k] = a[k] + g[k];
+        }
+#pragma unroll
+        for (int k = 0; k < H; ++k) split(a[k], x[2 * k], x[2 * k + 1]);
+        Vec o;
+        pack(o, x);
+        out[i * 32 + lane] = o;
+      }
+    __syncwarp();                            // every lane has read the stage
+    if (lane == 0 && row + stages * step < A.rows) fetch(row + stages * step, st);
+    if (++st == stages) {
+      st = 0;
+      ph ^= 1;
+    }
+  }
+  // the warps' sums, in warp order, through the rings' memory
+  __syncthreads();
+  float* all = reinterpret_cast<float*>(rings);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int j = (i * 32 + lane) * V;
+    if (j >= d) continue;
+#pragma unroll
+    for (int k = 0; k < H; ++k) {
+      *reinterpret_cast<F2*>(all + (size_t)warp * 2 * d + j + 2 * k) = ag[i][k];
+      *reinterpret_cast<F2*>(all + (size_t)warp * 2 * d + d + j + 2 * k) = ab[i][k];
+    }
+  }
+  __syncthreads();
+  float* part = A.part + (int64_t)blockIdx.x * 2 * d;
+  for (int j = threadIdx.x; j < 2 * d; j += blockDim.x) {
+    float x = 0.f;
+    for (int w = 0; w < warps; ++w) x += all[(size_t)w * 2 * d + j];
+    part[j] = x;
+  }
+}
+
+// dscale | dbias = the blocks' partial rows added in block order: 32 groups of
 // blocks per column, then the groups in order.
-__global__ void __launch_bounds__(256) layer_norm_params_kernel(const float* __restrict__ part, int blocks, int d,
-                                                                float* __restrict__ dscale,
-                                                                float* __restrict__ dbias) {
-  __shared__ float red[8][33];
+__global__ void __launch_bounds__(1024) layer_norm_params_kernel(const float* __restrict__ part, int blocks, int d,
+                                                                 float* __restrict__ dscale,
+                                                                 float* __restrict__ dbias, int* err) {
+  if (blocks == 0 && blockIdx.x == 0 && threadIdx.x == 0) *err = 0;
+  __shared__ float red[32][33];
   const int c = threadIdx.x & 31, g = threadIdx.x >> 5;
   const int j = blockIdx.x * 32 + c;
   float x = 0.f;
   if (j < 2 * d) {
     const float* p = part + j;
     int b = g;
-    for (; b + 56 < blocks; b += 64) {      // eight loads in flight
+    for (; b + 7 * 32 < blocks; b += 8 * 32) {      // eight loads in flight
       float a[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) a[i] = p[(int64_t)(b + 8 * i) * 2 * d];
+      for (int i = 0; i < 8; ++i) a[i] = p[(int64_t)(b + 32 * i) * 2 * d];
 #pragma unroll
       for (int i = 0; i < 8; ++i) x += a[i];
     }
-    for (; b < blocks; b += 8) x += p[(int64_t)b * 2 * d];
+    float a[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a[i] = b + 32 * i < blocks ? p[(int64_t)(b + 32 * i) * 2 * d] : 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x += a[i];
   }
   red[g][c] = x;
   __syncthreads();
-  if (g == 0 && j < 2 * d) {
-    float t = red[0][c];
-#pragma unroll
-    for (int i = 1; i < 8; ++i) t += red[i][c];
-    (j < d ? dscale[j] : dbias[j - d]) = t;
-  }
+  // warp g: column g of this block's 32
+  const float t = warp_sum(red[c][g]);
+  const int k = blockIdx.x * 32 + g;
+  if (c == 0 && k < 2 * d) (k < d ? dscale[k] : dbias[k - d]) = t;
 }
 
 // Threads of a row: the power of two that holds its width at 16 values each.
@@ -280,44 +858,160 @@ int sm_count() {
 
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+// The block-per-row layouts: threads a row, vectors a thread, rows at a time.
+struct Wide {
+  int nt, nv, r;
+};
+
+bool wide_rows(int d, int v) { return d > 32 * VALS && d % v == 0; }
+
+Wide wide_for(int d, int v) {
+  const int vecs = (d + v - 1) / v;
+  if (vecs <= 1024) return {(vecs + 31) / 32 * 32, 1, 1};
+  const int nv = vecs <= 2048 ? 2 : 4;
+  return {((vecs + nv - 1) / nv + 31) / 32 * 32, nv, 1};
+}
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// The ring layout of the gradient: rows of up to 256 vectors (16-bit) or 512
+// (float32), 64 columns a lane; as many warps as the rings leave room for.
+struct Ring {
+  int warps, stages;
+  size_t smem;
+};
+
+bool ring_rows(int d, int v) { return wide_rows(d, v) && d <= 2048; }
+
+Ring ring_for(int d, int esize) {
+  const size_t rbp = ((size_t)d * esize + 127) / 128 * 128, head = 128 + 512 + ((size_t)d * 4 + 127) / 128 * 128;
+  const size_t room = 227 * 1024 - head, row = rbp * 2;
+  const size_t most = d > 1024 ? 8 : 12;                     // 128 sums a lane leave registers for 8 warps
+  Ring r{};
+  r.stages = 3 * row * most <= room ? 3 : 2;
+  const size_t w = room / (row * r.stages);
+  r.warps = (int)(w < most ? w : most);
+  r.smem = head + row * r.stages * r.warps;
+  return r;
+}
+
 template <typename E>
 cudaError_t norm_forward_t(NormArgs& A, bool vec, cudaStream_t s) {
   constexpr int V = 16 / sizeof(E);
-  const bool wide = A.tpr > 32;
-  const int nt = wide ? A.tpr : NT;
-  const int64_t need = (A.rows + nt / A.tpr - 1) / (nt / A.tpr);
-  const int grid = (int)(need < (1 << 20) ? need : (1 << 20));
-  if (vec)
-    wide ? layer_norm_kernel<E, V, true><<<grid, nt, 0, s>>>(A) : layer_norm_kernel<E, V, false><<<grid, nt, 0, s>>>(A);
-  else
-    wide ? layer_norm_kernel<E, 1, true><<<grid, nt, 0, s>>>(A) : layer_norm_kernel<E, 1, false><<<grid, nt, 0, s>>>(A);
+  constexpr int64_t MOST = 1 << 20;
+  const int vecs = A.d / V;
+  const bool warp = A.d > 32 * VALS && (vec ? vecs <= 512 : A.d <= 2048);
+  if (warp) {
+    const int64_t grid = ceil_div(A.rows, 4);
+    if (grid >= (1ll << 31)) return cudaErrorInvalidValue;
+    const unsigned g = (unsigned)grid;
+    if (!vec)
+      A.d <= 1024 ? layer_norm_warp_kernel<E, 1, 32><<<g, 128, 0, s>>>(A)
+                  : layer_norm_warp_kernel<E, 1, 64><<<g, 128, 0, s>>>(A);
+    else if (vecs <= 128)
+      layer_norm_warp_kernel<E, V, 4><<<g, 128, 0, s>>>(A);
+    else if (vecs <= 256)
+      layer_norm_warp_kernel<E, V, 8><<<g, 128, 0, s>>>(A);
+    else
+      layer_norm_warp_kernel<E, V, 16><<<g, 128, 0, s>>>(A);
+  } else if (vec && vecs > 512) {
+    const Wide w = wide_for(A.d, V);
+    const int grid = (int)(A.rows < MOST ? A.rows : MOST);
+    if (w.nv == 1)
+      layer_norm_wide_kernel<E, 1, 1024><<<grid, w.nt, 0, s>>>(A);
+    else if (w.nv == 2)
+      layer_norm_wide_kernel<E, 2, 1024><<<grid, w.nt, 0, s>>>(A);
+    else if constexpr (sizeof(E) == 4)   // 16-bit rows end at two vectors
+      layer_norm_wide_kernel<E, 4, 1024><<<grid, w.nt, 0, s>>>(A);
+  } else {
+    const bool wide = A.tpr > 32;
+    const int nt = wide ? A.tpr : NT;
+    const int64_t need = ceil_div(A.rows, nt / A.tpr);
+    const int grid = (int)(need < MOST ? need : MOST);
+    if (vec)
+      layer_norm_kernel<E, V, 0><<<grid, nt, 0, s>>>(A);
+    else if (wide)
+      layer_norm_kernel<E, 1, 1024><<<grid, nt, 0, s>>>(A);
+    else
+      layer_norm_kernel<E, 1, 0><<<grid, nt, 0, s>>>(A);
+  }
   count_launch();
   return cudaGetLastError();
+}
+
+template <typename E, int NV, int MAXW>
+cudaError_t launch_ring(const NormArgs& A, const Ring& r, int grid, cudaStream_t s) {
+  auto kern = layer_norm_ring_backward_kernel<E, NV, MAXW>;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)r.smem);
+  if (e != cudaSuccess) return e;
+  kern<<<grid, r.warps * 32, r.smem, s>>>(A, r.stages);
+  return cudaSuccess;
 }
 
 template <typename E>
 cudaError_t norm_backward_t(NormArgs& A, bool vec, int grid, cudaStream_t s) {
   constexpr int V = 16 / sizeof(E);
-  const bool wide = A.tpr > 32;
-  const int nt = wide ? A.tpr : NT;
-  const size_t sm = wide ? 0 : (size_t)nt * VALS * sizeof(float);   // 16 KB
-  if (vec)
-    wide ? layer_norm_backward_kernel<E, V, true><<<grid, nt, sm, s>>>(A)
-         : layer_norm_backward_kernel<E, V, false><<<grid, nt, sm, s>>>(A);
-  else
-    wide ? layer_norm_backward_kernel<E, 1, true><<<grid, nt, sm, s>>>(A)
-         : layer_norm_backward_kernel<E, 1, false><<<grid, nt, sm, s>>>(A);
+  if (vec && ring_rows(A.d, V)) {
+    const Ring r = ring_for(A.d, sizeof(E));
+    cudaError_t e;
+    if (A.d <= 1024)
+      e = launch_ring<E, 32 / V, 12>(A, r, grid, s);
+    else
+      e = launch_ring<E, 64 / V, 8>(A, r, grid, s);
+    if (e != cudaSuccess) return e;
+  } else if (vec && wide_rows(A.d, V)) {
+    const Wide w = wide_for(A.d, V);
+    if (w.nv == 1 && w.nt <= 512)
+      layer_norm_wide_backward_kernel<E, 1, 1, 512, true><<<grid, w.nt, 0, s>>>(A);
+    else if (w.nv == 1)
+      layer_norm_wide_backward_kernel<E, 1, 1, 1024, false><<<grid, w.nt, 0, s>>>(A);
+    else if (w.nv == 2)
+      layer_norm_wide_backward_kernel<E, 1, 2, 1024, false><<<grid, w.nt, 0, s>>>(A);
+    else if constexpr (sizeof(E) == 4)
+      layer_norm_wide_backward_kernel<E, 1, 4, 1024, false><<<grid, w.nt, 0, s>>>(A);
+  } else {
+    const bool wide = A.tpr > 32;
+    const int nt = wide ? A.tpr : NT;
+    const size_t sm = wide ? 0 : (size_t)nt * VALS * sizeof(float);   // 16 KB
+    if (vec)
+      layer_norm_backward_kernel<E, V, 0><<<grid, nt, sm, s>>>(A);
+    else if (A.tpr > 256)
+      layer_norm_backward_kernel<E, 1, 1024><<<grid, nt, sm, s>>>(A);
+    else if (wide)
+      layer_norm_backward_kernel<E, 1, 256><<<grid, nt, sm, s>>>(A);
+    else
+      layer_norm_backward_kernel<E, 1, 0><<<grid, nt, sm, s>>>(A);
+  }
   count_launch();
   return cudaGetLastError();
 }
 
+// Blocks of the gradient's row pass: as many as are resident at once.
+int backward_blocks(int64_t rows, int d, int v, bool vec) {
+  int64_t need, per_sm;
+  if (vec && ring_rows(d, v)) {
+    need = ceil_div(rows, ring_for(d, 16 / v).warps);
+    per_sm = 1;
+  } else if (vec && wide_rows(d, v)) {
+    const Wide w = wide_for(d, v);
+    need = ceil_div(rows, w.r);
+    per_sm = w.nt <= 256 ? 512 / w.nt : 1;
+  } else {
+    const int tpr = norm_tpr(d), nt = tpr > 32 ? tpr : NT;
+    need = ceil_div(rows, nt / tpr);
+    per_sm = nt <= 256 ? 512 / nt : 1;
+  }
+  const int64_t cap = per_sm * sm_count();
+  return (int)(need < cap ? need : cap);
+}
+
 }  // namespace
 
-int norm_backward_blocks(int64_t rows, int d) {
-  const int tpr = norm_tpr(d), nt = tpr > 32 ? tpr : NT;
-  const int64_t need = (rows + nt / tpr - 1) / (nt / tpr);
-  const int64_t cap = (int64_t)sm_count() * (nt >= 1024 ? 1 : nt >= 512 ? 1 : 512 / nt);
-  return (int)(need < cap ? need : cap);
+// The most that any alignment of the call's tensors takes.
+int norm_backward_blocks(int64_t rows, int d, int dtype) {
+  const int v = dtype == MEMLAYER_F32 ? 4 : 8;
+  const int a = backward_blocks(rows, d, v, true), b = backward_blocks(rows, d, v, false);
+  return a > b ? a : b;
 }
 
 cudaError_t launch_layer_norm(const memlayer_norm_config& c, const memlayer_norm_args& a, cudaStream_t s) {
@@ -338,7 +1032,7 @@ cudaError_t launch_layer_norm(const memlayer_norm_config& c, const memlayer_norm
   A.sum = a.sum;
   const int v = c.dtype == MEMLAYER_F32 ? 4 : 8;
   const bool vec = c.d_model % v == 0 && a.x_stride % v == 0 && (!a.residual || a.residual_stride % v == 0) &&
-                   al16(a.x) && al16(a.residual) && al16(a.y) && al16(a.sum);
+                   al16(a.x) && al16(a.residual) && al16(a.y) && al16(a.sum) && al16(a.scale) && al16(a.bias);
   switch (c.dtype) {
     case MEMLAYER_F16: return norm_forward_t<__half>(A, vec, s);
     case MEMLAYER_BF16: return norm_forward_t<__nv_bfloat16>(A, vec, s);
@@ -347,7 +1041,7 @@ cudaError_t launch_layer_norm(const memlayer_norm_config& c, const memlayer_norm
 }
 
 cudaError_t launch_layer_norm_backward(const memlayer_norm_config& c, const memlayer_norm_grads& g, float* part,
-                                       cudaStream_t s) {
+                                       int* err, cudaStream_t s) {
   NormArgs A{};
   A.rows = c.rows;
   A.d = c.d_model;
@@ -363,11 +1057,12 @@ cudaError_t launch_layer_norm_backward(const memlayer_norm_config& c, const meml
   A.scale = g.scale;
   A.dx = g.dx;
   A.part = part;
+  A.err = err;
   const int v = c.dtype == MEMLAYER_F32 ? 4 : 8;
   const bool vec = c.d_model % v == 0 && g.x_stride % v == 0 && g.dy_stride % v == 0 &&
                    (!g.dresidual || g.dresidual_stride % v == 0) && al16(g.x) && al16(g.dy) && al16(g.dresidual) &&
-                   al16(g.dx);
-  const int grid = norm_backward_blocks(c.rows, c.d_model);
+                   al16(g.dx) && al16(g.scale);
+  const int grid = backward_blocks(c.rows, c.d_model, v, vec);
   cudaError_t e = cudaSuccess;
   if (grid > 0) switch (c.dtype) {
       case MEMLAYER_F16: e = norm_backward_t<__half>(A, vec, grid, s); break;
@@ -375,7 +1070,7 @@ cudaError_t launch_layer_norm_backward(const memlayer_norm_config& c, const meml
       default: e = norm_backward_t<float>(A, vec, grid, s); break;
     }
   if (e != cudaSuccess) return e;
-  layer_norm_params_kernel<<<(2 * c.d_model + 31) / 32, 256, 0, s>>>(part, grid, c.d_model, g.dscale, g.dbias);
+  layer_norm_params_kernel<<<(2 * c.d_model + 31) / 32, 1024, 0, s>>>(part, grid, c.d_model, g.dscale, g.dbias, err);
   count_launch();
   return cudaGetLastError();
 }

@@ -86,7 +86,8 @@ int32_t memlayer_layer_norm_backward_workspace_size(const memlayer_norm_config* 
   const int st = check_norm(cfg);
   if (st) return st;
   if (!bytes) return MEMLAYER_ERR_BAD_POINTER;
-  *bytes = (size_t)norm_backward_blocks(cfg->rows, cfg->d_model) * 2 * cfg->d_model * sizeof(float);
+  // the head holds the status word
+  *bytes = 512 + (size_t)norm_backward_blocks(cfg->rows, cfg->d_model, cfg->dtype) * 2 * cfg->d_model * sizeof(float);
   return MEMLAYER_OK;
 }
 
@@ -104,8 +105,9 @@ int32_t memlayer_layer_norm_backward(const memlayer_norm_config* cfg, const meml
       !aligned(g->dbias, 4))
     return MEMLAYER_ERR_BAD_POINTER;
   if (cfg->rows > 0 && (!g->dx || !aligned(g->dx, es))) return MEMLAYER_ERR_BAD_POINTER;
-  if (need > 0 && (st = check_workspace(workspace, workspace_bytes, need))) return st;
-  return cuda_status(launch_layer_norm_backward(*cfg, *g, (float*)workspace, (cudaStream_t)stream));
+  if ((st = check_workspace(workspace, workspace_bytes, need))) return st;
+  char* ws = (char*)workspace;
+  return cuda_status(launch_layer_norm_backward(*cfg, *g, (float*)(ws + 512), (int*)(ws + 256), (cudaStream_t)stream));
 }
 
 int32_t memlayer_cross_entropy_workspace_size(const memlayer_loss_config* cfg, int32_t backward, size_t* bytes) {
@@ -142,7 +144,7 @@ int32_t memlayer_cross_entropy_backward(const memlayer_loss_config* cfg, const m
   return cuda_status(launch_loss_backward(*cfg, *a, *g, (char*)workspace, (cudaStream_t)stream));
 }
 
-int32_t memlayer_cross_entropy_status(const void* workspace, int32_t* code, void* stream) {
+int32_t memlayer_train_status(const void* workspace, int32_t* code, void* stream) {
   if (!workspace || !code) return MEMLAYER_ERR_BAD_POINTER;
   int v = 0;
   if (cudaMemcpyAsync(&v, (const char*)workspace + 256, sizeof(int), cudaMemcpyDeviceToHost, (cudaStream_t)stream) !=

@@ -12,7 +12,8 @@ Activations are float32, float16 or bfloat16 CUDA tensors and results have
 their type; parameters of the norm, losses and statistics are float32.  Input
 rows may be strided (a slice of a wider tensor); other layouts are copied.
 The kernels run on the tensors' device, on ``stream`` or that device's
-current stream.
+current stream.  With ``check=True`` a call waits for its kernels and raises
+where they recorded a failure.
 """
 
 from __future__ import annotations
@@ -35,20 +36,20 @@ def _on_tensor_device(fn):
     def wrapped(first, *args, stream: Optional[torch.cuda.Stream] = None, **kw):
         if not isinstance(first, torch.Tensor) or not first.is_cuda:
             raise TypeError(f"{fn.__name__}: the first argument must be a CUDA tensor (no CPU path)")
-        if stream is not None:
-            if stream.device != first.device:
-                raise ValueError("stream belongs to another device than the tensors")
-            with torch.cuda.stream(stream):
-                return fn(first, *args, **kw)
-        if first.get_device() != torch.cuda.current_device():
+        if stream is None and first.get_device() == torch._C._cuda_getDevice():
+            return fn(first, *args, **kw)
+        if stream is None:
             with torch.cuda.device(first.device):
                 return fn(first, *args, **kw)
-        return fn(first, *args, **kw)
+        if stream.device != first.device:
+            raise ValueError("stream belongs to another device than the tensors")
+        with torch.cuda.stream(stream):
+            return fn(first, *args, **kw)
     return wrapped
 
 
 def _stream(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
 def _rows(t: torch.Tensor, name: str, like: torch.Tensor) -> Tuple[torch.Tensor, int]:
@@ -86,6 +87,13 @@ def _dtype(t: torch.Tensor) -> int:
         raise TypeError(f"{t.dtype} is not supported (float32, float16 or bfloat16)") from None
 
 
+def _check_status(ws: torch.Tensor, stream: int) -> None:
+    code = C.c_int32(0)
+    L.check(L.lib().memlayer_train_status(ws.data_ptr(), C.byref(code), stream), "memlayer_train_status")
+    if code.value:
+        raise L.DeviceError(f"device status {code.value}: {L.DEVICE_ERRORS.get(code.value, 'unknown')}")
+
+
 @_on_tensor_device
 def layer_norm(x: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor, *,
                residual: Optional[torch.Tensor] = None, eps: float = 1e-6):
@@ -101,8 +109,8 @@ def layer_norm(x: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor, *,
     xr, ldx = _rows(x, "x", x)
     rr, ldr = (None, 0) if residual is None else _rows(residual, "residual", x)
     sc, bi = _vector(scale, "scale", d, x), _vector(bias, "bias", d, x)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    total = None if rr is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = torch.empty_like(xr, memory_format=torch.contiguous_format)
+    total = None if rr is None else torch.empty_like(y)
     cfg = L.MemlayerNormConfig(x.numel() // d if d else 0, d, code, eps)
     a = L.MemlayerNormArgs(xr.data_ptr(), ldx, None if rr is None else rr.data_ptr(), ldr, sc.data_ptr(),
                            bi.data_ptr(), y.data_ptr(), None if total is None else total.data_ptr())
@@ -112,7 +120,7 @@ def layer_norm(x: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor, *,
 
 @_on_tensor_device
 def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, scale: torch.Tensor, *,
-                        dresidual: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                        dresidual: Optional[torch.Tensor] = None, eps: float = 1e-6, check: bool = False,
                         ) -> Tuple[torch.Tensor, Dict[str, torch.Tensor]]:
     """Gradients of ``sum(dy * layer_norm(x, scale, bias))``: ``(dx, {"scale",
     "bias"})``.  ``x`` is the forward's normalised input (its sum when it had
@@ -126,7 +134,7 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, scale: torch.Tensor, 
     xr, ldx = _rows(x, "x", dy)
     rr, ldr = (None, 0) if dresidual is None else _rows(dresidual, "dresidual", dy)
     sc = _vector(scale, "scale", d, dy)
-    dx = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device)
+    dx = torch.empty_like(g, memory_format=torch.contiguous_format)
     dp = torch.empty(2, d, dtype=torch.float32, device=dy.device)
     cfg = L.MemlayerNormConfig(dy.numel() // d if d else 0, d, code, eps)
     nb = C.c_size_t()
@@ -135,8 +143,11 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, scale: torch.Tensor, 
     ws = _workspace(nb.value, dy.device)
     a = L.MemlayerNormGrads(g.data_ptr(), ldg, xr.data_ptr(), ldx, None if rr is None else rr.data_ptr(), ldr,
                             sc.data_ptr(), dx.data_ptr(), dp.data_ptr(), dp.data_ptr() + 4 * d)
-    L.check(L.lib().memlayer_layer_norm_backward(C.byref(cfg), C.byref(a), ws.data_ptr(), nb.value, _stream(dy)),
+    s = _stream(dy)
+    L.check(L.lib().memlayer_layer_norm_backward(C.byref(cfg), C.byref(a), ws.data_ptr(), nb.value, s),
             "memlayer_layer_norm_backward")
+    if check:
+        _check_status(ws, s)
     return dx, {"scale": dp[0], "bias": dp[1]}
 
 
@@ -170,14 +181,6 @@ def _loss_workspace(cfg, backward: int, device):
     return _workspace(nb.value, device), nb.value
 
 
-def _check_loss_status(ws: torch.Tensor, stream: int) -> None:
-    code = C.c_int32(0)
-    L.check(L.lib().memlayer_cross_entropy_status(ws.data_ptr(), C.byref(code), stream),
-            "memlayer_cross_entropy_status")
-    if code.value:
-        raise L.DeviceError(f"device status {code.value}: {L.DEVICE_ERRORS.get(code.value, 'unknown')}")
-
-
 @_on_tensor_device
 def linear_cross_entropy(h: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, *, ignore_index: int = -100,
                          check: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -185,8 +188,7 @@ def linear_cross_entropy(h: torch.Tensor, weight: torch.Tensor, targets: torch.T
     ``targets``, without storing them: ``(loss, lse)``, float32 of the shape
     of ``targets``, ``lse`` being log sum exp of the logits.  A token whose
     target is ``ignore_index`` has loss 0; any other target outside the
-    vocabulary gives NaN, and raises with ``check=True`` (which waits for the
-    call)."""
+    vocabulary gives NaN, and raises with ``check=True``."""
     cfg, hr, ldh, wr, ldw, t = _loss_args(h, weight, targets, ignore_index)
     loss = torch.empty(t.shape, dtype=torch.float32, device=h.device)
     lse = torch.empty_like(loss)
@@ -195,7 +197,7 @@ def linear_cross_entropy(h: torch.Tensor, weight: torch.Tensor, targets: torch.T
     s = _stream(h)
     L.check(L.lib().memlayer_cross_entropy(C.byref(cfg), C.byref(a), ws.data_ptr(), nb, s), "memlayer_cross_entropy")
     if check:
-        _check_loss_status(ws, s)
+        _check_status(ws, s)
     return loss, lse
 
 
@@ -212,8 +214,8 @@ def linear_cross_entropy_backward(h: torch.Tensor, weight: torch.Tensor, targets
     n = t.numel()
     ls, dl = _vector(lse, "lse", n, h), _vector(dloss, "dloss", n, h)
     de = None if dlse is None else _vector(dlse, "dlse", n, h)
-    dh = torch.empty(h.shape, dtype=h.dtype, device=h.device)
-    dw = torch.empty(weight.shape, dtype=h.dtype, device=h.device)
+    dh = torch.empty_like(hr, memory_format=torch.contiguous_format)
+    dw = torch.empty_like(wr, memory_format=torch.contiguous_format)
     ws, nb = _loss_workspace(cfg, 1, h.device)
     a = L.MemlayerLossArgs(hr.data_ptr(), ldh, wr.data_ptr(), ldw, t.data_ptr(), None, None)
     g = L.MemlayerLossGrads(ls.data_ptr(), dl.data_ptr(), None if de is None else de.data_ptr(), dh.data_ptr(),
@@ -222,13 +224,14 @@ def linear_cross_entropy_backward(h: torch.Tensor, weight: torch.Tensor, targets
     L.check(L.lib().memlayer_cross_entropy_backward(C.byref(cfg), C.byref(a), C.byref(g), ws.data_ptr(), nb, s),
             "memlayer_cross_entropy_backward")
     if check:
-        _check_loss_status(ws, s)
+        _check_status(ws, s)
     return dh, dw
 
 
 @_on_tensor_device
 def orthogonalize(update: torch.Tensor, *, steps: int = 5,
-                  coefficients: Sequence[float] = (3.4445, -4.7750, 2.0315), eps: float = 1e-7) -> torch.Tensor:
+                  coefficients: Sequence[float] = (3.4445, -4.7750, 2.0315), eps: float = 1e-7,
+                  check: bool = False) -> torch.Tensor:
     """Newton-Schulz orthogonalisation of the matrices ``update [..., m, n]``
     (gradients or momenta of Dense kernels): ``X = U / (|U|_F + eps)``, then
     ``steps`` times ``X <- (a I + b X X^T + c (X X^T)^2) X``, which brings
@@ -247,6 +250,9 @@ def orthogonalize(update: torch.Tensor, *, steps: int = 5,
     L.check(L.lib().memlayer_orthogonalize_workspace_size(C.byref(cfg), C.byref(nb)),
             "memlayer_orthogonalize_workspace_size")
     ws = _workspace(nb.value, u.device)
-    L.check(L.lib().memlayer_orthogonalize(C.byref(cfg), u.data_ptr(), out.data_ptr(), ws.data_ptr(), nb.value,
-                                           _stream(u)), "memlayer_orthogonalize")
+    s = _stream(u)
+    L.check(L.lib().memlayer_orthogonalize(C.byref(cfg), u.data_ptr(), out.data_ptr(), ws.data_ptr(), nb.value, s),
+            "memlayer_orthogonalize")
+    if check:
+        _check_status(ws, s)
     return out

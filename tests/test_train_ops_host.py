@@ -148,7 +148,7 @@ def test_loss_workspace_refused():
                   lib.memlayer_cross_entropy(C.byref(c), C.byref(loss_args()), ws, size, None))
             assert st == L.ERR_WORKSPACE
     code = C.c_int32()
-    assert lib.memlayer_cross_entropy_status(None, C.byref(code), None) == L.ERR_BAD_POINTER
+    assert lib.memlayer_train_status(None, C.byref(code), None) == L.ERR_BAD_POINTER
 
 
 def test_loss_workspace_does_not_hold_the_logits():
