@@ -4,6 +4,7 @@
 // whose rows TMA cannot address.
 #include <cudaTypedefs.h>
 
+#include <atomic>
 #include <mutex>
 
 #include "gemm16.cuh"
@@ -128,10 +129,24 @@ PFN_cuTensorMapEncodeTiled_v12000 encode16_fn() {
 namespace g16 {
 
 int device_sms() {
-  int dev = 0, sms = 148;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  static std::atomic<int> known[64];       // by device; 0: not asked yet
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 148;   // sizes can be asked for without a GPU
+  if (dev < 64 && (sms = known[dev].load(std::memory_order_relaxed))) return sms;
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+  if (dev < 64) known[dev].store(sms, std::memory_order_relaxed);
   return sms;
+}
+
+cudaError_t allow_smem(const void* kernel, std::atomic<uint64_t>* done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (bit && (done->load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_LIMIT);
+  if (e == cudaSuccess) done->fetch_or(bit, std::memory_order_relaxed);
+  return e;
 }
 
 cudaError_t make_operand(CUtensorMap* map, const void* base, int64_t rows, int64_t k, int64_t pitch, bool mn,

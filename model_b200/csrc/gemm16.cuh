@@ -34,6 +34,8 @@
 // Every mbarrier wait is bounded.
 #pragma once
 
+#include <atomic>
+
 #include "tc_common.cuh"
 
 namespace ml {
@@ -66,7 +68,9 @@ struct Prod {
   int m_tiles, n_tiles, splits, batch;
   int kq, kq_total;
   uint32_t amn, bmn;                      // operand is MN-major
-  __host__ __device__ int total() const { return m_tiles * n_tiles * splits * batch; }
+  int tri;                                // a symmetric result: only the tiles mt >= nt (square tiles)
+  __host__ __device__ int tiles() const { return tri ? m_tiles * (m_tiles + 1) / 2 : m_tiles * n_tiles; }
+  __host__ __device__ int total() const { return tiles() * splits * batch; }
 };
 
 // The tiles of one launch, over `clusters` clusters (CTAs or pairs).
@@ -115,10 +119,18 @@ struct Sched {
       t.q = 1;
     }
     const Prod& p = prod[t.q];
-    t.mt = lin % p.m_tiles;
-    lin /= p.m_tiles;
-    t.nt = lin % p.n_tiles;
-    lin /= p.n_tiles;
+    const int at = lin % p.tiles();
+    lin /= p.tiles();
+    if (p.tri) {
+      int r = (int)((sqrtf(8.f * at + 1.f) - 1.f) * 0.5f);
+      while ((r + 1) * (r + 2) / 2 <= at) ++r;
+      while (r * (r + 1) / 2 > at) --r;
+      t.mt = r;
+      t.nt = at - r * (r + 1) / 2;
+    } else {
+      t.mt = at % p.m_tiles;
+      t.nt = at / p.m_tiles;
+    }
     t.ks = lin % p.splits;
     t.z = lin / p.splits;
     return t;
@@ -271,6 +283,10 @@ __device__ __forceinline__ void bulk_store(const CUtensorMap* map, uint32_t src,
   asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
 
+__device__ __forceinline__ void st_shared16(uint32_t at, uint32_t a) {
+  asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"((uint16_t)a) : "memory");
+}
+
 __device__ __forceinline__ void st_shared(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
@@ -293,6 +309,15 @@ __device__ __forceinline__ uint32_t at16(uint32_t buf, int r, int c) {
 }
 __device__ __forceinline__ uint32_t at32(uint32_t buf, int r, int c) {
   return buf + r * 128 + (((c >> 2) ^ (r & 7)) << 4) + (c & 3) * 4;
+}
+
+// The calling lane's row of 32 16-bit values as a column of the block (its transpose).
+__device__ __forceinline__ void stage16_transposed(uint32_t buf, int lane, const uint32_t (&h)[16]) {
+#pragma unroll
+  for (int c = 0; c < 16; ++c) {
+    st_shared16(at16(buf, 2 * c, lane), h[c]);
+    st_shared16(at16(buf, 2 * c + 1, lane), h[c] >> 16);
+  }
 }
 
 // The calling lane's row of 32 float32 values staged in the output's type.
@@ -346,7 +371,28 @@ __device__ __forceinline__ void copy_rows(int dtype, uint32_t buf, void* out, in
   }
 }
 
-// A segment's columns (64 or 128) added to a thread's sums.  They have to
+// Two matrices of 16-bit pieces (hi, lo): each half of the staging buffer is
+// written as soon as the store that last used it has been read, so one store
+// is always in flight.
+__device__ __forceinline__ void store_pieces(const CUtensorMap* map, uint32_t buf, const uint32_t (&h)[16],
+                                             const uint32_t (&l)[16], int x, int y, int z, bool on,
+                                             bool transposed = false) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    if (lane == 0) bulk_wait<1, true>();
+    __syncwarp();
+    if (transposed)
+      stage16_transposed(buf + q * 2048, lane, q ? l : h);
+    else
+      stage16(buf + q * 2048, lane, q ? l : h);
+    tc::fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0 && on) bulk_store(map + q, buf + q * 2048, x, y, z, false);
+  }
+}
+
+// A segment's columns (32, 64 or 128) added to a thread's sums.  They have to
 // stay in registers (hence the redistribution of the CTA's): spilled, a
 // segment's drain took 4,000 to 6,000 cycles instead of 700.
 __device__ __forceinline__ void add_segment(uint32_t taddr, float (&sum)[128], int cols, int sg) {
@@ -355,7 +401,7 @@ __device__ __forceinline__ void add_segment(uint32_t taddr, float (&sum)[128], i
     if (c >= cols) break;
     uint32_t v[32], w[32];
     tc::tmem_ld32(taddr + c, v);
-    tc::tmem_ld32(taddr + c + 32, w);
+    tc::tmem_ld32(taddr + (cols > 32 ? c + 32 : c), w);
     tc::tmem_wait_ld();
     if (sg == 0) {
 #pragma unroll
@@ -397,6 +443,12 @@ struct Unscale {
   __device__ __forceinline__ float operator()(float x) const { return x * a * b; }
 };
 
+// Programmatic dependent launch: a kernel may start while the one before it
+// in the stream still runs, up to the wait; it sees all of that kernel's (and,
+// as each of them waits, every earlier one's) results after it.
+__device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void allow_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // ---- the kernel --------------------------------------------------------------------
 __host__ __device__ inline uint32_t a_bytes() { return 128 * 128; }                  // one piece, one stage, one CTA
 __host__ __device__ inline uint32_t b_bytes(int BN, int cg) { return (uint32_t)(BN / cg) * 128; }
@@ -437,6 +489,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem_base = ctl->tmem_base;
+  allow_next();
+  wait_previous();
 
   if (warp < EPI_WARPS) {
     // kSum keeps 128 sums a thread: 384 x 168 registers dealt out again, 256 x 224 + 128 x 56
@@ -642,6 +696,8 @@ inline int smem_stages(int BN, int cg, int pa, int pb, bool store) {
 }
 
 int device_sms();
+// Lets `kernel` use all of an SM's shared memory, once per device (`done`: its devices so far).
+cudaError_t allow_smem(const void* kernel, std::atomic<uint64_t>* done);
 
 template <class EPI, int CG, int PA, int PB>
 cudaError_t launch_one(const Maps& maps, Sched S, const typename EPI::Args& ea, int* err, cudaStream_t s) {
@@ -649,19 +705,22 @@ cudaError_t launch_one(const Maps& maps, Sched S, const typename EPI::Args& ea, 
   const size_t smem = 1024 + CTL_BYTES + (size_t)S.stages * (PA * a_bytes() + PB * b_bytes(S.BN, CG)) +
                       (EPI::kStore ? EPI_WARPS * STAGING : 0);
   auto kern = gemm16_kernel<EPI, CG, PA, PB>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static std::atomic<uint64_t> done{0};
+  cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), &done);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(S.clusters * CG);
   cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = CG;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   e = cudaLaunchKernelEx(&cfg, kern, maps, S, ea, err);
   count_launch();
   return e != cudaSuccess ? e : cudaGetLastError();

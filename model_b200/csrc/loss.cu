@@ -310,19 +310,18 @@ struct EpiGrad {
           h[j] = *reinterpret_cast<const uint32_t*>(&u);
         }
       }
-      // the halves of the staging buffer: hi and lo, or this block and the one before
       const int lane = threadIdx.x & 31;
-      const uint32_t b0 = buf + (PIECES == 2 ? 0 : turn * 2048);
-      turn ^= 1;
-      if (lane == 0) g16::bulk_wait<PIECES == 2 ? 0 : 1, true>();
-      __syncwarp();
-      g16::stage16(b0, lane, h);
-      if constexpr (PIECES == 2) g16::stage16(b0 + 2048, lane, o);
-      tc::fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0 && on) {           // lane 0 has the block's first row
-        g16::bulk_store(&A.out[0], b0, col0 + cc, (int)row, 0, false);
-        if constexpr (PIECES == 2) g16::bulk_store(&A.out[1], b0 + 2048, col0 + cc, (int)row, 0, false);
+      if constexpr (PIECES == 2) {
+        g16::store_pieces(A.out, buf, h, o, col0 + cc, (int)row, 0, on);   // lane 0 has the block's first row
+      } else {                         // the halves of the staging buffer in turn
+        const uint32_t b0 = buf + turn * 2048;
+        turn ^= 1;
+        if (lane == 0) g16::bulk_wait<1, true>();
+        __syncwarp();
+        g16::stage16(b0, lane, h);
+        tc::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0 && on) g16::bulk_store(&A.out[0], b0, col0 + cc, (int)row, 0, false);
       }
     }
   }

@@ -11,7 +11,10 @@
 // epilogue reads a matrix: the first product's epilogue writes P and
 // R = b I + c P, the second's a I + R P, the third's the next X (the output's
 // type in the last step).  Majors instead of transposes: the m > n products
-// read X along its other index.
+// read X along its other index.  The first two are symmetric: only the tiles
+// on and below the diagonal are computed, the epilogue writes the others as
+// their transposes.  A long k with few tiles is cut into slices, whose float32
+// partials a small kernel adds.
 //
 // Entries of X, P, R and Q are bounded by their singular values, which the
 // host bounds for the given coefficients before it launches (the usual
@@ -41,7 +44,7 @@ inline int seg_for(int64_t K) { return K > 512 ? 2 : 1; }
 constexpr float SCALE = 4096.f, BOUND = 15.f;   // 15 x 2^12 < 65504
 
 // ---- |U|_F and the pieces of X_0 -----------------------------------------------
-constexpr int NORM_CHUNKS = 256;
+constexpr int NORM_CHUNKS = 1024;
 
 template <typename E> __device__ __forceinline__ float up_f(E x);
 template <> __device__ __forceinline__ float up_f(float x) { return x; }
@@ -54,17 +57,36 @@ template <typename E>
 __global__ void __launch_bounds__(256) orth_norm_kernel(const E* __restrict__ u, int64_t n, int chunks,
                                                         double* __restrict__ part) {
   __shared__ double red[8];
-  const int64_t per = ((n + chunks - 1) / chunks + 7) / 8 * 8;
+  // whole 16-byte vectors per chunk; a matrix that starts or ends inside one
+  // goes by single elements
+  constexpr int V = 16 / sizeof(E);
+  const int64_t per = ((n + chunks - 1) / chunks + V - 1) / V * V;
   const int64_t b = blockIdx.x * per, e = b + per < n ? b + per : n;
   const E* x = u + blockIdx.y * n;
   double s[4] = {0., 0., 0., 0.};
-  for (int64_t i = b + threadIdx.x; i < e; i += 1024) {
+  auto take = [&](int j, float f) {
+    const double v = f;
+    s[j & 3] = fma(v, v, s[j & 3]);
+  };
+  if (((reinterpret_cast<uintptr_t>(x) | (uintptr_t)(n * sizeof(E))) & 15) == 0) {
+    struct alignas(16) Vec { E v[V]; };
+    for (int64_t i = b + threadIdx.x * V; i < e; i += 2 * 256 * V) {
+      Vec p = *reinterpret_cast<const Vec*>(x + i), q{};
+      const bool two = i + 256 * V < e;
+      if (two) q = *reinterpret_cast<const Vec*>(x + i + 256 * V);
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (i + j * 256 < e) {
-        const double v = up_f(x[i + j * 256]);
-        s[j] = fma(v, v, s[j]);
+      for (int j = 0; j < V; ++j) take(j, up_f(p.v[j]));
+      if (two) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) take(j, up_f(q.v[j]));
       }
+    }
+  } else {
+    for (int64_t i = b + threadIdx.x; i < e; i += 1024) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (i + j * 256 < e) take(j, up_f(x[i + j * 256]));
+    }
   }
   double t = (s[0] + s[1]) + (s[2] + s[3]);
 #pragma unroll
@@ -118,7 +140,8 @@ struct PolyArgs {
   int N;
   int two;                             // a second output follows
   float s[2], diag[2];                 // output q = s[q] acc + diag[q] I (in scaled units)
-  int type;                            // -1: pieces; else memlayer_dtype of the plain output
+  int type;                            // -1: pieces; -2: float32 partials of k slices (out[0][0]); else
+                                       // memlayer_dtype of the plain output
   int tma;                             // the plain output's rows are 16 bytes apart
   void* plain;                         // [batch][M][N]
 };
@@ -134,8 +157,7 @@ struct EpiPoly {
     turn = 0;
   }
   static __device__ __forceinline__ void pieces(const CUtensorMap* map, uint32_t buf, const uint32_t (&v)[32],
-                                                float s, float diag, int at, int col, int row0, int z) {
-    const int lane = threadIdx.x & 31;
+                                                float s, float diag, int at, int col, int row0, int z, bool mirror) {
     uint32_t h[16], l[16];
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
@@ -147,16 +169,17 @@ struct EpiPoly {
       h[j] = *reinterpret_cast<const uint32_t*>(&a);
       l[j] = *reinterpret_cast<const uint32_t*>(&b);
     }
+    g16::store_pieces(map, buf, h, l, col, row0, z, true);
+    if (mirror) g16::store_pieces(map, buf, h, l, row0, col, z, true, true);
+  }
+  __device__ __forceinline__ void partial(const Args& A, uint32_t (&v)[32], int row0, int col, int z) {
+    const int lane = threadIdx.x & 31;
     if (lane == 0) g16::bulk_wait<0, true>();
     __syncwarp();
-    g16::stage16(buf, lane, h);
-    g16::stage16(buf + 2048, lane, l);
+    g16::stage32(buf, lane, v);
     tc::fence_proxy_async_smem();
     __syncwarp();
-    if (lane == 0) {
-      g16::bulk_store(map, buf, col, row0, z, false);
-      g16::bulk_store(map + 1, buf + 2048, col, row0, z, false);
-    }
+    if (lane == 0) g16::bulk_store(&A.out[0][0], buf, col, row0, z, false);
   }
   __device__ __forceinline__ void plain(const Args& A, uint32_t (&v)[32], int64_t row0, int col, int z) {
     const int lane = threadIdx.x & 31;
@@ -198,16 +221,79 @@ struct EpiPoly {
       for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(sum[cc + j]);
       if (A.type >= 0) {
         plain(A, v, row0, col, t.z);
+      } else if (A.type == -2) {
+        partial(A, v, (int)row0, col, t.ks * S.prod[0].batch + t.z);
       } else {
         const int64_t d = row - col;                         // the diagonal's column in this block
         const int at = d >= 0 && d < 32 ? (int)d : -1;
-        pieces(A.out[0], buf, v, A.s[0], A.diag[0], at, col, (int)row0, t.z);
-        if (A.two) pieces(A.out[1], buf, v, A.s[1], A.diag[1], at, col, (int)row0, t.z);
+        const bool mirror = S.prod[0].tri && t.mt > t.nt;
+        for (int q = 0; q < 1 + A.two; ++q)
+          pieces(A.out[q], buf, v, A.s[q], A.diag[q], at, col, (int)row0, t.z, mirror);
       }
     }
   }
   __device__ __forceinline__ void end(const Args&, const Sched&, int) {}
 };
+
+// The slices' partials of a symmetric product [slices][batch][s][lds], added in
+// slice order, to its outputs' pieces: a 32 x 32 block on or below the
+// diagonal per thread block (the tiles above it were not computed), written
+// as it is and transposed.
+struct JoinArgs {
+  const float* part;
+  int slices, s, lds;
+  int64_t se;                          // entries from hi to lo
+  __half* out[2];
+  int two;
+  float sc[2], diag[2];
+};
+
+__global__ void __launch_bounds__(256) orth_join_kernel(JoinArgs A) {
+  __shared__ float t[32][33];
+  int rb = (int)((sqrtf(8.f * blockIdx.x + 1.f) - 1.f) * 0.5f);
+  while ((rb + 1) * (rb + 2) / 2 <= (int)blockIdx.x) ++rb;
+  while (rb * (rb + 1) / 2 > (int)blockIdx.x) --rb;
+  const int cb = blockIdx.x - rb * (rb + 1) / 2;
+  const int64_t one = (int64_t)A.s * A.lds, all = one * gridDim.y, z = blockIdx.y;
+  const int i = threadIdx.x >> 3, j0 = (threadIdx.x & 7) * 4;
+  // lds is a multiple of 8: four columns are inside the pitch together
+  const int r = rb * 32 + i, c = cb * 32 + j0;
+  const bool in = r < A.s && c < A.lds;
+  float x[4] = {0.f, 0.f, 0.f, 0.f};
+  if (in) {
+    const float* p = A.part + z * one + (int64_t)r * A.lds + c;
+    for (int k = 0; k < A.slices; ++k) {
+      const float4 v = *reinterpret_cast<const float4*>(p + k * all);
+      x[0] += v.x;
+      x[1] += v.y;
+      x[2] += v.z;
+      x[3] += v.w;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) t[i][j0 + j] = x[j];
+  __syncthreads();
+  auto put = [&](int row, int col, const float (&v)[4]) {
+    for (int q = 0; q < 1 + A.two; ++q) {
+      alignas(8) __half2 h[2], l[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        g16::split2(v[2 * j] * A.sc[q] + (col + 2 * j == row ? A.diag[q] : 0.f),
+                    v[2 * j + 1] * A.sc[q] + (col + 2 * j + 1 == row ? A.diag[q] : 0.f), h[j], l[j]);
+      __half* o = A.out[q] + z * one + (int64_t)row * A.lds + col;
+      *reinterpret_cast<uint2*>(o) = *reinterpret_cast<uint2*>(h);
+      *reinterpret_cast<uint2*>(o + A.se) = *reinterpret_cast<uint2*>(l);
+    }
+  };
+  if (in) put(r, c, x);
+  if (rb != cb) {
+    const int tr = cb * 32 + i, tc = rb * 32 + j0;
+    float y[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = t[j0 + j][i];
+    if (tr < A.s && tc < A.lds) put(tr, tc, y);
+  }
+}
 
 // ---- plan -----------------------------------------------------------------------
 int64_t up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
@@ -218,9 +304,43 @@ struct Plan {
   int64_t B, m, n, s;                  // s: the smaller side
   bool tall;
   int64_t ldx, lds;
-  size_t o_part, o_x[2], o_p, o_r, o_q, bytes;   // hi then lo in each
+  size_t o_part, o_x[2], o_p, o_r, o_q, o_k, bytes;   // hi then lo in each
   int64_t xe, se;                      // entries of one piece of X, of an s x s matrix
 };
+
+struct Tiling {
+  int cg, BN, tri, slices;
+};
+
+// Tile and slices of k with the least estimated time: rounds of tiles over
+// the clusters, each its stages and an epilogue, in SM cycles as measured at
+// 4096^3 (large tiles) and 256^3 (small ones); joining slices costs a small
+// kernel.  Symmetric products take square tiles on and below the diagonal, or
+// small ones everywhere (12 tiles of 128 x 128 took 176 us for 4 x 256 x 256,
+// 32 of 128 x 64 148).
+Tiling tiling(int64_t M, int64_t N, int64_t K, int64_t batch, bool symmetric) {
+  struct Shape { int cg, BN, tri; double stage, epilogue; };
+  const Shape all[4] = {{2, 256, 1, 1900, 6000}, {2, 128, 0, 1100, 4000}, {1, 128, 1, 1000, 4000}, {1, 64, 0, 750, 3000}};
+  const int64_t kq = up(K, g16::BK) / g16::BK;
+  Tiling best{1, 64, 0, 1};
+  double least = 1e300;
+  for (const Shape& t : all) {
+    if (symmetric && t.cg == 2 && !t.tri) continue;
+    const bool tri = symmetric && t.tri;
+    const int64_t mt = up(M, 128 * t.cg) / (128 * t.cg), nt = up(N, t.BN) / t.BN;
+    const int64_t tiles = (tri ? mt * (mt + 1) / 2 : mt * nt) * batch, clusters = g16::device_sms() / t.cg;
+    for (int64_t n = 1; n <= (symmetric ? kq / 4 : 1) || n == 1; n *= 2) {
+      if (n > 1 && tiles * n > clusters) break;
+      const int64_t rounds = (tiles * n + clusters - 1) / clusters, per = (kq + n - 1) / n;
+      const double cost = rounds * (per * t.stage + t.epilogue) + (n > 1 ? 8000 : 0);
+      if (cost < least) {
+        least = cost;
+        best = {t.cg, t.BN, tri, (int)n};
+      }
+    }
+  }
+  return best;
+}
 
 bool make_plan(const memlayer_orth_config& c, Plan* out) {
   Plan p{};
@@ -247,23 +367,13 @@ bool make_plan(const memlayer_orth_config& c, Plan* out) {
   p.o_p = take(2 * p.se * 2);
   p.o_r = take(2 * p.se * 2);
   p.o_q = take(2 * p.se * 2);
+  // partials of the first two products' slices
+  const int s1 = tiling(p.s, p.s, p.tall ? p.m : p.n, p.B, true).slices, s2 = tiling(p.s, p.s, p.s, p.B, true).slices;
+  const int sl = s1 > s2 ? s1 : s2;
+  if (sl > 1) p.o_k = take((int64_t)sl * p.B * p.s * p.lds * 4);
   p.bytes = off;
   *out = p;
   return true;
-}
-
-struct Tiling {
-  int cg, BN;
-};
-
-// The largest tile that still gives every cluster one; the smallest where
-// none does (few products' tiles: more SMs share the work).
-Tiling tiling(int64_t M, int64_t N, int64_t batch) {
-  const int sms = g16::device_sms();
-  const Tiling all[3] = {{2, 256}, {2, 128}, {1, 128}};
-  for (const Tiling& t : all)
-    if (up(M, 128 * t.cg) / (128 * t.cg) * (up(N, t.BN) / t.BN) * batch >= sms / t.cg) return t;
-  return all[2];
 }
 
 #define OR_TRY(x)                             \
@@ -277,31 +387,62 @@ struct Mat {
   int64_t lo, ld, batch;               // batch: entries between matrices
 };
 
-// A(i, k): M rows; B(j, k): N rows; k of length K.
-cudaError_t product(const Plan& p, const Mat& a, bool amn, const Mat& b, bool bmn, int64_t M, int64_t N, int64_t K,
-                    PolyArgs& ea, int* err, cudaStream_t s) {
-  const Tiling t = tiling(M, N, p.B);
-  Maps m{};
-  for (int q = 0; q < 2; ++q) {
-    OR_TRY(g16::make_operand(&m.a[0][q], a.p + q * a.lo, M, K, a.ld, amn, 128, 0, (int)p.B, a.batch));
-    OR_TRY(g16::make_operand(&m.b[0][q], b.p + q * b.lo, N, K, b.ld, bmn, t.BN / t.cg, 0, (int)p.B, b.batch));
-  }
-  Sched S{};
-  Prod& r = S.prod[0];
-  r.m_tiles = (int)(up(M, 128 * t.cg) / (128 * t.cg));
-  r.n_tiles = (int)(up(N, t.BN) / t.BN);
-  r.splits = 1;
+// One of the three products: its tiles and the maps of its operands (built
+// once a call for each of the two buffers that X alternates between).
+struct Product {
+  Maps maps[2];
+  Sched S;
+  Tiling t;
+  int64_t M, N;
+};
+
+// A(i, k): M rows; B(j, k): N rows; k of length K.  tri: the result is symmetric.
+cudaError_t make_product(const Plan& p, const Mat (&a)[2], bool amn, const Mat (&b)[2], bool bmn, int64_t M, int64_t N,
+                         int64_t K, bool tri, int buffers, Product* out) {
+  Product& P = *out;
+  P.t = tiling(M, N, K, p.B, tri);
+  P.M = M;
+  P.N = N;
+  for (int k = 0; k < buffers; ++k)
+    for (int q = 0; q < 2; ++q) {
+      OR_TRY(g16::make_operand(&P.maps[k].a[0][q], a[k].p + q * a[k].lo, M, K, a[k].ld, amn, 128, 0, (int)p.B,
+                               a[k].batch));
+      OR_TRY(g16::make_operand(&P.maps[k].b[0][q], b[k].p + q * b[k].lo, N, K, b[k].ld, bmn, P.t.BN / P.t.cg, 0,
+                               (int)p.B, b[k].batch));
+    }
+  Prod& r = P.S.prod[0];
+  r.m_tiles = (int)(up(M, 128 * P.t.cg) / (128 * P.t.cg));
+  r.n_tiles = (int)(up(N, P.t.BN) / P.t.BN);
   r.batch = (int)p.B;
-  r.kq = r.kq_total = (int)(up(K, g16::BK) / g16::BK);
+  r.kq_total = (int)(up(K, g16::BK) / g16::BK);
+  r.kq = (r.kq_total + P.t.slices - 1) / P.t.slices;
+  r.splits = (r.kq_total + r.kq - 1) / r.kq;
   r.amn = amn;
   r.bmn = bmn;
-  S.BN = t.BN;
-  S.seg = seg_for(K);
-  g16::distribute(&S, g16::device_sms() / t.cg, 0);
-  ea.M = M;
-  ea.N = (int)N;
-  return t.cg == 2 ? g16::launch_one<EpiPoly, 2, 2, 2>(m, S, ea, err, s)
-                   : g16::launch_one<EpiPoly, 1, 2, 2>(m, S, ea, err, s);
+  r.tri = P.t.tri;
+  P.S.BN = P.t.BN;
+  P.S.seg = seg_for(K);
+  g16::distribute(&P.S, g16::device_sms() / P.t.cg, 0);
+  return cudaSuccess;
+}
+
+cudaError_t launch(const Product& P, int buffer, const PolyArgs& ea, int* err, cudaStream_t s) {
+  return P.t.cg == 2 ? g16::launch_one<EpiPoly, 2, 2, 2>(P.maps[buffer], P.S, ea, err, s)
+                     : g16::launch_one<EpiPoly, 1, 2, 2>(P.maps[buffer], P.S, ea, err, s);
+}
+
+// A symmetric product to its outputs' pieces; `raw`: the partials of its slices as an output.
+cudaError_t symmetric(const Plan& p, const Product& P, int buffer, const PolyArgs& ea, const PolyArgs& raw,
+                      __half* o0, __half* o1, char* ws, cudaStream_t s) {
+  int* err = reinterpret_cast<int*>(ws + O_ERR);
+  if (P.S.prod[0].splits == 1) return launch(P, buffer, ea, err, s);
+  OR_TRY(launch(P, buffer, raw, err, s));
+  const JoinArgs j{reinterpret_cast<float*>(ws + p.o_k), P.S.prod[0].splits, (int)p.s, (int)p.lds, p.se, {o0, o1},
+                   ea.two, {ea.s[0], ea.s[1]}, {ea.diag[0], ea.diag[1]}};
+  const int64_t nb = (p.s + 31) / 32;
+  orth_join_kernel<<<dim3((unsigned)(nb * (nb + 1) / 2), (unsigned)p.B), 256, 0, s>>>(j);
+  count_launch();
+  return cudaGetLastError();
 }
 
 template <typename E>
@@ -364,7 +505,17 @@ cudaError_t launch_orthogonalize(const memlayer_orth_config& c, const void* upda
   __half *x[2] = {reinterpret_cast<__half*>(ws + p.o_x[0]), reinterpret_cast<__half*>(ws + p.o_x[1])};
   __half *P = reinterpret_cast<__half*>(ws + p.o_p), *R = reinterpret_cast<__half*>(ws + p.o_r),
          *Q = reinterpret_cast<__half*>(ws + p.o_q);
-  const Mat MP{P, p.se, p.lds, p.s * p.lds}, MR{R, p.se, p.lds, p.s * p.lds}, MQ{Q, p.se, p.lds, p.s * p.lds};
+  const Mat X[2] = {{x[0], p.xe, p.ldx, p.m * p.ldx}, {x[1], p.xe, p.ldx, p.m * p.ldx}};
+  auto square = [&](const __half* q) { return Mat{q, p.se, p.lds, p.s * p.lds}; };
+  const Mat MP[2] = {square(P), square(P)}, MR[2] = {square(R), square(R)}, MQ[2] = {square(Q), square(Q)};
+  const int buffers = c.steps > 1 ? 2 : 1;
+  Product gram{}, poly{}, apply{};
+  OR_TRY(make_product(p, X, p.tall, X, p.tall, p.s, p.s, p.tall ? p.m : p.n, true, buffers, &gram));
+  OR_TRY(make_product(p, MR, false, MP, false, p.s, p.s, p.s, true, 1, &poly));
+  if (p.tall)
+    OR_TRY(make_product(p, X, false, MQ, false, p.m, p.n, p.n, false, buffers, &apply));
+  else
+    OR_TRY(make_product(p, MQ, false, X, true, p.m, p.n, p.m, false, buffers, &apply));
   auto pieces = [&](CUtensorMap* map, __half* q, int64_t lo, int64_t rows, int64_t cols, int64_t ld) {
     for (int i = 0; i < 2; ++i) {
       const cudaError_t e = g16::make_store(map + i, q + i * lo, rows, cols, ld, MEMLAYER_F16, p.B, rows * ld);
@@ -372,39 +523,48 @@ cudaError_t launch_orthogonalize(const memlayer_orth_config& c, const void* upda
     }
     return cudaSuccess;
   };
-  PolyArgs a1{}, a2{}, a3{};
+  auto sizes = [&](PolyArgs& a, const Product& q) {
+    a.M = q.M;
+    a.N = (int)q.N;
+    a.type = -1;
+  };
+  PolyArgs a1{}, a2{}, a3[2]{}, last{}, r1{}, r2{};
   OR_TRY(pieces(a1.out[0], P, p.se, p.s, p.s, p.lds));
   OR_TRY(pieces(a1.out[1], R, p.se, p.s, p.s, p.lds));
   OR_TRY(pieces(a2.out[0], Q, p.se, p.s, p.s, p.lds));
   // accumulators carry SCALE^2, pieces SCALE
-  a1.type = a2.type = -1;
+  sizes(a1, gram);
   a1.two = 1;
   a1.s[0] = 1.f / SCALE;
   a1.s[1] = c.c / SCALE;
   a1.diag[1] = c.b * SCALE;
+  sizes(a2, poly);
   a2.s[0] = 1.f / SCALE;
   a2.diag[0] = c.a * SCALE;
+  for (PolyArgs* r : {&r1, &r2}) {
+    const Product& q = r == &r1 ? gram : poly;
+    sizes(*r, q);
+    r->type = -2;
+    if (q.S.prod[0].splits > 1)
+      OR_TRY(g16::make_store(&r->out[0][0], ws + p.o_k, p.s, p.s, p.lds, MEMLAYER_F32, q.S.prod[0].splits * p.B,
+                             p.s * p.lds));
+  }
+  for (int k = 0; k < buffers; ++k) {
+    sizes(a3[k], apply);
+    a3[k].s[0] = 1.f / SCALE;
+    OR_TRY(pieces(a3[k].out[0], x[k], p.xe, p.m, p.n, p.ldx));
+  }
   const int64_t es = c.dtype == MEMLAYER_F32 ? 4 : 2;
+  sizes(last, apply);
+  last.type = c.dtype;
+  last.s[0] = 1.f / (SCALE * SCALE);
+  last.plain = out;
+  last.tma = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && p.n * es % 16 == 0;
+  if (last.tma) OR_TRY(g16::make_store(&last.out[0][0], out, p.m, p.n, p.n, c.dtype, p.B, p.m * p.n));
   for (int k = 0; k < c.steps; ++k) {
-    const Mat X{x[k & 1], p.xe, p.ldx, p.m * p.ldx};
-    __half* next = x[(k + 1) & 1];
-    OR_TRY(product(p, X, p.tall, X, p.tall, p.s, p.s, p.tall ? p.m : p.n, a1, err, s));
-    OR_TRY(product(p, MR, false, MP, false, p.s, p.s, p.s, a2, err, s));
-    if (k + 1 < c.steps) {
-      a3.type = -1;
-      a3.s[0] = 1.f / SCALE;
-      OR_TRY(pieces(a3.out[0], next, p.xe, p.m, p.n, p.ldx));
-    } else {
-      a3.type = c.dtype;
-      a3.s[0] = 1.f / (SCALE * SCALE);
-      a3.plain = out;
-      a3.tma = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && p.n * es % 16 == 0;
-      if (a3.tma) OR_TRY(g16::make_store(&a3.out[0][0], out, p.m, p.n, p.n, c.dtype, p.B, p.m * p.n));
-    }
-    if (p.tall)
-      OR_TRY(product(p, X, false, MQ, false, p.m, p.n, p.n, a3, err, s));
-    else
-      OR_TRY(product(p, MQ, false, X, true, p.m, p.n, p.m, a3, err, s));
+    OR_TRY(symmetric(p, gram, k & 1, a1, r1, P, R, ws, s));
+    OR_TRY(symmetric(p, poly, 0, a2, r2, Q, nullptr, ws, s));
+    OR_TRY(launch(apply, k & 1, k + 1 < c.steps ? a3[(k + 1) & 1] : last, err, s));
   }
   return cudaSuccess;
 }
