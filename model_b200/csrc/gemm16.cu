@@ -19,6 +19,8 @@ constexpr int NTH = 256;
 
 // Bits of the largest finite |x| (order of non-negative floats = order of bits).
 __global__ void __launch_bounds__(NTH) amax_kernel(AmaxArgs A) {
+  allow_next();
+  wait_previous();
   __shared__ unsigned red[NTH / 32];
   int i = 0, b = blockIdx.x;
   while (b >= A.m[i].blocks) b -= A.m[i++].blocks;
@@ -70,6 +72,8 @@ __global__ void __launch_bounds__(NTH) amax_kernel(AmaxArgs A) {
 // (16-bit source), zeros in the padding columns.
 template <typename E>
 __global__ void __launch_bounds__(NTH) pieces_kernel(PiecesArgs A) {
+  allow_next();
+  wait_previous();
   int i = 0, b = blockIdx.x;
   while (b >= A.m[i].blocks) b -= A.m[i++].blocks;
   const PiecesMat M = A.m[i];
@@ -221,9 +225,8 @@ cudaError_t launch_amax(AmaxArgs A, cudaStream_t s) {
     total += A.m[i].blocks;
   }
   if (!total) return cudaSuccess;
-  amax_kernel<<<total, NTH, 0, s>>>(A);
   count_launch();
-  return cudaGetLastError();
+  return launch_dependent(amax_kernel, dim3(total), NTH, 0, s, A);
 }
 
 cudaError_t launch_pieces(PiecesArgs A, int dtype, cudaStream_t s) {
@@ -234,12 +237,10 @@ cudaError_t launch_pieces(PiecesArgs A, int dtype, cudaStream_t s) {
     total += A.m[i].blocks;
   }
   if (!total) return cudaSuccess;
-  if (dtype == MEMLAYER_F32)
-    pieces_kernel<float><<<total, NTH, 0, s>>>(A);
-  else
-    pieces_kernel<unsigned short><<<total, NTH, 0, s>>>(A);   // 16 bits as they are
   count_launch();
-  return cudaGetLastError();
+  // 16-bit sources: their bits as they are
+  return dtype == MEMLAYER_F32 ? launch_dependent(pieces_kernel<float>, dim3(total), NTH, 0, s, A)
+                               : launch_dependent(pieces_kernel<unsigned short>, dim3(total), NTH, 0, s, A);
 }
 
 }  // namespace ml

@@ -36,6 +36,7 @@
 
 #include <atomic>
 
+#include "dependent.cuh"
 #include "tc_common.cuh"
 
 namespace ml {
@@ -442,12 +443,6 @@ struct Unscale {
   }
   __device__ __forceinline__ float operator()(float x) const { return x * a * b; }
 };
-
-// Programmatic dependent launch: a kernel may start while the one before it
-// in the stream still runs, up to the wait; it sees all of that kernel's (and,
-// as each of them waits, every earlier one's) results after it.
-__device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void allow_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // ---- the kernel --------------------------------------------------------------------
 __host__ __device__ inline uint32_t a_bytes() { return 128 * 128; }                  // one piece, one stage, one CTA

@@ -32,6 +32,8 @@ namespace ml {
 
 namespace {
 
+int64_t up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
+
 using g16::Maps;
 using g16::Prod;
 using g16::Sched;
@@ -162,16 +164,20 @@ struct EpiStats {
 // Joins the partial (maximum, sum) pairs of a row, in slot order per lane and
 // a fixed tree over the lanes.  One warp per row.
 __global__ void __launch_bounds__(256) loss_join_kernel(const float2* __restrict__ part, const float* __restrict__ zt,
-                                                        const int* __restrict__ targets, int64_t T, int V, Sched S,
-                                                        int rows_per_tile, int ignore,
+                                                        const int* __restrict__ targets, int64_t T, int V, const __grid_constant__ Sched S,
+                                                        int rows_per_tile, int blocks, int ignore,
                                                         float* __restrict__ loss, float* __restrict__ lse,
                                                         int* __restrict__ err) {
+  allow_next();
+  wait_previous();
   const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   if (row >= T) return;
-  const int mt = (int)(row / rows_per_tile), nt = S.prod[0].n_tiles;
-  const int c0 = S.owner(mt * nt), c1 = S.owner(mt * nt + nt - 1);
-  const int n = (c1 - c0 + 1) * 2;
+  int n = blocks;                      // one pair a block of the few-token kernel, else two a cluster
+  if (n == 0) {
+    const int mt = (int)(row / rows_per_tile), nt = S.prod[0].n_tiles;
+    n = (S.owner(mt * nt + nt - 1) - S.owner(mt * nt) + 1) * 2;
+  }
   float m = -INFINITY, s = 0.f;
   for (int i = lane; i < n; i += 32) {
     const float2 p = part[(int64_t)i * T + row];
@@ -202,6 +208,123 @@ __global__ void __launch_bounds__(256) loss_join_kernel(const float2* __restrict
   }
 }
 
+// ---- few float32 tokens --------------------------------------------------------------
+// Up to 16 float32 tokens: the weight is read once and everything else waits
+// for it, while the two-piece form of the tensor cores would read it twice
+// more.  A block takes 128 vocabulary entries, a thread one of them against
+// four tokens (float32 FMAs, two columns an instruction); 64 columns of the
+// block's rows at a time come through a ring of asynchronous copies, deep
+// enough for all of a 256-wide row.  16 x 256 over 16,384 entries: the call
+// takes 20 us instead of the 30 of pieces and tiles.
+constexpr int FEW = 16, FEW_V = 128, FEW_K = 64, FEW_PITCH = FEW_K + 4, FEW_STAGES = 4, FEW_M = 4;
+
+struct FewArgs {
+  const float *h, *w;
+  int64_t ldh, ldw;
+  int T, V, d;
+  const int* targets;
+  float2* part;                        // [block][T]
+  float* zt;
+  int* err;
+};
+
+__device__ __forceinline__ void copy16(float* dst, const float* src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tc::smem_u32(dst)), "l"(src), "r"(in ? 16 : 0)
+               : "memory");
+}
+
+__global__ void __launch_bounds__(FEW_V * (FEW / FEW_M)) loss_few_kernel(FewArgs A) {
+  extern __shared__ float4 few_raw[];
+  float* ws = reinterpret_cast<float*>(few_raw);                       // [stages][128][68]
+  float* hs = ws + FEW_STAGES * FEW_V * FEW_PITCH;                     // [tokens rounded up to 4][columns to 64]
+  allow_next();
+  const int t = threadIdx.x, nt = blockDim.x, v0 = blockIdx.x * FEW_V, chunks = (A.d + FEW_K - 1) / FEW_K;
+  const int cols = chunks * FEW_K, tokens = nt / FEW_V * FEW_M;
+  if (blockIdx.x == 0 && t == 0) *A.err = 0;
+  auto fetch = [&](int c) {            // 16 lanes a row; zeros past the end
+    if (c < chunks) {
+      float* st = ws + (c % FEW_STAGES) * FEW_V * FEW_PITCH;
+      const int col = c * FEW_K + (t & 15) * 4;
+      for (int r = t >> 4; r < FEW_V; r += nt >> 4) {
+        const bool in = v0 + r < A.V && col < A.d;
+        copy16(st + r * FEW_PITCH + (t & 15) * 4, in ? A.w + (int64_t)(v0 + r) * A.ldw + col : A.w, in);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  for (int e = t; e < tokens * (cols / 4); e += nt) {
+    const int m = e / (cols / 4), k = (e - m * (cols / 4)) * 4;
+    const bool in = m < A.T && k < A.d;
+    copy16(hs + m * cols + k, in ? A.h + m * A.ldh + k : A.w, in);
+  }
+#pragma unroll
+  for (int c = 0; c < FEW_STAGES - 1; ++c) fetch(c);                   // the tokens are in the first group
+  const int r = t & (FEW_V - 1), m0 = t / FEW_V * FEW_M;               // a warp's tokens are the same
+  unsigned long long acc[FEW_M] = {};                                  // (even columns, odd columns)
+  for (int c = 0; c < chunks; ++c) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(FEW_STAGES - 2) : "memory");
+    __syncthreads();                   // the chunk is in for every thread, the one before is read
+    fetch(c + FEW_STAGES - 1);
+    const ulonglong2* row =
+        reinterpret_cast<const ulonglong2*>(ws + (c % FEW_STAGES) * FEW_V * FEW_PITCH + r * FEW_PITCH);
+    const float* hk = hs + m0 * cols + c * FEW_K;
+#pragma unroll
+    for (int k4 = 0; k4 < FEW_K / 4; ++k4) {
+      const ulonglong2 w = row[k4];
+#pragma unroll
+      for (int m = 0; m < FEW_M; ++m) {
+        const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(hk + m * cols + k4 * 4);
+        asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc[m]) : "l"(w.x), "l"(x.x));
+        asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc[m]) : "l"(w.y), "l"(x.y));
+      }
+    }
+  }
+  // a token's 128 logits: one warp finds their maximum and sum
+  __syncthreads();
+  float* zs = ws;                      // [tokens][128]
+#pragma unroll
+  for (int m = 0; m < FEW_M; ++m) {
+    float a, b;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(acc[m]));
+    zs[(m0 + m) * FEW_V + r] = v0 + r < A.V ? a + b : -INFINITY;
+  }
+  __syncthreads();
+  for (int m = t >> 5; m < A.T; m += nt >> 5) {
+    const int lane = t & 31;
+    float z[FEW_V / 32];
+    float mx = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < FEW_V / 32; ++i) {
+      z[i] = zs[m * FEW_V + i * 32 + lane] * LOG2E;
+      mx = fmaxf(mx, z[i]);
+    }
+    mx = warp_max(mx);
+    const float ref = mx == -INFINITY ? 0.f : mx;
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < FEW_V / 32; ++i) s += g16::exp2_fast(z[i] - ref);
+    s = warp_sum(s);
+    if (lane == 0) {
+      A.part[(int64_t)blockIdx.x * A.T + m] = make_float2(mx, s);
+      const unsigned at = (unsigned)(A.targets[m] - v0);
+      if (at < FEW_V && v0 + (int)at < A.V) A.zt[m] = zs[m * FEW_V + at];
+    }
+  }
+}
+
+int few_threads(int64_t T) { return FEW_V * (int)((T + FEW_M - 1) / FEW_M); }
+
+size_t few_smem(int64_t T, int d) {
+  return (size_t)(FEW_STAGES * FEW_V * FEW_PITCH + up(T, FEW_M) * up(d, FEW_K)) * sizeof(float);
+}
+
+// Rows of 16-byte vectors, and the tokens fit beside the ring.
+bool few_tokens(const memlayer_loss_config& c, const memlayer_loss_args& a) {
+  auto rows16 = [](const void* p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 4 == 0; };
+  return c.dtype == MEMLAYER_F32 && c.tokens <= FEW && c.d_model % 4 == 0 && rows16(a.h, a.h_stride) &&
+         rows16(a.weight, a.weight_stride) && few_smem(c.tokens, c.d_model) <= g16::SMEM_LIMIT;
+}
+
 // ---- backward ---------------------------------------------------------------------
 // Per token: the factor of p, the factor of the one-hot target and the target
 // (-1: none); the largest of the factors' magnitudes for the scale of dz.
@@ -210,6 +333,8 @@ __global__ void __launch_bounds__(256) loss_rows_kernel(const int* __restrict__ 
                                                         const float* __restrict__ dlse, int64_t T, int V, int ignore,
                                                         float2* __restrict__ coef, int* __restrict__ tgt,
                                                         unsigned* __restrict__ amax, int* __restrict__ err) {
+  allow_next();
+  wait_previous();
   unsigned mx = 0;
   for (int64_t t = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; t < T; t += (int64_t)gridDim.x * blockDim.x) {
     const int v = targets[t];
@@ -420,6 +545,8 @@ struct EpiOut {
 // entries a thread (both buffers come 256-byte aligned or are written one by one).
 __global__ void __launch_bounds__(256) loss_slices_kernel(const float* __restrict__ P, int S, int64_t n, void* out,
                                                           int type, int vec) {
+  allow_next();
+  wait_previous();
   auto put = [&](int64_t e, float x) {
     if (type == MEMLAYER_F32)
       reinterpret_cast<float*>(out)[e] = x;
@@ -465,14 +592,11 @@ cudaError_t launch_slices(const float* P, int S, int64_t n, void* out, int type,
   int64_t blocks = (items + 255) / 256;
   const int64_t cap = 8 * g16::device_sms();
   if (blocks > cap) blocks = cap;
-  loss_slices_kernel<<<(unsigned)blocks, 256, 0, s>>>(P, S, n, out, type, vec);
   count_launch();
-  return cudaGetLastError();
+  return launch_dependent(loss_slices_kernel, dim3((unsigned)blocks), 256, 0, s, P, S, n, out, type, vec);
 }
 
 // ---- plan -----------------------------------------------------------------------
-int64_t up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
-
 struct Plan {
   int P, PZ;                           // pieces of h and W, of dz
   int cg, BN;                          // CTAs per tile; columns per tile of the logits
@@ -567,7 +691,8 @@ bool plan(const memlayer_loss_config& c, bool backward, Plan* out) {
     p.o_wl = take(V * p.ld * 2);
   }
   if (!backward) {
-    p.o_part = take((int64_t)p.slots * 2 * T * 8);
+    const int64_t few = f32 && T <= FEW ? up(V, FEW_V) / FEW_V * T * 8 : 0, part = (int64_t)p.slots * 2 * T * 8;
+    p.o_part = take(few > part ? few : part);
     p.o_zt = take(T * 4);
   } else {
     p.o_coef = take(T * 8);
@@ -648,6 +773,20 @@ cudaError_t launch_loss_forward(const memlayer_loss_config& c, const memlayer_lo
   Plan p;
   if (!plan(c, false, &p)) return cudaErrorInvalidValue;
   int* err = reinterpret_cast<int*>(ws + O_ERR);
+  if (c.tokens > 0 && few_tokens(c, a)) {
+    FewArgs f{(const float*)a.h, (const float*)a.weight, a.h_stride, a.weight_stride, (int)c.tokens, c.vocab_size,
+              c.d_model, a.targets, reinterpret_cast<float2*>(ws + p.o_part), reinterpret_cast<float*>(ws + p.o_zt),
+              err};
+    static std::atomic<uint64_t> done{0};
+    LS_TRY(g16::allow_smem(reinterpret_cast<const void*>(loss_few_kernel), &done));
+    const int blocks = (c.vocab_size + FEW_V - 1) / FEW_V;
+    loss_few_kernel<<<blocks, few_threads(c.tokens), few_smem(c.tokens, c.d_model), s>>>(f);
+    count_launch(2);
+    LS_TRY(cudaGetLastError());
+    return launch_dependent(loss_join_kernel, dim3((unsigned)((c.tokens + 7) / 8)), 256, 0, s, (const float2*)f.part,
+                            (const float*)f.zt, a.targets, c.tokens, c.vocab_size, Sched{}, 1, blocks, c.ignore_index,
+                            a.loss, a.lse, err);
+  }
   LS_TRY(cudaMemsetAsync(ws + O_ERR, 0, HEAD - O_ERR, s));
   if (c.tokens == 0) return cudaSuccess;
   Operands o{};
@@ -682,11 +821,10 @@ cudaError_t launch_loss_forward(const memlayer_loss_config& c, const memlayer_lo
     LS_TRY((launch<EpiStats<true>, 2, 2>(p.cg, m, S, ea, err, s)));
   else
     LS_TRY((launch<EpiStats<false>, 2, 2>(p.cg, m, S, ea, err, s)));
-  loss_join_kernel<<<(unsigned)((c.tokens + 7) / 8), 256, 0, s>>>(ea.part, ea.zt, a.targets, c.tokens, c.vocab_size,
-                                                                  S, 128 * p.cg, c.ignore_index, a.loss,
-                                                                  a.lse, err);
   count_launch();
-  return cudaGetLastError();
+  return launch_dependent(loss_join_kernel, dim3((unsigned)((c.tokens + 7) / 8)), 256, 0, s, (const float2*)ea.part,
+                          (const float*)ea.zt, a.targets, c.tokens, c.vocab_size, S, 128 * p.cg, 0, c.ignore_index,
+                          a.loss, a.lse, err);
 }
 
 cudaError_t launch_loss_backward(const memlayer_loss_config& c, const memlayer_loss_args& a,
@@ -708,10 +846,9 @@ cudaError_t launch_loss_backward(const memlayer_loss_config& c, const memlayer_l
   int* tgt = reinterpret_cast<int*>(ws + p.o_tgt);
   {
     const int64_t b = (T + 255) / 256;
-    loss_rows_kernel<<<(unsigned)(b < 592 ? b : 592), 256, 0, s>>>(a.targets, g.dloss, g.dlse, T, c.vocab_size,
-                                                                   c.ignore_index, coef, tgt, words + 2, err);
     count_launch();
-    LS_TRY(cudaGetLastError());
+    LS_TRY(launch_dependent(loss_rows_kernel, dim3((unsigned)(b < 592 ? b : 592)), 256, 0, s, a.targets, g.dloss, g.dlse,
+                            T, c.vocab_size, c.ignore_index, coef, tgt, words + 2, err));
   }
   uint16_t *gh = reinterpret_cast<uint16_t*>(ws + p.o_g), *gl = reinterpret_cast<uint16_t*>(ws + p.o_g2);
   float* acc_h = reinterpret_cast<float*>(ws + p.o_dh);

@@ -30,6 +30,7 @@
 // so the result does not depend on timing (no atomics).
 #include "norm.cuh"
 
+#include "dependent.cuh"
 #include "tc_common.cuh"
 
 namespace ml {
@@ -162,6 +163,7 @@ template <typename E, int VEC, int MAXT>
 __global__ void __launch_bounds__(MAXT ? MAXT : NT, MAXT ? 1 : 2) layer_norm_backward_kernel(NormArgs A) {
   constexpr bool WIDE = MAXT > 0;
   __shared__ float red[32];
+  allow_next();                            // of the kernel that adds the partials
   extern __shared__ float cols[];          // !WIDE: [groups][VALS * tpr]
   using Part = RowPart<E, VEC>;
   const int tpr = A.tpr, d = A.d;
@@ -538,6 +540,7 @@ template <typename E, int R, int NV, int MAXT, bool AHEAD>
 __global__ void __launch_bounds__(MAXT, MAXT <= 256 ? 2 : 1) layer_norm_wide_backward_kernel(NormArgs A) {
   constexpr int V = 16 / sizeof(E), H = V / 2;
   using Vec = Vec16<E, V>;
+  allow_next();                            // of the kernel that adds the partials
   __shared__ alignas(16) float red[2][3 * R * 32];
   const int d = A.d, t = threadIdx.x, nt = blockDim.x;
   for (int i = t; i < 2 * 3 * R * 32; i += nt) (&red[0][0])[i] = 0.f;   // slots without a warp
@@ -670,6 +673,7 @@ __global__ void __launch_bounds__(MAXW * 32, 1) layer_norm_ring_backward_kernel(
   constexpr int V = 16 / sizeof(E), H = V / 2;
   using Vec = Vec16<E, V>;
   extern __shared__ uint8_t smem_raw[];
+  allow_next();                              // of the kernel that adds the partials
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const int d = A.d, rb = d * (int)sizeof(E);
   constexpr int tensors = 2;
@@ -813,6 +817,7 @@ __global__ void __launch_bounds__(MAXW * 32, 1) layer_norm_ring_backward_kernel(
 __global__ void __launch_bounds__(1024) layer_norm_params_kernel(const float* __restrict__ part, int blocks, int d,
                                                                  float* __restrict__ dscale,
                                                                  float* __restrict__ dbias, int* err) {
+  wait_previous();
   if (blocks == 0 && blockIdx.x == 0 && threadIdx.x == 0) *err = 0;
   __shared__ float red[32][33];
   const int c = threadIdx.x & 31, g = threadIdx.x >> 5;
@@ -1070,9 +1075,9 @@ cudaError_t launch_layer_norm_backward(const memlayer_norm_config& c, const meml
       default: e = norm_backward_t<float>(A, vec, grid, s); break;
     }
   if (e != cudaSuccess) return e;
-  layer_norm_params_kernel<<<(2 * c.d_model + 31) / 32, 1024, 0, s>>>(part, grid, c.d_model, g.dscale, g.dbias, err);
   count_launch();
-  return cudaGetLastError();
+  return launch_dependent(layer_norm_params_kernel, dim3((2 * c.d_model + 31) / 32), 1024, 0, s, part, grid, c.d_model,
+                          g.dscale, g.dbias, err);
 }
 
 }  // namespace ml

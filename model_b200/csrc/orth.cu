@@ -57,6 +57,7 @@ template <typename E>
 __global__ void __launch_bounds__(256) orth_norm_kernel(const E* __restrict__ u, int64_t n, int chunks,
                                                         double* __restrict__ part) {
   __shared__ double red[8];
+  allow_next();
   // whole 16-byte vectors per chunk; a matrix that starts or ends inside one
   // goes by single elements
   constexpr int V = 16 / sizeof(E);
@@ -105,6 +106,8 @@ __global__ void __launch_bounds__(256) orth_init_kernel(const E* __restrict__ u,
                                                         const double* __restrict__ part, int chunks,
                                                         __half* __restrict__ hi, __half* __restrict__ lo) {
   __shared__ double inv_s;
+  allow_next();
+  wait_previous();
   if (threadIdx.x < 32) {
     double t = 0.;
     for (int i = threadIdx.x; i < chunks; i += 32) t += part[blockIdx.y * chunks + i];
@@ -250,6 +253,8 @@ struct JoinArgs {
 
 __global__ void __launch_bounds__(256) orth_join_kernel(JoinArgs A) {
   __shared__ float t[32][33];
+  allow_next();
+  wait_previous();
   int rb = (int)((sqrtf(8.f * blockIdx.x + 1.f) - 1.f) * 0.5f);
   while ((rb + 1) * (rb + 2) / 2 <= (int)blockIdx.x) ++rb;
   while (rb * (rb + 1) / 2 > (int)blockIdx.x) --rb;
@@ -440,9 +445,8 @@ cudaError_t symmetric(const Plan& p, const Product& P, int buffer, const PolyArg
   const JoinArgs j{reinterpret_cast<float*>(ws + p.o_k), P.S.prod[0].splits, (int)p.s, (int)p.lds, p.se, {o0, o1},
                    ea.two, {ea.s[0], ea.s[1]}, {ea.diag[0], ea.diag[1]}};
   const int64_t nb = (p.s + 31) / 32;
-  orth_join_kernel<<<dim3((unsigned)(nb * (nb + 1) / 2), (unsigned)p.B), 256, 0, s>>>(j);
   count_launch();
-  return cudaGetLastError();
+  return launch_dependent(orth_join_kernel, dim3((unsigned)(nb * (nb + 1) / 2), (unsigned)p.B), 256, 0, s, j);
 }
 
 template <typename E>
@@ -459,10 +463,9 @@ cudaError_t start(const memlayer_orth_config& c, const Plan& p, const E* u, char
   const int64_t cap = up(8 * g16::device_sms(), p.B) / p.B;
   if (blocks > cap) blocks = cap;
   __half* x = reinterpret_cast<__half*>(ws + p.o_x[0]);
-  orth_init_kernel<E><<<dim3((unsigned)blocks, (unsigned)p.B), 256, 0, s>>>(
-      u, (int)p.m, (int)p.n, (int)p.ldx, (double)c.epsilon, part, (int)chunks, x, x + p.xe);
   count_launch();
-  return cudaGetLastError();
+  return launch_dependent(orth_init_kernel<E>, dim3((unsigned)blocks, (unsigned)p.B), 256, 0, s, u, (int)p.m, (int)p.n,
+                          (int)p.ldx, (double)c.epsilon, (const double*)part, (int)chunks, x, x + p.xe);
 }
 
 }  // namespace

@@ -52,16 +52,25 @@ def _stream(t: torch.Tensor) -> int:
     return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
-def _rows(t: torch.Tensor, name: str, like: torch.Tensor) -> Tuple[torch.Tensor, int]:
-    """``t`` (shape and type of ``like``) and the stride between its rows."""
-    if t is not like:
-        if not isinstance(t, torch.Tensor) or not t.is_cuda:
-            raise TypeError(f"{name} must be a CUDA tensor (no CPU path)")
-        if t.device != like.device or t.dtype != like.dtype:
-            raise TypeError(f"{name} must have the device and type of the first tensor")
-        if t.shape != like.shape:
-            raise ValueError(f"{name} must have shape {tuple(like.shape)}")
-    d = t.shape[-1]
+def _call(entry: str, *args) -> None:
+    # ctypes takes a structure by reference where the signature has a pointer
+    status = getattr(L.lib(), entry)(*args)
+    if status:
+        raise L.MemlayerError(status, entry)
+
+
+def _like(t: torch.Tensor, name: str, like: torch.Tensor) -> torch.Tensor:
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise TypeError(f"{name} must be a CUDA tensor (no CPU path)")
+    if t.device != like.device or t.dtype != like.dtype:
+        raise TypeError(f"{name} must have the device and type of the first tensor")
+    if t.shape != like.shape:
+        raise ValueError(f"{name} must have shape {tuple(like.shape)}")
+    return t
+
+
+def _rows(t: torch.Tensor, d: int) -> Tuple[torch.Tensor, int]:
+    """``t`` with rows of ``d`` entries that a stride apart describes, and that stride."""
     if t.is_contiguous():
         return t, d
     if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= d:
@@ -75,7 +84,7 @@ def _vector(t: torch.Tensor, name: str, n: int, like: torch.Tensor) -> torch.Ten
         raise TypeError(f"{name} must be a CUDA tensor on the device of the first tensor")
     if t.numel() != n:
         raise ValueError(f"{name} must have {n} entries")
-    if t.dtype != torch.float32:
+    if t.dtype is not torch.float32:
         t = t.to(torch.float32)
     return t if t.is_contiguous() else t.contiguous()
 
@@ -89,7 +98,7 @@ def _dtype(t: torch.Tensor) -> int:
 
 def _check_status(ws: torch.Tensor, stream: int) -> None:
     code = C.c_int32(0)
-    L.check(L.lib().memlayer_train_status(ws.data_ptr(), C.byref(code), stream), "memlayer_train_status")
+    _call("memlayer_train_status", ws.data_ptr(), code, stream)
     if code.value:
         raise L.DeviceError(f"device status {code.value}: {L.DEVICE_ERRORS.get(code.value, 'unknown')}")
 
@@ -106,16 +115,20 @@ def layer_norm(x: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor, *,
     if x.dim() == 0:
         raise ValueError("x must have at least one dimension")
     d = x.shape[-1]
-    xr, ldx = _rows(x, "x", x)
-    rr, ldr = (None, 0) if residual is None else _rows(residual, "residual", x)
+    xr, ldx = _rows(x, d)
     sc, bi = _vector(scale, "scale", d, x), _vector(bias, "bias", d, x)
     y = torch.empty_like(xr, memory_format=torch.contiguous_format)
-    total = None if rr is None else torch.empty_like(y)
     cfg = L.MemlayerNormConfig(x.numel() // d if d else 0, d, code, eps)
-    a = L.MemlayerNormArgs(xr.data_ptr(), ldx, None if rr is None else rr.data_ptr(), ldr, sc.data_ptr(),
-                           bi.data_ptr(), y.data_ptr(), None if total is None else total.data_ptr())
-    L.check(L.lib().memlayer_layer_norm(C.byref(cfg), C.byref(a), _stream(x)), "memlayer_layer_norm")
-    return y if total is None else (y, total)
+    if residual is None:
+        a = L.MemlayerNormArgs(xr.data_ptr(), ldx, None, 0, sc.data_ptr(), bi.data_ptr(), y.data_ptr(), None)
+        _call("memlayer_layer_norm", cfg, a, _stream(x))
+        return y
+    rr, ldr = _rows(_like(residual, "residual", x), d)
+    total = torch.empty_like(y)
+    a = L.MemlayerNormArgs(xr.data_ptr(), ldx, rr.data_ptr(), ldr, sc.data_ptr(), bi.data_ptr(), y.data_ptr(),
+                           total.data_ptr())
+    _call("memlayer_layer_norm", cfg, a, _stream(x))
+    return y, total
 
 
 @_on_tensor_device
@@ -130,25 +143,23 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, scale: torch.Tensor, 
     if dy.dim() == 0:
         raise ValueError("dy must have at least one dimension")
     d = dy.shape[-1]
-    g, ldg = _rows(dy, "dy", dy)
-    xr, ldx = _rows(x, "x", dy)
-    rr, ldr = (None, 0) if dresidual is None else _rows(dresidual, "dresidual", dy)
+    g, ldg = _rows(dy, d)
+    xr, ldx = _rows(_like(x, "x", dy), d)
+    rr, ldr = (None, 0) if dresidual is None else _rows(_like(dresidual, "dresidual", dy), d)
     sc = _vector(scale, "scale", d, dy)
     dx = torch.empty_like(g, memory_format=torch.contiguous_format)
-    dp = torch.empty(2, d, dtype=torch.float32, device=dy.device)
+    ds, db = sc.new_empty(d), sc.new_empty(d)
     cfg = L.MemlayerNormConfig(dy.numel() // d if d else 0, d, code, eps)
     nb = C.c_size_t()
-    L.check(L.lib().memlayer_layer_norm_backward_workspace_size(C.byref(cfg), C.byref(nb)),
-            "memlayer_layer_norm_backward_workspace_size")
+    _call("memlayer_layer_norm_backward_workspace_size", cfg, nb)
     ws = _workspace(nb.value, dy.device)
     a = L.MemlayerNormGrads(g.data_ptr(), ldg, xr.data_ptr(), ldx, None if rr is None else rr.data_ptr(), ldr,
-                            sc.data_ptr(), dx.data_ptr(), dp.data_ptr(), dp.data_ptr() + 4 * d)
+                            sc.data_ptr(), dx.data_ptr(), ds.data_ptr(), db.data_ptr())
     s = _stream(dy)
-    L.check(L.lib().memlayer_layer_norm_backward(C.byref(cfg), C.byref(a), ws.data_ptr(), nb.value, s),
-            "memlayer_layer_norm_backward")
+    _call("memlayer_layer_norm_backward", cfg, a, ws.data_ptr(), nb.value, s)
     if check:
         _check_status(ws, s)
-    return dx, {"scale": dp[0], "bias": dp[1]}
+    return dx, {"scale": ds, "bias": db}
 
 
 def _loss_args(h, weight, targets, ignore_index):
@@ -165,19 +176,19 @@ def _loss_args(h, weight, targets, ignore_index):
         raise ValueError("ignore_index must fit 32 bits")
     V, d = weight.shape
     if targets.dtype != torch.int32:
-        # an id that 32 bits cannot hold stays out of range
-        targets = torch.where((targets >= -2 ** 31) & (targets < 2 ** 31), targets, 2 ** 31 - 1).to(torch.int32)
+        # an id that 32 bits cannot hold stays out of range, and is not the ignored one
+        bad = -1 if ignore_index != -1 else -2
+        targets = torch.where((targets >= -2 ** 31) & (targets < 2 ** 31), targets, bad).to(torch.int32)
     t = targets.contiguous()
-    hr, ldh = _rows(h, "h", h)
-    wr, ldw = _rows(weight, "weight", weight)
+    hr, ldh = _rows(h, d)
+    wr, ldw = _rows(weight, d)
     cfg = L.MemlayerLossConfig(t.numel(), d, V, code, ignore_index)
     return cfg, hr, ldh, wr, ldw, t
 
 
 def _loss_workspace(cfg, backward: int, device):
     nb = C.c_size_t()
-    L.check(L.lib().memlayer_cross_entropy_workspace_size(C.byref(cfg), backward, C.byref(nb)),
-            "memlayer_cross_entropy_workspace_size")
+    _call("memlayer_cross_entropy_workspace_size", cfg, backward, nb)
     return _workspace(nb.value, device), nb.value
 
 
@@ -195,7 +206,7 @@ def linear_cross_entropy(h: torch.Tensor, weight: torch.Tensor, targets: torch.T
     ws, nb = _loss_workspace(cfg, 0, h.device)
     a = L.MemlayerLossArgs(hr.data_ptr(), ldh, wr.data_ptr(), ldw, t.data_ptr(), loss.data_ptr(), lse.data_ptr())
     s = _stream(h)
-    L.check(L.lib().memlayer_cross_entropy(C.byref(cfg), C.byref(a), ws.data_ptr(), nb, s), "memlayer_cross_entropy")
+    _call("memlayer_cross_entropy", cfg, a, ws.data_ptr(), nb, s)
     if check:
         _check_status(ws, s)
     return loss, lse
@@ -221,8 +232,7 @@ def linear_cross_entropy_backward(h: torch.Tensor, weight: torch.Tensor, targets
     g = L.MemlayerLossGrads(ls.data_ptr(), dl.data_ptr(), None if de is None else de.data_ptr(), dh.data_ptr(),
                             dw.data_ptr())
     s = _stream(h)
-    L.check(L.lib().memlayer_cross_entropy_backward(C.byref(cfg), C.byref(a), C.byref(g), ws.data_ptr(), nb, s),
-            "memlayer_cross_entropy_backward")
+    _call("memlayer_cross_entropy_backward", cfg, a, g, ws.data_ptr(), nb, s)
     if check:
         _check_status(ws, s)
     return dh, dw
@@ -247,12 +257,10 @@ def orthogonalize(update: torch.Tensor, *, steps: int = 5,
     out = torch.empty_like(u)
     cfg = L.MemlayerOrthConfig(u.numel() // (m * n) if m * n else 0, m, n, code, steps, a, b, c, eps)
     nb = C.c_size_t()
-    L.check(L.lib().memlayer_orthogonalize_workspace_size(C.byref(cfg), C.byref(nb)),
-            "memlayer_orthogonalize_workspace_size")
+    _call("memlayer_orthogonalize_workspace_size", cfg, nb)
     ws = _workspace(nb.value, u.device)
     s = _stream(u)
-    L.check(L.lib().memlayer_orthogonalize(C.byref(cfg), u.data_ptr(), out.data_ptr(), ws.data_ptr(), nb.value, s),
-            "memlayer_orthogonalize")
+    _call("memlayer_orthogonalize", cfg, u.data_ptr(), out.data_ptr(), ws.data_ptr(), nb.value, s)
     if check:
         _check_status(ws, s)
     return out

@@ -280,6 +280,18 @@ def test_loss_and_gradient(T, d, V, t):
     LossRef(h, w, y, dl).check(*run_loss(h, w, y, dl, check=True))
 
 
+@pytest.mark.parametrize("T", [1, 3, 16, 17])
+@pytest.mark.parametrize("d,V", [(4, 127), (36, 128), (100, 129), (256, 1000), (1500, 300)])
+def test_loss_of_few_float32_tokens(T, d, V):
+    h, w, y, dl = loss_case(T, d, V, F32, seed=T + d, gap=4 if T > 4 else 0)
+    LossRef(h, w, y).check(*mb.linear_cross_entropy(h, w, y, check=True))
+    wide = torch.zeros(V, d + 8, device="cuda")                   # rows 16 bytes apart, and rows that are not
+    wide[:, 4:d + 4] = w
+    LossRef(h, w, y).check(*mb.linear_cross_entropy(h, wide[:, 4:d + 4], y, check=True))
+    wide[:, 3:d + 3] = w
+    LossRef(h, w, y).check(*mb.linear_cross_entropy(h, wide[:, 3:d + 3], y, check=True))
+
+
 @pytest.mark.parametrize("t", TYPES)
 def test_loss_gradient_of_lse_and_weighted_tokens(t):
     h, w, y, dl = loss_case(200, 96, 700, t, seed=4, gap=3)
