@@ -51,7 +51,7 @@ constexpr uint32_t CTL_BYTES = 1024;
 constexpr uint32_t SMEM_LIMIT = 227 * 1024;
 
 struct Ctl {
-  uint64_t full[MAX_STAGES], empty[MAX_STAGES], tfull[2], tempty[2];
+  uint64_t full[MAX_STAGES], empty[MAX_STAGES], tfull[2], tempty[2], stored;
   uint32_t tmem_base;
   int abort;
 };
@@ -99,6 +99,7 @@ struct Sched {
   }
   __device__ __forceinline__ int count(int c) const {
     if (contiguous) return first(c + 1) - first(c);
+    if (c >= clusters) return 0;
     const int g = c < r ? 0 : 1, i = g ? c - r : c;
     return q + (c < r) + x[g] + (i < e[g]);
   }
@@ -372,24 +373,27 @@ __device__ __forceinline__ void copy_rows(int dtype, uint32_t buf, void* out, in
   }
 }
 
-// Two matrices of 16-bit pieces (hi, lo): each half of the staging buffer is
-// written as soon as the store that last used it has been read, so one store
-// is always in flight.
+// The warp's block of two matrices of 16-bit pieces (hi, lo), a half of the
+// staging buffer each, or its transpose.  One proxy fence for both: fences
+// are most of what a small product's stores take.
 __device__ __forceinline__ void store_pieces(const CUtensorMap* map, uint32_t buf, const uint32_t (&h)[16],
                                              const uint32_t (&l)[16], int x, int y, int z, bool on,
                                              bool transposed = false) {
   const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int q = 0; q < 2; ++q) {
-    if (lane == 0) bulk_wait<1, true>();
-    __syncwarp();
-    if (transposed)
-      stage16_transposed(buf + q * 2048, lane, q ? l : h);
-    else
-      stage16(buf + q * 2048, lane, q ? l : h);
-    tc::fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0 && on) bulk_store(map + q, buf + q * 2048, x, y, z, false);
+  if (lane == 0) bulk_wait<0, true>();
+  __syncwarp();
+  if (transposed) {
+    stage16_transposed(buf, lane, h);
+    stage16_transposed(buf + 2048, lane, l);
+  } else {
+    stage16(buf, lane, h);
+    stage16(buf + 2048, lane, l);
+  }
+  tc::fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0 && on) {
+    bulk_store(map, buf, x, y, z, false);
+    bulk_store(map + 1, buf + 2048, x, y, z, false);
   }
 }
 
@@ -448,228 +452,305 @@ struct Unscale {
 __host__ __device__ inline uint32_t a_bytes() { return 128 * 128; }                  // one piece, one stage, one CTA
 __host__ __device__ inline uint32_t b_bytes(int BN, int cg) { return (uint32_t)(BN / cg) * 128; }
 
-template <class EPI, int CG, int PA, int PB>
-__global__ void __launch_bounds__(THREADS, 1)
-    gemm16_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Sched S,
-                  const __grid_constant__ typename EPI::Args ea, int* err) {
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  Ctl* ctl = reinterpret_cast<Ctl*>(smem);
-  uint8_t* ring = smem + CTL_BYTES;
-  volatile int* abort = &ctl->abort;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = CG == 2 ? cluster_rank() : 0;
-  const int cluster = blockIdx.x / CG;
-  const uint32_t ab = a_bytes(), bb = b_bytes(S.BN, CG), stage_bytes = PA * ab + PB * bb;
-  constexpr bool SUM = EPI::kSum;
-  const int cnt = S.count(cluster);
+// What a CTA's roles share.
+struct Cta {
+  Ctl* ctl;
+  uint8_t* ring;
+  volatile int* abort;
+  int* err;
+  uint32_t rank, stage_bytes, tmem_base;
+  int cluster, stages;
+};
 
+// Positions in the stage ring and between the two accumulators, kept by each
+// role (over several products in a kernel that runs more than one).
+struct RingPos {
+  int s = 0;
+  uint32_t ph = 0;
+  __device__ __forceinline__ void next(int stages) {
+    if (++s == stages) {
+      s = 0;
+      ph ^= 1;
+    }
+  }
+};
+struct AccPos {
+  int acc = 0;
+  uint32_t ph = 0;
+  __device__ __forceinline__ void next() {
+    acc ^= 1;
+    if (acc == 0) ph ^= 1;
+  }
+};
+
+// Barriers and TMEM; all threads call.
+template <int CG, int PA, int PB>
+__device__ __forceinline__ Cta begin_cta(uint8_t* smem_raw, int BN, int stages, int* err) {
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  Cta c;
+  c.ctl = reinterpret_cast<Ctl*>(smem);
+  c.ring = smem + CTL_BYTES;
+  c.abort = &c.ctl->abort;
+  c.err = err;
+  c.rank = CG == 2 ? cluster_rank() : 0;
+  c.stage_bytes = PA * a_bytes() + PB * b_bytes(BN, CG);
+  c.cluster = blockIdx.x / CG;
+  c.stages = stages;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < S.stages; ++s) {
-      tc::mbar_init(&ctl->full[s], 1);
-      tc::mbar_init(&ctl->empty[s], 1);
+    for (int s = 0; s < stages; ++s) {
+      tc::mbar_init(&c.ctl->full[s], 1);
+      tc::mbar_init(&c.ctl->empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
-      tc::mbar_init(&ctl->tfull[b], 1);
-      tc::mbar_init(&ctl->tempty[b], CG * EPI_WARPS);
+      tc::mbar_init(&c.ctl->tfull[b], 1);
+      tc::mbar_init(&c.ctl->tempty[b], CG * EPI_WARPS);
     }
-    ctl->abort = 0;
+    tc::mbar_init(&c.ctl->stored, EPI_WARPS);
+    c.ctl->abort = 0;
     tc::fence_mbar_init();
   }
-  if (warp == 9) tmem_alloc<CG>(&ctl->tmem_base, 512);
+  if (threadIdx.x >> 5 == 9) tmem_alloc<CG>(&c.ctl->tmem_base, 512);
   tc::fence_before_sync();
   if constexpr (CG == 2)
     cluster_sync();
   else
     __syncthreads();
   tc::fence_after_sync();
-  const uint32_t tmem_base = ctl->tmem_base;
-  allow_next();
-  wait_previous();
+  c.tmem_base = c.ctl->tmem_base;
+  return c;
+}
 
-  if (warp < EPI_WARPS) {
-    // kSum keeps 128 sums a thread: 384 x 168 registers dealt out again, 256 x 224 + 128 x 56
-    if constexpr (SUM) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
-    const int quarter = warp & 3, half = warp >> 2;
-    EPI epi;
-    epi.begin(ea, S, cluster, ring + (size_t)S.stages * stage_bytes + warp * STAGING);
-    int acc = 0;
-    uint32_t aph = 0;
-    uint32_t tempty[2];
-    for (int b = 0; b < 2; ++b) {
-      tempty[b] = tc::smem_u32(&ctl->tempty[b]);
-      if constexpr (CG == 2) tempty[b] = map_to_cta(tempty[b], 0);
-    }
-    for (int i = 0; i < cnt; ++i) {
-      const Tile t = S.tile(cluster, i);
-      const int64_t row = (int64_t)t.mt * (128 * CG) + rank * 128 + quarter * 32 + lane;
-      const int nseg = SUM ? (S.stages_of(t) + S.seg - 1) / S.seg : 1;
-      bool ok = true;
-      for (int sg = 0; sg < nseg; ++sg) {
-        if (!__all_sync(FULL, tc::mbar_wait(&ctl->tfull[acc], aph, abort, err, 15))) {
-          ok = false;
-          break;
-        }
-        tc::fence_after_sync();
-        const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * 256);
-        if constexpr (SUM)
-          add_segment(taddr + half * (S.BN >> 1), epi.sum, S.BN >> 1, sg);
-        else
-          epi.tile(ea, S, t, row, half, taddr);
-        tc::fence_before_sync();
-        __syncwarp();
-        if (lane == 0) {
-          if constexpr (CG == 2)
-            arrive_cluster(tempty[acc]);
-          else
-            tc::mbar_arrive(&ctl->tempty[acc]);
-        }
-        if constexpr (SUM) {               // the accumulator is free before the stores
-          if (sg == nseg - 1) epi.store(ea, S, t, row, half);
-        }
-        acc ^= 1;
-        if (acc == 0) aph ^= 1;
-      }
-      if (!ok) break;
-    }
-    epi.end(ea, S, half);
-    if constexpr (EPI::kStore) {
-      if (lane == 0) bulk_wait<0, false>();   // the stores are done with the staging buffers
-    }
-  } else {
-    if constexpr (SUM) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == 8) {
-      if (lane == 0) {
-        for (int q = 0; q < 2 && S.prod[q].m_tiles > 0; ++q)
-          for (int p = 0; p < 2; ++p) {
-            if (p < PA) tc::prefetch_tmap(&maps.a[q][p]);
-            if (p < PB) tc::prefetch_tmap(&maps.b[q][p]);
-          }
-        int s = 0;
-        uint32_t ph = 0;
-        bool ok = true;
-        for (int i = 0; i < cnt && ok; ++i) {
-          const Tile t = S.tile(cluster, i);
-          const int nk = S.stages_of(t);
-          const uint32_t amn = S.prod[t.q].amn, bmn = S.prod[t.q].bmn;
-          const int ar = t.mt * (128 * CG) + (int)rank * 128;
-          const int br = t.nt * S.BN + (int)rank * (S.BN / CG);
-          for (int kc = 0; kc < nk; ++kc) {
-            if (!tc::mbar_wait(&ctl->empty[s], ph ^ 1, abort, err, 11)) {
-              ok = false;
-              break;
-            }
-            const int k = (t.ks * S.prod[t.q].kq + kc) * BK;
-            const uint32_t st = tc::smem_u32(ring + (size_t)s * stage_bytes);
-            if (rank == 0) tc::mbar_expect_tx(&ctl->full[s], CG * stage_bytes);
-            uint32_t bar = tc::smem_u32(&ctl->full[s]);
-            if constexpr (CG == 2) bar = map_to_cta(bar, 0);
-  #pragma unroll
-            for (int p = 0; p < PA; ++p) {
-              const uint32_t da = st + p * ab;
-              const CUtensorMap* ma = &maps.a[t.q][p];
-              if (amn) {
-                tma_load_3d<CG>(da, ma, bar, ar, k, t.z);
-                tma_load_3d<CG>(da + 8192, ma, bar, ar + 64, k, t.z);
-              } else {
-                tma_load_3d<CG>(da, ma, bar, k, ar, t.z);
-              }
-            }
-  #pragma unroll
-            for (int p = 0; p < PB; ++p) {
-              const uint32_t db = st + PA * ab + p * bb;
-              const CUtensorMap* mb = &maps.b[t.q][p];
-              if (bmn) {
-                for (int c = 0; c < S.BN / CG; c += 64) tma_load_3d<CG>(db + (c >> 6) * 8192, mb, bar, br + c, k, t.z);
-              } else {
-                tma_load_3d<CG>(db, mb, bar, k, br, t.z);
-              }
-            }
-            if (++s == S.stages) {
-              s = 0;
-              ph ^= 1;
-            }
-          }
-        }
-        // every stage read (in a pair: the leader's arrivals on this CTA's barriers are in)
-        for (int j = 0; j < S.stages && ok; ++j) {
-          ok = tc::mbar_wait(&ctl->empty[s], ph ^ 1, abort, err, 11);
-          if (++s == S.stages) {
-            s = 0;
-            ph ^= 1;
-          }
-        }
-      }
-    } else if (warp == 9) {
-      if (lane == 0 && rank == 0) {
-        int s = 0, acc = 0;
-        uint32_t ph = 0, aph = 0;
-        bool ok = true;
-        for (int i = 0; i < cnt && ok; ++i) {
-          const Tile t = S.tile(cluster, i);
-          const int nk = S.stages_of(t);
-          const uint32_t amn = S.prod[t.q].amn, bmn = S.prod[t.q].bmn;
-          const uint32_t idesc = idesc_16(128 * CG, S.BN, S.bf16, amn, bmn);
-          // 16 k: 32 bytes along a K-major row, 16 rows of 128 bytes of an MN-major block
-          const uint32_t astep = amn ? 2048 : 32, bstep = bmn ? 2048 : 32;
-          const uint64_t adesc = amn ? sdesc_mn_sw128(0) : tc::sdesc_k_sw128(0);
-          const uint64_t bdesc = bmn ? sdesc_mn_sw128(0) : tc::sdesc_k_sw128(0);
-          const int nseg = SUM ? (nk + S.seg - 1) / S.seg : 1;
-          for (int sg = 0; sg < nseg && ok; ++sg) {
-            if (!tc::mbar_wait(&ctl->tempty[acc], aph ^ 1, abort, err, 12)) {
-              ok = false;
-              break;
-            }
-            tc::fence_after_sync();
-            const uint32_t d = tmem_base + (uint32_t)(acc * 256);
-            const int kc0 = nk * sg / nseg, kc1 = nk * (sg + 1) / nseg;
-            for (int kc = kc0; kc < kc1; ++kc) {
-              if (!tc::mbar_wait(&ctl->full[s], ph, abort, err, 13)) {
-                ok = false;
-                break;
-              }
-              tc::fence_after_sync();
-              const uint32_t sa = tc::smem_u32(ring + (size_t)s * stage_bytes), sb = sa + PA * ab;
-              uint32_t more = kc > kc0;
-              auto step = [&](uint32_t a, uint32_t b) {
-                mma_f16<CG>(d, adesc | ((a >> 4) & 0x3FFF), bdesc | ((b >> 4) & 0x3FFF), idesc, more);
-                more = 1;
-              };
-              if constexpr (PA == 2) {
-#pragma unroll
-                for (int k16 = 0; k16 < BK / 16; ++k16) step(sa + ab + k16 * astep, sb + k16 * bstep);
-              }
-              if constexpr (PB == 2) {
-#pragma unroll
-                for (int k16 = 0; k16 < BK / 16; ++k16) step(sa + k16 * astep, sb + bb + k16 * bstep);
-              }
-#pragma unroll
-              for (int k16 = 0; k16 < BK / 16; ++k16) step(sa + k16 * astep, sb + k16 * bstep);
-              commit<CG>(&ctl->empty[s]);
-              if (++s == S.stages) {
-                s = 0;
-                ph ^= 1;
-              }
-            }
-            if (!ok) break;
-            commit<CG>(&ctl->tfull[acc]);
-            acc ^= 1;
-            if (acc == 0) aph ^= 1;
-          }
-        }
-      }
-    }
-  }
+template <int CG>
+__device__ __forceinline__ void end_cta(const Cta& c) {
   __syncwarp();
   tc::fence_before_sync();
   if constexpr (CG == 2)
     cluster_sync();
   else
     __syncthreads();
-  if (warp == 9) {
+  if (threadIdx.x >> 5 == 9) {
     tc::fence_after_sync();
-    tmem_dealloc<CG>(tmem_base, 512);
+    tmem_dealloc<CG>(c.tmem_base, 512);
   }
+}
+
+// Epilogue warps: the cluster's tiles of one product.
+template <class EPI, int CG>
+__device__ __forceinline__ bool drain(const Cta& c, EPI& epi, const typename EPI::Args& ea, const Sched& S, AccPos& at) {
+  constexpr bool SUM = EPI::kSum;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quarter = warp & 3, half = warp >> 2;
+  const int cnt = S.count(c.cluster);
+  uint32_t tempty[2];
+  for (int b = 0; b < 2; ++b) {
+    tempty[b] = tc::smem_u32(&c.ctl->tempty[b]);
+    if constexpr (CG == 2) tempty[b] = map_to_cta(tempty[b], 0);
+  }
+  for (int i = 0; i < cnt; ++i) {
+    const Tile t = S.tile(c.cluster, i);
+    const int64_t row = (int64_t)t.mt * (128 * CG) + c.rank * 128 + quarter * 32 + lane;
+    const int nseg = SUM ? (S.stages_of(t) + S.seg - 1) / S.seg : 1;
+    for (int sg = 0; sg < nseg; ++sg) {
+      if (!__all_sync(FULL, tc::mbar_wait(&c.ctl->tfull[at.acc], at.ph, c.abort, c.err, 15))) return false;
+      tc::fence_after_sync();
+      const uint32_t taddr = c.tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(at.acc * 256);
+      if constexpr (SUM)
+        add_segment(taddr + half * (S.BN >> 1), epi.sum, S.BN >> 1, sg);
+      else
+        epi.tile(ea, S, t, row, half, taddr);
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (CG == 2)
+          arrive_cluster(tempty[at.acc]);
+        else
+          tc::mbar_arrive(&c.ctl->tempty[at.acc]);
+      }
+      if constexpr (SUM) {                 // the accumulator is free before the stores
+        if (sg == nseg - 1) epi.store(ea, S, t, row, half);
+      }
+      at.next();
+    }
+  }
+  return true;
+}
+
+// Producer (one thread): the stages of the cluster's tiles.
+template <int CG, int PA, int PB>
+__device__ __forceinline__ bool produce(const Cta& c, const Maps& maps, const Sched& S, RingPos& at) {
+  const uint32_t ab = a_bytes(), bb = b_bytes(S.BN, CG);
+  const int cnt = S.count(c.cluster);
+  for (int i = 0; i < cnt; ++i) {
+    const Tile t = S.tile(c.cluster, i);
+    const int nk = S.stages_of(t);
+    const uint32_t amn = S.prod[t.q].amn, bmn = S.prod[t.q].bmn;
+    const int ar = t.mt * (128 * CG) + (int)c.rank * 128;
+    const int br = t.nt * S.BN + (int)c.rank * (S.BN / CG);
+    for (int kc = 0; kc < nk; ++kc) {
+      if (!tc::mbar_wait(&c.ctl->empty[at.s], at.ph ^ 1, c.abort, c.err, 11)) return false;
+      const int k = (t.ks * S.prod[t.q].kq + kc) * BK;
+      const uint32_t st = tc::smem_u32(c.ring + (size_t)at.s * c.stage_bytes);
+      if (c.rank == 0) tc::mbar_expect_tx(&c.ctl->full[at.s], CG * c.stage_bytes);
+      uint32_t bar = tc::smem_u32(&c.ctl->full[at.s]);
+      if constexpr (CG == 2) bar = map_to_cta(bar, 0);
+#pragma unroll
+      for (int p = 0; p < PA; ++p) {
+        const uint32_t da = st + p * ab;
+        const CUtensorMap* ma = &maps.a[t.q][p];
+        if (amn) {
+          tma_load_3d<CG>(da, ma, bar, ar, k, t.z);
+          tma_load_3d<CG>(da + 8192, ma, bar, ar + 64, k, t.z);
+        } else {
+          tma_load_3d<CG>(da, ma, bar, k, ar, t.z);
+        }
+      }
+#pragma unroll
+      for (int p = 0; p < PB; ++p) {
+        const uint32_t db = st + PA * ab + p * bb;
+        const CUtensorMap* mb = &maps.b[t.q][p];
+        if (bmn) {
+          for (int n = 0; n < S.BN / CG; n += 64) tma_load_3d<CG>(db + (n >> 6) * 8192, mb, bar, br + n, k, t.z);
+        } else {
+          tma_load_3d<CG>(db, mb, bar, k, br, t.z);
+        }
+      }
+      at.next(c.stages);
+    }
+  }
+  return true;
+}
+
+// Producer, at the end: every stage read (in a pair: the leader's arrivals on
+// this CTA's barriers are in); after a wait that gave up, time for the copies
+// in flight to land.
+__device__ __forceinline__ void finish_producing(const Cta& c, bool ok, RingPos& at) {
+  for (int j = 0; j < c.stages && ok; ++j) {
+    ok = tc::mbar_wait(&c.ctl->empty[at.s], at.ph ^ 1, c.abort, c.err, 11);
+    at.next(c.stages);
+  }
+  if (!ok) {
+    const long long t0 = clock64();
+    while (clock64() - t0 < 2000000) {}    // about a millisecond
+  }
+}
+
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
+}
+
+// MMA issuer (a whole warp, of the leader in a pair): every lane walks the
+// tiles, one issues.  The operands are then the same in every lane for the
+// compiler, too, and stay in uniform registers, where the instruction wants
+// them; issued by one lane of a divergent branch, twelve MMAs took 1,100 to
+// 1,750 cycles whatever their size.
+template <int CG, int PA, int PB, bool SUM>
+__device__ __forceinline__ bool issue(const Cta& c, const Sched& S, RingPos& at, AccPos& ac) {
+  const uint32_t ab = a_bytes() >> 4, bb = b_bytes(S.BN, CG) >> 4;
+  const uint32_t ring = tc::smem_u32(c.ring);
+  const int cnt = S.count(c.cluster);
+  const bool one = elect_one();
+  for (int i = 0; i < cnt; ++i) {
+    const Tile t = S.tile(c.cluster, i);
+    const int nk = S.stages_of(t);
+    const uint32_t amn = S.prod[t.q].amn, bmn = S.prod[t.q].bmn;
+    const uint32_t idesc = idesc_16(128 * CG, S.BN, S.bf16, amn, bmn);
+    // 16 k: 32 bytes along a K-major row, 16 rows of 128 bytes of an MN-major block
+    const uint32_t astep = amn ? 2048 >> 4 : 32 >> 4, bstep = bmn ? 2048 >> 4 : 32 >> 4;
+    const uint64_t adesc = amn ? sdesc_mn_sw128(0) : tc::sdesc_k_sw128(0);
+    const uint64_t bdesc = bmn ? sdesc_mn_sw128(0) : tc::sdesc_k_sw128(0);
+    const int nseg = SUM ? (nk + S.seg - 1) / S.seg : 1;
+    for (int sg = 0; sg < nseg; ++sg) {
+      if (!__all_sync(FULL, tc::mbar_wait(&c.ctl->tempty[ac.acc], ac.ph ^ 1, c.abort, c.err, 12))) return false;
+      tc::fence_after_sync();
+      const uint32_t d = c.tmem_base + (uint32_t)(ac.acc * 256);
+      const int kc0 = nk * sg / nseg, kc1 = nk * (sg + 1) / nseg;
+      for (int kc = kc0; kc < kc1; ++kc) {
+        if (!__all_sync(FULL, tc::mbar_wait(&c.ctl->full[at.s], at.ph, c.abort, c.err, 13))) return false;
+        tc::fence_after_sync();
+        // descriptors hold addresses in 16 bytes, 14 bits of them; the steps stay inside
+        const uint32_t sa = ((ring + at.s * c.stage_bytes) >> 4) & 0x3FFF, sb = sa + PA * ab;
+        const uint64_t a0 = adesc + sa, b0 = bdesc + sb;
+        const uint32_t more = kc > kc0;
+        if (one) {
+          if constexpr (PA == 2) {
+#pragma unroll
+            for (int k16 = 0; k16 < BK / 16; ++k16)
+              mma_f16<CG>(d, a0 + ab + k16 * astep, b0 + k16 * bstep, idesc, k16 ? 1 : more);
+          }
+          if constexpr (PB == 2) {
+#pragma unroll
+            for (int k16 = 0; k16 < BK / 16; ++k16)
+              mma_f16<CG>(d, a0 + k16 * astep, b0 + bb + k16 * bstep, idesc, k16 || PA == 2 ? 1 : more);
+          }
+#pragma unroll
+          for (int k16 = 0; k16 < BK / 16; ++k16)
+            mma_f16<CG>(d, a0 + k16 * astep, b0 + k16 * bstep, idesc, k16 || PA + PB > 2 ? 1 : more);
+          commit<CG>(&c.ctl->empty[at.s]);
+          if (kc == kc1 - 1) commit<CG>(&c.ctl->tfull[ac.acc]);
+        }
+        __syncwarp();
+        at.next(c.stages);
+      }
+      ac.next();
+    }
+  }
+  return true;
+}
+
+template <int PA, int PB>
+__device__ __forceinline__ void prefetch(const Maps& maps, const Sched& S) {
+  for (int q = 0; q < 2 && S.prod[q].m_tiles > 0; ++q)
+    for (int p = 0; p < 2; ++p) {
+      if (p < PA) tc::prefetch_tmap(&maps.a[q][p]);
+      if (p < PB) tc::prefetch_tmap(&maps.b[q][p]);
+    }
+}
+
+// kSum keeps 128 sums a thread: 384 x 168 registers dealt out again, 256 x 224
+// + 128 x 56.
+template <bool SUM>
+__device__ __forceinline__ void more_registers() {
+  if constexpr (SUM) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+}
+template <bool SUM>
+__device__ __forceinline__ void fewer_registers() {
+  if constexpr (SUM) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+}
+
+template <class EPI, int CG, int PA, int PB>
+__global__ void __launch_bounds__(THREADS, 1)
+    gemm16_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Sched S,
+                  const __grid_constant__ typename EPI::Args ea, int* err) {
+  extern __shared__ uint8_t smem_raw[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Cta c = begin_cta<CG, PA, PB>(smem_raw, S.BN, S.stages, err);
+  allow_next();
+  wait_previous();
+  if (warp < EPI_WARPS) {
+    more_registers<EPI::kSum>();
+    EPI epi;
+    AccPos at;
+    epi.begin(ea, S, c.cluster, c.ring + (size_t)c.stages * c.stage_bytes + warp * STAGING);
+    drain<EPI, CG>(c, epi, ea, S, at);
+    epi.end(ea, S, warp >> 2);
+    if constexpr (EPI::kStore) {
+      if (lane == 0) bulk_wait<0, false>();   // the stores are done with the staging buffers
+    }
+  } else {
+    fewer_registers<EPI::kSum>();
+    if (warp == 8 && lane == 0) {
+      prefetch<PA, PB>(maps, S);
+      RingPos at;
+      const bool ok = produce<CG, PA, PB>(c, maps, S, at);
+      finish_producing(c, ok, at);
+    } else if (warp == 9 && c.rank == 0) {
+      RingPos at;
+      AccPos ac;
+      issue<CG, PA, PB, EPI::kSum>(c, S, at, ac);
+    }
+  }
+  end_cta<CG>(c);
 }
 
 // ---- host side -------------------------------------------------------------------
@@ -694,11 +775,15 @@ int device_sms();
 // Lets `kernel` use all of an SM's shared memory, once per device (`done`: its devices so far).
 cudaError_t allow_smem(const void* kernel, std::atomic<uint64_t>* done);
 
+inline size_t smem_bytes(int BN, int cg, int pa, int pb, bool store) {
+  return 1024 + CTL_BYTES + (size_t)smem_stages(BN, cg, pa, pb, store) * (pa * a_bytes() + pb * b_bytes(BN, cg)) +
+         (store ? EPI_WARPS * STAGING : 0);
+}
+
 template <class EPI, int CG, int PA, int PB>
 cudaError_t launch_one(const Maps& maps, Sched S, const typename EPI::Args& ea, int* err, cudaStream_t s) {
   S.stages = smem_stages(S.BN, CG, PA, PB, EPI::kStore);
-  const size_t smem = 1024 + CTL_BYTES + (size_t)S.stages * (PA * a_bytes() + PB * b_bytes(S.BN, CG)) +
-                      (EPI::kStore ? EPI_WARPS * STAGING : 0);
+  const size_t smem = smem_bytes(S.BN, CG, PA, PB, EPI::kStore);
   auto kern = gemm16_kernel<EPI, CG, PA, PB>;
   static std::atomic<uint64_t> done{0};
   cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), &done);
