@@ -31,6 +31,11 @@
 // its own 128 rows of A and half of the rows of B, the leader issues for
 // both, and each CTA drains its own 128 rows.  Accumulators are
 // double-buffered in TMEM, so an epilogue runs beside the next tile's MMAs.
+// NB = 2 takes two column tiles at once instead, an accumulator each: A is
+// staged once for both.  TMA brings an SM 32 to 39 bytes a cycle whatever is
+// asked of it (the bound of 16-bit products: 47 instead of 62 bytes a cycle at
+// the tensor cores' full rate), and over a long k the drain that nothing
+// overlaps is a few percent.
 // Every mbarrier wait is bounded.
 #pragma once
 
@@ -484,7 +489,7 @@ struct AccPos {
 };
 
 // Barriers and TMEM; all threads call.
-template <int CG, int PA, int PB>
+template <int CG, int PA, int PB, int NB>
 __device__ __forceinline__ Cta begin_cta(uint8_t* smem_raw, int BN, int stages, int* err) {
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   Cta c;
@@ -493,7 +498,7 @@ __device__ __forceinline__ Cta begin_cta(uint8_t* smem_raw, int BN, int stages, 
   c.abort = &c.ctl->abort;
   c.err = err;
   c.rank = CG == 2 ? cluster_rank() : 0;
-  c.stage_bytes = PA * a_bytes() + PB * b_bytes(BN, CG);
+  c.stage_bytes = PA * a_bytes() + NB * PB * b_bytes(BN, CG);
   c.cluster = blockIdx.x / CG;
   c.stages = stages;
   if (threadIdx.x == 0) {
@@ -535,7 +540,7 @@ __device__ __forceinline__ void end_cta(const Cta& c) {
 }
 
 // Epilogue warps: the cluster's tiles of one product.
-template <class EPI, int CG>
+template <class EPI, int CG, int NB>
 __device__ __forceinline__ bool drain(const Cta& c, EPI& epi, const typename EPI::Args& ea, const Sched& S, AccPos& at) {
   constexpr bool SUM = EPI::kSum;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quarter = warp & 3, half = warp >> 2;
@@ -546,10 +551,11 @@ __device__ __forceinline__ bool drain(const Cta& c, EPI& epi, const typename EPI
     if constexpr (CG == 2) tempty[b] = map_to_cta(tempty[b], 0);
   }
   for (int i = 0; i < cnt; ++i) {
-    const Tile t = S.tile(c.cluster, i);
+    Tile t = S.tile(c.cluster, i);
     const int64_t row = (int64_t)t.mt * (128 * CG) + c.rank * 128 + quarter * 32 + lane;
-    const int nseg = SUM ? (S.stages_of(t) + S.seg - 1) / S.seg : 1;
-    for (int sg = 0; sg < nseg; ++sg) {
+    const int nseg = SUM ? (S.stages_of(t) + S.seg - 1) / S.seg : NB;
+    t.nt *= NB;
+    for (int sg = 0; sg < nseg; ++sg) {    // segments of k, or the column tiles
       if (!__all_sync(FULL, tc::mbar_wait(&c.ctl->tfull[at.acc], at.ph, c.abort, c.err, 15))) return false;
       tc::fence_after_sync();
       const uint32_t taddr = c.tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(at.acc * 256);
@@ -557,6 +563,7 @@ __device__ __forceinline__ bool drain(const Cta& c, EPI& epi, const typename EPI
         add_segment(taddr + half * (S.BN >> 1), epi.sum, S.BN >> 1, sg);
       else
         epi.tile(ea, S, t, row, half, taddr);
+      if constexpr (!SUM) ++t.nt;
       tc::fence_before_sync();
       __syncwarp();
       if (lane == 0) {
@@ -575,7 +582,7 @@ __device__ __forceinline__ bool drain(const Cta& c, EPI& epi, const typename EPI
 }
 
 // Producer (one thread): the stages of the cluster's tiles.
-template <int CG, int PA, int PB>
+template <int CG, int PA, int PB, int NB>
 __device__ __forceinline__ bool produce(const Cta& c, const Maps& maps, const Sched& S, RingPos& at) {
   const uint32_t ab = a_bytes(), bb = b_bytes(S.BN, CG);
   const int cnt = S.count(c.cluster);
@@ -584,7 +591,7 @@ __device__ __forceinline__ bool produce(const Cta& c, const Maps& maps, const Sc
     const int nk = S.stages_of(t);
     const uint32_t amn = S.prod[t.q].amn, bmn = S.prod[t.q].bmn;
     const int ar = t.mt * (128 * CG) + (int)c.rank * 128;
-    const int br = t.nt * S.BN + (int)c.rank * (S.BN / CG);
+    const int br = t.nt * NB * S.BN + (int)c.rank * (S.BN / CG);
     for (int kc = 0; kc < nk; ++kc) {
       if (!tc::mbar_wait(&c.ctl->empty[at.s], at.ph ^ 1, c.abort, c.err, 11)) return false;
       const int k = (t.ks * S.prod[t.q].kq + kc) * BK;
@@ -604,13 +611,14 @@ __device__ __forceinline__ bool produce(const Cta& c, const Maps& maps, const Sc
         }
       }
 #pragma unroll
-      for (int p = 0; p < PB; ++p) {
+      for (int p = 0; p < NB * PB; ++p) {  // the column tiles' pieces
         const uint32_t db = st + PA * ab + p * bb;
-        const CUtensorMap* mb = &maps.b[t.q][p];
+        const CUtensorMap* mb = &maps.b[t.q][p % PB];
+        const int r = br + p / PB * S.BN;
         if (bmn) {
-          for (int n = 0; n < S.BN / CG; n += 64) tma_load_3d<CG>(db + (n >> 6) * 8192, mb, bar, br + n, k, t.z);
+          for (int n = 0; n < S.BN / CG; n += 64) tma_load_3d<CG>(db + (n >> 6) * 8192, mb, bar, r + n, k, t.z);
         } else {
-          tma_load_3d<CG>(db, mb, bar, k, br, t.z);
+          tma_load_3d<CG>(db, mb, bar, k, r, t.z);
         }
       }
       at.next(c.stages);
@@ -644,7 +652,7 @@ __device__ __forceinline__ bool elect_one() {
 // compiler, too, and stay in uniform registers, where the instruction wants
 // them; issued by one lane of a divergent branch, twelve MMAs took 1,100 to
 // 1,750 cycles whatever their size.
-template <int CG, int PA, int PB, bool SUM>
+template <int CG, int PA, int PB, int NB, bool SUM>
 __device__ __forceinline__ bool issue(const Cta& c, const Sched& S, RingPos& at, AccPos& ac) {
   const uint32_t ab = a_bytes() >> 4, bb = b_bytes(S.BN, CG) >> 4;
   const uint32_t ring = tc::smem_u32(c.ring);
@@ -661,38 +669,49 @@ __device__ __forceinline__ bool issue(const Cta& c, const Sched& S, RingPos& at,
     const uint64_t bdesc = bmn ? sdesc_mn_sw128(0) : tc::sdesc_k_sw128(0);
     const int nseg = SUM ? (nk + S.seg - 1) / S.seg : 1;
     for (int sg = 0; sg < nseg; ++sg) {
-      if (!__all_sync(FULL, tc::mbar_wait(&c.ctl->tempty[ac.acc], ac.ph ^ 1, c.abort, c.err, 12))) return false;
-      tc::fence_after_sync();
-      const uint32_t d = c.tmem_base + (uint32_t)(ac.acc * 256);
+      if (NB == 1) {
+        if (!__all_sync(FULL, tc::mbar_wait(&c.ctl->tempty[ac.acc], ac.ph ^ 1, c.abort, c.err, 12))) return false;
+        tc::fence_after_sync();
+      }
       const int kc0 = nk * sg / nseg, kc1 = nk * (sg + 1) / nseg;
       for (int kc = kc0; kc < kc1; ++kc) {
         if (!__all_sync(FULL, tc::mbar_wait(&c.ctl->full[at.s], at.ph, c.abort, c.err, 13))) return false;
         tc::fence_after_sync();
         // descriptors hold addresses in 16 bytes, 14 bits of them; the steps stay inside
         const uint32_t sa = ((ring + at.s * c.stage_bytes) >> 4) & 0x3FFF, sb = sa + PA * ab;
-        const uint64_t a0 = adesc + sa, b0 = bdesc + sb;
+        const uint64_t a0 = adesc + sa;
         const uint32_t more = kc > kc0;
-        if (one) {
-          if constexpr (PA == 2) {
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          if (NB == 2 && kc == kc0) {      // each column tile waits for its own accumulator
+            if (!__all_sync(FULL, tc::mbar_wait(&c.ctl->tempty[nb], ac.ph ^ 1, c.abort, c.err, 12))) return false;
+            tc::fence_after_sync();
+          }
+          const uint32_t d = c.tmem_base + (uint32_t)((NB == 2 ? nb : ac.acc) * 256);
+          const uint64_t b0 = bdesc + sb + nb * PB * bb;
+          if (one) {
+            if constexpr (PA == 2) {
+#pragma unroll
+              for (int k16 = 0; k16 < BK / 16; ++k16)
+                mma_f16<CG>(d, a0 + ab + k16 * astep, b0 + k16 * bstep, idesc, k16 ? 1 : more);
+            }
+            if constexpr (PB == 2) {
+#pragma unroll
+              for (int k16 = 0; k16 < BK / 16; ++k16)
+                mma_f16<CG>(d, a0 + k16 * astep, b0 + bb + k16 * bstep, idesc, k16 || PA == 2 ? 1 : more);
+            }
 #pragma unroll
             for (int k16 = 0; k16 < BK / 16; ++k16)
-              mma_f16<CG>(d, a0 + ab + k16 * astep, b0 + k16 * bstep, idesc, k16 ? 1 : more);
+              mma_f16<CG>(d, a0 + k16 * astep, b0 + k16 * bstep, idesc, k16 || PA + PB > 2 ? 1 : more);
+            if (nb == NB - 1) commit<CG>(&c.ctl->empty[at.s]);
+            if (kc == kc1 - 1) commit<CG>(&c.ctl->tfull[NB == 2 ? nb : ac.acc]);
           }
-          if constexpr (PB == 2) {
-#pragma unroll
-            for (int k16 = 0; k16 < BK / 16; ++k16)
-              mma_f16<CG>(d, a0 + k16 * astep, b0 + bb + k16 * bstep, idesc, k16 || PA == 2 ? 1 : more);
-          }
-#pragma unroll
-          for (int k16 = 0; k16 < BK / 16; ++k16)
-            mma_f16<CG>(d, a0 + k16 * astep, b0 + k16 * bstep, idesc, k16 || PA + PB > 2 ? 1 : more);
-          commit<CG>(&c.ctl->empty[at.s]);
-          if (kc == kc1 - 1) commit<CG>(&c.ctl->tfull[ac.acc]);
         }
         __syncwarp();
         at.next(c.stages);
       }
       ac.next();
+      if (NB == 2) ac.next();
     }
   }
   return true;
@@ -718,13 +737,13 @@ __device__ __forceinline__ void fewer_registers() {
   if constexpr (SUM) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
 }
 
-template <class EPI, int CG, int PA, int PB>
+template <class EPI, int CG, int PA, int PB, int NB>
 __global__ void __launch_bounds__(THREADS, 1)
     gemm16_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Sched S,
                   const __grid_constant__ typename EPI::Args ea, int* err) {
   extern __shared__ uint8_t smem_raw[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const Cta c = begin_cta<CG, PA, PB>(smem_raw, S.BN, S.stages, err);
+  const Cta c = begin_cta<CG, PA, PB, NB>(smem_raw, S.BN, S.stages, err);
   allow_next();
   wait_previous();
   if (warp < EPI_WARPS) {
@@ -732,7 +751,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     EPI epi;
     AccPos at;
     epi.begin(ea, S, c.cluster, c.ring + (size_t)c.stages * c.stage_bytes + warp * STAGING);
-    drain<EPI, CG>(c, epi, ea, S, at);
+    drain<EPI, CG, NB>(c, epi, ea, S, at);
     epi.end(ea, S, warp >> 2);
     if constexpr (EPI::kStore) {
       if (lane == 0) bulk_wait<0, false>();   // the stores are done with the staging buffers
@@ -742,12 +761,12 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (warp == 8 && lane == 0) {
       prefetch<PA, PB>(maps, S);
       RingPos at;
-      const bool ok = produce<CG, PA, PB>(c, maps, S, at);
+      const bool ok = produce<CG, PA, PB, NB>(c, maps, S, at);
       finish_producing(c, ok, at);
     } else if (warp == 9 && c.rank == 0) {
       RingPos at;
       AccPos ac;
-      issue<CG, PA, PB, EPI::kSum>(c, S, at, ac);
+      issue<CG, PA, PB, NB, EPI::kSum>(c, S, at, ac);
     }
   }
   end_cta<CG>(c);
@@ -765,9 +784,12 @@ cudaError_t make_operand(CUtensorMap* map, const void* base, int64_t rows, int64
 cudaError_t make_store(CUtensorMap* map, void* base, int64_t rows, int64_t cols, int64_t pitch, int dtype,
                        int64_t z = 1, int64_t zstride = 0);
 
-inline int smem_stages(int BN, int cg, int pa, int pb, bool store) {
-  const uint32_t st = pa * a_bytes() + pb * b_bytes(BN, cg);
-  const int n = (int)((SMEM_LIMIT - 1024 - CTL_BYTES - (store ? EPI_WARPS * STAGING : 0)) / st);
+inline uint32_t stage_size(int BN, int cg, int pa, int pb, int nb) {
+  return pa * a_bytes() + nb * pb * b_bytes(BN, cg);
+}
+
+inline int smem_stages(int BN, int cg, int pa, int pb, int nb, bool store) {
+  const int n = (int)((SMEM_LIMIT - 1024 - CTL_BYTES - (store ? EPI_WARPS * STAGING : 0)) / stage_size(BN, cg, pa, pb, nb));
   return n > MAX_STAGES ? MAX_STAGES : n;
 }
 
@@ -775,16 +797,13 @@ int device_sms();
 // Lets `kernel` use all of an SM's shared memory, once per device (`done`: its devices so far).
 cudaError_t allow_smem(const void* kernel, std::atomic<uint64_t>* done);
 
-inline size_t smem_bytes(int BN, int cg, int pa, int pb, bool store) {
-  return 1024 + CTL_BYTES + (size_t)smem_stages(BN, cg, pa, pb, store) * (pa * a_bytes() + pb * b_bytes(BN, cg)) +
-         (store ? EPI_WARPS * STAGING : 0);
-}
-
-template <class EPI, int CG, int PA, int PB>
+template <class EPI, int CG, int PA, int PB, int NB = 1>
 cudaError_t launch_one(const Maps& maps, Sched S, const typename EPI::Args& ea, int* err, cudaStream_t s) {
-  S.stages = smem_stages(S.BN, CG, PA, PB, EPI::kStore);
-  const size_t smem = smem_bytes(S.BN, CG, PA, PB, EPI::kStore);
-  auto kern = gemm16_kernel<EPI, CG, PA, PB>;
+  static_assert(NB == 1 || !EPI::kSum, "segments use both accumulators");
+  S.stages = smem_stages(S.BN, CG, PA, PB, NB, EPI::kStore);
+  const size_t smem = 1024 + CTL_BYTES + (size_t)S.stages * stage_size(S.BN, CG, PA, PB, NB) +
+                      (EPI::kStore ? EPI_WARPS * STAGING : 0);
+  auto kern = gemm16_kernel<EPI, CG, PA, PB, NB>;
   static std::atomic<uint64_t> done{0};
   cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), &done);
   if (e != cudaSuccess) return e;

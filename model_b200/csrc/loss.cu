@@ -604,7 +604,7 @@ struct Plan {
   int slots;                           // partial pairs per row and column half
   int64_t ld;                          // row pitch of the 16-bit forms
   int vc;                              // columns of a vocabulary piece = row pitch of its dz
-  int oBN;                             // columns per tile of the gradient products
+  int oBN, oNB;                        // columns per tile of the gradient products, tiles at once
   int s_h, s_w;                        // k slices of dh and of dW
   size_t o_hh, o_hl, o_wh, o_wl, o_part, o_zt, o_coef, o_tgt, o_g, o_g2, o_dh, o_dw, bytes;
 };
@@ -633,7 +633,7 @@ Prod product(int64_t m_tiles, int64_t n_tiles, int splits, int64_t k, bool amn, 
 // first; returns which place dh has.
 int out_products(const Plan& p, int64_t T, int64_t vc, int64_t d, Sched* S) {
   const int rt = 128 * p.cg;
-  const int64_t nd = up(d, p.oBN) / p.oBN;
+  const int64_t nd = up(d, p.oBN * p.oNB) / (p.oBN * p.oNB);
   const Prod w = product(up(vc, rt) / rt, nd, p.s_w, T, true, true);
   const Prod h = product(up(T, rt) / rt, nd, p.s_h, vc, false, true);
   const int at = h.kq > w.kq ? 0 : 1;
@@ -651,7 +651,7 @@ void piece_plan(int64_t T, int64_t V, int64_t d, int sms, Plan* p) {
   const int64_t n = (V + most - 1) / most;
   p->vc = (int)up((V + n - 1) / n, 256);
   const int rt = 128 * p->cg;
-  const int64_t nd = up(d, p->oBN) / p->oBN, kh = up(p->vc, 64) / 64, kw = up(T, 64) / 64;
+  const int64_t nd = up(d, p->oBN * p->oNB) / (p->oBN * p->oNB), kh = up(p->vc, 64) / 64, kw = up(T, 64) / 64;
   const double ideal = (double)(up(T, rt) / rt * nd * kh + up(p->vc, rt) / rt * nd * kw) / (sms / p->cg);
   const double cap = ideal * 1.25 < 16 ? 16 : ideal * 1.25;
   p->s_h = kh > cap ? (int)(kh / cap + 0.999) : 1;
@@ -698,6 +698,10 @@ bool plan(const memlayer_loss_config& c, bool backward, Plan* out) {
     p.o_coef = take(T * 8);
     p.o_tgt = take(T * 4);
     p.oBN = d > 128 ? 256 : 128;
+    // 16-bit products with an even number of column tiles take two at once:
+    // 8192 x 1024 x 32768 bf16 791 us instead of 956, 1999 x 512 x 30011 f16
+    // 100 instead of 124 (an odd one would multiply by columns that are not there)
+    p.oNB = p.cg == 2 && p.PZ == 1 && up(d, 256) / 256 % 2 == 0 ? 2 : 1;
     piece_plan(T, V, d, sms, &p);
     p.o_g = take(T * p.vc * 2);
     if (p.PZ == 2) p.o_g2 = take(T * p.vc * 2);
@@ -928,8 +932,9 @@ cudaError_t launch_loss_backward(const memlayer_loss_config& c, const memlayer_l
     if (f32)
       LS_TRY((launch<EpiOut<true>, 2, 2>(p.cg, m2, S2, ea, err, s)));
     else
-      LS_TRY(p.PZ == 2 ? (g16::launch_one<EpiOut<false>, 1, 2, 1>(m2, S2, ea, err, s))
-                       : (g16::launch_one<EpiOut<false>, 2, 1, 1>(m2, S2, ea, err, s)));
+      LS_TRY(p.PZ == 2    ? (g16::launch_one<EpiOut<false>, 1, 2, 1>(m2, S2, ea, err, s))
+             : p.oNB == 2 ? (g16::launch_one<EpiOut<false>, 2, 1, 1, 2>(m2, S2, ea, err, s))
+                          : (g16::launch_one<EpiOut<false>, 2, 1, 1>(m2, S2, ea, err, s)));
     if (sw > 1)
       LS_TRY(launch_slices(reinterpret_cast<float*>(ws + p.o_dw), sw, (int64_t)vc * d, dwp, c.dtype, s));
     if (i == 0) p.s_h = sh;            // slices of the first (largest) piece
