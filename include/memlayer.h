@@ -666,7 +666,7 @@ int32_t memlayer_layer_norm_backward(const memlayer_norm_config* cfg, const meml
 typedef struct {
   int64_t tokens;                /* T */
   int32_t d_model;               /* 1 .. 65536 */
-  int32_t vocab_size;            /* V */
+  int32_t vocab_size;            /* V, at most 2^31 - 256 */
   int32_t dtype;                 /* memlayer_dtype of h, weight, dh, dweight */
   int32_t ignore_index;          /* a target of this value carries no loss */
 } memlayer_loss_config;

@@ -56,7 +56,7 @@ constexpr uint32_t CTL_BYTES = 1024;
 constexpr uint32_t SMEM_LIMIT = 227 * 1024;
 
 struct Ctl {
-  uint64_t full[MAX_STAGES], empty[MAX_STAGES], tfull[2], tempty[2], stored;
+  uint64_t full[MAX_STAGES], empty[MAX_STAGES], tfull[2], tempty[2];
   uint32_t tmem_base;
   int abort;
 };
@@ -467,8 +467,7 @@ struct Cta {
   int cluster, stages;
 };
 
-// Positions in the stage ring and between the two accumulators, kept by each
-// role (over several products in a kernel that runs more than one).
+// Positions in the stage ring and between the two accumulators, kept by each role.
 struct RingPos {
   int s = 0;
   uint32_t ph = 0;
@@ -510,7 +509,6 @@ __device__ __forceinline__ Cta begin_cta(uint8_t* smem_raw, int BN, int stages, 
       tc::mbar_init(&c.ctl->tfull[b], 1);
       tc::mbar_init(&c.ctl->tempty[b], CG * EPI_WARPS);
     }
-    tc::mbar_init(&c.ctl->stored, EPI_WARPS);
     c.ctl->abort = 0;
     tc::fence_mbar_init();
   }

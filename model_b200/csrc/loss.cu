@@ -164,8 +164,9 @@ struct EpiStats {
 // Joins the partial (maximum, sum) pairs of a row, in slot order per lane and
 // a fixed tree over the lanes.  One warp per row.
 __global__ void __launch_bounds__(256) loss_join_kernel(const float2* __restrict__ part, const float* __restrict__ zt,
-                                                        const int* __restrict__ targets, int64_t T, int V, const __grid_constant__ Sched S,
-                                                        int rows_per_tile, int blocks, int ignore,
+                                                        const int* __restrict__ targets, int64_t T, int V,
+                                                        const __grid_constant__ Sched S, int rows_per_tile, int blocks,
+                                                        int ignore,
                                                         float* __restrict__ loss, float* __restrict__ lse,
                                                         int* __restrict__ err) {
   allow_next();
@@ -851,8 +852,8 @@ cudaError_t launch_loss_backward(const memlayer_loss_config& c, const memlayer_l
   {
     const int64_t b = (T + 255) / 256;
     count_launch();
-    LS_TRY(launch_dependent(loss_rows_kernel, dim3((unsigned)(b < 592 ? b : 592)), 256, 0, s, a.targets, g.dloss, g.dlse,
-                            T, c.vocab_size, c.ignore_index, coef, tgt, words + 2, err));
+    LS_TRY(launch_dependent(loss_rows_kernel, dim3((unsigned)(b < 592 ? b : 592)), 256, 0, s, a.targets, g.dloss,
+                            g.dlse, T, c.vocab_size, c.ignore_index, coef, tgt, words + 2, err));
   }
   uint16_t *gh = reinterpret_cast<uint16_t*>(ws + p.o_g), *gl = reinterpret_cast<uint16_t*>(ws + p.o_g2);
   float* acc_h = reinterpret_cast<float*>(ws + p.o_dh);

@@ -30,8 +30,7 @@
 // so the result does not depend on timing (no atomics).
 #include "norm.cuh"
 
-#include "dependent.cuh"
-#include "tc_common.cuh"
+#include "gemm16.cuh"
 
 namespace ml {
 
@@ -665,9 +664,9 @@ __global__ void __launch_bounds__(MAXT, MAXT <= 256 ? 2 : 1) layer_norm_wide_bac
 
 // The gradient of rows that a warp holds: a warp per row, without a barrier.
 // Each warp streams its rows of x and dy through a ring of its own in shared
-// memory (bulk copies, signalled by mbarriers) and reads them from there: the mean, the three sums around it, dx.  The columns' parameter sums
-// stay in its registers over all of its rows; the block adds its warps' at
-// the end.
+// memory (bulk copies, signalled by mbarriers) and reads them from there: the
+// mean, the three sums around it, dx.  The columns' parameter sums stay in its
+// registers over all of its rows; the block adds its warps' at the end.
 template <typename E, int NV, int MAXW>
 __global__ void __launch_bounds__(MAXW * 32, 1) layer_norm_ring_backward_kernel(NormArgs A, int stages) {
   constexpr int V = 16 / sizeof(E), H = V / 2;
@@ -676,7 +675,7 @@ __global__ void __launch_bounds__(MAXW * 32, 1) layer_norm_ring_backward_kernel(
   allow_next();                              // of the kernel that adds the partials
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const int d = A.d, rb = d * (int)sizeof(E);
-  constexpr int tensors = 2;
+  constexpr int tensors = 2;                 // x and dy
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem) + warp * 4;              // 4 stages at most
   volatile int* abort = reinterpret_cast<int*>(smem + 12 * 32);
@@ -723,7 +722,11 @@ __global__ void __launch_bounds__(MAXW * 32, 1) layer_norm_ring_backward_kernel(
       for (int i = 0; i < NV; ++i)
         if ((i * 32 + lane) * V < d) e[i] = es[i * 32 + lane];
     }
-    if (!__all_sync(FULL, tc::mbar_wait(&full[st], ph, abort, A.err, 11))) break;
+    if (!__all_sync(FULL, tc::mbar_wait(&full[st], ph, abort, A.err, 11))) {
+      const long long t0 = clock64();        // time for the copies in flight to land
+      while (clock64() - t0 < 2000000) {}    // about a millisecond
+      break;
+    }
     const uint8_t* at = ring + (size_t)st * tensors * rbp;
     const Vec* xs = reinterpret_cast<const Vec*>(at);
     const Vec* gs = reinterpret_cast<const Vec*>(at + rbp);
@@ -854,13 +857,6 @@ int norm_tpr(int d) {
   return t;
 }
 
-int sm_count() {
-  int dev = 0, sms = 148;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  return sms;
-}
-
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // The block-per-row layouts: threads a row, vectors a thread, rows at a time.
@@ -947,7 +943,8 @@ cudaError_t norm_forward_t(NormArgs& A, bool vec, cudaStream_t s) {
 template <typename E, int NV, int MAXW>
 cudaError_t launch_ring(const NormArgs& A, const Ring& r, int grid, cudaStream_t s) {
   auto kern = layer_norm_ring_backward_kernel<E, NV, MAXW>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)r.smem);
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t e = g16::allow_smem(reinterpret_cast<const void*>(kern), &done);
   if (e != cudaSuccess) return e;
   kern<<<grid, r.warps * 32, r.smem, s>>>(A, r.stages);
   return cudaSuccess;
@@ -1006,7 +1003,7 @@ int backward_blocks(int64_t rows, int d, int v, bool vec) {
     need = ceil_div(rows, nt / tpr);
     per_sm = nt <= 256 ? 512 / nt : 1;
   }
-  const int64_t cap = per_sm * sm_count();
+  const int64_t cap = per_sm * g16::device_sms();
   return (int)(need < cap ? need : cap);
 }
 

@@ -1,6 +1,5 @@
 // C ABI of the training step's operators around the memory layer: argument
-// checks for norm.cu, loss.cu
-// and orth.cu.
+// checks for norm.cu, loss.cu and orth.cu.
 #include <math.h>
 #include <stdint.h>
 
@@ -35,7 +34,8 @@ int check_norm(const memlayer_norm_config* c) {
 int check_loss(const memlayer_loss_config* c) {
   if (!c) return MEMLAYER_ERR_BAD_POINTER;
   if (c->tokens < 0 || c->tokens >= (1ll << 31) || c->d_model < 1 || c->vocab_size < 1) return MEMLAYER_ERR_BAD_SHAPE;
-  if (!dtype_ok(c->dtype) || c->d_model > 65536) return MEMLAYER_ERR_UNSUPPORTED;
+  // the last column tile's columns stay below 2^31
+  if (!dtype_ok(c->dtype) || c->d_model > 65536 || c->vocab_size > 0x7FFFFF00) return MEMLAYER_ERR_UNSUPPORTED;
   return MEMLAYER_OK;
 }
 

@@ -131,6 +131,14 @@ def layer_norm(x: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor, *,
     return y, total
 
 
+# The sizes depend on the device (its SMs) beside the arguments.
+@functools.lru_cache(maxsize=256)
+def _norm_workspace_bytes(rows: int, d: int, code: int, eps: float, device: int) -> int:
+    nb = C.c_size_t()
+    _call("memlayer_layer_norm_backward_workspace_size", L.MemlayerNormConfig(rows, d, code, eps), nb)
+    return nb.value
+
+
 @_on_tensor_device
 def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, scale: torch.Tensor, *,
                         dresidual: Optional[torch.Tensor] = None, eps: float = 1e-6, check: bool = False,
@@ -150,13 +158,12 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, scale: torch.Tensor, 
     dx = torch.empty_like(g, memory_format=torch.contiguous_format)
     ds, db = sc.new_empty(d), sc.new_empty(d)
     cfg = L.MemlayerNormConfig(dy.numel() // d if d else 0, d, code, eps)
-    nb = C.c_size_t()
-    _call("memlayer_layer_norm_backward_workspace_size", cfg, nb)
-    ws = _workspace(nb.value, dy.device)
+    nb = _norm_workspace_bytes(cfg.rows, d, code, eps, dy.get_device())
+    ws = _workspace(nb, dy.device)
     a = L.MemlayerNormGrads(g.data_ptr(), ldg, xr.data_ptr(), ldx, None if rr is None else rr.data_ptr(), ldr,
                             sc.data_ptr(), dx.data_ptr(), ds.data_ptr(), db.data_ptr())
     s = _stream(dy)
-    _call("memlayer_layer_norm_backward", cfg, a, ws.data_ptr(), nb.value, s)
+    _call("memlayer_layer_norm_backward", cfg, a, ws.data_ptr(), nb, s)
     if check:
         _check_status(ws, s)
     return dx, {"scale": ds, "bias": db}
@@ -186,10 +193,16 @@ def _loss_args(h, weight, targets, ignore_index):
     return cfg, hr, ldh, wr, ldw, t
 
 
-def _loss_workspace(cfg, backward: int, device):
+@functools.lru_cache(maxsize=256)
+def _loss_workspace_bytes(tokens: int, d: int, vocab: int, code: int, backward: int, device: int) -> int:
     nb = C.c_size_t()
-    _call("memlayer_cross_entropy_workspace_size", cfg, backward, nb)
-    return _workspace(nb.value, device), nb.value
+    _call("memlayer_cross_entropy_workspace_size", L.MemlayerLossConfig(tokens, d, vocab, code, 0), backward, nb)
+    return nb.value
+
+
+def _loss_workspace(cfg, backward: int, device):
+    nb = _loss_workspace_bytes(cfg.tokens, cfg.d_model, cfg.vocab_size, cfg.dtype, backward, device.index)
+    return _workspace(nb, device), nb
 
 
 @_on_tensor_device

@@ -109,7 +109,10 @@ def loss_grads(**kw):
     (dict(tokens=-1), L.ERR_BAD_SHAPE), (dict(tokens=1 << 31), L.ERR_BAD_SHAPE), (dict(d_model=0), L.ERR_BAD_SHAPE),
     (dict(vocab_size=0), L.ERR_BAD_SHAPE), (dict(dtype=9), L.ERR_UNSUPPORTED), (dict(d_model=65537), L.ERR_UNSUPPORTED),
     # 2^23 x 2^23 tiles would not fit the kernels' tile counter
-    (dict(tokens=(1 << 31) - 1, vocab_size=(1 << 31) - 1), L.ERR_UNSUPPORTED)])
+    (dict(tokens=(1 << 31) - 1, vocab_size=(1 << 31) - 1), L.ERR_UNSUPPORTED),
+    (dict(tokens=(1 << 31) - 1, vocab_size=(1 << 31) - 256), L.ERR_UNSUPPORTED),
+    # the last column tile would end past 2^31
+    (dict(tokens=1, vocab_size=(1 << 31) - 255), L.ERR_UNSUPPORTED)])
 def test_loss_sizes_refused(bad, status):
     lib, n = L.lib(), C.c_size_t()
     c = loss_cfg(**bad)
