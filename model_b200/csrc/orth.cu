@@ -14,7 +14,8 @@
 // read X along its other index.  The first two are symmetric: only the tiles
 // on and below the diagonal are computed, the epilogue writes the others as
 // their transposes.  A long k with few tiles is cut into slices, whose float32
-// partials a small kernel adds.
+// partials a small kernel adds.  Matrices that a cluster's shared memory holds
+// take orth_chain.cu instead.
 //
 // Entries of X, P, R and Q are bounded by their singular values, which the
 // host bounds for the given coefficients before it launches (the usual
@@ -41,7 +42,7 @@ using g16::Tile;
 // tensor time, so products of k > 512, whose float32 error is larger anyway,
 // take two.
 inline int seg_for(int64_t K) { return K > 512 ? 2 : 1; }
-constexpr float SCALE = 4096.f, BOUND = 15.f;   // 15 x 2^12 < 65504
+constexpr float SCALE = kOrthScale, BOUND = 15.f;   // 15 x 2^12 < 65504
 
 // ---- |U|_F and the pieces of X_0 -----------------------------------------------
 constexpr int NORM_CHUNKS = 1024;
@@ -358,6 +359,11 @@ bool make_plan(const memlayer_orth_config& c, Plan* out) {
   p.lds = up(p.s, 8);
   p.xe = p.B * p.m * p.ldx;
   p.se = p.B * p.s * p.lds;
+  if (orth_in_cluster(c)) {            // needs the status word only
+    p.bytes = HEAD;
+    *out = p;
+    return true;
+  }
   size_t off = HEAD;
   auto take = [&](int64_t bytes) {
     const size_t o = off;
@@ -498,6 +504,7 @@ cudaError_t launch_orthogonalize(const memlayer_orth_config& c, const void* upda
   Plan p;
   if (!make_plan(c, &p)) return cudaErrorInvalidValue;
   int* err = reinterpret_cast<int*>(ws + O_ERR);
+  if (p.B > 0 && orth_in_cluster(c)) return launch_orth_chain(c, update, out, err, s);
   OR_TRY(cudaMemsetAsync(err, 0, sizeof(int), s));
   if (p.B == 0) return cudaSuccess;
   switch (c.dtype) {

@@ -485,6 +485,19 @@ def test_orthogonalize(shape, t):
     orth_within(x, orth_ref(u, 5, MUON, 1e-7), t)
 
 
+# one to eight CTAs a matrix, the last one's columns partly or all past the end; and the first sizes beyond
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("shape", [(16, 128, 256), (3, 128, 257), (3, 257, 65), (64, 512), (2, 65, 513), (513, 64), (2, 127, 1025),
+                                   (1030, 128), (128, 2048), (2048, 17), (3, 2047), (40, 8, 1100), (128, 2049), (2049, 64),
+                                   (129, 130), (2, 200, 129), (130, 1000)])
+def test_orthogonalize_small_sides(shape, t):
+    u = (1e-3 * torch.randn(*shape, device="cuda", generator=gen(sum(shape)))).to(t)
+    x = mb.orthogonalize(u, check=True)
+    assert x.dtype == t and x.shape == u.shape
+    orth_within(x, orth_ref(u, 5, MUON, 1e-7), t)
+    assert torch.equal(mb.orthogonalize(u), x)
+
+
 @pytest.mark.parametrize("steps,coef", [(1, MUON), (12, (1.5, -0.5, 0.0)), (8, (1.875, -1.25, 0.375))])
 def test_orthogonalize_other_iterations(steps, coef):
     u = torch.randn(96, 160, device="cuda", generator=gen(1))
