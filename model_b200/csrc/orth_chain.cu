@@ -13,8 +13,8 @@
 // once each way, and a product costs its MMAs, the drain of its accumulators
 // and a block barrier instead of a launch and the load of its operands.  Five
 // steps of float32, launches of orth.cu against this: 12 x 64 x 64 91 -> 29 us,
-// 128 x 128 103 -> 40, 4 x 128 x 256 116 -> 54, 64 x 1000 103 -> 60,
-// 128 x 2048 121 -> 79 (of which the cluster's sums are 35), 1000 x 64 x 64
+// 128 x 128 103 -> 39, 4 x 128 x 256 116 -> 52, 64 x 1000 103 -> 60,
+// 128 x 2048 121 -> 78 (of which the cluster's sums are 25), 1000 x 64 x 64
 // 324 -> 183.  Latency bounds it: a step's products wait for each other.
 //
 // Shared memory holds the rows of X and of P in blocks of 64 columns, 128
@@ -57,7 +57,7 @@ struct ChainArgs {
   int C, lc, steps;                            // CTAs a matrix, columns of each (a multiple of 64)
   float a, b, c;
   double eps;
-  int vec_in, vec_out;                         // eight columns as 16-byte vectors
+  int vec_in, vec_out;                         // eight columns in one access
   int* err;
 };
 
@@ -157,8 +157,32 @@ __device__ __forceinline__ void waited8(uint32_t at, float (&x)[8]) {
   x[4] = w.x, x[5] = w.y, x[6] = w.z, x[7] = w.w;
 }
 
+// Eight neighbouring values of global memory, in one access.
 template <typename E>
-struct alignas(16) Eight { E e[8]; };
+struct alignas(8 * sizeof(E)) Eight { E e[8]; };
+template <typename E>
+__device__ __forceinline__ Eight<E> read8(const E* p) {
+  return *reinterpret_cast<const Eight<E>*>(p);
+}
+template <>
+__device__ __forceinline__ Eight<float> read8(const float* p) {
+  Eight<float> v;
+  asm volatile("ld.global.v8.f32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=f"(v.e[0]), "=f"(v.e[1]), "=f"(v.e[2]), "=f"(v.e[3]), "=f"(v.e[4]), "=f"(v.e[5]), "=f"(v.e[6]),
+                 "=f"(v.e[7])
+               : "l"(p));
+  return v;
+}
+template <typename E>
+__device__ __forceinline__ void write8(E* p, const Eight<E>& v) {
+  *reinterpret_cast<Eight<E>*>(p) = v;
+}
+template <>
+__device__ __forceinline__ void write8(float* p, const Eight<float>& v) {
+  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(v.e[0]), "f"(v.e[1]),
+               "f"(v.e[2]), "f"(v.e[3]), "f"(v.e[4]), "f"(v.e[5]), "f"(v.e[6]), "f"(v.e[7])
+               : "memory");
+}
 
 // The two-piece product of 64 k, small terms first; a whole warp calls, lane
 // `one` issues (the operands stay in uniform registers).
@@ -253,7 +277,7 @@ __global__ void __launch_bounds__(NT, 1) orth_chain_kernel(const __grid_constant
       for (int i = 0; i < AHEAD; ++i) {
         int r, c;
         in[i] = item(e0 + i * NT, r, c) && r < S && c0 + c * 8 < L;
-        v[i] = *reinterpret_cast<const Eight<E>*>(in[i] ? u + at8(r, c) : u);
+        v[i] = read8(in[i] ? u + at8(r, c) : u);
       }
       float x[AHEAD][8];
 #pragma unroll
@@ -507,7 +531,7 @@ __global__ void __launch_bounds__(NT, 1) orth_chain_kernel(const __grid_constant
       Eight<E> v;
 #pragma unroll
       for (int j = 0; j < 8; ++j) v.e[j] = down<E>(x[j] * un);
-      *reinterpret_cast<Eight<E>*>(p) = v;
+      write8(p, v);
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
@@ -572,9 +596,10 @@ cudaError_t launch_orth_chain(const memlayer_orth_config& c, const void* update,
   a.b = c.b;
   a.c = c.c;
   a.eps = (double)c.epsilon;
-  const bool rows16 = !a.tall && c.cols % 8 == 0;
-  a.vec_in = rows16 && (reinterpret_cast<uintptr_t>(update) & 15) == 0;
-  a.vec_out = rows16 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+  const bool rows8 = !a.tall && c.cols % 8 == 0;
+  const uintptr_t mask = c.dtype == MEMLAYER_F32 ? 31 : 15;
+  a.vec_in = rows8 && (reinterpret_cast<uintptr_t>(update) & mask) == 0;
+  a.vec_out = rows8 && (reinterpret_cast<uintptr_t>(out) & mask) == 0;
   a.err = err;
   switch (c.dtype) {
     case MEMLAYER_F16: return launch<__half>(a, c.batch, s);
