@@ -11,7 +11,7 @@
 // in registers, so the variance is the centred one -- E[x^2] - E[x]^2 loses
 // the variance of a row whose mean is large -- and the gradient recomputes
 // mean and rstd from the row it reads anyway instead of reading them back.
-// Statistics and sums are float32 whatever the storage type.  Two layouts:
+// Statistics and sums are float32 whatever the storage type.  Three layouts:
 //
 //   group   a row in a power of two of threads, 16 values each; up to a warp
 //           (512 columns) its sums are shuffles.  Also every width whose rows
@@ -21,14 +21,21 @@
 //           parameter sums in registers (64 columns a lane), so few warps fit
 //           an SM; a ring of rows in shared memory, filled by bulk copies,
 //           keeps HBM busy beside them.  In a block per row its reductions
-//           took four times the instructions (16384 x 2048 bf16: 113 us);
-//   wide    beyond: a block per row.
+//           took four times the instructions (16384 x 2048 bf16: 113 us for
+//           the 66 of the ring);
+//   wide    beyond, a block per row.  Also packed rows of more than 512
+//           columns whose width is no multiple of a vector, by vectors that
+//           the rows begin inside of (forward and gradient of 9557 x 2498
+//           bf16 68 + 130 us, by single elements 211 + 304).
 //
 // The parameter gradients: dscale / dbias of the columns stay in registers over
 // all of a block's rows; it adds its row groups in shared memory and writes one
 // partial row; a second kernel adds the partials in block order,
 // so the result does not depend on timing (no atomics).
 #include "norm.cuh"
+
+#include <algorithm>
+#include <numeric>
 
 #include "gemm16.cuh"
 
@@ -443,116 +450,205 @@ __global__ void __launch_bounds__(128) layer_norm_warp_kernel(NormArgs A) {
   }
 }
 
+// Rows one after another in memory whose width is no multiple of a vector
+// (SHIFT): row r starts r d mod V entries into one.  A block takes rows of
+// the same start, so its columns keep their threads; the vectors at a row's
+// ends hold entries of the rows beside it, which are loaded with them (but
+// not past the last row), count for nothing and are not stored.
+template <int V>
+__device__ __forceinline__ bool at_edge(int j, int d) { return j < 0 || j + V > d; }
+template <int V>
+__device__ __forceinline__ bool in_row(int j, int k, int d) { return (unsigned)(j + k) < (unsigned)d; }
+
+template <typename E, int V, bool SHIFT>
+__device__ __forceinline__ Vec16<E, V> load_part(const E* row, int j, int d, bool last) {
+  if (SHIFT && last && j + V > d) {
+    Vec16<E, V> v;
+#pragma unroll
+    for (int k = 0; k < V; ++k) v.e[k] = j + k < d ? row[j + k] : Elem<E>::down(0.f);
+    return v;
+  }
+  return *reinterpret_cast<const Vec16<E, V>*>(row + j);
+}
+template <typename E, int V, bool SHIFT>
+__device__ __forceinline__ void store_part(E* row, int j, int d, const Vec16<E, V>& v) {
+  if (SHIFT && at_edge<V>(j, d)) {
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+      if (in_row<V>(j, k, d)) row[j + k] = v.e[k];
+  } else {
+    *reinterpret_cast<Vec16<E, V>*>(row + j) = v;
+  }
+}
+// The entries of other rows replaced.
+template <int V, bool SHIFT>
+__device__ __forceinline__ void keep_row(float (&x)[V], int j, int d, float other) {
+  if (SHIFT && at_edge<V>(j, d)) {
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+      if (!in_row<V>(j, k, d)) x[k] = other;
+  }
+}
+template <int V, bool SHIFT>
+__device__ __forceinline__ void keep_row(F2 (&x)[V / 2], int j, int d, float other) {
+  if (SHIFT && at_edge<V>(j, d)) {
+#pragma unroll
+    for (int k = 0; k < V / 2; ++k) {
+      float a, b;
+      split(x[k], a, b);
+      x[k] = f2(in_row<V>(j, 2 * k, d) ? a : other, in_row<V>(j, 2 * k + 1, d) ? b : other);
+    }
+  }
+}
+// The parameters of a thread's columns: aligned, or entry by entry, zeros outside.
+template <int V, bool SHIFT>
+__device__ __forceinline__ void load_columns(const float* p, int j, int d, float (&x)[V]) {
+  if constexpr (SHIFT) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) x[k] = in_row<V>(j, k, d) ? p[j + k] : 0.f;
+  } else {
+    load_f32(p + j, x);
+  }
+}
+template <int V, bool SHIFT>
+__device__ __forceinline__ int block_shift(int d) { return SHIFT ? (int)((blockIdx.x * (unsigned)d) & (V - 1)) : 0; }
+
 // A row in a block, for rows that a warp does not hold: thread t has columns
-// (i blockDim + t) V .. + V, i < NV.
-template <typename E, int NV, int MAXT>
-__global__ void __launch_bounds__(MAXT, 1) layer_norm_wide_kernel(NormArgs A) {
+// (i blockDim + t) V .. + V, i < NV (less the shift).
+template <typename E, int NV, int MAXT, int MINB, bool SHIFT>
+__global__ void __launch_bounds__(MAXT, MINB) layer_norm_wide_kernel(NormArgs A) {
   constexpr int V = 16 / sizeof(E);
   using Vec = Vec16<E, V>;
   __shared__ alignas(16) float red[2][32];
-  const int d = A.d, t = threadIdx.x, nt = blockDim.x;
+  const int d = A.d, t = threadIdx.x, nt = blockDim.x, o = block_shift<V, SHIFT>(d);
   if (t < 64) (&red[0][0])[t] = 0.f;     // slots without a warp
   __syncthreads();
+  float scale[NV][V], bias[NV][V];       // SHIFT: kept over the block's rows
+  if constexpr (SHIFT) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int j = (i * nt + t) * V - o;
+      if (j >= d) continue;
+      load_columns<V, true>(A.scale, j, d, scale[i]);
+      load_columns<V, true>(A.bias, j, d, bias[i]);
+    }
+  }
   for (int64_t row = blockIdx.x; row < A.rows; row += gridDim.x) {
-    Vec p[NV];
+    const bool last = row + 1 == A.rows;
+    Vec p[NV], q[NV];
     float s[1] = {0.f}, s2[1] = {0.f};
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int j = (i * nt + t) * V;
-      if (j < d) p[i] = *reinterpret_cast<const Vec*>(reinterpret_cast<const E*>(A.x) + row * A.ldx + j);
+      const int j = (i * nt + t) * V - o;
+      if (j >= d) continue;
+      p[i] = load_part<E, V, SHIFT>(reinterpret_cast<const E*>(A.x) + row * A.ldx, j, d, last);
+      if (A.r) q[i] = load_part<E, V, SHIFT>(reinterpret_cast<const E*>(A.r) + row * A.ldr, j, d, last);
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int j = (i * nt + t) * V;
+      const int j = (i * nt + t) * V - o;
       if (j >= d) continue;
       float a[V];
       unpack(p[i], a);
       if (A.r) {
         float b[V];
-        unpack(*reinterpret_cast<const Vec*>(reinterpret_cast<const E*>(A.r) + row * A.ldr + j), b);
+        unpack(q[i], b);
 #pragma unroll
         for (int k = 0; k < V; ++k) a[k] += b[k];
         pack(p[i], a);
         unpack(p[i], a);
-        if (A.sum) *reinterpret_cast<Vec*>(reinterpret_cast<E*>(A.sum) + row * (int64_t)d + j) = p[i];
+        if (A.sum) store_part<E, V, SHIFT>(reinterpret_cast<E*>(A.sum) + row * (int64_t)d, j, d, p[i]);
       }
+      keep_row<V, SHIFT>(a, j, d, 0.f);
 #pragma unroll
       for (int k = 0; k < V; ++k) s[0] += a[k];
     }
     block_sums(s, red[0]);
     const float mean = s[0] * A.inv_d;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if ((i * nt + t) * V < d) {
-        float a[V];
-        unpack(p[i], a);
+    for (int i = 0; i < NV; ++i) {
+      const int j = (i * nt + t) * V - o;
+      if (j >= d) continue;
+      float a[V];
+      unpack(p[i], a);
+      keep_row<V, SHIFT>(a, j, d, mean);
 #pragma unroll
-        for (int k = 0; k < V; ++k) {
-          const float c = a[k] - mean;
-          s2[0] = fmaf(c, c, s2[0]);
-        }
+      for (int k = 0; k < V; ++k) {
+        const float c = a[k] - mean;
+        s2[0] = fmaf(c, c, s2[0]);
       }
+    }
     block_sums(s2, red[1]);
     const float rstd = 1.0f / sqrtf(s2[0] * A.inv_d + A.eps);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int j = (i * nt + t) * V;
+      const int j = (i * nt + t) * V - o;
       if (j >= d) continue;
       float a[V], sc[V], bi[V];
       unpack(p[i], a);
-      load_f32(A.scale + j, sc);
-      load_f32(A.bias + j, bi);
+      if constexpr (SHIFT) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+          sc[k] = scale[i][k];
+          bi[k] = bias[i][k];
+        }
+      } else {
+        load_f32(A.scale + j, sc);
+        load_f32(A.bias + j, bi);
+      }
 #pragma unroll
       for (int k = 0; k < V; ++k) a[k] = fmaf((a[k] - mean) * rstd, sc[k], bi[k]);
       pack(p[i], a);
-      *reinterpret_cast<Vec*>(reinterpret_cast<E*>(A.y) + row * (int64_t)d + j) = p[i];
+      store_part<E, V, SHIFT>(reinterpret_cast<E*>(A.y) + row * (int64_t)d, j, d, p[i]);
     }
   }
 }
 
 // R rows of a block's batch, as loaded.
-template <typename E, int R, int NV>
+template <typename E, int R, int NV, bool SHIFT>
 struct Batch {
   static constexpr int V = 16 / sizeof(E);
   Vec16<E, V> p[R][NV], q[R][NV], e[R][NV];
-  __device__ __forceinline__ void load(const NormArgs& A, int64_t base) {
-    using Vec = Vec16<E, V>;
+  __device__ __forceinline__ void load(const NormArgs& A, int64_t base, int o) {
     const int t = threadIdx.x, nt = blockDim.x;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      if (base + r >= A.rows) break;
+      const int64_t row = base + r;
+      if (row >= A.rows) break;
+      const bool last = row + 1 == A.rows;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int j = (i * nt + t) * V;
+        const int j = (i * nt + t) * V - o;
         if (j >= A.d) continue;
-        p[r][i] = *reinterpret_cast<const Vec*>(reinterpret_cast<const E*>(A.x) + (base + r) * A.ldx + j);
-        q[r][i] = *reinterpret_cast<const Vec*>(reinterpret_cast<const E*>(A.dy) + (base + r) * A.lddy + j);
-        if (A.dr) e[r][i] = *reinterpret_cast<const Vec*>(reinterpret_cast<const E*>(A.dr) + (base + r) * A.lddr + j);
+        p[r][i] = load_part<E, V, SHIFT>(reinterpret_cast<const E*>(A.x) + row * A.ldx, j, A.d, last);
+        q[r][i] = load_part<E, V, SHIFT>(reinterpret_cast<const E*>(A.dy) + row * A.lddy, j, A.d, last);
+        if (A.dr) e[r][i] = load_part<E, V, SHIFT>(reinterpret_cast<const E*>(A.dr) + row * A.lddr, j, A.d, last);
       }
     }
   }
 };
 
 // AHEAD: the next batch's loads are issued before this one's sums, so HBM is
-// busy during the barriers (where the registers allow it).
-template <typename E, int R, int NV, int MAXT, bool AHEAD>
-__global__ void __launch_bounds__(MAXT, MAXT <= 256 ? 2 : 1) layer_norm_wide_backward_kernel(NormArgs A) {
+// busy during the barriers (where the registers allow it: shifted 16-bit rows
+// would spill, 155 us for 130 at 9557 x 2498).
+template <typename E, int R, int NV, int MAXT, int MINB, bool AHEAD, bool SHIFT>
+__global__ void __launch_bounds__(MAXT, MINB) layer_norm_wide_backward_kernel(NormArgs A) {
   constexpr int V = 16 / sizeof(E), H = V / 2;
   using Vec = Vec16<E, V>;
   allow_next();                            // of the kernel that adds the partials
   __shared__ alignas(16) float red[2][3 * R * 32];
-  const int d = A.d, t = threadIdx.x, nt = blockDim.x;
+  const int d = A.d, t = threadIdx.x, nt = blockDim.x, o = block_shift<V, SHIFT>(d);
   for (int i = t; i < 2 * 3 * R * 32; i += nt) (&red[0][0])[i] = 0.f;   // slots without a warp
   __syncthreads();
   if (blockIdx.x == 0 && threadIdx.x == 0) *A.err = 0;
   F2 ag[NV][H], ab[NV][H], sc[NV][H];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int j = (i * nt + t) * V;
+    const int j = (i * nt + t) * V - o;
     float f[V];
 #pragma unroll
     for (int k = 0; k < V; ++k) f[k] = 0.f;
-    if (j < d) load_f32(A.scale + j, f);
+    if (j < d) load_columns<V, SHIFT>(A.scale, j, d, f);
 #pragma unroll
     for (int k = 0; k < H; ++k) {
       ag[i][k] = ab[i][k] = f2(0.f);
@@ -560,15 +656,15 @@ __global__ void __launch_bounds__(MAXT, MAXT <= 256 ? 2 : 1) layer_norm_wide_bac
     }
   }
   const int64_t step = (int64_t)gridDim.x * R;
-  Batch<E, R, NV> next;
-  if constexpr (AHEAD) next.load(A, (int64_t)blockIdx.x * R);
+  Batch<E, R, NV, SHIFT> next;
+  if constexpr (AHEAD) next.load(A, (int64_t)blockIdx.x * R, o);
   for (int64_t base = (int64_t)blockIdx.x * R; base < A.rows; base += step) {
-    Batch<E, R, NV> b;
+    Batch<E, R, NV, SHIFT> b;
     if constexpr (AHEAD) {
       b = next;
-      next.load(A, base + step);
+      next.load(A, base + step, o);
     } else {
-      b.load(A, base);
+      b.load(A, base, o);
     }
     float s[R];
 #pragma unroll
@@ -576,9 +672,10 @@ __global__ void __launch_bounds__(MAXT, MAXT <= 256 ? 2 : 1) layer_norm_wide_bac
       F2 acc = f2(0.f);
 #pragma unroll
       for (int i = 0; i < NV; ++i)
-        if ((i * nt + t) * V < d) {
+        if (const int j = (i * nt + t) * V - o; j < d) {
           F2 a[H];
           unpack2(b.p[r][i], a);
+          keep_row<V, SHIFT>(a, j, d, 0.f);
 #pragma unroll
           for (int k = 0; k < H; ++k) acc = acc + a[k];
         }
@@ -589,14 +686,17 @@ __global__ void __launch_bounds__(MAXT, MAXT <= 256 ? 2 : 1) layer_norm_wide_bac
     float m[3 * R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const F2 mean = f2(-(s[r] * A.inv_d));
+      const float mean_f = s[r] * A.inv_d;
+      const F2 mean = f2(-mean_f);
       F2 s2 = f2(0.f), sg = f2(0.f), sgc = f2(0.f);
 #pragma unroll
       for (int i = 0; i < NV; ++i)
-        if ((i * nt + t) * V < d) {
+        if (const int j = (i * nt + t) * V - o; j < d) {
           F2 a[H], g[H];
           unpack2(b.p[r][i], a);
           unpack2(b.q[r][i], g);
+          keep_row<V, SHIFT>(a, j, d, mean_f);
+          keep_row<V, SHIFT>(g, j, d, 0.f);
 #pragma unroll
           for (int k = 0; k < H; ++k) {
             const F2 c = a[k] + mean, gy = g[k] * sc[i][k];
@@ -618,7 +718,7 @@ __global__ void __launch_bounds__(MAXT, MAXT <= 256 ? 2 : 1) layer_norm_wide_bac
                c2 = f2(-(m[3 * r + 2] * rstd_f * A.inv_d));
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int j = (i * nt + t) * V;
+        const int j = (i * nt + t) * V - o;
         if (j >= d) continue;
         F2 a[H], g[H];
         float x[V];
@@ -638,26 +738,26 @@ __global__ void __launch_bounds__(MAXT, MAXT <= 256 ? 2 : 1) layer_norm_wide_bac
         }
 #pragma unroll
         for (int k = 0; k < H; ++k) split(a[k], x[2 * k], x[2 * k + 1]);
-        Vec o;
-        pack(o, x);
-        *reinterpret_cast<Vec*>(reinterpret_cast<E*>(A.dx) + (base + r) * (int64_t)d + j) = o;
+        Vec v;
+        pack(v, x);
+        store_part<E, V, SHIFT>(reinterpret_cast<E*>(A.dx) + (base + r) * (int64_t)d, j, d, v);
       }
     }
   }
   float* out = A.part + (int64_t)blockIdx.x * 2 * d;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    const int j = (i * nt + t) * V;
+    const int j = (i * nt + t) * V - o;
     if (j >= d) continue;
 #pragma unroll
     for (int k = 0; k < H; ++k) {
       float a, c;
       split(ag[i][k], a, c);
-      out[j + 2 * k] = a;
-      out[j + 2 * k + 1] = c;
+      if (!SHIFT || in_row<V>(j, 2 * k, d)) out[j + 2 * k] = a;
+      if (!SHIFT || in_row<V>(j, 2 * k + 1, d)) out[j + 2 * k + 1] = c;
       split(ab[i][k], a, c);
-      out[d + j + 2 * k] = a;
-      out[d + j + 2 * k + 1] = c;
+      if (!SHIFT || in_row<V>(j, 2 * k, d)) out[d + j + 2 * k] = a;
+      if (!SHIFT || in_row<V>(j, 2 * k + 1, d)) out[d + j + 2 * k + 1] = c;
     }
   }
 }
@@ -861,19 +961,41 @@ bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // The block-per-row layouts: threads a row, vectors a thread, rows at a time.
 struct Wide {
-  int nt, nv, r;
+  int nt, nv;
+  // Blocks of an SM where `most` of 256 threads fit, more of smaller ones.
+  int per_sm(int most) const { return nt <= 256 ? most * 256 / nt : 1; }
 };
 
 bool wide_rows(int d, int v) { return d > 32 * VALS && d % v == 0; }
 
+// Up to 4096 columns in blocks of at most 256 threads, several on an SM
+// (gradient of 4096 x 4096 float32 56 us, in one block of 1024 105); beyond in
+// one of up to 1024.
 Wide wide_for(int d, int v) {
   const int vecs = (d + v - 1) / v;
-  if (vecs <= 1024) return {(vecs + 31) / 32 * 32, 1, 1};
-  const int nv = vecs <= 2048 ? 2 : 4;
-  return {((vecs + nv - 1) / nv + 31) / 32 * 32, nv, 1};
+  int nv = 1;
+  if (vecs * v <= 4096)
+    while (vecs > 256 * nv) nv *= 2;
+  else
+    nv = vecs <= 1024 ? 1 : vecs <= 2048 ? 2 : 4;
+  return {((vecs + nv - 1) / nv + 31) / 32 * 32, nv};
 }
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// How a call's rows are read: by entries, by 16-byte vectors, or by vectors
+// that rows packed one after another start inside of (SHIFT).
+enum Access { ENTRIES, VECTORS, SHIFTED };
+
+bool shifted_rows(int d, int v) { return wide_rows(d, 1) && wide_for(d + v - 1, v).nt <= 1024; }
+
+// Blocks for shifted rows: at most `most`, and then a multiple of the rows
+// after which starts repeat.
+int shifted_grid(int64_t rows, int d, int v, int64_t most) {
+  if (rows <= most) return (int)rows;
+  const int period = v / std::gcd(d, v);
+  return (int)(most / period * period);
+}
 
 // The ring layout of the gradient: rows of up to 256 vectors (16-bit) or 512
 // (float32), 64 columns a lane; as many warps as the rings leave room for.
@@ -897,10 +1019,35 @@ Ring ring_for(int d, int esize) {
 }
 
 template <typename E>
-cudaError_t norm_forward_t(NormArgs& A, bool vec, cudaStream_t s) {
+cudaError_t norm_forward_t(NormArgs& A, Access how, cudaStream_t s) {
   constexpr int V = 16 / sizeof(E);
   constexpr int64_t MOST = 1 << 20;
   const int vecs = A.d / V;
+  const bool vec = how == VECTORS;
+  if (how == SHIFTED) {
+    // 16-bit rows of up to 4096 columns: a vector a thread in blocks of up to
+    // 512 (9557 x 2498 68 us, two vectors in blocks of 160 82)
+    Wide w = wide_for(A.d + V - 1, V);
+    if (V == 8 && w.nv == 2 && w.nt <= 256) w = {(int)ceil_div(A.d + V - 1, V * 32) * 32, 1};
+    const int most = w.nt > 256 ? 1024 / w.nt : w.per_sm(w.nv * V > 8 ? 3 : 4);
+    const int grid = shifted_grid(A.rows, A.d, V, (int64_t)most * g16::device_sms());
+    if (w.nt > 256 && w.nv == 1)
+      layer_norm_wide_kernel<E, 1, 1024, 1, true><<<grid, w.nt, 0, s>>>(A);
+    else if (w.nt > 256 && w.nv == 2)
+      layer_norm_wide_kernel<E, 2, 1024, 1, true><<<grid, w.nt, 0, s>>>(A);
+    else if (w.nt > 256)
+      layer_norm_wide_kernel<E, 4, 1024, 1, true><<<grid, w.nt, 0, s>>>(A);
+    else if (w.nv == 1)
+      layer_norm_wide_kernel<E, 1, 256, 4, true><<<grid, w.nt, 0, s>>>(A);
+    else if constexpr (V == 4) {
+      if (w.nv == 2)
+        layer_norm_wide_kernel<E, 2, 256, 4, true><<<grid, w.nt, 0, s>>>(A);
+      else
+        layer_norm_wide_kernel<E, 4, 256, 3, true><<<grid, w.nt, 0, s>>>(A);
+    }
+    count_launch();
+    return cudaGetLastError();
+  }
   const bool warp = A.d > 32 * VALS && (vec ? vecs <= 512 : A.d <= 2048);
   if (warp) {
     const int64_t grid = ceil_div(A.rows, 4);
@@ -919,11 +1066,11 @@ cudaError_t norm_forward_t(NormArgs& A, bool vec, cudaStream_t s) {
     const Wide w = wide_for(A.d, V);
     const int grid = (int)(A.rows < MOST ? A.rows : MOST);
     if (w.nv == 1)
-      layer_norm_wide_kernel<E, 1, 1024><<<grid, w.nt, 0, s>>>(A);
+      layer_norm_wide_kernel<E, 1, 1024, 1, false><<<grid, w.nt, 0, s>>>(A);
     else if (w.nv == 2)
-      layer_norm_wide_kernel<E, 2, 1024><<<grid, w.nt, 0, s>>>(A);
+      layer_norm_wide_kernel<E, 2, 1024, 1, false><<<grid, w.nt, 0, s>>>(A);
     else if constexpr (sizeof(E) == 4)   // 16-bit rows end at two vectors
-      layer_norm_wide_kernel<E, 4, 1024><<<grid, w.nt, 0, s>>>(A);
+      layer_norm_wide_kernel<E, 4, 1024, 1, false><<<grid, w.nt, 0, s>>>(A);
   } else {
     const bool wide = A.tpr > 32;
     const int nt = wide ? A.tpr : NT;
@@ -950,10 +1097,33 @@ cudaError_t launch_ring(const NormArgs& A, const Ring& r, int grid, cudaStream_t
   return cudaSuccess;
 }
 
-template <typename E>
-cudaError_t norm_backward_t(NormArgs& A, bool vec, int grid, cudaStream_t s) {
+// Blocks of 256 threads an SM holds with the gradient's registers: by columns a thread.
+int backward_resident(int cols) { return cols <= 4 ? 4 : cols <= 8 ? 3 : 2; }
+
+template <typename E, bool SHIFT>
+void launch_wide_backward(const NormArgs& A, const Wide& w, int grid, cudaStream_t s) {
   constexpr int V = 16 / sizeof(E);
-  if (vec && ring_rows(A.d, V)) {
+  if (w.nt > 256 && w.nv == 1)
+    layer_norm_wide_backward_kernel<E, 1, 1, 1024, 1, false, SHIFT><<<grid, w.nt, 0, s>>>(A);
+  else if (w.nt > 256 && w.nv == 2)
+    layer_norm_wide_backward_kernel<E, 1, 2, 1024, 1, false, SHIFT><<<grid, w.nt, 0, s>>>(A);
+  else if (w.nt > 256)
+    layer_norm_wide_backward_kernel<E, 1, 4, 1024, 1, false, SHIFT><<<grid, w.nt, 0, s>>>(A);
+  else if (w.nv == 1)
+    layer_norm_wide_backward_kernel<E, 1, 1, 256, V == 4 ? 4 : 3, V == 4 || !SHIFT, SHIFT><<<grid, w.nt, 0, s>>>(A);
+  else if (w.nv == 2)
+    layer_norm_wide_backward_kernel<E, 1, 2, 256, V == 4 ? 3 : 2, V == 4 || !SHIFT, SHIFT><<<grid, w.nt, 0, s>>>(A);
+  else if constexpr (V == 4)
+    layer_norm_wide_backward_kernel<E, 1, 4, 256, 2, false, SHIFT><<<grid, w.nt, 0, s>>>(A);
+}
+
+template <typename E>
+cudaError_t norm_backward_t(NormArgs& A, Access how, int grid, cudaStream_t s) {
+  constexpr int V = 16 / sizeof(E);
+  const bool vec = how == VECTORS;
+  if (how == SHIFTED) {
+    launch_wide_backward<E, true>(A, wide_for(A.d + V - 1, V), grid, s);
+  } else if (vec && ring_rows(A.d, V)) {
     const Ring r = ring_for(A.d, sizeof(E));
     cudaError_t e;
     if (A.d <= 1024)
@@ -962,15 +1132,7 @@ cudaError_t norm_backward_t(NormArgs& A, bool vec, int grid, cudaStream_t s) {
       e = launch_ring<E, 64 / V, 8>(A, r, grid, s);
     if (e != cudaSuccess) return e;
   } else if (vec && wide_rows(A.d, V)) {
-    const Wide w = wide_for(A.d, V);
-    if (w.nv == 1 && w.nt <= 512)
-      layer_norm_wide_backward_kernel<E, 1, 1, 512, true><<<grid, w.nt, 0, s>>>(A);
-    else if (w.nv == 1)
-      layer_norm_wide_backward_kernel<E, 1, 1, 1024, false><<<grid, w.nt, 0, s>>>(A);
-    else if (w.nv == 2)
-      layer_norm_wide_backward_kernel<E, 1, 2, 1024, false><<<grid, w.nt, 0, s>>>(A);
-    else if constexpr (sizeof(E) == 4)
-      layer_norm_wide_backward_kernel<E, 1, 4, 1024, false><<<grid, w.nt, 0, s>>>(A);
+    launch_wide_backward<E, false>(A, wide_for(A.d, V), grid, s);
   } else {
     const bool wide = A.tpr > 32;
     const int nt = wide ? A.tpr : NT;
@@ -989,15 +1151,20 @@ cudaError_t norm_backward_t(NormArgs& A, bool vec, int grid, cudaStream_t s) {
 }
 
 // Blocks of the gradient's row pass: as many as are resident at once.
-int backward_blocks(int64_t rows, int d, int v, bool vec) {
+int backward_blocks(int64_t rows, int d, int v, Access how) {
   int64_t need, per_sm;
+  const bool vec = how == VECTORS;
+  if (how == SHIFTED) {
+    const Wide w = wide_for(d + v - 1, v);
+    return shifted_grid(rows, d, v, (int64_t)w.per_sm(backward_resident(w.nv * v)) * g16::device_sms());
+  }
   if (vec && ring_rows(d, v)) {
     need = ceil_div(rows, ring_for(d, 16 / v).warps);
     per_sm = 1;
   } else if (vec && wide_rows(d, v)) {
     const Wide w = wide_for(d, v);
-    need = ceil_div(rows, w.r);
-    per_sm = w.nt <= 256 ? 512 / w.nt : 1;
+    need = rows;
+    per_sm = w.per_sm(backward_resident(w.nv * v));
   } else {
     const int tpr = norm_tpr(d), nt = tpr > 32 ? tpr : NT;
     need = ceil_div(rows, nt / tpr);
@@ -1012,8 +1179,9 @@ int backward_blocks(int64_t rows, int d, int v, bool vec) {
 // The most that any alignment of the call's tensors takes.
 int norm_backward_blocks(int64_t rows, int d, int dtype) {
   const int v = dtype == MEMLAYER_F32 ? 4 : 8;
-  const int a = backward_blocks(rows, d, v, true), b = backward_blocks(rows, d, v, false);
-  return a > b ? a : b;
+  int most = 0;
+  for (Access how : {ENTRIES, VECTORS, SHIFTED}) most = std::max(most, backward_blocks(rows, d, v, how));
+  return most;
 }
 
 cudaError_t launch_layer_norm(const memlayer_norm_config& c, const memlayer_norm_args& a, cudaStream_t s) {
@@ -1033,12 +1201,18 @@ cudaError_t launch_layer_norm(const memlayer_norm_config& c, const memlayer_norm
   A.y = a.y;
   A.sum = a.sum;
   const int v = c.dtype == MEMLAYER_F32 ? 4 : 8;
-  const bool vec = c.d_model % v == 0 && a.x_stride % v == 0 && (!a.residual || a.residual_stride % v == 0) &&
-                   al16(a.x) && al16(a.residual) && al16(a.y) && al16(a.sum) && al16(a.scale) && al16(a.bias);
+  const bool base = al16(a.x) && al16(a.residual) && al16(a.y) && al16(a.sum);
+  Access how = ENTRIES;
+  if (base && al16(a.scale) && al16(a.bias) && c.d_model % v == 0 && a.x_stride % v == 0 &&
+      (!a.residual || a.residual_stride % v == 0))
+    how = VECTORS;
+  else if (base && shifted_rows(c.d_model, v) && a.x_stride == c.d_model &&
+           (!a.residual || a.residual_stride == c.d_model))
+    how = SHIFTED;
   switch (c.dtype) {
-    case MEMLAYER_F16: return norm_forward_t<__half>(A, vec, s);
-    case MEMLAYER_BF16: return norm_forward_t<__nv_bfloat16>(A, vec, s);
-    default: return norm_forward_t<float>(A, vec, s);
+    case MEMLAYER_F16: return norm_forward_t<__half>(A, how, s);
+    case MEMLAYER_BF16: return norm_forward_t<__nv_bfloat16>(A, how, s);
+    default: return norm_forward_t<float>(A, how, s);
   }
 }
 
@@ -1061,15 +1235,20 @@ cudaError_t launch_layer_norm_backward(const memlayer_norm_config& c, const meml
   A.part = part;
   A.err = err;
   const int v = c.dtype == MEMLAYER_F32 ? 4 : 8;
-  const bool vec = c.d_model % v == 0 && g.x_stride % v == 0 && g.dy_stride % v == 0 &&
-                   (!g.dresidual || g.dresidual_stride % v == 0) && al16(g.x) && al16(g.dy) && al16(g.dresidual) &&
-                   al16(g.dx) && al16(g.scale);
-  const int grid = backward_blocks(c.rows, c.d_model, v, vec);
+  const bool base = al16(g.x) && al16(g.dy) && al16(g.dresidual) && al16(g.dx);
+  Access how = ENTRIES;
+  if (base && al16(g.scale) && c.d_model % v == 0 && g.x_stride % v == 0 && g.dy_stride % v == 0 &&
+      (!g.dresidual || g.dresidual_stride % v == 0))
+    how = VECTORS;
+  else if (base && shifted_rows(c.d_model, v) && g.x_stride == c.d_model && g.dy_stride == c.d_model &&
+           (!g.dresidual || g.dresidual_stride == c.d_model))
+    how = SHIFTED;
+  const int grid = backward_blocks(c.rows, c.d_model, v, how);
   cudaError_t e = cudaSuccess;
   if (grid > 0) switch (c.dtype) {
-      case MEMLAYER_F16: e = norm_backward_t<__half>(A, vec, grid, s); break;
-      case MEMLAYER_BF16: e = norm_backward_t<__nv_bfloat16>(A, vec, grid, s); break;
-      default: e = norm_backward_t<float>(A, vec, grid, s); break;
+      case MEMLAYER_F16: e = norm_backward_t<__half>(A, how, grid, s); break;
+      case MEMLAYER_BF16: e = norm_backward_t<__nv_bfloat16>(A, how, grid, s); break;
+      default: e = norm_backward_t<float>(A, how, grid, s); break;
     }
   if (e != cudaSuccess) return e;
   count_launch();

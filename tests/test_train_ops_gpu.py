@@ -114,6 +114,42 @@ def test_norm_forward_and_backward(M, d, t):
     check_norm_backward(dx, dp, dy, s, scale, dr, 1e-5, t)
 
 
+# packed rows that begin inside of a 16-byte vector: fewer and more of them than blocks, one or several vectors a thread
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("M,d", [(1, 513), (2, 515), (9, 516), (3001, 514), (2003, 1001), (1501, 2047), (1200, 2498), (700, 4097),
+                                 (310, 8201), (5, 9001), (3, 16381), (2, 16383)])
+def test_norm_rows_between_vectors(M, d, t):
+    x, r, scale, bias, dy, dr = norm_case(M, d, t, seed=M + d)
+    y, s = mb.layer_norm(x, scale, bias, residual=r, eps=1e-5)
+    assert torch.equal(s, (x.float() + r.float()).to(t))
+    want, tol, *_ = norm_ref(s, scale, bias, 1e-5)
+    within(y, want, tol + half_step(t) * want.abs() + tiny(t), "y")
+    within(mb.layer_norm(s, scale, bias, eps=1e-5), want, tol + half_step(t) * want.abs() + tiny(t), "y alone")
+    dx, dp = mb.layer_norm_backward(dy, s, scale, dresidual=dr, eps=1e-5, check=True)
+    check_norm_backward(dx, dp, dy, s, scale, dr, 1e-5, t)
+    dx, dp = mb.layer_norm_backward(dy, s, scale, eps=1e-5)
+    check_norm_backward(dx, dp, dy, s, scale, None, 1e-5, t)
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_norm_rows_between_vectors_keep_to_themselves(t):
+    M, d = 1500, 1003
+    x, _, scale, bias, dy, _ = norm_case(M, d, t, seed=21)
+    clean, (cdx, _) = mb.layer_norm(x, scale, bias), mb.layer_norm_backward(dy, x, scale)
+    bad = list(range(1, M, 7))
+    x[bad, 0], x[bad, d - 1], dy[bad, d - 1] = float("nan"), float("inf"), float("nan")
+    y, (dx, _) = mb.layer_norm(x, scale, bias), mb.layer_norm_backward(dy, x, scale)
+    keep = [i for i in range(M) if i % 7 != 1]
+    assert torch.equal(y[keep], clean[keep]) and torch.equal(dx[keep], cdx[keep])
+    assert torch.isnan(y[bad]).all() and torch.isnan(dx[bad]).all()
+    # what is around the rows stays as it was
+    room = torch.full((M * d + 64,), 7.0, device="cuda").to(t)
+    inner = room[32:32 + M * d].view(M, d)
+    inner.copy_(cdx)
+    before = room.clone()
+    assert torch.equal(mb.layer_norm(inner, scale, bias), mb.layer_norm(cdx, scale, bias)) and torch.equal(room, before)
+
+
 @pytest.mark.parametrize("t", TYPES)
 def test_norm_many_rows(t):
     x, _, scale, bias, dy, _ = norm_case(20011, 48, t, seed=5)
