@@ -548,6 +548,62 @@ def test_orthogonalize_brings_singular_values_near_one():
     assert 0.6 < float(s.min()) and float(s.max()) < 1.22
 
 
+@pytest.mark.parametrize("shape", [(100, 200), (60, 700), (700, 60), (128, 2048)])
+def test_orthogonalize_special_values_of_small_sides(shape):
+    u = torch.randn(*shape, device="cuda", generator=gen(7))
+    a = mb.orthogonalize(u, eps=0.0)
+    for s in (2.0 ** 70, 2.0 ** -70):                                      # as below
+        assert torch.equal(mb.orthogonalize(u * s, eps=0.0), a)
+    assert not mb.orthogonalize(torch.zeros(2, *shape, device="cuda")).any()
+    b = torch.stack([u, u, u, u])
+    b[1, shape[0] - 1, shape[1] - 1], b[2, 0, 0] = float("nan"), float("inf")
+    x = mb.orthogonalize(b, eps=0.0)
+    assert torch.equal(x[0], a) and torch.equal(x[3], a) and torch.isnan(x[1:3]).all()
+    for off in (1, 4):                                                     # 4- and 16-byte aligned
+        shifted = torch.empty(u.numel() + off, device="cuda")[off:].view(*shape)
+        shifted.copy_(u)
+        assert torch.equal(mb.orthogonalize(shifted, eps=0.0), a)
+    # what is around the result stays as it was
+    room = torch.full((u.numel() + 64,), 3.0, device="cuda")
+    cfg = L.MemlayerOrthConfig(1, *shape, L.F32, 5, 3.4445, -4.7750, 2.0315, 0.0)
+    ws = torch.empty(512, dtype=torch.uint8, device="cuda")
+    assert L.lib().memlayer_orthogonalize(cfg, u.data_ptr(), room[32:].data_ptr(), ws.data_ptr(), 512,
+                                          torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(room[32:-32].view(*shape), a) and (room[:32] == 3).all() and (room[-32:] == 3).all()
+
+
+def test_small_updates_beside_other_calls():
+    us = [torch.randn(*s, device="cuda", generator=gen(i)) for i, s in enumerate([(30, 64, 64), (9, 128, 700), (2, 300, 300),
+                                                                                  (4, 1500, 100)])]
+    h, w = torch.randn(700, 256, device="cuda", generator=gen(8)), torch.randn(3000, 256, device="cuda", generator=gen(9)) * 0.1
+    y = torch.randint(0, 3000, (700,), device="cuda", generator=gen(10))
+    want, loss = [mb.orthogonalize(u) for u in us], mb.linear_cross_entropy(h, w, y)[0]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(5)]
+    got = []
+    for _ in range(20):
+        got.append([mb.orthogonalize(u, stream=s) for u, s in zip(us, streams)]
+                   + [mb.linear_cross_entropy(h, w, y, stream=streams[4])[0]])
+    torch.cuda.synchronize()
+    for x in got:
+        assert all(torch.equal(a, b) for a, b in zip(x, want + [loss]))
+
+
+def test_small_update_captured_and_replayed():
+    u = torch.randn(3, 100, 900, device="cuda", generator=gen(11))
+    mb.orthogonalize(u)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x = mb.orthogonalize(u)
+        z = mb.orthogonalize(x, steps=2)
+    for i in range(3):
+        u.copy_(torch.randn(3, 100, 900, device="cuda", generator=gen(20 + i)))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(x, mb.orthogonalize(u)) and torch.equal(z, mb.orthogonalize(x, steps=2))
+
+
 def test_orthogonalize_scales_and_special_values():
     u = torch.randn(40, 56, device="cuda", generator=gen(4))
     a = mb.orthogonalize(u, eps=0.0)
