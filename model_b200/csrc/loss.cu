@@ -210,14 +210,15 @@ __global__ void __launch_bounds__(256) loss_join_kernel(const float2* __restrict
 }
 
 // ---- few float32 tokens --------------------------------------------------------------
-// Up to 16 float32 tokens: the weight is read once and everything else waits
+// Up to 24 float32 tokens: the weight is read once and everything else waits
 // for it, while the two-piece form of the tensor cores would read it twice
 // more.  A block takes 128 vocabulary entries, a thread one of them against
 // four tokens (float32 FMAs, two columns an instruction); 64 columns of the
 // block's rows at a time come through a ring of asynchronous copies, deep
-// enough for all of a 256-wide row.  16 x 256 over 16,384 entries: the call
-// takes 20 us instead of the 30 of pieces and tiles.
-constexpr int FEW = 16, FEW_V = 128, FEW_K = 64, FEW_PITCH = FEW_K + 4, FEW_STAGES = 4, FEW_M = 4;
+// enough for all of a 256-wide row.  Over 16,384 entries of 256, on the device:
+// 17 tokens 16.5 us instead of the 20.6 of pieces and tiles, 24 18.5 instead of
+// 22.6, 32 22.6 instead of 20.8.
+constexpr int FEW = 24, FEW_V = 128, FEW_K = 64, FEW_PITCH = FEW_K + 4, FEW_STAGES = 4, FEW_M = 4;
 
 struct FewArgs {
   const float *h, *w;

@@ -316,7 +316,7 @@ def test_loss_and_gradient(T, d, V, t):
     LossRef(h, w, y, dl).check(*run_loss(h, w, y, dl, check=True))
 
 
-@pytest.mark.parametrize("T", [1, 3, 16, 17])
+@pytest.mark.parametrize("T", [1, 3, 16, 17, 24, 25])
 @pytest.mark.parametrize("d,V", [(4, 127), (36, 128), (100, 129), (256, 1000), (1500, 300)])
 def test_loss_of_few_float32_tokens(T, d, V):
     h, w, y, dl = loss_case(T, d, V, F32, seed=T + d, gap=4 if T > 4 else 0)
