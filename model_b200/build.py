@@ -4,6 +4,8 @@ Every ``csrc/*.cu`` file is compiled for sm_100a only
 (``-gencode arch=compute_100a,code=sm_100a``) and linked into one shared
 library that exports the C ABI of ``include/memlayer.h``.  nvcc
 cross-compiles without a GPU, so this runs on any machine with CUDA 12.9.
+``csrc/fast_calls.cpp``, the training operators' calls from torch tensors, is
+compiled beside it against this interpreter and its torch.
 """
 
 from __future__ import annotations
@@ -13,6 +15,7 @@ import glob
 import os
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
@@ -20,6 +23,7 @@ CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 BUILD = os.path.join(ROOT, "_build")
 LIB = os.path.join(PKG, "libmemlayer.so")
+FAST = os.path.join(PKG, "_fast" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -32,6 +36,21 @@ def _stale(obj: str, deps) -> bool:
         return True
     t = os.path.getmtime(obj)
     return any(os.path.getmtime(d) > t for d in deps)
+
+
+def _fast_command():
+    """The compiler's command for the extension module, and the module's dependencies."""
+    import torch
+    tdir = os.path.dirname(torch.__file__)
+    tinc, cuda = os.path.join(tdir, "include"), os.path.dirname(os.path.dirname(NVCC))
+    src = os.path.join(CSRC, "fast_calls.cpp")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", src, "-o", FAST, "-I", INCLUDE,
+           "-I", tinc, "-I", os.path.join(tinc, "torch", "csrc", "api", "include"),
+           "-I", os.path.join(cuda, "include"), "-I", sysconfig.get_paths()["include"],
+           "-L", PKG, "-l:" + os.path.basename(LIB), "-L", os.path.join(tdir, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python",
+           "-Wl,-rpath,$ORIGIN"]
+    return cmd, [src, os.path.join(INCLUDE, "memlayer.h")]
 
 
 def build(verbose: bool = False, ptxas_verbose: bool = False) -> str:
@@ -51,7 +70,7 @@ def build(verbose: bool = False, ptxas_verbose: bool = False) -> str:
     def run(cmd):
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
-            raise RuntimeError(f"nvcc failed ({' '.join(cmd)}):\n{r.stdout}\n{r.stderr}")
+            raise RuntimeError(f"{os.path.basename(cmd[0])} failed ({' '.join(cmd)}):\n{r.stdout}\n{r.stderr}")
         return r.stdout + r.stderr
 
     with cf.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as ex:
@@ -61,6 +80,9 @@ def build(verbose: bool = False, ptxas_verbose: bool = False) -> str:
     if jobs or not os.path.exists(LIB):
         run([NVCC, *ARCH, "-shared", "-o", LIB, *objs, "-lcudart_static", "-Xlinker",
              "-rpath=/usr/local/cuda/lib64", "-lrt", "-ldl", "-lpthread"])
+    cmd, deps = _fast_command()
+    if _stale(FAST, deps):
+        run(cmd)
     # the XLA FFI handlers of the JAX binding, where JAX is installed
     from model_b200 import jax_ffi
     jax_ffi.build(verbose=verbose)

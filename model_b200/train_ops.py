@@ -14,6 +14,11 @@ rows may be strided (a slice of a wider tensor); other layouts are copied.
 The kernels run on the tensors' device, on ``stream`` or that device's
 current stream.  With ``check=True`` a call waits for its kernels and raises
 where they recorded a failure.
+
+The usual calls -- contiguous tensors of the current device, its current
+stream, no check -- go through an extension module (``csrc/fast_calls.cpp``)
+that answers None to all others; those, and every error, take the general way
+over ctypes here.
 """
 
 from __future__ import annotations
@@ -27,6 +32,11 @@ import torch
 from . import _lib as L
 from .memory import _DTYPES, _workspace
 
+try:
+    from . import _fast
+except ImportError:          # not built for this interpreter: every call takes the general way
+    _fast = None
+
 
 def _on_tensor_device(fn):
     """Runs ``fn`` (first argument: a CUDA tensor) with that tensor's device
@@ -35,7 +45,7 @@ def _on_tensor_device(fn):
     @functools.wraps(fn)
     def wrapped(first, *args, stream: Optional[torch.cuda.Stream] = None, **kw):
         if not isinstance(first, torch.Tensor) or not first.is_cuda:
-            raise TypeError(f"{fn.__name__}: the first argument must be a CUDA tensor (no CPU path)")
+            raise TypeError(f"{fn.__name__[1:]}: the first argument must be a CUDA tensor (no CPU path)")
         if stream is None and first.get_device() == torch._C._cuda_getDevice():
             return fn(first, *args, **kw)
         if stream is None:
@@ -103,14 +113,23 @@ def _check_status(ws: torch.Tensor, stream: int) -> None:
         raise L.DeviceError(f"device status {code.value}: {L.DEVICE_ERRORS.get(code.value, 'unknown')}")
 
 
-@_on_tensor_device
 def layer_norm(x: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor, *,
-               residual: Optional[torch.Tensor] = None, eps: float = 1e-6):
+               residual: Optional[torch.Tensor] = None, eps: float = 1e-6,
+               stream: Optional[torch.cuda.Stream] = None):
     """LayerNorm over the last dimension of ``x [..., d]`` (flax's epsilon by
     default): ``y = (x - mean) / sqrt(var + eps) * scale + bias``.  With
     ``residual`` the norm reads ``x + residual`` (rounded to the type of
     ``x``) and ``(y, x + residual)`` is returned, the second being what
     ``layer_norm_backward`` takes as its input."""
+    if _fast is not None and stream is None:
+        out = _fast.layer_norm(x, scale, bias, residual, eps)
+        if out is not None:
+            return out
+    return _layer_norm(x, scale, bias, residual, eps, stream=stream)
+
+
+@_on_tensor_device
+def _layer_norm(x, scale, bias, residual, eps):
     code = _dtype(x)
     if x.dim() == 0:
         raise ValueError("x must have at least one dimension")
@@ -131,22 +150,23 @@ def layer_norm(x: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor, *,
     return y, total
 
 
-# The sizes depend on the device (its SMs) beside the arguments.
-@functools.lru_cache(maxsize=256)
-def _norm_workspace_bytes(rows: int, d: int, code: int, eps: float, device: int) -> int:
-    nb = C.c_size_t()
-    _call("memlayer_layer_norm_backward_workspace_size", L.MemlayerNormConfig(rows, d, code, eps), nb)
-    return nb.value
-
-
-@_on_tensor_device
 def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, scale: torch.Tensor, *,
                         dresidual: Optional[torch.Tensor] = None, eps: float = 1e-6, check: bool = False,
+                        stream: Optional[torch.cuda.Stream] = None,
                         ) -> Tuple[torch.Tensor, Dict[str, torch.Tensor]]:
     """Gradients of ``sum(dy * layer_norm(x, scale, bias))``: ``(dx, {"scale",
     "bias"})``.  ``x`` is the forward's normalised input (its sum when it had
     a residual; ``dx`` is then the gradient of both summands).  ``dresidual``,
     the gradient that reaches ``x`` beside the norm, is added to ``dx``."""
+    if _fast is not None and stream is None and not check:
+        out = _fast.layer_norm_backward(dy, x, scale, dresidual, eps)
+        if out is not None:
+            return out[0], {"scale": out[1], "bias": out[2]}
+    return _layer_norm_backward(dy, x, scale, dresidual, eps, check, stream=stream)
+
+
+@_on_tensor_device
+def _layer_norm_backward(dy, x, scale, dresidual, eps, check):
     code = _dtype(dy)
     if dy.dim() == 0:
         raise ValueError("dy must have at least one dimension")
@@ -158,12 +178,13 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, scale: torch.Tensor, 
     dx = torch.empty_like(g, memory_format=torch.contiguous_format)
     ds, db = sc.new_empty(d), sc.new_empty(d)
     cfg = L.MemlayerNormConfig(dy.numel() // d if d else 0, d, code, eps)
-    nb = _norm_workspace_bytes(cfg.rows, d, code, eps, dy.get_device())
-    ws = _workspace(nb, dy.device)
+    nb = C.c_size_t()
+    _call("memlayer_layer_norm_backward_workspace_size", cfg, nb)
+    ws = _workspace(nb.value, dy.device)
     a = L.MemlayerNormGrads(g.data_ptr(), ldg, xr.data_ptr(), ldx, None if rr is None else rr.data_ptr(), ldr,
                             sc.data_ptr(), dx.data_ptr(), ds.data_ptr(), db.data_ptr())
     s = _stream(dy)
-    _call("memlayer_layer_norm_backward", cfg, a, ws.data_ptr(), nb, s)
+    _call("memlayer_layer_norm_backward", cfg, a, ws.data_ptr(), nb.value, s)
     if check:
         _check_status(ws, s)
     return dx, {"scale": ds, "bias": db}
@@ -193,26 +214,29 @@ def _loss_args(h, weight, targets, ignore_index):
     return cfg, hr, ldh, wr, ldw, t
 
 
-@functools.lru_cache(maxsize=256)
-def _loss_workspace_bytes(tokens: int, d: int, vocab: int, code: int, backward: int, device: int) -> int:
-    nb = C.c_size_t()
-    _call("memlayer_cross_entropy_workspace_size", L.MemlayerLossConfig(tokens, d, vocab, code, 0), backward, nb)
-    return nb.value
-
-
 def _loss_workspace(cfg, backward: int, device):
-    nb = _loss_workspace_bytes(cfg.tokens, cfg.d_model, cfg.vocab_size, cfg.dtype, backward, device.index)
-    return _workspace(nb, device), nb
+    nb = C.c_size_t()
+    _call("memlayer_cross_entropy_workspace_size", cfg, backward, nb)
+    return _workspace(nb.value, device), nb.value
 
 
-@_on_tensor_device
 def linear_cross_entropy(h: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, *, ignore_index: int = -100,
-                         check: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
+                         check: bool = False, stream: Optional[torch.cuda.Stream] = None,
+                         ) -> Tuple[torch.Tensor, torch.Tensor]:
     """Softmax cross entropy of the logits ``h @ weight.T`` against integer
     ``targets``, without storing them: ``(loss, lse)``, float32 of the shape
     of ``targets``, ``lse`` being log sum exp of the logits.  A token whose
     target is ``ignore_index`` has loss 0; any other target outside the
     vocabulary gives NaN, and raises with ``check=True``."""
+    if _fast is not None and stream is None and not check:
+        out = _fast.linear_cross_entropy(h, weight, targets, ignore_index)
+        if out is not None:
+            return out
+    return _linear_cross_entropy(h, weight, targets, ignore_index, check, stream=stream)
+
+
+@_on_tensor_device
+def _linear_cross_entropy(h, weight, targets, ignore_index, check):
     cfg, hr, ldh, wr, ldw, t = _loss_args(h, weight, targets, ignore_index)
     loss = torch.empty(t.shape, dtype=torch.float32, device=h.device)
     lse = torch.empty_like(loss)
@@ -225,15 +249,24 @@ def linear_cross_entropy(h: torch.Tensor, weight: torch.Tensor, targets: torch.T
     return loss, lse
 
 
-@_on_tensor_device
 def linear_cross_entropy_backward(h: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, lse: torch.Tensor,
                                   dloss: torch.Tensor, *, dlse: Optional[torch.Tensor] = None,
                                   ignore_index: int = -100, check: bool = False,
+                                  stream: Optional[torch.cuda.Stream] = None,
                                   ) -> Tuple[torch.Tensor, torch.Tensor]:
     """``(dh, dweight)`` of ``sum(dloss * loss) + sum(dlse * lse)`` for the
     forward on the same ``h``, ``weight`` and ``targets`` that gave ``lse``
     (a mean over n tokens: ``dloss`` filled with 1 / n).  ``dloss`` is not
     read at ignored tokens; ``h`` must be finite there too."""
+    if _fast is not None and stream is None and not check:
+        out = _fast.linear_cross_entropy_backward(h, weight, targets, lse, dloss, dlse, ignore_index)
+        if out is not None:
+            return out
+    return _linear_cross_entropy_backward(h, weight, targets, lse, dloss, dlse, ignore_index, check, stream=stream)
+
+
+@_on_tensor_device
+def _linear_cross_entropy_backward(h, weight, targets, lse, dloss, dlse, ignore_index, check):
     cfg, hr, ldh, wr, ldw, t = _loss_args(h, weight, targets, ignore_index)
     n = t.numel()
     ls, dl = _vector(lse, "lse", n, h), _vector(dloss, "dloss", n, h)
@@ -251,16 +284,24 @@ def linear_cross_entropy_backward(h: torch.Tensor, weight: torch.Tensor, targets
     return dh, dw
 
 
-@_on_tensor_device
 def orthogonalize(update: torch.Tensor, *, steps: int = 5,
                   coefficients: Sequence[float] = (3.4445, -4.7750, 2.0315), eps: float = 1e-7,
-                  check: bool = False) -> torch.Tensor:
+                  check: bool = False, stream: Optional[torch.cuda.Stream] = None) -> torch.Tensor:
     """Newton-Schulz orthogonalisation of the matrices ``update [..., m, n]``
     (gradients or momenta of Dense kernels): ``X = U / (|U|_F + eps)``, then
     ``steps`` times ``X <- (a I + b X X^T + c (X X^T)^2) X``, which brings
     every singular value near 1.  Returns a tensor like ``update``; the caller
     scales and subtracts it.  Products run on 22-bit operands whatever the
     type; coefficients whose iteration would leave their range are refused."""
+    if _fast is not None and stream is None and not check:
+        out = _fast.orthogonalize(update, steps, *coefficients, eps)
+        if out is not None:
+            return out
+    return _orthogonalize(update, steps, coefficients, eps, check, stream=stream)
+
+
+@_on_tensor_device
+def _orthogonalize(update, steps, coefficients, eps, check):
     code = _dtype(update)
     if update.dim() < 2:
         raise ValueError("update must be [..., m, n]")

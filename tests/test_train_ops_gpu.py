@@ -704,6 +704,64 @@ def test_stream_argument():
     assert torch.equal(d, mb.orthogonalize(w))
 
 
+@pytest.mark.parametrize("t", TYPES)
+def test_extension_and_general_way_agree(t):
+    from model_b200 import train_ops
+    fast, here = train_ops._fast, torch.cuda.current_stream()          # with a stream: the general way
+    x, r, scale, bias, dy, dr = norm_case(90, 70, t, seed=51)
+    h, w, y, dl = loss_case(90, 70, 300, t, seed=52)
+    u = torch.randn(2, 90, 40, device="cuda", generator=gen(53)).to(t)
+    x3 = x.view(9, 10, 70)
+    pairs = [
+        (fast.layer_norm(x, scale, bias, r, 1e-5), mb.layer_norm(x, scale, bias, residual=r, eps=1e-5, stream=here)),
+        ((fast.layer_norm(x3, scale, bias, None, 1e-6),), (mb.layer_norm(x3, scale, bias, stream=here),)),
+        ((fast.orthogonalize(u, 4, 3.4445, -4.775, 2.0315, 1e-7),), (mb.orthogonalize(u, steps=4, stream=here),)),
+        (fast.linear_cross_entropy(h, w, y, -100), mb.linear_cross_entropy(h, w, y, stream=here))]
+    lse = pairs[-1][1][1]
+    pairs.append((fast.linear_cross_entropy_backward(h, w, y, lse, dl, dl, -100),
+                  mb.linear_cross_entropy_backward(h, w, y, lse, dl, dlse=dl, stream=here)))
+    dx, dp = mb.layer_norm_backward(dy, x, scale, dresidual=dr, stream=here)
+    pairs.append((fast.layer_norm_backward(dy, x, scale, dr, 1e-6), (dx, dp["scale"], dp["bias"])))
+    for got, want in pairs:
+        assert len(got) == len(want)
+        for p, q in zip(got, want):
+            assert torch.equal(p, q) and p.shape == q.shape and p.dtype == q.dtype and p.is_contiguous()
+            assert not p.requires_grad and p.device == q.device
+    # parameters and tensors that carry gradients are taken, their results carry none
+    p = torch.nn.Parameter(scale.clone())
+    z = fast.layer_norm(x.float().requires_grad_(), p, bias, None, 1e-6)
+    assert z is not None and not z.requires_grad
+    assert fast.layer_norm(torch.empty(0, 70, device="cuda", dtype=t), scale, bias, None, 1e-6).shape == (0, 70)
+
+
+def test_extension_leaves_the_rest_to_the_general_way():
+    from model_b200 import train_ops
+    fast = train_ops._fast
+    x, _, scale, bias, dy, _ = norm_case(12, 32, F32, seed=54)
+    h, w, y, dl = loss_case(12, 32, 50, F32, seed=55)
+    class Sub(torch.Tensor):
+        pass
+    other = torch.zeros(12, 32)                                          # on the CPU
+    for args in ((x[:, ::2], scale[:16], bias[:16]), (x.t(), scale[:12], bias[:12]), (x.double(), scale, bias),
+                 (x, scale.half(), bias), (x, scale[:31], bias), (x, scale, bias.cpu()), (x.as_subclass(Sub), scale, bias),
+                 (torch.tensor(1.0, device="cuda"), scale, bias), (torch.empty(3, 0, device="cuda"), scale[:0], bias[:0])):
+        assert fast.layer_norm(*args, None, 1e-6) is None
+    assert fast.layer_norm(x, scale, bias, other, 1e-6) is None and fast.layer_norm(x, scale, bias, x[:3], 1e-6) is None
+    assert fast.layer_norm(x, scale, bias, None, -1.0) is None and fast.layer_norm(x, scale, bias, None, "1") is None
+    assert fast.layer_norm_backward(dy, x.half(), scale, None, 1e-6) is None
+    assert fast.linear_cross_entropy(h, w, y.long(), -100) is None and fast.linear_cross_entropy(h, w, y[:5], -100) is None
+    assert fast.linear_cross_entropy(h, w, y, 2 ** 31) is None and fast.linear_cross_entropy(h, w.half(), y, -100) is None
+    assert fast.linear_cross_entropy_backward(h, w, y, dl[:3], dl, None, -100) is None
+    assert fast.orthogonalize(h, 5, 30.0, 1.0, 1.0, 1e-7) is None and fast.orthogonalize(h[0], 5, 1., 1., 1., 1e-7) is None
+    # the public functions take or refuse them as before
+    assert torch.equal(mb.layer_norm(x.t(), scale[:12], bias[:12]), mb.layer_norm(x.t().contiguous(), scale[:12], bias[:12]))
+    assert torch.equal(mb.linear_cross_entropy(h, w, y.long())[0], mb.linear_cross_entropy(h, w, y)[0])
+    with pytest.raises(TypeError):
+        mb.layer_norm(x.double(), scale, bias)
+    with pytest.raises(L.MemlayerError):
+        mb.layer_norm(x, scale, bias, eps=-1.0)
+
+
 def test_captured_and_replayed():
     run = all_of_them()
     want = run()

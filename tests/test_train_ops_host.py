@@ -226,3 +226,23 @@ def test_model_hidden_arguments_refused():
     assert f(C.byref(c), C.byref(p), None, 2, 8, FAKE, FAKE, 1 << 30, None) == L.ERR_BAD_POINTER
     assert f(C.byref(c), C.byref(p), FAKE, 2, 8, None, FAKE, 1 << 30, None) == L.ERR_BAD_POINTER
     assert f(C.byref(c), C.byref(p), FAKE, 2, 8, FAKE, None, 0, None) == L.ERR_WORKSPACE
+
+
+def test_extension_declines_what_it_does_not_take():
+    import torch
+    from model_b200 import train_ops
+    fast = train_ops._fast
+    assert fast is not None, "csrc/fast_calls.cpp is not built"
+    x, v = torch.zeros(2, 4), torch.zeros(4)
+    calls = [(fast.layer_norm, (x, v, v, None, 1e-6)), (fast.layer_norm_backward, (x, x, v, None, 1e-6)),
+             (fast.linear_cross_entropy, (x, x, torch.zeros(2, dtype=torch.int32), -100)),
+             (fast.linear_cross_entropy_backward, (x, x, torch.zeros(2, dtype=torch.int32), v, v, None, -100)),
+             (fast.orthogonalize, (x, 5, 3.4445, -4.775, 2.0315, 1e-7))]
+    for f, args in calls:                    # tensors without a GPU, other things, too few and too many of them
+        assert f(*args) is None and f(*args[:-1]) is None and f(*args, 1) is None and f() is None
+        assert f(*([None] * len(args))) is None and f(*(["x"] * len(args))) is None and f(*([3] * len(args))) is None
+    for call in (lambda: train_ops.layer_norm(x, v, v), lambda: train_ops.layer_norm_backward(x, x, v),
+                 lambda: train_ops.linear_cross_entropy(x, x, v), lambda: train_ops.orthogonalize(x),
+                 lambda: train_ops.linear_cross_entropy_backward(x, x, v, v, v)):
+        with pytest.raises(TypeError, match="CUDA tensor"):
+            call()
