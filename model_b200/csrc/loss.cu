@@ -240,6 +240,7 @@ __global__ void __launch_bounds__(FEW_V * (FEW / FEW_M)) loss_few_kernel(FewArgs
   float* ws = reinterpret_cast<float*>(few_raw);                       // [stages][128][68]
   float* hs = ws + FEW_STAGES * FEW_V * FEW_PITCH;                     // [tokens rounded up to 4][columns to 64]
   allow_next();
+  wait_previous();
   const int t = threadIdx.x, nt = blockDim.x, v0 = blockIdx.x * FEW_V, chunks = (A.d + FEW_K - 1) / FEW_K;
   const int cols = chunks * FEW_K, tokens = nt / FEW_V * FEW_M;
   if (blockIdx.x == 0 && t == 0) *A.err = 0;
@@ -786,9 +787,9 @@ cudaError_t launch_loss_forward(const memlayer_loss_config& c, const memlayer_lo
     static std::atomic<uint64_t> done{0};
     LS_TRY(g16::allow_smem(reinterpret_cast<const void*>(loss_few_kernel), &done));
     const int blocks = (c.vocab_size + FEW_V - 1) / FEW_V;
-    loss_few_kernel<<<blocks, few_threads(c.tokens), few_smem(c.tokens, c.d_model), s>>>(f);
     count_launch(2);
-    LS_TRY(cudaGetLastError());
+    LS_TRY(launch_dependent(loss_few_kernel, dim3((unsigned)blocks), few_threads(c.tokens),
+                            few_smem(c.tokens, c.d_model), s, f));
     return launch_dependent(loss_join_kernel, dim3((unsigned)((c.tokens + 7) / 8)), 256, 0, s, (const float2*)f.part,
                             (const float*)f.zt, a.targets, c.tokens, c.vocab_size, Sched{}, 1, blocks, c.ignore_index,
                             a.loss, a.lse, err);

@@ -32,6 +32,9 @@
 // all of a block's rows; it adds its row groups in shared memory and writes one
 // partial row; a second kernel adds the partials in block order,
 // so the result does not depend on timing (no atomics).
+//
+// Launches are dependent ones: a kernel's start hides behind the end of the
+// one before it (8192 x 256 float32, forward and gradient: 22.3 us for 24.6).
 #include "norm.cuh"
 
 #include <algorithm>
@@ -124,6 +127,8 @@ template <typename E, int VEC, int MAXT>
 __global__ void __launch_bounds__(MAXT ? MAXT : NT, MAXT ? 1 : 2) layer_norm_kernel(NormArgs A) {
   constexpr bool WIDE = MAXT > 0;
   __shared__ float red[32];
+  allow_next();
+  wait_previous();
   using Part = RowPart<E, VEC>;
   const int tpr = A.tpr, d = A.d;
   const int t = threadIdx.x & (tpr - 1), g = threadIdx.x / tpr, groups = blockDim.x / tpr;
@@ -169,7 +174,8 @@ template <typename E, int VEC, int MAXT>
 __global__ void __launch_bounds__(MAXT ? MAXT : NT, MAXT ? 1 : 2) layer_norm_backward_kernel(NormArgs A) {
   constexpr bool WIDE = MAXT > 0;
   __shared__ float red[32];
-  allow_next();                            // of the kernel that adds the partials
+  allow_next();
+  wait_previous();
   extern __shared__ float cols[];          // !WIDE: [groups][VALS * tpr]
   using Part = RowPart<E, VEC>;
   const int tpr = A.tpr, d = A.d;
@@ -381,6 +387,8 @@ __device__ __forceinline__ void pack(Vec16<__nv_bfloat16, 8>& v, const float (&x
 template <typename E, int V, int NV>
 __global__ void __launch_bounds__(128) layer_norm_warp_kernel(NormArgs A) {
   using Vec = Vec16<E, V>;
+  allow_next();
+  wait_previous();
   const int d = A.d, lane = threadIdx.x & 31;
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   if (row >= A.rows) return;
@@ -521,6 +529,8 @@ __global__ void __launch_bounds__(MAXT, MINB) layer_norm_wide_kernel(NormArgs A)
   using Vec = Vec16<E, V>;
   __shared__ alignas(16) float red[2][32];
   const int d = A.d, t = threadIdx.x, nt = blockDim.x, o = block_shift<V, SHIFT>(d);
+  allow_next();
+  wait_previous();
   if (t < 64) (&red[0][0])[t] = 0.f;     // slots without a warp
   __syncthreads();
   float scale[NV][V], bias[NV][V];       // SHIFT: kept over the block's rows
@@ -635,7 +645,8 @@ template <typename E, int R, int NV, int MAXT, int MINB, bool AHEAD, bool SHIFT>
 __global__ void __launch_bounds__(MAXT, MINB) layer_norm_wide_backward_kernel(NormArgs A) {
   constexpr int V = 16 / sizeof(E), H = V / 2;
   using Vec = Vec16<E, V>;
-  allow_next();                            // of the kernel that adds the partials
+  allow_next();
+  wait_previous();
   __shared__ alignas(16) float red[2][3 * R * 32];
   const int d = A.d, t = threadIdx.x, nt = blockDim.x, o = block_shift<V, SHIFT>(d);
   for (int i = t; i < 2 * 3 * R * 32; i += nt) (&red[0][0])[i] = 0.f;   // slots without a warp
@@ -772,7 +783,7 @@ __global__ void __launch_bounds__(MAXW * 32, 1) layer_norm_ring_backward_kernel(
   constexpr int V = 16 / sizeof(E), H = V / 2;
   using Vec = Vec16<E, V>;
   extern __shared__ uint8_t smem_raw[];
-  allow_next();                              // of the kernel that adds the partials
+  allow_next();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const int d = A.d, rb = d * (int)sizeof(E);
   constexpr int tensors = 2;                 // x and dy
@@ -785,9 +796,10 @@ __global__ void __launch_bounds__(MAXW * 32, 1) layer_norm_ring_backward_kernel(
   uint8_t* ring = rings + (size_t)warp * stages * tensors * rbp;
   if (lane == 0)
     for (int i = 0; i < stages; ++i) tc::mbar_init(&full[i], 1);
-  if (blockIdx.x == 0 && threadIdx.x == 0) *A.err = 0;
   if (threadIdx.x == 0) *abort = 0;
   tc::fence_mbar_init();
+  wait_previous();
+  if (blockIdx.x == 0 && threadIdx.x == 0) *A.err = 0;
   for (int j = threadIdx.x; j < d; j += blockDim.x) scale_s[j] = A.scale[j];
   __syncthreads();
 
@@ -1032,18 +1044,18 @@ cudaError_t norm_forward_t(NormArgs& A, Access how, cudaStream_t s) {
     const int most = w.nt > 256 ? 1024 / w.nt : w.per_sm(w.nv * V > 8 ? 3 : 4);
     const int grid = shifted_grid(A.rows, A.d, V, (int64_t)most * g16::device_sms());
     if (w.nt > 256 && w.nv == 1)
-      layer_norm_wide_kernel<E, 1, 1024, 1, true><<<grid, w.nt, 0, s>>>(A);
+      launch_dependent(layer_norm_wide_kernel<E, 1, 1024, 1, true>, dim3(grid), w.nt, 0, s, A);
     else if (w.nt > 256 && w.nv == 2)
-      layer_norm_wide_kernel<E, 2, 1024, 1, true><<<grid, w.nt, 0, s>>>(A);
+      launch_dependent(layer_norm_wide_kernel<E, 2, 1024, 1, true>, dim3(grid), w.nt, 0, s, A);
     else if (w.nt > 256)
-      layer_norm_wide_kernel<E, 4, 1024, 1, true><<<grid, w.nt, 0, s>>>(A);
+      launch_dependent(layer_norm_wide_kernel<E, 4, 1024, 1, true>, dim3(grid), w.nt, 0, s, A);
     else if (w.nv == 1)
-      layer_norm_wide_kernel<E, 1, 256, 4, true><<<grid, w.nt, 0, s>>>(A);
+      launch_dependent(layer_norm_wide_kernel<E, 1, 256, 4, true>, dim3(grid), w.nt, 0, s, A);
     else if constexpr (V == 4) {
       if (w.nv == 2)
-        layer_norm_wide_kernel<E, 2, 256, 4, true><<<grid, w.nt, 0, s>>>(A);
+        launch_dependent(layer_norm_wide_kernel<E, 2, 256, 4, true>, dim3(grid), w.nt, 0, s, A);
       else
-        layer_norm_wide_kernel<E, 4, 256, 3, true><<<grid, w.nt, 0, s>>>(A);
+        launch_dependent(layer_norm_wide_kernel<E, 4, 256, 3, true>, dim3(grid), w.nt, 0, s, A);
     }
     count_launch();
     return cudaGetLastError();
@@ -1054,34 +1066,34 @@ cudaError_t norm_forward_t(NormArgs& A, Access how, cudaStream_t s) {
     if (grid >= (1ll << 31)) return cudaErrorInvalidValue;
     const unsigned g = (unsigned)grid;
     if (!vec)
-      A.d <= 1024 ? layer_norm_warp_kernel<E, 1, 32><<<g, 128, 0, s>>>(A)
-                  : layer_norm_warp_kernel<E, 1, 64><<<g, 128, 0, s>>>(A);
+      A.d <= 1024 ? launch_dependent(layer_norm_warp_kernel<E, 1, 32>, dim3(g), 128, 0, s, A)
+                  : launch_dependent(layer_norm_warp_kernel<E, 1, 64>, dim3(g), 128, 0, s, A);
     else if (vecs <= 128)
-      layer_norm_warp_kernel<E, V, 4><<<g, 128, 0, s>>>(A);
+      launch_dependent(layer_norm_warp_kernel<E, V, 4>, dim3(g), 128, 0, s, A);
     else if (vecs <= 256)
-      layer_norm_warp_kernel<E, V, 8><<<g, 128, 0, s>>>(A);
+      launch_dependent(layer_norm_warp_kernel<E, V, 8>, dim3(g), 128, 0, s, A);
     else
-      layer_norm_warp_kernel<E, V, 16><<<g, 128, 0, s>>>(A);
+      launch_dependent(layer_norm_warp_kernel<E, V, 16>, dim3(g), 128, 0, s, A);
   } else if (vec && vecs > 512) {
     const Wide w = wide_for(A.d, V);
     const int grid = (int)(A.rows < MOST ? A.rows : MOST);
     if (w.nv == 1)
-      layer_norm_wide_kernel<E, 1, 1024, 1, false><<<grid, w.nt, 0, s>>>(A);
+      launch_dependent(layer_norm_wide_kernel<E, 1, 1024, 1, false>, dim3(grid), w.nt, 0, s, A);
     else if (w.nv == 2)
-      layer_norm_wide_kernel<E, 2, 1024, 1, false><<<grid, w.nt, 0, s>>>(A);
+      launch_dependent(layer_norm_wide_kernel<E, 2, 1024, 1, false>, dim3(grid), w.nt, 0, s, A);
     else if constexpr (sizeof(E) == 4)   // 16-bit rows end at two vectors
-      layer_norm_wide_kernel<E, 4, 1024, 1, false><<<grid, w.nt, 0, s>>>(A);
+      launch_dependent(layer_norm_wide_kernel<E, 4, 1024, 1, false>, dim3(grid), w.nt, 0, s, A);
   } else {
     const bool wide = A.tpr > 32;
     const int nt = wide ? A.tpr : NT;
     const int64_t need = ceil_div(A.rows, nt / A.tpr);
     const int grid = (int)(need < MOST ? need : MOST);
     if (vec)
-      layer_norm_kernel<E, V, 0><<<grid, nt, 0, s>>>(A);
+      launch_dependent(layer_norm_kernel<E, V, 0>, dim3(grid), nt, 0, s, A);
     else if (wide)
-      layer_norm_kernel<E, 1, 1024><<<grid, nt, 0, s>>>(A);
+      launch_dependent(layer_norm_kernel<E, 1, 1024>, dim3(grid), nt, 0, s, A);
     else
-      layer_norm_kernel<E, 1, 0><<<grid, nt, 0, s>>>(A);
+      launch_dependent(layer_norm_kernel<E, 1, 0>, dim3(grid), nt, 0, s, A);
   }
   count_launch();
   return cudaGetLastError();
@@ -1093,7 +1105,7 @@ cudaError_t launch_ring(const NormArgs& A, const Ring& r, int grid, cudaStream_t
   static std::atomic<uint64_t> done{0};
   const cudaError_t e = g16::allow_smem(reinterpret_cast<const void*>(kern), &done);
   if (e != cudaSuccess) return e;
-  kern<<<grid, r.warps * 32, r.smem, s>>>(A, r.stages);
+  launch_dependent(kern, dim3(grid), r.warps * 32, r.smem, s, A, r.stages);
   return cudaSuccess;
 }
 
@@ -1104,17 +1116,19 @@ template <typename E, bool SHIFT>
 void launch_wide_backward(const NormArgs& A, const Wide& w, int grid, cudaStream_t s) {
   constexpr int V = 16 / sizeof(E);
   if (w.nt > 256 && w.nv == 1)
-    layer_norm_wide_backward_kernel<E, 1, 1, 1024, 1, false, SHIFT><<<grid, w.nt, 0, s>>>(A);
+    launch_dependent(layer_norm_wide_backward_kernel<E, 1, 1, 1024, 1, false, SHIFT>, dim3(grid), w.nt, 0, s, A);
   else if (w.nt > 256 && w.nv == 2)
-    layer_norm_wide_backward_kernel<E, 1, 2, 1024, 1, false, SHIFT><<<grid, w.nt, 0, s>>>(A);
+    launch_dependent(layer_norm_wide_backward_kernel<E, 1, 2, 1024, 1, false, SHIFT>, dim3(grid), w.nt, 0, s, A);
   else if (w.nt > 256)
-    layer_norm_wide_backward_kernel<E, 1, 4, 1024, 1, false, SHIFT><<<grid, w.nt, 0, s>>>(A);
+    launch_dependent(layer_norm_wide_backward_kernel<E, 1, 4, 1024, 1, false, SHIFT>, dim3(grid), w.nt, 0, s, A);
   else if (w.nv == 1)
-    layer_norm_wide_backward_kernel<E, 1, 1, 256, V == 4 ? 4 : 3, V == 4 || !SHIFT, SHIFT><<<grid, w.nt, 0, s>>>(A);
+    launch_dependent(layer_norm_wide_backward_kernel<E, 1, 1, 256, V == 4 ? 4 : 3, V == 4 || !SHIFT, SHIFT>,
+                     dim3(grid), w.nt, 0, s, A);
   else if (w.nv == 2)
-    layer_norm_wide_backward_kernel<E, 1, 2, 256, V == 4 ? 3 : 2, V == 4 || !SHIFT, SHIFT><<<grid, w.nt, 0, s>>>(A);
+    launch_dependent(layer_norm_wide_backward_kernel<E, 1, 2, 256, V == 4 ? 3 : 2, V == 4 || !SHIFT, SHIFT>,
+                     dim3(grid), w.nt, 0, s, A);
   else if constexpr (V == 4)
-    layer_norm_wide_backward_kernel<E, 1, 4, 256, 2, false, SHIFT><<<grid, w.nt, 0, s>>>(A);
+    launch_dependent(layer_norm_wide_backward_kernel<E, 1, 4, 256, 2, false, SHIFT>, dim3(grid), w.nt, 0, s, A);
 }
 
 template <typename E>
@@ -1138,13 +1152,13 @@ cudaError_t norm_backward_t(NormArgs& A, Access how, int grid, cudaStream_t s) {
     const int nt = wide ? A.tpr : NT;
     const size_t sm = wide ? 0 : (size_t)nt * VALS * sizeof(float);   // 16 KB
     if (vec)
-      layer_norm_backward_kernel<E, V, 0><<<grid, nt, sm, s>>>(A);
+      launch_dependent(layer_norm_backward_kernel<E, V, 0>, dim3(grid), nt, sm, s, A);
     else if (A.tpr > 256)
-      layer_norm_backward_kernel<E, 1, 1024><<<grid, nt, sm, s>>>(A);
+      launch_dependent(layer_norm_backward_kernel<E, 1, 1024>, dim3(grid), nt, sm, s, A);
     else if (wide)
-      layer_norm_backward_kernel<E, 1, 256><<<grid, nt, sm, s>>>(A);
+      launch_dependent(layer_norm_backward_kernel<E, 1, 256>, dim3(grid), nt, sm, s, A);
     else
-      layer_norm_backward_kernel<E, 1, 0><<<grid, nt, sm, s>>>(A);
+      launch_dependent(layer_norm_backward_kernel<E, 1, 0>, dim3(grid), nt, sm, s, A);
   }
   count_launch();
   return cudaGetLastError();

@@ -59,6 +59,7 @@ __global__ void __launch_bounds__(256) orth_norm_kernel(const E* __restrict__ u,
                                                         double* __restrict__ part) {
   __shared__ double red[8];
   allow_next();
+  wait_previous();
   // whole 16-byte vectors per chunk; a matrix that starts or ends inside one
   // goes by single elements
   constexpr int V = 16 / sizeof(E);
@@ -461,9 +462,9 @@ cudaError_t start(const memlayer_orth_config& c, const Plan& p, const E* u, char
   int64_t chunks = (n + 4095) / 4096;
   if (chunks > NORM_CHUNKS) chunks = NORM_CHUNKS;
   double* part = reinterpret_cast<double*>(ws + p.o_part);
-  orth_norm_kernel<E><<<dim3((unsigned)chunks, (unsigned)p.B), 256, 0, s>>>(u, n, (int)chunks, part);
   count_launch();
-  OR_TRY(cudaGetLastError());
+  OR_TRY(launch_dependent(orth_norm_kernel<E>, dim3((unsigned)chunks, (unsigned)p.B), 256, 0, s, u, n, (int)chunks,
+                          part));
   const int64_t items = p.m * (p.ldx / 8);
   int64_t blocks = (items + 511) / 512;
   const int64_t cap = up(8 * g16::device_sms(), p.B) / p.B;

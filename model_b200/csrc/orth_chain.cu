@@ -233,9 +233,11 @@ __global__ void __launch_bounds__(NT, 1) orth_chain_kernel(const __grid_constant
     tc::mbar_init(&ctl->done[1], 1);
     ctl->abort = 0;
     tc::fence_mbar_init();
-    if (blockIdx.x == 0) *A.err = 0;
   }
   if (warp == 1) g16::tmem_alloc<1>(&ctl->tmem_base, 512);
+  allow_next();
+  wait_previous();
+  if (blockIdx.x == 0 && t == 0) *A.err = 0;
 
   // ---- X_0 = U / (|U|_F + eps): eight columns of a row at a time --------------------
   const int64_t base = (int64_t)(blockIdx.x / A.C) * A.m * A.n;
@@ -562,12 +564,14 @@ cudaError_t launch(const ChainArgs& a, int64_t batch, cudaStream_t s) {
   cfg.blockDim = dim3(NT);
   cfg.dynamicSmemBytes = SMEM;
   cfg.stream = s;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = a.C;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   count_launch();
   return cudaLaunchKernelEx(&cfg, kern, a);
 }
