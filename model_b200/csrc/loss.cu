@@ -463,6 +463,210 @@ struct EpiGrad {
   __device__ __forceinline__ void end(const Args&, const Sched&, int) {}
 };
 
+// ---- gradient of few tokens ----------------------------------------------------------
+// Up to 16 tokens of up to 1024 columns: the weight is read and its gradient
+// written once, and the products are small enough for float32 FMAs.  A block
+// takes 64 vocabulary entries at a time: a warp finds the logits of two of
+// them (lanes along the columns), the block turns them into dz in shared
+// memory, and a thread multiplies dz by its columns of h and of the weight
+// (from L2 now): dW goes out, dh stays in registers over all of its entries.
+// A second kernel adds the blocks' parts of dh in block order.  TM: tokens
+// rounded up.
+constexpr int FEWB = 16, FEWB_V = 64, FEWB_D = 1024, FEWB_T = 512;
+
+// Groups of threads that share a block's entries where the columns leave threads over.
+__host__ __device__ inline int few_groups(int d) {
+  const int dp = (d + 31) / 32 * 32;
+  return dp <= FEWB_T / 2 ? FEWB_T / dp : 1;
+}
+
+struct FewGradArgs {
+  const void *h, *w;
+  int64_t ldh, ldw;
+  int T, V, d, ignore;
+  const int* targets;
+  const float *lse, *dloss, *dlse;
+  void* dw;
+  float* part;                         // [block][group][T][d]
+  int* err;
+};
+
+template <typename E> __device__ __forceinline__ float to_f32(E x);
+template <> __device__ __forceinline__ float to_f32(float x) { return x; }
+template <> __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+template <> __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename E> __device__ __forceinline__ E from_f32(float x);
+template <> __device__ __forceinline__ float from_f32(float x) { return x; }
+template <> __device__ __forceinline__ __half from_f32(float x) { return __float2half_rn(x); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32(float x) { return __float2bfloat16_rn(x); }
+
+template <typename E, int TM>
+__global__ void __launch_bounds__(FEWB_T, TM <= 4 ? 2 : 1) loss_few_backward_kernel(const FewGradArgs A) {
+  constexpr int COLS = FEWB_D / FEWB_T;
+  extern __shared__ float4 few_raw[];
+  float* dz = reinterpret_cast<float*>(few_raw);                       // [64][TM]
+  float *q = dz + FEWB_V * TM, *g = q + TM, *l = g + TM;               // a token's factors and log sum
+  int* tg = reinterpret_cast<int*>(l + TM);                            // and target (-1: none)
+  float* hs = l + 2 * TM;                                              // [TM][d]
+  allow_next();
+  wait_previous();
+  const int t = threadIdx.x, warp = t >> 5, lane = t & 31, d = A.d;
+  const E *h = reinterpret_cast<const E*>(A.h), *w = reinterpret_cast<const E*>(A.w);
+  E* dw = reinterpret_cast<E*>(A.dw);
+  if (blockIdx.x == 0 && t == 0) *A.err = 0;
+  __syncthreads();
+  if (t < TM) {
+    const int v = t < A.T ? A.targets[t] : A.ignore;
+    const bool in = t < A.T && v >= 0 && v < A.V && v != A.ignore;
+    if (t < A.T && !in && v != A.ignore && blockIdx.x == 0) atomicCAS(A.err, 0, STATUS_TARGET);
+    g[t] = in ? A.dloss[t] : 0.f;
+    q[t] = g[t] + (A.dlse && t < A.T ? A.dlse[t] : 0.f);
+    l[t] = t < A.T ? A.lse[t] : 0.f;
+    tg[t] = in ? v : -1;
+  }
+  for (int e = t; e < TM * d; e += FEWB_T) {
+    const int m = e / d;
+    hs[e] = m < A.T ? to_f32(h[m * A.ldh + (e - m * d)]) : 0.f;
+  }
+  __syncthreads();
+  const int groups = few_groups(d), width = groups > 1 ? (d + 31) / 32 * 32 : FEWB_T;
+  const int group = groups > 1 ? t / width : 0, first = group < groups ? t - group * width : d;
+  float hr[COLS][TM], acc[COLS][TM];
+#pragma unroll
+  for (int i = 0; i < COLS; ++i)
+#pragma unroll
+    for (int m = 0; m < TM; ++m) {
+      const int c = first + i * FEWB_T;
+      hr[i][m] = c < d ? hs[m * d + c] : 0.f;
+      acc[i][m] = 0.f;
+    }
+  const int tiles = (A.V - 1) / FEWB_V + 1;
+  for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    const int v0 = tile * FEWB_V, rows = min(FEWB_V, A.V - v0);
+    for (int r = warp * 2; r < rows; r += FEWB_T / 32 * 2) {
+      const E *w0 = w + (v0 + r) * A.ldw, *w1 = r + 1 < rows ? w0 + A.ldw : w0;
+      float z[2][TM];
+#pragma unroll
+      for (int m = 0; m < TM; ++m) z[0][m] = z[1][m] = 0.f;
+#pragma unroll 4
+      for (int c = lane; c < d; c += 32) {
+        const float a = to_f32(w0[c]), b = to_f32(w1[c]);
+#pragma unroll
+        for (int m = 0; m < TM; ++m) {
+          const float x = hs[m * d + c];
+          z[0][m] = fmaf(a, x, z[0][m]);
+          z[1][m] = fmaf(b, x, z[1][m]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int m = 0; m < TM; ++m) {
+          const float x = warp_sum(z[i][m]);
+          if (lane == 0) dz[(r + i) * TM + m] = x;      // r is even: inside the 64 rows
+        }
+    }
+    __syncthreads();
+    for (int e = t; e < rows * TM; e += FEWB_T) {
+      const int m = e % TM, v = v0 + e / TM;
+      float x = g16::exp2_fast((dz[e] - l[m]) * LOG2E) * q[m];
+      if (tg[m] == v) x -= g[m];
+      dz[e] = q[m] == 0.f && g[m] == 0.f ? 0.f : x;     // an ignored token: nothing, whatever its logits are
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < COLS; ++i) {
+      const int c = first + i * FEWB_T;
+      if (c >= d) break;
+      const E* wc = w + v0 * A.ldw + c;
+      E* dc = dw + (int64_t)v0 * d + c;
+      auto entry = [&](int r) {
+        const float x = to_f32(wc[r * A.ldw]);
+        float o = 0.f;
+#pragma unroll
+        for (int m = 0; m < TM; ++m) {
+          const float y = dz[r * TM + m];
+          o = fmaf(y, hr[i][m], o);
+          acc[i][m] = fmaf(y, x, acc[i][m]);
+        }
+        dc[(int64_t)r * d] = from_f32<E>(o);
+      };
+      if (groups == 1) {               // unrolled for its loads; with a stride between them it took 1.4 times as long
+#pragma unroll 8
+        for (int r = 0; r < rows; ++r) entry(r);
+      } else {
+#pragma unroll 4
+        for (int r = group; r < rows; r += groups) entry(r);
+      }
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < COLS; ++i) {
+    const int c = first + i * FEWB_T;
+    if (c >= d) break;
+#pragma unroll
+    for (int m = 0; m < TM; ++m)
+      if (m < A.T) A.part[(((int64_t)blockIdx.x * groups + group) * A.T + m) * d + c] = acc[i][m];
+  }
+}
+
+// out = the blocks' parts [blocks][n] added in block order: 32 groups of
+// blocks an entry, then the groups in a fixed tree.
+template <typename E>
+__global__ void __launch_bounds__(1024) loss_few_dh_kernel(const float* __restrict__ part, int blocks, int n,
+                                                           E* __restrict__ out) {
+  __shared__ float red[32][33];
+  allow_next();
+  wait_previous();
+  const int c = threadIdx.x & 31, g = threadIdx.x >> 5, j = blockIdx.x * 32 + c;
+  float x = 0.f;
+  if (j < n) {
+#pragma unroll 4
+    for (int b = g; b < blocks; b += 32) x += part[(int64_t)b * n + j];
+  }
+  red[g][c] = x;
+  __syncthreads();
+  const float s = warp_sum(red[c][g]);
+  if (c == 0 && blockIdx.x * 32 + g < n) out[blockIdx.x * 32 + g] = from_f32<E>(s);
+}
+
+// 16-bit tensor cores are ahead of more than four tokens where a block would
+// take several times 64 entries (8 x 512 over 30,000 bf16 43 us for 50, 16 x
+// 1024 over 32,768 72 for 169), and behind elsewhere: 5 x 112 over 7,933 bf16
+// 25 for 14, 3 x 290 over 49,237 111 for 43, 4 x 856 over 10,146 float32 71
+// for 33, 16 x 256 over 16,384 49 for 35.
+bool few_backward(const memlayer_loss_config& c) {
+  return c.tokens <= FEWB && c.d_model <= FEWB_D &&
+         (c.tokens <= 4 || c.dtype == MEMLAYER_F32 || c.vocab_size <= FEWB_V * g16::device_sms());
+}
+
+int few_backward_blocks(const memlayer_loss_config& c) {
+  const int most = g16::device_sms() * (c.tokens <= 4 ? 2 : 1), tiles = (c.vocab_size - 1) / FEWB_V + 1;
+  return tiles < most ? tiles : most;
+}
+
+template <typename E, int TM>
+cudaError_t launch_few_backward(const FewGradArgs& a, int blocks, void* dh, cudaStream_t s) {
+  auto kern = loss_few_backward_kernel<E, TM>;
+  static std::atomic<uint64_t> done{0};
+  cudaError_t e = g16::allow_smem(reinterpret_cast<const void*>(kern), &done);
+  if (e != cudaSuccess) return e;
+  count_launch(2);
+  e = launch_dependent(kern, dim3((unsigned)blocks), FEWB_T, (size_t)TM * (FEWB_V + 4 + a.d) * sizeof(float), s, a);
+  if (e != cudaSuccess) return e;
+  const int n = a.T * a.d;
+  return launch_dependent(loss_few_dh_kernel<E>, dim3((unsigned)((n + 31) / 32)), 1024, 0, s, (const float*)a.part,
+                          blocks * few_groups(a.d), n, reinterpret_cast<E*>(dh));
+}
+
+template <typename E>
+cudaError_t few_backward_of(const FewGradArgs& a, int blocks, void* dh, cudaStream_t s) {
+  if (a.T <= 4) return launch_few_backward<E, 4>(a, blocks, dh, s);
+  if (a.T <= 8) return launch_few_backward<E, 8>(a, blocks, dh, s);
+  return launch_few_backward<E, FEWB>(a, blocks, dh, s);
+}
+
 struct OutOne {
   CUtensorMap map;                     // out as staged stores write it (tma)
   int64_t M;
@@ -686,6 +890,12 @@ bool plan(const memlayer_loss_config& c, bool backward, Plan* out) {
     off += (size_t)up(bytes, 256);
     return o;
   };
+  if (backward && few_backward(c)) {
+    p.o_dh = take((int64_t)few_backward_blocks(c) * few_groups(c.d_model) * T * d * 4);
+    p.bytes = off;
+    *out = p;
+    return true;
+  }
   // room for the 16-bit forms whether or not this call's strides need them
   p.o_hh = take(T * p.ld * 2);
   p.o_wh = take(V * p.ld * 2);
@@ -840,6 +1050,14 @@ cudaError_t launch_loss_backward(const memlayer_loss_config& c, const memlayer_l
   if (!plan(c, true, &p)) return cudaErrorInvalidValue;
   int* err = reinterpret_cast<int*>(ws + O_ERR);
   const int64_t T = c.tokens, V = c.vocab_size, d = c.d_model;
+  if (T > 0 && few_backward(c)) {
+    const FewGradArgs f{a.h, a.weight, a.h_stride, a.weight_stride, (int)T, c.vocab_size, c.d_model, c.ignore_index,
+                        a.targets, g.lse, g.dloss, g.dlse, g.dweight, reinterpret_cast<float*>(ws + p.o_dh), err};
+    const int blocks = few_backward_blocks(c);
+    return c.dtype == MEMLAYER_F32   ? few_backward_of<float>(f, blocks, g.dh, s)
+           : c.dtype == MEMLAYER_F16 ? few_backward_of<__half>(f, blocks, g.dh, s)
+                                     : few_backward_of<__nv_bfloat16>(f, blocks, g.dh, s);
+  }
   LS_TRY(cudaMemsetAsync(ws + O_ERR, 0, HEAD - O_ERR, s));
   const size_t esize = c.dtype == MEMLAYER_F32 ? 4 : 2;
   if (T == 0) return cudaMemsetAsync(g.dweight, 0, (size_t)V * d * esize, s);

@@ -329,6 +329,46 @@ def test_loss_of_few_float32_tokens(T, d, V):
 
 
 @pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("T", [1, 4, 5, 8, 9, 16, 17])
+@pytest.mark.parametrize("d,V", [(1, 1), (7, 63), (36, 65), (513, 129), (1024, 300), (1025, 130), (50, 21001)])
+def test_loss_gradient_of_few_tokens(T, d, V, t):
+    h, w, y, dl = loss_case(T, d, V, t, seed=T + d, gap=3 if T > 4 else 0)
+    dlse = 0.1 * torch.randn(T, device="cuda", generator=gen(2))
+    LossRef(h, w, y, dl, dlse).check(*run_loss(h, w, y, dl, dlse))
+    wide = torch.zeros(V, d + 3, dtype=t, device="cuda")                    # rows from odd addresses
+    wide[:, 1:d + 1] = w
+    LossRef(h, w, y, dl).check(*run_loss(h, wide[:, 1:d + 1], y, dl))
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_loss_gradient_of_few_tokens_special(t):
+    h, w, y, dl = loss_case(6, 40, 500, t, seed=3)
+    _, lse = mb.linear_cross_entropy(h, w, y)
+    dh, dw = mb.linear_cross_entropy_backward(h, w, y, lse, dl)
+    z = y.clone()
+    z[2] = -100                                                             # its dloss and lse are not read
+    nan = torch.full_like(dl, float("nan"))
+    a = mb.linear_cross_entropy_backward(h, w, z, torch.where(z < 0, nan, lse), torch.where(z < 0, nan, dl))
+    b = mb.linear_cross_entropy_backward(h, w, y, lse, torch.where(z < 0, torch.zeros_like(dl), dl))
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]) and not a[0][2].any()
+    z[2] = 500                                                              # out of range: loud, no gradient
+    c = mb.linear_cross_entropy_backward(h, w, z, lse, dl)
+    assert torch.equal(c[0], a[0]) and torch.equal(c[1], a[1])
+    with pytest.raises(L.DeviceError, match="27"):
+        mb.linear_cross_entropy_backward(h, w, z, lse, dl, check=True)
+    z[:] = 7                                                                # one entry for all
+    _, ls = mb.linear_cross_entropy(h, w, z)
+    d2, w2 = mb.linear_cross_entropy_backward(h, w, z, ls, dl)
+    LossRef(h, w, z, dl).check(*mb.linear_cross_entropy(h, w, z), d2, w2)
+    bad = h.clone()
+    bad[1, 3] = float("nan")                                                # stays in its token's dh; dW of all entries
+    _, ls = mb.linear_cross_entropy(bad, w, y)
+    d3, w3 = mb.linear_cross_entropy_backward(bad, w, y, ls, dl)
+    keep = [0, 2, 3, 4, 5]
+    assert torch.equal(d3[keep], dh[keep]) and torch.isnan(d3[1]).all() and torch.isnan(w3).all()
+
+
+@pytest.mark.parametrize("t", TYPES)
 def test_loss_gradient_of_lse_and_weighted_tokens(t):
     h, w, y, dl = loss_case(200, 96, 700, t, seed=4, gap=3)
     dl = dl * torch.randint(-1, 2, (200,), device="cuda")        # zero and negative weights
