@@ -42,6 +42,7 @@
 #include <atomic>
 
 #include "dependent.cuh"
+#include "staging_turn.cuh"
 #include "tc_common.cuh"
 
 namespace ml {
@@ -51,7 +52,7 @@ constexpr int THREADS = 384;
 constexpr int EPI_WARPS = 8;
 constexpr int BK = 64;                    // k elements per stage: 128-byte rows
 constexpr int MAX_STAGES = 8;
-constexpr uint32_t STAGING = 4096;        // an epilogue warp's 32 rows x 128 bytes
+constexpr uint32_t STAGING = 2 * STAGING_HALF;   // an epilogue warp's 32 rows x 128 bytes
 constexpr uint32_t CTL_BYTES = 1024;
 constexpr uint32_t SMEM_LIMIT = 227 * 1024;
 
@@ -288,6 +289,19 @@ __device__ __forceinline__ void bulk_store(const CUtensorMap* map, uint32_t src,
                  "r"(src), "r"(x), "r"(y), "r"(z)
                  : "memory");
   asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+
+// The place of the warp's next staged block, free to be written (staging_turn.cuh).
+__device__ __forceinline__ uint32_t staging_place(StagingTurn& turn, uint32_t buf, bool wide, bool bulk) {
+  const StagingTurn::Place p = turn.next(wide, bulk);
+  if ((threadIdx.x & 31) == 0) {
+    if (p.stand)
+      bulk_wait<1, true>();
+    else
+      bulk_wait<0, true>();
+  }
+  __syncwarp();
+  return buf + p.offset;
 }
 
 __device__ __forceinline__ void st_shared16(uint32_t at, uint32_t a) {

@@ -375,10 +375,10 @@ struct EpiGrad {
   using Args = GradArgs;
   float un, sg;
   uint32_t buf;
-  int turn;
+  StagingTurn turn;
   __device__ __forceinline__ void begin(const Args& A, const Sched&, int, uint8_t* staging) {
     buf = tc::smem_u32(staging);
-    turn = 0;
+    turn = StagingTurn{};
     un = logit_unscale(A.amax_h, A.amax_w);
     sg = g16::pow2(dz_exp(A.amax_g));
   }
@@ -442,10 +442,7 @@ struct EpiGrad {
       if constexpr (PIECES == 2) {
         g16::store_pieces(A.out, buf, h, o, col0 + cc, (int)row, 0, on);   // lane 0 has the block's first row
       } else {                         // the halves of the staging buffer in turn
-        const uint32_t b0 = buf + turn * 2048;
-        turn ^= 1;
-        if (lane == 0) g16::bulk_wait<1, true>();
-        __syncwarp();
+        const uint32_t b0 = g16::staging_place(turn, buf, false, true);
         g16::stage16(b0, lane, h);
         tc::fence_proxy_async_smem();
         __syncwarp();
@@ -688,27 +685,18 @@ struct EpiOut {
   using Args = OutArgs;
   float sum[128];                      // the thread's columns over the segments of k
   uint32_t buf;
-  int turn;
+  StagingTurn turn;                    // a cluster may have float32 partials of dh and 16-bit blocks of dW
   __device__ __forceinline__ void begin(const Args&, const Sched&, int, uint8_t* staging) {
     buf = tc::smem_u32(staging);
-    turn = 0;
+    turn = StagingTurn{};
   }
   // The warp's 32 rows x 32 columns.
   __device__ __forceinline__ void block(const OutOne& O, uint32_t (&v)[32], const g16::Unscale& un, int64_t row0,
                                         int col, int ks) {
     const int lane = threadIdx.x & 31;
-    const bool f32 = O.type == MEMLAYER_F32;
-    const uint32_t b = buf + (f32 ? 0 : turn * 2048);
-    turn ^= 1;
 #pragma unroll
     for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(un(__uint_as_float(v[j])));
-    if (lane == 0) {
-      if (f32)
-        g16::bulk_wait<0, true>();
-      else
-        g16::bulk_wait<1, true>();
-    }
-    __syncwarp();
+    const uint32_t b = g16::staging_place(turn, buf, O.type == MEMLAYER_F32, O.tma);
     g16::stage_as(O.type, b, lane, v);
     if (O.tma) {
       tc::fence_proxy_async_smem();

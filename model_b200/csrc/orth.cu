@@ -156,10 +156,10 @@ struct EpiPoly {
   using Args = PolyArgs;
   float sum[128];
   uint32_t buf;
-  int turn;
+  StagingTurn turn;
   __device__ __forceinline__ void begin(const Args&, const Sched&, int, uint8_t* staging) {
     buf = tc::smem_u32(staging);
-    turn = 0;
+    turn = StagingTurn{};
   }
   static __device__ __forceinline__ void pieces(const CUtensorMap* map, uint32_t buf, const uint32_t (&v)[32],
                                                 float s, float diag, int at, int col, int row0, int z, bool mirror) {
@@ -188,18 +188,9 @@ struct EpiPoly {
   }
   __device__ __forceinline__ void plain(const Args& A, uint32_t (&v)[32], int64_t row0, int col, int z) {
     const int lane = threadIdx.x & 31;
-    const bool f32 = A.type == MEMLAYER_F32;
-    const uint32_t b = buf + (f32 ? 0 : turn * 2048);
-    turn ^= 1;
 #pragma unroll
     for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * A.s[0]);
-    if (lane == 0) {
-      if (f32)
-        g16::bulk_wait<0, true>();
-      else
-        g16::bulk_wait<1, true>();
-    }
-    __syncwarp();
+    const uint32_t b = g16::staging_place(turn, buf, A.type == MEMLAYER_F32, A.tma);
     g16::stage_as(A.type, b, lane, v);
     if (A.tma) {
       tc::fence_proxy_async_smem();

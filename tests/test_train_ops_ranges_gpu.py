@@ -1,0 +1,76 @@
+"""The training operators where several of their parts meet: calls whose
+clusters work on both gradients, sums cut into slices, rows and tokens of very
+different magnitudes, padding with anything in it.  References, bounds and
+their derivation: test_train_ops_gpu.py."""
+
+import ctypes as C
+
+import pytest
+import torch
+
+import model_b200 as mb
+from model_b200 import _lib as L
+from test_train_ops_gpu import BF16, F16, F32, TYPES, U, LossRef, gen, half_step, loss_case, run_loss, tiny, within
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- loss: clusters with tiles of dh and of dW ------------------------------------------
+# dh is summed from float32 partials and dW written in 16 bits by the same warps (60 to 81 of the clusters)
+@pytest.mark.parametrize("t", [BF16, F16])
+@pytest.mark.parametrize("T,d,V", [(64, 768, 50257), (128, 1024, 32768), (32, 512, 65536), (64, 512, 65536), (1024, 768, 50257)])
+def test_loss_gradients_that_share_a_cluster(T, d, V, t):
+    h, w, y, dl = loss_case(T, d, V, t, seed=T + V, gap=7)
+    got = run_loss(h, w, y, dl, check=True)
+    LossRef(h, w, y, dl).check(*got)
+    for _ in range(5):
+        again = run_loss(h, w, y, dl)
+        assert all(torch.equal(a, b) for a, b in zip(got, again))
+
+
+def test_loss_dh_of_a_vocabulary_beyond_32_bits():
+    V, d = (1 << 21) + 5, 1032
+    g = gen(3)
+    w = torch.empty(V, d, dtype=BF16, device="cuda")
+    for i in range(0, V, 1 << 18):
+        w[i:i + (1 << 18)] = torch.randn(min(1 << 18, V - i), d, device="cuda", generator=g).to(BF16) * 0.05
+    h = torch.randn(3, d, device="cuda", generator=g).to(BF16)
+    y = torch.tensor([V - 1, 0, V // 2], dtype=torch.int32, device="cuda")
+    dl = torch.full((3,), 1 / 3, device="cuda")
+    loss, lse, dh, dw = run_loss(h, w, y, dl, check=True)
+    z = torch.cat([h.double() @ w[i:i + (1 << 17)].double().T for i in range(0, V, 1 << 17)], 1)
+    p = (z - torch.logsumexp(z, 1, keepdim=True)).exp() / 3
+    mag = p.clone()
+    at = torch.arange(3), y.long()
+    p[at] -= 1 / 3
+    mag[at] += 1 / 3
+    want, size = torch.zeros(3, d, dtype=torch.float64, device="cuda"), torch.zeros(3, d, dtype=torch.float64, device="cuda")
+    for i in range(0, V, 1 << 17):
+        block = w[i:i + (1 << 17)].double()
+        want += p[:, i:i + (1 << 17)] @ block
+        size += mag[:, i:i + (1 << 17)] @ block.abs()
+    # dz in two bf16 pieces 2^-16 of it, a logit of |z| <= 40 2^-15; truncating sums of at most V / 16 steps
+    tol = size * (2.0 ** -16 + 2.0 ** -15 + (V / 16 + 64) * 2 * U) + half_step(BF16) * want.abs()
+    within(dh, want, tol, "dh")
+
+
+# dh for TMA, dweight two bytes beside a 16-byte boundary: one goes out by bulk stores, the other entry by entry
+@pytest.mark.parametrize("t", [BF16, F16])
+@pytest.mark.parametrize("T,d,V", [(64, 768, 5000), (600, 256, 3000)])
+def test_loss_gradients_stored_both_ways(T, d, V, t):
+    h, w, y, dl = loss_case(T, d, V, t, seed=T + V)
+    _, lse = mb.linear_cross_entropy(h, w, y)
+    dh, dw = mb.linear_cross_entropy_backward(h, w, y, lse, dl)
+    code = {BF16: L.BF16, F16: L.F16}[t]
+    cfg, nb = L.MemlayerLossConfig(T, d, V, code, -100), C.c_size_t()
+    L.check(L.lib().memlayer_cross_entropy_workspace_size(cfg, 1, nb), "size")
+    ws = torch.empty(nb.value, dtype=torch.uint8, device="cuda")
+    for off_h, off_w in ((0, 1), (1, 0), (1, 1)):
+        oh, ow = (torch.full((n + 16,), 5.0, device="cuda").to(t) for n in (T * d, V * d))
+        a = L.MemlayerLossArgs(h.data_ptr(), d, w.data_ptr(), d, y.data_ptr(), None, None)
+        g = L.MemlayerLossGrads(lse.data_ptr(), dl.data_ptr(), None, oh[off_h:].data_ptr(), ow[off_w:].data_ptr())
+        L.check(L.lib().memlayer_cross_entropy_backward(cfg, a, g, ws.data_ptr(), nb.value,
+                                                        torch.cuda.current_stream().cuda_stream), "backward")
+        assert torch.equal(oh[off_h:off_h + T * d].view(T, d), dh) and torch.equal(ow[off_w:off_w + V * d].view(V, d), dw)
+        assert (oh[:off_h] == 5).all() and (oh[off_h + T * d:] == 5).all()
+        assert (ow[:off_w] == 5).all() and (ow[off_w + V * d:] == 5).all()
