@@ -396,7 +396,7 @@ __device__ __forceinline__ void copy_rows(int dtype, uint32_t buf, void* out, in
 // staging buffer each, or its transpose.  One proxy fence for both: fences
 // are most of what a small product's stores take.
 __device__ __forceinline__ void store_pieces(const CUtensorMap* map, uint32_t buf, const uint32_t (&h)[16],
-                                             const uint32_t (&l)[16], int x, int y, int z, bool on,
+                                             const uint32_t (&l)[16], int x, int y, int z,
                                              bool transposed = false) {
   const int lane = threadIdx.x & 31;
   if (lane == 0) bulk_wait<0, true>();
@@ -410,7 +410,7 @@ __device__ __forceinline__ void store_pieces(const CUtensorMap* map, uint32_t bu
   }
   tc::fence_proxy_async_smem();
   __syncwarp();
-  if (lane == 0 && on) {
+  if (lane == 0) {
     bulk_store(map, buf, x, y, z, false);
     bulk_store(map + 1, buf + 2048, x, y, z, false);
   }

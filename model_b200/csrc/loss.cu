@@ -385,6 +385,9 @@ struct EpiGrad {
   template <class Get>
   __device__ __forceinline__ void blocks(const Args& A, const Sched& S, const Tile& t, int64_t row, int half,
                                          Get get) {
+    // a warp whose 32 rows are past the last token has nothing to store, and
+    // stages nothing: what it staged last may still be on its way
+    if (row - (threadIdx.x & 31) >= A.T) return;
     const bool on = row < A.T;
     float l = 0.f, q = 0.f, g = 0.f;
     int tg = -1;
@@ -440,13 +443,13 @@ struct EpiGrad {
       }
       const int lane = threadIdx.x & 31;
       if constexpr (PIECES == 2) {
-        g16::store_pieces(A.out, buf, h, o, col0 + cc, (int)row, 0, on);   // lane 0 has the block's first row
+        g16::store_pieces(A.out, buf, h, o, col0 + cc, (int)row, 0);   // lane 0 has the block's first row
       } else {                         // the halves of the staging buffer in turn
         const uint32_t b0 = g16::staging_place(turn, buf, false, true);
         g16::stage16(b0, lane, h);
         tc::fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0 && on) g16::bulk_store(&A.out[0], b0, col0 + cc, (int)row, 0, false);
+        if (lane == 0) g16::bulk_store(&A.out[0], b0, col0 + cc, (int)row, 0, false);
       }
     }
   }

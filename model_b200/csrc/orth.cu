@@ -174,8 +174,8 @@ struct EpiPoly {
       h[j] = *reinterpret_cast<const uint32_t*>(&a);
       l[j] = *reinterpret_cast<const uint32_t*>(&b);
     }
-    g16::store_pieces(map, buf, h, l, col, row0, z, true);
-    if (mirror) g16::store_pieces(map, buf, h, l, row0, col, z, true, true);
+    g16::store_pieces(map, buf, h, l, col, row0, z);
+    if (mirror) g16::store_pieces(map, buf, h, l, row0, col, z, true);
   }
   __device__ __forceinline__ void partial(const Args& A, uint32_t (&v)[32], int row0, int col, int z) {
     const int lane = threadIdx.x & 31;

@@ -79,3 +79,11 @@ def test_the_model_finds_a_wait_that_is_too_short():
     # a half that the warp copies out itself, between two stores of the other
     blocks = [(0, 1), (0, 0), (0, 1)]
     assert conflicts(blocks, [(0, 0), (HALF, 1), (0, 1)]) == [2]
+
+
+def test_every_block_given_to_the_engine_has_to_reach_it(rule):
+    # 16-bit blocks staged as if for bulk stores that are then not issued (rows
+    # past the last token): the second one is written over the store before them
+    blocks = [(0, 1)] * 4
+    assert conflicts([(0, 1), (0, 1), (0, 0), (0, 0)], rule(blocks)) == [3]
+    assert not conflicts([(0, 1), (0, 1)], rule([(0, 1), (0, 1)]))

@@ -74,3 +74,14 @@ def test_loss_gradients_stored_both_ways(T, d, V, t):
         assert torch.equal(oh[off_h:off_h + T * d].view(T, d), dh) and torch.equal(ow[off_w:off_w + V * d].view(V, d), dw)
         assert (oh[:off_h] == 5).all() and (oh[off_h + T * d:] == 5).all()
         assert (ow[:off_w] == 5).all() and (ow[off_w + V * d:] == 5).all()
+
+
+# the last tokens fill one warp's rows or part of them: the warps behind have nothing to store
+@pytest.mark.parametrize("t", [BF16, F16])
+@pytest.mark.parametrize("T,d,V", [(545, 64, 9000), (769, 128, 5000), (1999, 96, 6007), (1057, 256, 4096)])
+def test_loss_gradient_of_a_partly_filled_row_tile(T, d, V, t):
+    h, w, y, dl = loss_case(T, d, V, t, seed=T, gap=11)
+    got = run_loss(h, w, y, dl, check=True)
+    LossRef(h, w, y, dl).check(*got)
+    for _ in range(5):
+        assert all(torch.equal(a, b) for a, b in zip(got, run_loss(h, w, y, dl)))
