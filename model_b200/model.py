@@ -25,7 +25,7 @@ import torch
 
 from . import _lib as L
 from .memory import MemoryPool, _cuda_f32, _raise_device_status, _workspace, on_stream
-from .train_ops import (layer_norm, layer_norm_backward, linear_cross_entropy,
+from .train_ops import (_targets, layer_norm, layer_norm_backward, linear_cross_entropy,
                         linear_cross_entropy_backward)
 
 
@@ -261,7 +261,7 @@ class PreparedModel:
                             dloss: Optional[torch.Tensor] = None, ignore_index: int = -100, check: bool = False,
                             stream=None):
         """``MemoryPoolLM.loss_and_head_grads`` on these parameters."""
-        targets = targets.to(self.device)
+        targets = _targets(targets.to(self.device), ignore_index)
         x = self.hidden(tokens, check=check)
         h = layer_norm(x, self.ln_final["scale"], self.ln_final["bias"])
         loss, lse = linear_cross_entropy(h, self.embedding, targets, ignore_index=ignore_index, check=check)

@@ -190,6 +190,21 @@ def _layer_norm_backward(dy, x, scale, dresidual, eps, check):
     return dx, {"scale": ds, "bias": db}
 
 
+def _targets(targets: torch.Tensor, ignore_index: int) -> torch.Tensor:
+    """``targets`` as int32; an id that 32 bits cannot hold stays out of range and is not the ignored one."""
+    t = targets.dtype
+    if t is torch.int32:
+        return targets
+    if t in (torch.uint8, torch.int8, torch.int16, torch.uint16):
+        # as they are: compared in their own type with 32-bit limits, every id would be out of range
+        return targets.to(torch.int32)
+    if t not in (torch.int64, torch.uint32):
+        raise ValueError(f"targets must be integers of at most 32 bits or int64, not {t}")
+    targets = targets.to(torch.int64)
+    bad = -1 if ignore_index != -1 else -2
+    return torch.where((targets >= -2 ** 31) & (targets < 2 ** 31), targets, bad).to(torch.int32)
+
+
 def _loss_args(h, weight, targets, ignore_index):
     code = _dtype(h)
     if not isinstance(weight, torch.Tensor) or weight.device != h.device or weight.dtype != h.dtype:
@@ -198,15 +213,12 @@ def _loss_args(h, weight, targets, ignore_index):
         raise ValueError("h must be [..., d] and weight [vocab, d]")
     if not isinstance(targets, torch.Tensor) or targets.device != h.device:
         raise TypeError("targets must be a tensor on the device of h")
-    if targets.is_floating_point() or targets.dtype == torch.bool or targets.shape != h.shape[:-1]:
-        raise ValueError(f"targets must be integers of shape {tuple(h.shape[:-1])}")
+    if targets.shape != h.shape[:-1]:
+        raise ValueError(f"targets must have shape {tuple(h.shape[:-1])}")
     if not -2 ** 31 <= ignore_index < 2 ** 31:
         raise ValueError("ignore_index must fit 32 bits")
     V, d = weight.shape
-    if targets.dtype != torch.int32:
-        # an id that 32 bits cannot hold stays out of range, and is not the ignored one
-        bad = -1 if ignore_index != -1 else -2
-        targets = torch.where((targets >= -2 ** 31) & (targets < 2 ** 31), targets, bad).to(torch.int32)
+    targets = _targets(targets, ignore_index)
     t = targets.contiguous()
     hr, ldh = _rows(h, d)
     wr, ldw = _rows(weight, d)

@@ -246,3 +246,33 @@ def test_extension_declines_what_it_does_not_take():
                  lambda: train_ops.linear_cross_entropy_backward(x, x, v, v, v)):
         with pytest.raises(TypeError, match="CUDA tensor"):
             call()
+
+
+# ---- targets of every integer type --------------------------------------------------------
+@pytest.mark.parametrize("t", [torch.uint8, torch.int8, torch.int16, torch.uint16, torch.int32, torch.uint32, torch.int64])
+def test_targets_of_any_integer_type_keep_their_ids(t):
+    from model_b200 import train_ops
+    h, w = torch.zeros(2, 3, 4), torch.zeros(100, 4)
+    y = torch.tensor([[0, 1, 99], [7, 100, 127]]).to(t)
+    assert train_ops._loss_args(h, w, y, -100)[-1].tolist() == [[0, 1, 99], [7, 100, 127]]
+    if t.is_signed:
+        y[0, 0] = -100
+        assert train_ops._loss_args(h, w, y, -100)[-1].tolist() == [[-100, 1, 99], [7, 100, 127]]
+
+
+def test_targets_beyond_32_bits_are_neither_ids_nor_ignored():
+    from model_b200 import train_ops
+    h, w = torch.zeros(4, 4), torch.zeros(100, 4)
+    y = torch.tensor([3 + 2 ** 32, -1 - 2 ** 32, 2 ** 31, 5])
+    for ignore in (-100, -1, -2, 3):
+        t = train_ops._loss_args(h, w, y, ignore)[-1]
+        assert t.dtype == torch.int32 and t[3] == 5 and not ((t[:3] >= 0) | (t[:3] == ignore)).any()
+    t = train_ops._loss_args(h, w, torch.tensor([2 ** 32 - 100, 1, 2, 3], dtype=torch.uint32), -100)[-1]
+    assert t.tolist() == [-1, 1, 2, 3]
+
+
+@pytest.mark.parametrize("t", [torch.bool, torch.float32, torch.complex64, torch.uint64])
+def test_targets_of_other_types_refused(t):
+    from model_b200 import train_ops
+    with pytest.raises(ValueError, match="targets must be integers"):
+        train_ops._loss_args(torch.zeros(4, 4), torch.zeros(100, 4), torch.zeros(4, dtype=t), -100)

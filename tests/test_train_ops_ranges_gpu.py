@@ -85,3 +85,27 @@ def test_loss_gradient_of_a_partly_filled_row_tile(T, d, V, t):
     LossRef(h, w, y, dl).check(*got)
     for _ in range(5):
         assert all(torch.equal(a, b) for a, b in zip(got, run_loss(h, w, y, dl)))
+
+
+@pytest.mark.parametrize("it", [torch.uint8, torch.int8, torch.int16, torch.uint16, torch.uint32, torch.int64])
+def test_loss_targets_of_any_integer_type(it):
+    h, w, y, dl = loss_case(40, 32, 120, F32, seed=9)
+    want = run_loss(h, w, y, dl)
+    got = run_loss(h, w, y.to(it), dl, check=True)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_model_head_with_targets_of_any_integer_type():
+    from model_b200 import MemoryPoolLM, ModelConfig
+    cfg = ModelConfig(vocab_size=200, max_len=32, d_model=64, n_layers=1, n_heads=2, ffn_mult=2, memory_layers=(),
+                      n_sub_keys=16, pool_heads=2, d_key=32, d_value=64, top_k=4)
+    m = MemoryPoolLM(cfg)
+    prep = m.prepare(m.init(1))
+    tok = torch.randint(0, 200, (2, 32), device="cuda", generator=gen(60))
+    tgt = torch.randint(0, 200, (2, 32), device="cuda", generator=gen(61))
+    tgt[0, :8] = 156                         # -100 in eight bits
+    loss, grads = m.loss_and_head_grads(prep, tok, tgt)
+    for it in (torch.uint8, torch.int16, torch.int32):
+        l2, g2 = m.loss_and_head_grads(prep, tok, tgt.to(it))
+        assert torch.equal(loss, l2) and torch.equal(grads["hidden"], g2["hidden"])
+        assert torch.equal(grads["embed"]["embedding"], g2["embed"]["embedding"])
