@@ -268,8 +268,9 @@ class PreparedModel:
         if dloss is None:
             n = (targets != ignore_index).sum().clamp(min=1)
             dloss = (1.0 / n).to(torch.float32).expand(targets.shape)
-        dh, dw = linear_cross_entropy_backward(h, self.embedding, targets, lse, dloss, ignore_index=ignore_index)
-        dx, dp = layer_norm_backward(dh, x, self.ln_final["scale"])
+        dh, dw = linear_cross_entropy_backward(h, self.embedding, targets, lse, dloss, ignore_index=ignore_index,
+                                               check=check)
+        dx, dp = layer_norm_backward(dh, x, self.ln_final["scale"], check=check)
         return loss, {"hidden": dx, "ln_final": dp, "embed": {"embedding": dw}}
 
 

@@ -276,3 +276,29 @@ def test_targets_of_other_types_refused(t):
     from model_b200 import train_ops
     with pytest.raises(ValueError, match="targets must be integers"):
         train_ops._loss_args(torch.zeros(4, 4), torch.zeros(100, 4), torch.zeros(4, dtype=t), -100)
+
+
+@pytest.mark.parametrize("check", [False, True])
+def test_head_gradients_pass_check_to_every_call(monkeypatch, check):
+    from model_b200 import model as M
+    seen = {}
+
+    def record(name, result):
+        def call(*args, check=None, **kw):
+            seen[name] = check
+            return result
+        return call
+    x, v = torch.zeros(2, 3, 4), torch.zeros(2, 3)
+    monkeypatch.setattr(M.PreparedModel, "hidden", record("hidden", x))
+    monkeypatch.setattr(M, "layer_norm", lambda *a, **k: x)                # has no status to check
+    monkeypatch.setattr(M, "linear_cross_entropy", record("loss", (v, v)))
+    monkeypatch.setattr(M, "linear_cross_entropy_backward", record("loss gradient", (x, x)))
+    monkeypatch.setattr(M, "layer_norm_backward", record("norm gradient", (x, {})))
+    prep = object.__new__(M.PreparedModel)
+    prep.device, prep.embedding, prep.ln_final = torch.device("cpu"), x, {"scale": v, "bias": v}
+    tokens = torch.zeros(2, 3, dtype=torch.int32)
+    prep.loss_and_head_grads(tokens, tokens, check=check)
+    assert seen == {k: check for k in ("hidden", "loss", "loss gradient", "norm gradient")}
+    seen.clear()
+    prep.loss(tokens, tokens, check=check)
+    assert seen == {"hidden": check, "loss": check}
