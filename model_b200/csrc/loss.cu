@@ -57,6 +57,12 @@ __device__ __forceinline__ float logit_unscale(const unsigned* amax_h, const uns
   return g16::pow2(max(-100, min(126, -exp_of(amax_h) - exp_of(amax_w))));
 }
 
+__device__ __forceinline__ unsigned long long pair(float a, float b) {
+  unsigned long long r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // The 32 columns from cc on of an epilogue thread's row: from its accumulator,
 // or from the sums of its segments.
 struct FromTmem {
@@ -80,7 +86,7 @@ struct StatsArgs {
   int V;
   const unsigned *amax_h, *amax_w;   // float32 operands: scale maxima (else null)
   const int* targets;
-  float2* part;                      // [slot][half][T] (maximum in log2 units, sum)
+  float2* part;                      // [slot][half][T] (maximum, sum of exp(z - maximum))
   float* zt;                         // [T] target logit
 };
 
@@ -105,7 +111,7 @@ struct EpiStats {
     if (!any || row >= A.T) return;
     // clusters before this one that hold tiles of the row block
     const int first = S.owner(mt * S.prod[0].n_tiles);
-    A.part[((int64_t)(slot - first) * 2 + half) * A.T + row] = make_float2(m * c, s);
+    A.part[((int64_t)(slot - first) * 2 + half) * A.T + row] = make_float2(m * un, s);
   }
   template <class Get>
   __device__ __forceinline__ void blocks(const Args& A, const Sched& S, const Tile& t, int64_t r, int half, Get get) {
@@ -135,12 +141,25 @@ struct EpiStats {
       float mx = __uint_as_float(v[0]);
 #pragma unroll
       for (int j = 1; j < 32; ++j) mx = fmaxf(mx, __uint_as_float(v[j]));
+      // the difference first, then the factor: at the maximum it is 0 whatever
+      // the logits' size (v c - round(m c) is not: 4,000 for logits of 1e10),
+      // and elsewhere its error goes by the difference, not by the logits.
+      // Two columns an instruction: as many as one fused multiply-add each.
       const float mn = fmaxf(m, mx);
-      const float ref = mn == -INFINITY ? 0.f : mn * c;
+      const float ref = mn == -INFINITY ? 0.f : mn;
+      const unsigned long long nr = pair(-ref, -ref), cc2 = pair(c, c);
       float a[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int j = 0; j < 32; ++j) a[j & 3] += g16::exp2_fast(fmaf(__uint_as_float(v[j]), c, -ref));
-      s = fmaf(s, g16::exp2_fast(fmaf(m, c, -ref)), (a[0] + a[1]) + (a[2] + a[3]));
+      for (int j = 0; j < 32; j += 2) {
+        unsigned long long x = pair(__uint_as_float(v[j]), __uint_as_float(v[j + 1]));
+        asm("add.rn.f32x2 %0, %0, %1;" : "+l"(x) : "l"(nr));
+        asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(x) : "l"(cc2));
+        float e0, e1;
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(e0), "=f"(e1) : "l"(x));
+        a[j & 3] += g16::exp2_fast(e0);
+        a[(j & 3) + 1] += g16::exp2_fast(e1);
+      }
+      s = fmaf(s, g16::exp2_fast((m - ref) * c), (a[0] + a[1]) + (a[2] + a[3]));
       m = mn;
       const unsigned at = (unsigned)(target - (col0 + cc));
       if (at < 32u && (int)at < left) {
@@ -184,7 +203,7 @@ __global__ void __launch_bounds__(256) loss_join_kernel(const float2* __restrict
     const float2 p = part[(int64_t)i * T + row];
     const float mn = fmaxf(m, p.x);
     const float ref = mn == -INFINITY ? 0.f : mn;
-    s = s * exp2f(m - ref) + p.y * exp2f(p.x - ref);
+    s = s * exp2f((m - ref) * LOG2E) + p.y * exp2f((p.x - ref) * LOG2E);
     m = mn;
   }
 #pragma unroll
@@ -192,11 +211,11 @@ __global__ void __launch_bounds__(256) loss_join_kernel(const float2* __restrict
     const float m2 = __shfl_xor_sync(FULL, m, o), s2 = __shfl_xor_sync(FULL, s, o);
     const float mn = fmaxf(m, m2);
     const float ref = mn == -INFINITY ? 0.f : mn;
-    s = s * exp2f(m - ref) + s2 * exp2f(m2 - ref);
+    s = s * exp2f((m - ref) * LOG2E) + s2 * exp2f((m2 - ref) * LOG2E);
     m = mn;
   }
   if (lane == 0) {
-    const float l = (m + log2f(s)) * LN2;
+    const float l = fmaf(log2f(s), LN2, m);
     lse[row] = l;
     const int t = targets[row];
     const bool in = t >= 0 && t < V;
@@ -298,14 +317,14 @@ __global__ void __launch_bounds__(FEW_V * (FEW / FEW_M)) loss_few_kernel(FewArgs
     float mx = -INFINITY;
 #pragma unroll
     for (int i = 0; i < FEW_V / 32; ++i) {
-      z[i] = zs[m * FEW_V + i * 32 + lane] * LOG2E;
+      z[i] = zs[m * FEW_V + i * 32 + lane];
       mx = fmaxf(mx, z[i]);
     }
     mx = warp_max(mx);
     const float ref = mx == -INFINITY ? 0.f : mx;
     float s = 0.f;
 #pragma unroll
-    for (int i = 0; i < FEW_V / 32; ++i) s += g16::exp2_fast(z[i] - ref);
+    for (int i = 0; i < FEW_V / 32; ++i) s += g16::exp2_fast((z[i] - ref) * LOG2E);
     s = warp_sum(s);
     if (lane == 0) {
       A.part[(int64_t)blockIdx.x * A.T + m] = make_float2(mx, s);
@@ -569,7 +588,9 @@ __global__ void __launch_bounds__(FEWB_T, TM <= 4 ? 2 : 1) loss_few_backward_ker
     __syncthreads();
     for (int e = t; e < rows * TM; e += FEWB_T) {
       const int m = e % TM, v = v0 + e / TM;
-      float x = g16::exp2_fast((dz[e] - l[m]) * LOG2E) * q[m];
+      const float lp = dz[e] - l[m];
+      // p <= 1, though the forward added these logits in another order (a NaN stays)
+      float x = g16::exp2_fast(lp > 0.f ? 0.f : lp * LOG2E) * q[m];
       if (tg[m] == v) x -= g[m];
       dz[e] = q[m] == 0.f && g[m] == 0.f ? 0.f : x;     // an ignored token: nothing, whatever its logits are
     }

@@ -109,3 +109,33 @@ def test_model_head_with_targets_of_any_integer_type():
         l2, g2 = m.loss_and_head_grads(prep, tok, tgt.to(it))
         assert torch.equal(loss, l2) and torch.equal(grads["hidden"], g2["hidden"])
         assert torch.equal(grads["embed"]["embedding"], g2["embed"]["embedding"])
+
+
+# ---- loss: large logits -----------------------------------------------------------------
+# the largest logit's own term is exp(0) whatever its size; one entry has all the probability
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("size", [1e3, 1e6, 1e9, 1e12])
+@pytest.mark.parametrize("T,d,V", [(1, 64, 300), (16, 64, 1000), (24, 36, 500), (40, 130, 700), (200, 64, 3000), (300, 640, 300)])
+def test_loss_of_large_logits(T, d, V, size, t):
+    h, w, y, dl = loss_case(T, d, V, F32, seed=T + d)
+    at = (h.double() @ w.double().T).argmax(1)
+    y[::2] = at[::2].int()
+    if t == F16:
+        size = min(size, 1e8)                     # its range
+    a = (size / 3) ** 0.5
+    h, w = (h * a).to(t), (w * a).to(t)
+    ref = LossRef(h, w, y, dl)
+    # an exponential below the smallest normal float is 0, and bf16 holds what is left of it beside such
+    # logits: 2^-126 of every term on top of the bounds (dw of entries of a probability of 1e-40 is 1e-40)
+    none = 2.0 ** -126 * dl.double()[:, None].expand(T, V)
+    ref.dh_tol, ref.dw_tol = ref.dh_tol + none @ w.double().abs(), ref.dw_tol + none.T @ h.double().abs()
+    loss, lse, dh, dw = run_loss(h, w, y, dl, check=True)
+    ref.check(loss, lse, dh, dw)
+    z = h.double() @ w.double().T
+    top = z.max(1).values
+    clear = (z < top[:, None] - 100).sum(1) == V - 1       # nothing else counts: lse is the logit itself
+    assert size < 1e3 or clear.any()
+    hit = clear & (y == z.argmax(1))
+    assert not loss[hit].any()
+    if T > 24:                                    # the gradient finds the forward's logits again: p is 1, dz 0
+        assert not dh[hit].any()
