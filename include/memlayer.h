@@ -695,13 +695,16 @@ int32_t memlayer_cross_entropy_workspace_size(const memlayer_loss_config* cfg, i
  * (model.py:125 under the trainer's loss) without the [T, V] logits.  A
  * target outside [0, V) that is not ignore_index gives a NaN loss and, in the
  * backward, no gradient; it records status 27, read with
- * memlayer_train_status.  float32 products keep 22 bits of each
- * operand (relative to its matrix's largest entry). */
+ * memlayer_train_status.  float32 products keep 22 bits of each operand:
+ * of h relative to the token's largest entry, of the weight relative to its
+ * largest entry. */
 int32_t memlayer_cross_entropy(const memlayer_loss_config* cfg, const memlayer_loss_args* args, void* workspace,
                                size_t workspace_bytes, void* stream);
 
 /* dh and dweight of sum(dloss * loss) + sum(dlse * lse); args as in the
- * forward (loss and lse there are not used).  h must be finite at ignored
+ * forward (loss and lse there are not used).  The sums over tokens of a
+ * float32 dweight keep 22 bits relative to the largest entry of h among the
+ * tokens that have a gradient.  h must be finite at ignored
  * tokens too: their zero gradient multiplies it in dweight. */
 int32_t memlayer_cross_entropy_backward(const memlayer_loss_config* cfg, const memlayer_loss_args* args,
                                         const memlayer_loss_grads* grads, void* workspace, size_t workspace_bytes,

@@ -1,7 +1,6 @@
-// Host side of the 16-bit tensor-core GEMM (gemm16.cuh) and the kernels that
-// put its operands into 16-bit form: the largest magnitude of float32
-// matrices, their split into f16 pieces, and the copy of 16-bit matrices
-// whose rows TMA cannot address.
+// Host side of the 16-bit tensor-core GEMM (gemm16.cuh) and the kernel that
+// puts its operands into 16-bit form: float32 matrices split into f16 pieces,
+// 16-bit matrices whose rows TMA cannot address copied.
 #include <cudaTypedefs.h>
 
 #include <atomic>
@@ -15,58 +14,7 @@ namespace ml {
 
 namespace {
 
-constexpr int NTH = 256;
-
-// Bits of the largest finite |x| (order of non-negative floats = order of bits).
-__global__ void __launch_bounds__(NTH) amax_kernel(AmaxArgs A) {
-  allow_next();
-  wait_previous();
-  __shared__ unsigned red[NTH / 32];
-  int i = 0, b = blockIdx.x;
-  while (b >= A.m[i].blocks) b -= A.m[i++].blocks;
-  const AmaxMat M = A.m[i];
-  unsigned mx = 0;
-  auto take = [&](float x) {
-    const unsigned u = __float_as_uint(x) & 0x7FFFFFFFu;
-    if (u < 0x7F800000u && u > mx) mx = u;
-  };
-  const int64_t step = (int64_t)M.blocks * NTH, at = (int64_t)b * NTH + threadIdx.x;
-  if (M.pitch == M.cols && (reinterpret_cast<uintptr_t>(M.x) & 15) == 0) {
-    const int64_t n = M.rows * M.cols, n4 = n >> 2;
-    const float4* x4 = reinterpret_cast<const float4*>(M.x);
-    int64_t e = at;
-    for (; e + 3 * step < n4; e += 4 * step) {     // four loads in flight
-      float4 v[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = x4[e + j * step];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        take(v[j].x);
-        take(v[j].y);
-        take(v[j].z);
-        take(v[j].w);
-      }
-    }
-    for (; e < n4; e += step) {
-      const float4 v = x4[e];
-      take(v.x);
-      take(v.y);
-      take(v.z);
-      take(v.w);
-    }
-    if (at < (n & 3)) take(M.x[(n4 << 2) + at]);
-  } else {
-    const int64_t n = M.rows * M.cols;
-    for (int64_t e = at; e < n; e += step) take(M.x[(e / M.cols) * M.pitch + e % M.cols]);
-  }
-  mx = __reduce_max_sync(FULL, mx);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = mx;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < NTH / 32; ++w) mx = max(mx, red[w]);
-    if (mx) atomicMax(M.out, mx);                  // a maximum: the order does not matter
-  }
-}
+constexpr int NTH = PIECE_THREADS;
 
 // 8 columns a thread: hi / lo pieces of x s (float32 source) or a plain copy
 // (16-bit source), zeros in the padding columns.
@@ -86,9 +34,13 @@ __global__ void __launch_bounds__(NTH) pieces_kernel(PiecesArgs A) {
     const int64_t r = e / c8;
     const int c = (int)(e - r * c8) * 8;
     const E* p = src + r * M.pitch + c;
+    const bool skip = M.row_tgt && M.row_tgt[r] == PIECE_SKIP;
     if constexpr (sizeof(E) == 4) {
       float v[8];
-      if (vec && c + 8 <= M.cols) {
+      if (skip) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = 0.f;
+      } else if (vec && c + 8 <= M.cols) {
         const float4 a = *reinterpret_cast<const float4*>(p), q = *reinterpret_cast<const float4*>(p + 4);
         v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
         v[4] = q.x; v[5] = q.y; v[6] = q.z; v[7] = q.w;
@@ -108,11 +60,6 @@ __global__ void __launch_bounds__(NTH) pieces_kernel(PiecesArgs A) {
       *reinterpret_cast<uint4*>(reinterpret_cast<E*>(M.hi) + r * M.ld + c) = *reinterpret_cast<uint4*>(v);
     }
   }
-}
-
-int blocks_for(int64_t items, int per_thread) {
-  const int64_t b = (items + (int64_t)NTH * per_thread - 1) / ((int64_t)NTH * per_thread), cap = 8 * g16::device_sms();
-  return (int)(b < 1 ? 1 : b < cap ? b : cap);
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encode16_fn() {
@@ -214,27 +161,12 @@ double distribute(Sched* S, int most, double over) {
 
 }  // namespace g16
 
-cudaError_t launch_amax(AmaxArgs A, cudaStream_t s) {
-  int total = 0;
-  for (int i = 0; i < 4; ++i) {
-    if (A.m[i].rows * A.m[i].cols == 0) {
-      A.m[i].blocks = 0;
-      continue;
-    }
-    A.m[i].blocks = blocks_for(A.m[i].rows * A.m[i].cols, 16);
-    total += A.m[i].blocks;
-  }
-  if (!total) return cudaSuccess;
-  count_launch();
-  return launch_dependent(amax_kernel, dim3(total), NTH, 0, s, A);
-}
-
 cudaError_t launch_pieces(PiecesArgs A, int dtype, cudaStream_t s) {
   int total = 0;
-  for (int i = 0; i < 2; ++i) {
-    const int64_t n = A.m[i].rows * (A.m[i].ld >> 3);
-    A.m[i].blocks = n ? blocks_for(n, 2) : 0;
-    total += A.m[i].blocks;
+  for (PiecesMat& M : A.m) {
+    const int64_t n = M.rows * (M.ld >> 3);
+    M.blocks = n ? piece_blocks(n, 2) : 0;
+    total += M.blocks;
   }
   if (!total) return cudaSuccess;
   count_launch();

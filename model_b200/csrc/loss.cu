@@ -16,8 +16,8 @@
 // piece's [T, piece] matrix in the workspace), and one launch multiplies it
 // both ways, dW of the piece and its part of dh.
 //
-// float32 operands run as two f16 pieces each (22 bits, see gemm16.cuh), dz
-// too; 16-bit operands as they are, dz rounded once to their type (its
+// float32 operands run as two f16 pieces each (22 bits, see gemm16.cuh; h with
+// a scale a token), dz too; 16-bit operands as they are, dz rounded once to their type (its
 // relative error, 2^-9 or 2^-12, averages out over the sums it enters).  f16
 // dz carries a power-of-two scale from the largest |dloss|.  Statistics,
 // exponentials and sums are float32.
@@ -51,10 +51,91 @@ constexpr int LOGIT_SEG = 8;
 
 __device__ __forceinline__ int exp_of(const unsigned* amax) { return amax ? g16::scale_exp(*amax) : 0; }
 
-// Factor that turns an accumulator of the logits back: a normal float (beyond
-// that range logits are zero or infinite for every purpose).
-__device__ __forceinline__ float logit_unscale(const unsigned* amax_h, const unsigned* amax_w) {
-  return g16::pow2(max(-100, min(126, -exp_of(amax_h) - exp_of(amax_w))));
+// Factor that turns an accumulator of a token's logits back: a normal float
+// (beyond that range logits are zero or infinite for every purpose).  top_h:
+// the tokens' largest magnitudes (float32 operands, else null).
+__device__ __forceinline__ float logit_unscale(const unsigned* top_h, int64_t row, bool on, const unsigned* amax_w) {
+  return g16::pow2(max(-100, min(126, -(on && top_h ? g16::scale_exp(top_h[row]) : 0) - exp_of(amax_w))));
+}
+
+// ---- float32 tokens as pieces ------------------------------------------------------
+// Each token gets a scale of its own, from its largest entry: with one for all
+// of them a single huge one -- padding, too, where anything may stand -- takes
+// the others' bits (a row of 1e10 among ones of 1 put their lse 0.02 off).
+// A logit belongs to one token, so the epilogues take the scale out by row.
+// The gradient's dW sums over tokens; for it h is split once more, by the
+// largest entry of the tokens that have a gradient.  The first blocks look for
+// the weight's largest magnitude meanwhile.
+struct TokenArgs {
+  AmaxMat w;
+  const float* h;
+  int64_t T, ldh, ld;
+  int d, tpr;                          // tpr: threads a token, 32 or all
+  __half *hi, *lo;                     // [T][ld]
+  unsigned* top;                       // [T] bits of the largest finite magnitude
+};
+
+__global__ void __launch_bounds__(PIECE_THREADS) loss_tokens_kernel(TokenArgs A) {
+  __shared__ unsigned red[PIECE_THREADS / 32];
+  allow_next();
+  wait_previous();
+  if ((int)blockIdx.x < A.w.blocks) {
+    amax_block(A.w, blockIdx.x);
+    return;
+  }
+  const int t = threadIdx.x & (A.tpr - 1), groups = PIECE_THREADS / A.tpr, d = A.d;
+  const bool vec = A.ldh % 4 == 0 && d % 4 == 0 && (reinterpret_cast<uintptr_t>(A.h) & 15) == 0;
+  const int64_t step = (int64_t)(gridDim.x - A.w.blocks) * groups;
+  for (int64_t base = (int64_t)(blockIdx.x - A.w.blocks) * groups; base < A.T; base += step) {
+    const int64_t row = base + threadIdx.x / A.tpr;
+    const bool on = row < A.T;
+    const float* x = A.h + (on ? row : 0) * A.ldh;
+    unsigned mx = 0;
+    if (vec) {
+#pragma unroll 2
+      for (int c = t * 4; c < d; c += A.tpr * 4) {
+        const float4 v = *reinterpret_cast<const float4*>(x + c);
+        mx = max(max(mx, max(finite_bits(v.x), finite_bits(v.y))), max(finite_bits(v.z), finite_bits(v.w)));
+      }
+    } else {
+      for (int c = t; c < d; c += A.tpr) mx = max(mx, finite_bits(x[c]));
+    }
+    mx = __reduce_max_sync(FULL, mx);
+    if (A.tpr > 32) {
+      __syncthreads();                 // the slots of the token before are read
+      if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = mx;
+      __syncthreads();
+      for (int w = 0; w < PIECE_THREADS / 32; ++w) mx = max(mx, red[w]);
+    }
+    if (!on) continue;
+    if (t == 0) A.top[row] = mx;
+    const float sc = g16::pow2(g16::scale_exp(mx));
+    for (int c = t * 8; c < (int)A.ld; c += A.tpr * 8) {
+      float v[8];
+      if (vec && c + 8 <= d) {
+        const float4 a = *reinterpret_cast<const float4*>(x + c), b = *reinterpret_cast<const float4*>(x + c + 4);
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+        v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = c + j < d ? x[c + j] : 0.f;
+      }
+      __half2 h[4], l[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) g16::split2(v[2 * j] * sc, v[2 * j + 1] * sc, h[j], l[j]);
+      *reinterpret_cast<uint4*>(A.hi + row * A.ld + c) = *reinterpret_cast<uint4*>(h);
+      *reinterpret_cast<uint4*>(A.lo + row * A.ld + c) = *reinterpret_cast<uint4*>(l);
+    }
+  }
+}
+
+cudaError_t launch_tokens(TokenArgs A, cudaStream_t s) {
+  A.w.blocks = piece_blocks(A.w.rows * A.w.cols, 16);
+  A.tpr = A.d <= 2048 ? 32 : PIECE_THREADS;
+  const int64_t need = (A.T * A.tpr + PIECE_THREADS - 1) / PIECE_THREADS, cap = 8 * g16::device_sms();
+  count_launch();
+  return launch_dependent(loss_tokens_kernel, dim3((unsigned)(A.w.blocks + (need < cap ? need : cap))), PIECE_THREADS, 0, s,
+                          A);
 }
 
 __device__ __forceinline__ unsigned long long pair(float a, float b) {
@@ -84,7 +165,7 @@ struct FromSums {
 struct StatsArgs {
   int64_t T;
   int V;
-  const unsigned *amax_h, *amax_w;   // float32 operands: scale maxima (else null)
+  const unsigned *top_h, *amax_w;    // float32 operands: largest magnitudes, a token's and the weight's (else null)
   const int* targets;
   float2* part;                      // [slot][half][T] (maximum, sum of exp(z - maximum))
   float* zt;                         // [T] target logit
@@ -101,8 +182,6 @@ struct EpiStats {
   bool any;
 
   __device__ __forceinline__ void begin(const Args& A, const Sched&, int cluster, uint8_t*) {
-    un = logit_unscale(A.amax_h, A.amax_w);
-    c = un * LOG2E;
     mt = -1;
     slot = cluster;
     any = false;
@@ -123,6 +202,8 @@ struct EpiStats {
       s = 0.f;
       any = true;
       target = row < A.T ? A.targets[row] : -1;
+      un = logit_unscale(A.top_h, row, row < A.T, A.amax_w);
+      c = un * LOG2E;
     }
     const int hw = S.BN >> 1;
     const int col0 = t.nt * S.BN + half * hw;
@@ -349,28 +430,36 @@ bool few_tokens(const memlayer_loss_config& c, const memlayer_loss_args& a) {
 
 // ---- backward ---------------------------------------------------------------------
 // Per token: the factor of p, the factor of the one-hot target and the target
-// (-1: none); the largest of the factors' magnitudes for the scale of dz.
+// (-1: none; PIECE_SKIP: no gradient at all); the largest of the factors'
+// magnitudes for the scale of dz, the largest entry of the tokens that have a
+// gradient for that of dW's h.
 __global__ void __launch_bounds__(256) loss_rows_kernel(const int* __restrict__ targets,
                                                         const float* __restrict__ dloss,
                                                         const float* __restrict__ dlse, int64_t T, int V, int ignore,
+                                                        const unsigned* __restrict__ top_h,
                                                         float2* __restrict__ coef, int* __restrict__ tgt,
-                                                        unsigned* __restrict__ amax, int* __restrict__ err) {
+                                                        unsigned* __restrict__ amax, unsigned* __restrict__ amax_h,
+                                                        int* __restrict__ err) {
   allow_next();
   wait_previous();
-  unsigned mx = 0;
+  unsigned mx = 0, mh = 0;
   for (int64_t t = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; t < T; t += (int64_t)gridDim.x * blockDim.x) {
     const int v = targets[t];
     const bool in = v >= 0 && v < V && v != ignore;
     if (!in && v != ignore) atomicCAS(err, 0, STATUS_TARGET);
     const float g = in ? dloss[t] : 0.f, q = g + (dlse ? dlse[t] : 0.f);
     coef[t] = make_float2(q, g);
-    tgt[t] = in ? v : -1;
-    const unsigned a = __float_as_uint(g) & 0x7FFFFFFFu, b = __float_as_uint(q) & 0x7FFFFFFFu;
-    if (a < 0x7F800000u) mx = max(mx, a);
-    if (b < 0x7F800000u) mx = max(mx, b);
+    const bool none = g == 0.f && q == 0.f;
+    tgt[t] = none ? PIECE_SKIP : in ? v : -1;
+    mx = max(mx, max(finite_bits(g), finite_bits(q)));
+    if (top_h && !none) mh = max(mh, top_h[t]);
   }
   mx = __reduce_max_sync(FULL, mx);
-  if ((threadIdx.x & 31) == 0 && mx) atomicMax(amax, mx);
+  mh = __reduce_max_sync(FULL, mh);
+  if ((threadIdx.x & 31) == 0) {
+    if (mx) atomicMax(amax, mx);
+    if (mh) atomicMax(amax_h, mh);
+  }
 }
 
 // Scale of dz: |p q - [target] g| <= 2 max(|q|, |g|) < 2^15.
@@ -379,7 +468,7 @@ __device__ __forceinline__ int dz_exp(const unsigned* amax) { return amax ? g16:
 struct GradArgs {
   int64_t T;
   int v0, vc;                          // the piece: columns [v0, v0 + vc)
-  const unsigned *amax_h, *amax_w, *amax_g;
+  const unsigned *top_h, *amax_w, *amax_g;
   const float* lse;
   const float2* coef;
   const int* tgt;
@@ -392,13 +481,12 @@ struct EpiGrad {
   static constexpr bool kSum = SUM, kStore = true;
   float sum[128];
   using Args = GradArgs;
-  float un, sg;
+  float sg;
   uint32_t buf;
   StagingTurn turn;
   __device__ __forceinline__ void begin(const Args& A, const Sched&, int, uint8_t* staging) {
     buf = tc::smem_u32(staging);
     turn = StagingTurn{};
-    un = logit_unscale(A.amax_h, A.amax_w);
     sg = g16::pow2(dz_exp(A.amax_g));
   }
   template <class Get>
@@ -408,6 +496,7 @@ struct EpiGrad {
     // stages nothing: what it staged last may still be on its way
     if (row - (threadIdx.x & 31) >= A.T) return;
     const bool on = row < A.T;
+    const float un = logit_unscale(A.top_h, row, on, A.amax_w);
     float l = 0.f, q = 0.f, g = 0.f;
     int tg = -1;
     if (on) {
@@ -825,10 +914,11 @@ struct Plan {
   int vc;                              // columns of a vocabulary piece = row pitch of its dz
   int oBN, oNB;                        // columns per tile of the gradient products, tiles at once
   int s_h, s_w;                        // k slices of dh and of dW
-  size_t o_hh, o_hl, o_wh, o_wl, o_part, o_zt, o_coef, o_tgt, o_g, o_g2, o_dh, o_dw, bytes;
+  size_t o_hh, o_hl, o_top, o_h2, o_wh, o_wl, o_part, o_zt, o_coef, o_tgt, o_g, o_g2, o_dh, o_dw, bytes;
 };
 
-constexpr size_t O_ERR = 256, O_AMAX = 512, HEAD = 1024;   // amax words: h, W, dz
+constexpr size_t O_ERR = 256, O_AMAX = 512, HEAD = 1024;   // amax words: W, dz, dW's h
+enum { AMAX_W, AMAX_G, AMAX_H };
 
 // 16-bit matrices TMA can address: rows 16 bytes apart, 16-byte base.
 bool tma_rows(const void* p, int64_t stride) { return stride % 8 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -914,6 +1004,8 @@ bool plan(const memlayer_loss_config& c, bool backward, Plan* out) {
   if (f32) {
     p.o_hl = take(T * p.ld * 2);
     p.o_wl = take(V * p.ld * 2);
+    p.o_top = take(T * 4);
+    if (backward) p.o_h2 = take(2 * T * p.ld * 2);   // hi, lo
   }
   if (!backward) {
     const int64_t few = f32 && T <= FEW ? up(V, FEW_V) / FEW_V * T * 8 : 0, part = (int64_t)p.slots * 2 * T * 8;
@@ -939,49 +1031,61 @@ bool plan(const memlayer_loss_config& c, bool backward, Plan* out) {
 }
 
 struct Operands {
-  const void *h[2], *w[2];
-  int64_t ldh, ldw;
+  const void *h[2], *w[2], *h2[2];     // h2: dW's
+  int64_t ldh, ldw, ldh2;
 };
-
-// Operands in 16-bit form: the caller's where TMA can address them, else the workspace's.
-cudaError_t prepare(const memlayer_loss_config& c, const memlayer_loss_args& a, const Plan& p, char* ws, Operands* o,
-                    cudaStream_t s) {
-  unsigned* amax = reinterpret_cast<unsigned*>(ws + O_AMAX);
-  const bool f32 = c.dtype == MEMLAYER_F32;
-  o->h[0] = a.h;
-  o->w[0] = a.weight;
-  o->ldh = a.h_stride;
-  o->ldw = a.weight_stride;
-  const bool ch = f32 || !tma_rows(a.h, a.h_stride), cw = f32 || !tma_rows(a.weight, a.weight_stride);
-  cudaError_t e;
-  if (f32) {
-    AmaxArgs A{};
-    A.m[0] = {(const float*)a.h, c.tokens, c.d_model, a.h_stride, amax, 0};
-    A.m[1] = {(const float*)a.weight, c.vocab_size, c.d_model, a.weight_stride, amax + 1, 0};
-    if ((e = launch_amax(A, s)) != cudaSuccess) return e;
-  }
-  if (!ch && !cw) return cudaSuccess;
-  PiecesArgs B{};
-  if (ch) {
-    o->h[0] = ws + p.o_hh;
-    o->h[1] = ws + p.o_hl;
-    o->ldh = p.ld;
-    B.m[0] = {a.h, c.tokens, c.d_model, a.h_stride, ws + p.o_hh, ws + p.o_hl, p.ld, amax, 0};
-  }
-  if (cw) {
-    o->w[0] = ws + p.o_wh;
-    o->w[1] = ws + p.o_wl;
-    o->ldw = p.ld;
-    B.m[1] = {a.weight, c.vocab_size, c.d_model, a.weight_stride, ws + p.o_wh, ws + p.o_wl, p.ld, amax + 1, 0};
-  }
-  return launch_pieces(B, c.dtype, s);
-}
 
 #define LS_TRY(x)                             \
   do {                                        \
     const cudaError_t e_ = (x);               \
     if (e_ != cudaSuccess) return e_;         \
   } while (0)
+
+// Operands in 16-bit form: the caller's where TMA can address them, else the
+// workspace's.  g: the gradient's arguments, whose tokens it looks through (null: none).
+cudaError_t prepare(const memlayer_loss_config& c, const memlayer_loss_args& a, const memlayer_loss_grads* g,
+                    const Plan& p, char* ws, Operands* o, cudaStream_t s) {
+  unsigned* amax = reinterpret_cast<unsigned*>(ws + O_AMAX);
+  unsigned* top = reinterpret_cast<unsigned*>(ws + p.o_top);
+  int* tgt = reinterpret_cast<int*>(ws + p.o_tgt);
+  const bool f32 = c.dtype == MEMLAYER_F32;
+  o->h[0] = o->h2[0] = a.h;
+  o->w[0] = a.weight;
+  o->ldh = o->ldh2 = a.h_stride;
+  o->ldw = a.weight_stride;
+  PiecesArgs B{};
+  if (f32 || !tma_rows(a.weight, a.weight_stride)) {
+    o->w[0] = ws + p.o_wh;
+    o->w[1] = ws + p.o_wl;
+    o->ldw = p.ld;
+    B.m[0] = {a.weight, c.vocab_size, c.d_model, a.weight_stride, ws + p.o_wh, ws + p.o_wl, p.ld, amax + AMAX_W, nullptr, 0};
+  }
+  if (f32 || !tma_rows(a.h, a.h_stride)) {
+    o->h[0] = o->h2[0] = ws + p.o_hh;
+    o->h[1] = ws + p.o_hl;
+    o->ldh = o->ldh2 = p.ld;
+    if (!f32) B.m[1] = {a.h, c.tokens, c.d_model, a.h_stride, ws + p.o_hh, nullptr, p.ld, nullptr, nullptr, 0};
+  }
+  if (f32)
+    LS_TRY(launch_tokens({{(const float*)a.weight, c.vocab_size, c.d_model, a.weight_stride, amax + AMAX_W, 0},
+                          (const float*)a.h, c.tokens, a.h_stride, p.ld, c.d_model, 0, (__half*)(ws + p.o_hh),
+                          (__half*)(ws + p.o_hl), top}, s));
+  if (g) {
+    const int64_t b = (c.tokens + 255) / 256;
+    count_launch();
+    LS_TRY(launch_dependent(loss_rows_kernel, dim3((unsigned)(b < 592 ? b : 592)), 256, 0, s, a.targets, g->dloss,
+                            g->dlse, c.tokens, c.vocab_size, c.ignore_index, (const unsigned*)(f32 ? top : nullptr),
+                            reinterpret_cast<float2*>(ws + p.o_coef), tgt, amax + AMAX_G, amax + AMAX_H,
+                            reinterpret_cast<int*>(ws + O_ERR)));
+    if (f32) {
+      char *hi = ws + p.o_h2, *lo = hi + c.tokens * p.ld * 2;
+      o->h2[0] = hi;
+      o->h2[1] = lo;
+      B.m[2] = {a.h, c.tokens, c.d_model, a.h_stride, hi, lo, p.ld, amax + AMAX_H, tgt, 0};
+    }
+  }
+  return launch_pieces(B, c.dtype, s);
+}
 
 template <class EPI, int PA, int PB>
 cudaError_t launch(int cg, const Maps& m, const Sched& S, const typename EPI::Args& ea, int* err, cudaStream_t s) {
@@ -1019,7 +1123,7 @@ cudaError_t launch_loss_forward(const memlayer_loss_config& c, const memlayer_lo
   LS_TRY(cudaMemsetAsync(ws + O_ERR, 0, HEAD - O_ERR, s));
   if (c.tokens == 0) return cudaSuccess;
   Operands o{};
-  LS_TRY(prepare(c, a, p, ws, &o, s));
+  LS_TRY(prepare(c, a, nullptr, p, ws, &o, s));
   const int bf16 = c.dtype == MEMLAYER_BF16;
   Maps m{};
   for (int i = 0; i < p.P; ++i) {
@@ -1033,12 +1137,12 @@ cudaError_t launch_loss_forward(const memlayer_loss_config& c, const memlayer_lo
   S.clusters = sms < S.prod[0].total() ? sms : S.prod[0].total();
   S.BN = p.BN;
   S.bf16 = bf16;
-  const unsigned* amax = p.P == 2 ? reinterpret_cast<unsigned*>(ws + O_AMAX) : nullptr;
+  const bool f32 = c.dtype == MEMLAYER_F32;
   StatsArgs ea{};
   ea.T = c.tokens;
   ea.V = c.vocab_size;
-  ea.amax_h = amax;
-  ea.amax_w = amax ? amax + 1 : nullptr;
+  ea.top_h = f32 ? reinterpret_cast<unsigned*>(ws + p.o_top) : nullptr;
+  ea.amax_w = f32 ? reinterpret_cast<unsigned*>(ws + O_AMAX) + AMAX_W : nullptr;
   ea.targets = a.targets;
   ea.part = reinterpret_cast<float2*>(ws + p.o_part);
   ea.zt = reinterpret_cast<float*>(ws + p.o_zt);
@@ -1074,19 +1178,14 @@ cudaError_t launch_loss_backward(const memlayer_loss_config& c, const memlayer_l
   const size_t esize = c.dtype == MEMLAYER_F32 ? 4 : 2;
   if (T == 0) return cudaMemsetAsync(g.dweight, 0, (size_t)V * d * esize, s);
   Operands o{};
-  LS_TRY(prepare(c, a, p, ws, &o, s));
+  LS_TRY(prepare(c, a, &g, p, ws, &o, s));
   unsigned* words = reinterpret_cast<unsigned*>(ws + O_AMAX);
   const bool f32 = c.dtype == MEMLAYER_F32;
   const int bf16 = c.dtype == MEMLAYER_BF16;
-  const unsigned *ah = f32 ? words : nullptr, *aw = f32 ? words + 1 : nullptr, *ag = bf16 ? nullptr : words + 2;
-  float2* coef = reinterpret_cast<float2*>(ws + p.o_coef);
-  int* tgt = reinterpret_cast<int*>(ws + p.o_tgt);
-  {
-    const int64_t b = (T + 255) / 256;
-    count_launch();
-    LS_TRY(launch_dependent(loss_rows_kernel, dim3((unsigned)(b < 592 ? b : 592)), 256, 0, s, a.targets, g.dloss,
-                            g.dlse, T, c.vocab_size, c.ignore_index, coef, tgt, words + 2, err));
-  }
+  const unsigned *top = f32 ? reinterpret_cast<unsigned*>(ws + p.o_top) : nullptr, *aw = f32 ? words + AMAX_W : nullptr,
+                 *ah = f32 ? words + AMAX_H : nullptr, *ag = bf16 ? nullptr : words + AMAX_G;
+  const float2* coef = reinterpret_cast<float2*>(ws + p.o_coef);
+  const int* tgt = reinterpret_cast<int*>(ws + p.o_tgt);
   uint16_t *gh = reinterpret_cast<uint16_t*>(ws + p.o_g), *gl = reinterpret_cast<uint16_t*>(ws + p.o_g2);
   float* acc_h = reinterpret_cast<float*>(ws + p.o_dh);
   const int sms = g16::device_sms() / p.cg;
@@ -1109,7 +1208,7 @@ cudaError_t launch_loss_backward(const memlayer_loss_config& c, const memlayer_l
     S.BN = p.BN;
     S.bf16 = bf16;
     g16::distribute(&S, sms, 0);
-    GradArgs ga{T, v0, vc, ah, aw, ag, g.lse, coef, tgt, {}};
+    GradArgs ga{T, v0, vc, top, aw, ag, g.lse, coef, tgt, {}};
     LS_TRY(g16::make_store(&ga.out[0], gh, T, p.vc, p.vc, f32 ? MEMLAYER_F16 : c.dtype));
     if (p.PZ == 2) LS_TRY(g16::make_store(&ga.out[1], gl, T, p.vc, p.vc, f32 ? MEMLAYER_F16 : c.dtype));
     S.seg = LOGIT_SEG;
@@ -1135,7 +1234,7 @@ cudaError_t launch_loss_backward(const memlayer_loss_config& c, const memlayer_l
       LS_TRY(g16::make_operand(&m2.a[qh][q], gz[q], T, vc, p.vc, false, 128, bf16));
     }
     for (int q = 0; q < p.P; ++q) {
-      LS_TRY(g16::make_operand(&m2.b[qw][q], o.h[q], d, T, o.ldh, true, 0, bf16));
+      LS_TRY(g16::make_operand(&m2.b[qw][q], o.h2[q], d, T, o.ldh2, true, 0, bf16));
       LS_TRY(g16::make_operand(&m2.b[qh][q], (const char*)o.w[q] + woff, d, vc, o.ldw, true, 0, bf16));
     }
     const int sw = S2.prod[qw].splits, sh = S2.prod[qh].splits;

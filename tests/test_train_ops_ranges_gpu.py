@@ -139,3 +139,42 @@ def test_loss_of_large_logits(T, d, V, size, t):
     assert not loss[hit].any()
     if T > 24:                                    # the gradient finds the forward's logits again: p is 1, dz 0
         assert not dh[hit].any()
+
+
+# ---- loss: tokens of very different magnitudes -------------------------------------------
+# float32 states run as two 16-bit pieces: each token's have to keep their digits whatever the others hold
+@pytest.mark.parametrize("huge", [1e6, 1e10, 1e30])
+@pytest.mark.parametrize("T,d,V", [(40, 24, 300), (200, 64, 700), (300, 1100, 400), (600, 130, 1001), (530, 256, 6000)])
+def test_loss_of_tokens_beside_a_huge_one(T, d, V, huge):
+    h, w, y, dl = loss_case(T, d, V, F32, seed=T + d)
+    y[3], y[T - 1] = -100, -100
+    h[3] *= huge                                  # padding with something in it
+    h[T - 1] = huge
+    loss, lse, dh, dw = run_loss(h, w, y, dl, check=True)
+    keep = torch.tensor([i for i in range(T) if i not in (3, T - 1)], device="cuda")
+    ref = LossRef(h[keep], w, y[keep], dl[keep])
+    ref.check(loss[keep], lse[keep], dh[keep], dw)         # ignored tokens add nothing to dW
+    assert not loss[[3, T - 1]].any() and not dh[[3, T - 1]].any()
+    # live ones: the others' loss, lse and dh are theirs; dW's sums keep their digits beside its largest term
+    y[3] = 5
+    loss, lse, dh, dw = run_loss(h, w, y, dl, check=True)
+    ref.check(loss[keep], lse[keep], dh[keep], ref.dw)
+    LossRef(h[3:4], w, y[3:4], dl[3:4]).check(loss[3:4], lse[3:4], dh[3:4], LossRef(h[3:4], w, y[3:4], dl[3:4]).dw)
+    live = torch.cat([keep, torch.tensor([3], device="cuda")])
+    all_ = LossRef(h[live], w, y[live], dl[live])
+    within(dw, all_.dw, all_.dw_tol, "dw")
+
+
+def test_loss_of_tokens_beside_tiny_ones():
+    h, w, y, dl = loss_case(150, 48, 500, F32, seed=8, gap=4)
+    scale = 10.0 ** (torch.arange(150, device="cuda") % 30 - 25).double()
+    h = (h.double() * scale[:, None]).float()
+    loss, lse, dh, dw = run_loss(h, w, y, dl, check=True)
+    for e in range(30):
+        at = torch.arange(e, 150, 30, device="cuda")
+        ref = LossRef(h[at], w, y[at], dl[at])
+        within(lse[at], ref.lse, ref.lse_tol, "lse")
+        within(loss[at], ref.loss, ref.loss_tol, "loss")
+        within(dh[at], ref.dh, ref.dh_tol, "dh")
+    ref = LossRef(h, w, y, dl)
+    within(dw, ref.dw, ref.dw_tol, "dw")
