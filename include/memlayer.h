@@ -702,9 +702,10 @@ int32_t memlayer_cross_entropy(const memlayer_loss_config* cfg, const memlayer_l
                                size_t workspace_bytes, void* stream);
 
 /* dh and dweight of sum(dloss * loss) + sum(dlse * lse); args as in the
- * forward (loss and lse there are not used).  The sums over tokens of a
- * float32 dweight keep 22 bits relative to the largest entry of h among the
- * tokens that have a gradient.  h must be finite at ignored
+ * forward (loss and lse there are not used).  A token's dh keeps its
+ * digits whatever the other tokens weigh; dweight sums over tokens, and there
+ * float32 and float16 calls hold each term to 2^-39 of the largest
+ * (|dloss| + |dlse|) |h| of a token, or better.  h must be finite at ignored
  * tokens too: their zero gradient multiplies it in dweight. */
 int32_t memlayer_cross_entropy_backward(const memlayer_loss_config* cfg, const memlayer_loss_args* args,
                                         const memlayer_loss_grads* grads, void* workspace, size_t workspace_bytes,

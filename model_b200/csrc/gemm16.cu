@@ -16,8 +16,8 @@ namespace {
 
 constexpr int NTH = PIECE_THREADS;
 
-// 8 columns a thread: hi / lo pieces of x s (float32 source) or a plain copy
-// (16-bit source), zeros in the padding columns.
+// 8 columns a thread: hi / lo pieces of x s (float32 source) or a copy
+// (16-bit source; scaled: f16), zeros in the padding columns.
 template <typename E>
 __global__ void __launch_bounds__(NTH) pieces_kernel(PiecesArgs A) {
   allow_next();
@@ -28,35 +28,37 @@ __global__ void __launch_bounds__(NTH) pieces_kernel(PiecesArgs A) {
   const int c8 = (int)(M.ld >> 3);
   const int64_t n = M.rows * c8;
   const E* src = reinterpret_cast<const E*>(M.x);
-  const float sc = sizeof(E) == 4 ? g16::scale_of(M.amax) : 1.f;
-  const bool vec = sizeof(E) == 4 && M.pitch % 4 == 0 && (reinterpret_cast<uintptr_t>(M.x) & 15) == 0;
+  const int e0 = M.peak ? piece_exp(*M.peak) : sizeof(E) == 4 && M.amax ? g16::scale_exp(*M.amax) : 0;
+  constexpr int V = 16 / sizeof(E);
+  struct alignas(16) Vec { E e[V]; };
+  const bool vec = M.pitch % V == 0 && (reinterpret_cast<uintptr_t>(M.x) & 15) == 0;
   for (int64_t e = (int64_t)b * NTH + threadIdx.x; e < n; e += (int64_t)M.blocks * NTH) {
     const int64_t r = e / c8;
     const int c = (int)(e - r * c8) * 8;
     const E* p = src + r * M.pitch + c;
-    const bool skip = M.row_tgt && M.row_tgt[r] == PIECE_SKIP;
+    alignas(16) E v[8];
+    if (M.row_tgt && M.row_tgt[r] == PIECE_SKIP) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = E(0);
+    } else if (vec && c + 8 <= M.cols) {
+#pragma unroll
+      for (int j = 0; j < 8; j += V) *reinterpret_cast<Vec*>(v + j) = *reinterpret_cast<const Vec*>(p + j);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = c + j < M.cols ? p[j] : E(0);
+    }
+    const g16::Unscale sc(M.row_exp ? e0 - M.row_exp[r] : e0);
     if constexpr (sizeof(E) == 4) {
-      float v[8];
-      if (skip) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = 0.f;
-      } else if (vec && c + 8 <= M.cols) {
-        const float4 a = *reinterpret_cast<const float4*>(p), q = *reinterpret_cast<const float4*>(p + 4);
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-        v[4] = q.x; v[5] = q.y; v[6] = q.z; v[7] = q.w;
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = c + j < M.cols ? p[j] : 0.f;
-      }
       __half2 h[4], l[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) g16::split2(v[2 * j] * sc, v[2 * j + 1] * sc, h[j], l[j]);
+      for (int j = 0; j < 4; ++j) g16::split2(sc(v[2 * j]), sc(v[2 * j + 1]), h[j], l[j]);
       *reinterpret_cast<uint4*>(reinterpret_cast<__half*>(M.hi) + r * M.ld + c) = *reinterpret_cast<uint4*>(h);
       *reinterpret_cast<uint4*>(reinterpret_cast<__half*>(M.lo) + r * M.ld + c) = *reinterpret_cast<uint4*>(l);
     } else {
-      alignas(16) E v[8];
+      if (M.row_exp) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = c + j < M.cols ? p[j] : E(0);
+        for (int j = 0; j < 8; ++j) v[j] = __half_as_ushort(__float2half_rn(sc(__half2float(__ushort_as_half(v[j])))));
+      }
       *reinterpret_cast<uint4*>(reinterpret_cast<E*>(M.hi) + r * M.ld + c) = *reinterpret_cast<uint4*>(v);
     }
   }

@@ -18,9 +18,8 @@
 //
 // float32 operands run as two f16 pieces each (22 bits, see gemm16.cuh; h with
 // a scale a token), dz too; 16-bit operands as they are, dz rounded once to their type (its
-// relative error, 2^-9 or 2^-12, averages out over the sums it enters).  f16
-// dz carries a power-of-two scale from the largest |dloss|.  Statistics,
-// exponentials and sums are float32.
+// relative error, 2^-9 or 2^-12, averages out over the sums it enters).
+// Statistics, exponentials and sums are float32.
 #include "loss.cuh"
 
 #include <float.h>
@@ -49,6 +48,15 @@ constexpr int SEG = 3;
 // loss is up to 0.6e-6 off, without segments 1.3e-6 at a k of 1024.
 constexpr int LOGIT_SEG = 8;
 
+template <typename E> __device__ __forceinline__ float to_f32(E x);
+template <> __device__ __forceinline__ float to_f32(float x) { return x; }
+template <> __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+template <> __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename E> __device__ __forceinline__ E from_f32(float x);
+template <> __device__ __forceinline__ float from_f32(float x) { return x; }
+template <> __device__ __forceinline__ __half from_f32(float x) { return __float2half_rn(x); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32(float x) { return __float2bfloat16_rn(x); }
+
 __device__ __forceinline__ int exp_of(const unsigned* amax) { return amax ? g16::scale_exp(*amax) : 0; }
 
 // Factor that turns an accumulator of a token's logits back: a normal float
@@ -58,24 +66,32 @@ __device__ __forceinline__ float logit_unscale(const unsigned* top_h, int64_t ro
   return g16::pow2(max(-100, min(126, -(on && top_h ? g16::scale_exp(top_h[row]) : 0) - exp_of(amax_w))));
 }
 
-// ---- float32 tokens as pieces ------------------------------------------------------
-// Each token gets a scale of its own, from its largest entry: with one for all
-// of them a single huge one -- padding, too, where anything may stand -- takes
-// the others' bits (a row of 1e10 among ones of 1 put their lse 0.02 off).
-// A logit belongs to one token, so the epilogues take the scale out by row.
-// The gradient's dW sums over tokens; for it h is split once more, by the
-// largest entry of the tokens that have a gradient.  The first blocks look for
-// the weight's largest magnitude meanwhile.
+// ---- a scale for each token ----------------------------------------------------------
+// f16 operands carry powers of two, and each token has its own.  With one for
+// all of them a single huge token -- padding, too, where anything may stand --
+// takes the others' bits (a row of 1e10 among ones of 1 put their lse 0.02
+// off), and a token whose loss weighs 1e-9 of another's loses its dz.  h gets
+// its scale from the token's largest entry (float32 only), dz from the larger
+// of the token's two factors.  A logit and an entry of dh belong to one token,
+// so the epilogues take the scales out by row.  dW sums over tokens, and what
+// each of them adds has to carry the same power of two: there h is converted
+// once more, a token's rows times the inverse of its dz scale, all of them
+// such that the largest h / scale comes to 2^14 (a token's share of dW is that
+// size times p); tokens without a gradient are left out.  The first blocks
+// look for the weight's largest magnitude meanwhile.
 struct TokenArgs {
   AmaxMat w;
-  const float* h;
+  const void* h;
   int64_t T, ldh, ld;
   int d, tpr;                          // tpr: threads a token, 32 or all
-  __half *hi, *lo;                     // [T][ld]
+  __half *hi, *lo;                     // [T][ld] (float32)
   unsigned* top;                       // [T] bits of the largest finite magnitude
 };
 
+template <typename E>
 __global__ void __launch_bounds__(PIECE_THREADS) loss_tokens_kernel(TokenArgs A) {
+  constexpr int V = 16 / sizeof(E);
+  struct alignas(16) Vec { E e[V]; };
   __shared__ unsigned red[PIECE_THREADS / 32];
   allow_next();
   wait_previous();
@@ -84,21 +100,22 @@ __global__ void __launch_bounds__(PIECE_THREADS) loss_tokens_kernel(TokenArgs A)
     return;
   }
   const int t = threadIdx.x & (A.tpr - 1), groups = PIECE_THREADS / A.tpr, d = A.d;
-  const bool vec = A.ldh % 4 == 0 && d % 4 == 0 && (reinterpret_cast<uintptr_t>(A.h) & 15) == 0;
+  const bool vec = A.ldh % V == 0 && d % V == 0 && (reinterpret_cast<uintptr_t>(A.h) & 15) == 0;
   const int64_t step = (int64_t)(gridDim.x - A.w.blocks) * groups;
   for (int64_t base = (int64_t)(blockIdx.x - A.w.blocks) * groups; base < A.T; base += step) {
     const int64_t row = base + threadIdx.x / A.tpr;
     const bool on = row < A.T;
-    const float* x = A.h + (on ? row : 0) * A.ldh;
+    const E* x = reinterpret_cast<const E*>(A.h) + (on ? row : 0) * A.ldh;
     unsigned mx = 0;
     if (vec) {
 #pragma unroll 2
-      for (int c = t * 4; c < d; c += A.tpr * 4) {
-        const float4 v = *reinterpret_cast<const float4*>(x + c);
-        mx = max(max(mx, max(finite_bits(v.x), finite_bits(v.y))), max(finite_bits(v.z), finite_bits(v.w)));
+      for (int c = t * V; c < d; c += A.tpr * V) {
+        const Vec v = *reinterpret_cast<const Vec*>(x + c);
+#pragma unroll
+        for (int j = 0; j < V; ++j) mx = max(mx, finite_bits(to_f32(v.e[j])));
       }
     } else {
-      for (int c = t; c < d; c += A.tpr) mx = max(mx, finite_bits(x[c]));
+      for (int c = t; c < d; c += A.tpr) mx = max(mx, finite_bits(to_f32(x[c])));
     }
     mx = __reduce_max_sync(FULL, mx);
     if (A.tpr > 32) {
@@ -109,16 +126,17 @@ __global__ void __launch_bounds__(PIECE_THREADS) loss_tokens_kernel(TokenArgs A)
     }
     if (!on) continue;
     if (t == 0) A.top[row] = mx;
+    if constexpr (sizeof(E) == 2) continue;
     const float sc = g16::pow2(g16::scale_exp(mx));
     for (int c = t * 8; c < (int)A.ld; c += A.tpr * 8) {
       float v[8];
       if (vec && c + 8 <= d) {
-        const float4 a = *reinterpret_cast<const float4*>(x + c), b = *reinterpret_cast<const float4*>(x + c + 4);
+        const float4 a = *reinterpret_cast<const float4*>(x + c), b = *reinterpret_cast<const float4*>(x + c + V);
         v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
         v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
       } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = c + j < d ? x[c + j] : 0.f;
+        for (int j = 0; j < 8; ++j) v[j] = c + j < d ? to_f32(x[c + j]) : 0.f;
       }
       __half2 h[4], l[4];
 #pragma unroll
@@ -129,13 +147,14 @@ __global__ void __launch_bounds__(PIECE_THREADS) loss_tokens_kernel(TokenArgs A)
   }
 }
 
+template <typename E>
 cudaError_t launch_tokens(TokenArgs A, cudaStream_t s) {
-  A.w.blocks = piece_blocks(A.w.rows * A.w.cols, 16);
+  A.w.blocks = A.w.rows ? piece_blocks(A.w.rows * A.w.cols, 16) : 0;
   A.tpr = A.d <= 2048 ? 32 : PIECE_THREADS;
   const int64_t need = (A.T * A.tpr + PIECE_THREADS - 1) / PIECE_THREADS, cap = 8 * g16::device_sms();
   count_launch();
-  return launch_dependent(loss_tokens_kernel, dim3((unsigned)(A.w.blocks + (need < cap ? need : cap))), PIECE_THREADS, 0, s,
-                          A);
+  return launch_dependent(loss_tokens_kernel<E>, dim3((unsigned)(A.w.blocks + (need < cap ? need : cap))), PIECE_THREADS,
+                          0, s, A);
 }
 
 __device__ __forceinline__ unsigned long long pair(float a, float b) {
@@ -430,19 +449,19 @@ bool few_tokens(const memlayer_loss_config& c, const memlayer_loss_args& a) {
 
 // ---- backward ---------------------------------------------------------------------
 // Per token: the factor of p, the factor of the one-hot target and the target
-// (-1: none; PIECE_SKIP: no gradient at all); the largest of the factors'
-// magnitudes for the scale of dz, the largest entry of the tokens that have a
-// gradient for that of dW's h.
+// (-1: none; PIECE_SKIP: no gradient at all); where dz carries scales (top_h)
+// the token's, |p q - [target] g| <= 2 max(|q|, |g|) < 2^15, and the largest
+// exponent of h / scale over the tokens that have a gradient.
 __global__ void __launch_bounds__(256) loss_rows_kernel(const int* __restrict__ targets,
                                                         const float* __restrict__ dloss,
                                                         const float* __restrict__ dlse, int64_t T, int V, int ignore,
                                                         const unsigned* __restrict__ top_h,
                                                         float2* __restrict__ coef, int* __restrict__ tgt,
-                                                        unsigned* __restrict__ amax, unsigned* __restrict__ amax_h,
+                                                        int* __restrict__ exp_g, unsigned* __restrict__ peak,
                                                         int* __restrict__ err) {
   allow_next();
   wait_previous();
-  unsigned mx = 0, mh = 0;
+  unsigned mx = 0;
   for (int64_t t = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; t < T; t += (int64_t)gridDim.x * blockDim.x) {
     const int v = targets[t];
     const bool in = v >= 0 && v < V && v != ignore;
@@ -451,24 +470,21 @@ __global__ void __launch_bounds__(256) loss_rows_kernel(const int* __restrict__ 
     coef[t] = make_float2(q, g);
     const bool none = g == 0.f && q == 0.f;
     tgt[t] = none ? PIECE_SKIP : in ? v : -1;
-    mx = max(mx, max(finite_bits(g), finite_bits(q)));
-    if (top_h && !none) mh = max(mh, top_h[t]);
+    if (top_h) {
+      const int f = g16::scale_exp(max(finite_bits(g), finite_bits(q))) - 1;
+      exp_g[t] = f;
+      if (!none && top_h[t]) mx = max(mx, piece_peak((int)(top_h[t] >> 23) - 127 - f));
+    }
   }
   mx = __reduce_max_sync(FULL, mx);
-  mh = __reduce_max_sync(FULL, mh);
-  if ((threadIdx.x & 31) == 0) {
-    if (mx) atomicMax(amax, mx);
-    if (mh) atomicMax(amax_h, mh);
-  }
+  if ((threadIdx.x & 31) == 0 && mx) atomicMax(peak, mx);
 }
-
-// Scale of dz: |p q - [target] g| <= 2 max(|q|, |g|) < 2^15.
-__device__ __forceinline__ int dz_exp(const unsigned* amax) { return amax ? g16::scale_exp(*amax) - 1 : 0; }
 
 struct GradArgs {
   int64_t T;
   int v0, vc;                          // the piece: columns [v0, v0 + vc)
-  const unsigned *top_h, *amax_w, *amax_g;
+  const unsigned *top_h, *amax_w;
+  const int* exp_g;                    // the tokens' scales of dz (null: none)
   const float* lse;
   const float2* coef;
   const int* tgt;
@@ -481,13 +497,11 @@ struct EpiGrad {
   static constexpr bool kSum = SUM, kStore = true;
   float sum[128];
   using Args = GradArgs;
-  float sg;
   uint32_t buf;
   StagingTurn turn;
   __device__ __forceinline__ void begin(const Args& A, const Sched&, int, uint8_t* staging) {
     buf = tc::smem_u32(staging);
     turn = StagingTurn{};
-    sg = g16::pow2(dz_exp(A.amax_g));
   }
   template <class Get>
   __device__ __forceinline__ void blocks(const Args& A, const Sched& S, const Tile& t, int64_t row, int half,
@@ -501,6 +515,7 @@ struct EpiGrad {
     int tg = -1;
     if (on) {
       const float2 c = A.coef[row];
+      const float sg = A.exp_g ? g16::pow2(A.exp_g[row]) : 1.f;
       l = A.lse[row];
       q = c.x * sg;
       g = c.y * sg;
@@ -598,15 +613,6 @@ struct FewGradArgs {
   float* part;                         // [block][group][T][d]
   int* err;
 };
-
-template <typename E> __device__ __forceinline__ float to_f32(E x);
-template <> __device__ __forceinline__ float to_f32(float x) { return x; }
-template <> __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
-template <> __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <typename E> __device__ __forceinline__ E from_f32(float x);
-template <> __device__ __forceinline__ float from_f32(float x) { return x; }
-template <> __device__ __forceinline__ __half from_f32(float x) { return __float2half_rn(x); }
-template <> __device__ __forceinline__ __nv_bfloat16 from_f32(float x) { return __float2bfloat16_rn(x); }
 
 template <typename E, int TM>
 __global__ void __launch_bounds__(FEWB_T, TM <= 4 ? 2 : 1) loss_few_backward_kernel(const FewGradArgs A) {
@@ -786,7 +792,9 @@ struct OutOne {
   int type;                            // memlayer_dtype of out
   int add;                             // float32 only: added to what is there
   int tma;                             // rows are 16 bytes apart
-  const unsigned *amax_a, *amax_b;     // scale maxima of the operands (null: unscaled); amax_a is dz's
+  // scales of the operands (null: none): dz's by row (dh), dW's common one, the weight's
+  const int* exp_g;
+  const unsigned *peak, *amax_w;
 };
 struct OutArgs { OutOne o[2]; };
 
@@ -826,7 +834,7 @@ struct EpiOut {
   __device__ __forceinline__ void blocks(const Args& A, const Sched& S, const Tile& t, int64_t row, int half,
                                          Get get) {
     const OutOne& O = A.o[t.q];
-    const g16::Unscale un(-dz_exp(O.amax_a) - exp_of(O.amax_b));
+    const g16::Unscale un(-(O.exp_g && row < O.M ? O.exp_g[row] : 0) - (O.peak ? piece_exp(*O.peak) : 0) - exp_of(O.amax_w));
     const int64_t row0 = row - (threadIdx.x & 31);
     const int hw = S.BN >> 1;
     const int col0 = t.nt * S.BN + half * hw;
@@ -914,11 +922,11 @@ struct Plan {
   int vc;                              // columns of a vocabulary piece = row pitch of its dz
   int oBN, oNB;                        // columns per tile of the gradient products, tiles at once
   int s_h, s_w;                        // k slices of dh and of dW
-  size_t o_hh, o_hl, o_top, o_h2, o_wh, o_wl, o_part, o_zt, o_coef, o_tgt, o_g, o_g2, o_dh, o_dw, bytes;
+  size_t o_hh, o_hl, o_top, o_h2, o_wh, o_wl, o_part, o_zt, o_coef, o_tgt, o_exp, o_g, o_g2, o_dh, o_dw, bytes;
 };
 
-constexpr size_t O_ERR = 256, O_AMAX = 512, HEAD = 1024;   // amax words: W, dz, dW's h
-enum { AMAX_W, AMAX_G, AMAX_H };
+constexpr size_t O_ERR = 256, O_AMAX = 512, HEAD = 1024;
+enum { AMAX_W, PEAK };                 // words from O_AMAX on
 
 // 16-bit matrices TMA can address: rows 16 bytes apart, 16-byte base.
 bool tma_rows(const void* p, int64_t stride) { return stride % 8 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -1004,8 +1012,7 @@ bool plan(const memlayer_loss_config& c, bool backward, Plan* out) {
   if (f32) {
     p.o_hl = take(T * p.ld * 2);
     p.o_wl = take(V * p.ld * 2);
-    p.o_top = take(T * 4);
-    if (backward) p.o_h2 = take(2 * T * p.ld * 2);   // hi, lo
+    if (!backward) p.o_top = take(T * 4);
   }
   if (!backward) {
     const int64_t few = f32 && T <= FEW ? up(V, FEW_V) / FEW_V * T * 8 : 0, part = (int64_t)p.slots * 2 * T * 8;
@@ -1014,6 +1021,9 @@ bool plan(const memlayer_loss_config& c, bool backward, Plan* out) {
   } else {
     p.o_coef = take(T * 8);
     p.o_tgt = take(T * 4);
+    p.o_top = take(T * 4);
+    p.o_exp = take(T * 4);
+    p.o_h2 = take(p.P * T * p.ld * 2);   // hi, lo
     p.oBN = d > 128 ? 256 : 128;
     // 16-bit products with an even number of column tiles take two at once:
     // 8192 x 1024 x 32768 bf16 791 us instead of 956, 1999 x 512 x 30011 f16
@@ -1047,7 +1057,6 @@ cudaError_t prepare(const memlayer_loss_config& c, const memlayer_loss_args& a, 
                     const Plan& p, char* ws, Operands* o, cudaStream_t s) {
   unsigned* amax = reinterpret_cast<unsigned*>(ws + O_AMAX);
   unsigned* top = reinterpret_cast<unsigned*>(ws + p.o_top);
-  int* tgt = reinterpret_cast<int*>(ws + p.o_tgt);
   const bool f32 = c.dtype == MEMLAYER_F32;
   o->h[0] = o->h2[0] = a.h;
   o->w[0] = a.weight;
@@ -1058,30 +1067,36 @@ cudaError_t prepare(const memlayer_loss_config& c, const memlayer_loss_args& a, 
     o->w[0] = ws + p.o_wh;
     o->w[1] = ws + p.o_wl;
     o->ldw = p.ld;
-    B.m[0] = {a.weight, c.vocab_size, c.d_model, a.weight_stride, ws + p.o_wh, ws + p.o_wl, p.ld, amax + AMAX_W, nullptr, 0};
+    B.m[0] = {a.weight, c.vocab_size, c.d_model, a.weight_stride, ws + p.o_wh, ws + p.o_wl, p.ld, amax + AMAX_W};
   }
   if (f32 || !tma_rows(a.h, a.h_stride)) {
     o->h[0] = o->h2[0] = ws + p.o_hh;
     o->h[1] = ws + p.o_hl;
     o->ldh = o->ldh2 = p.ld;
-    if (!f32) B.m[1] = {a.h, c.tokens, c.d_model, a.h_stride, ws + p.o_hh, nullptr, p.ld, nullptr, nullptr, 0};
+    if (!f32) B.m[1] = {a.h, c.tokens, c.d_model, a.h_stride, ws + p.o_hh, nullptr, p.ld};
   }
-  if (f32)
-    LS_TRY(launch_tokens({{(const float*)a.weight, c.vocab_size, c.d_model, a.weight_stride, amax + AMAX_W, 0},
-                          (const float*)a.h, c.tokens, a.h_stride, p.ld, c.d_model, 0, (__half*)(ws + p.o_hh),
-                          (__half*)(ws + p.o_hl), top}, s));
+  const bool scaled = c.dtype != MEMLAYER_BF16;        // dz carries scales
+  TokenArgs ta{{}, a.h, c.tokens, a.h_stride, p.ld, c.d_model, 0, (__half*)(ws + p.o_hh), (__half*)(ws + p.o_hl), top};
+  if (f32) {
+    ta.w = {(const float*)a.weight, c.vocab_size, c.d_model, a.weight_stride, amax + AMAX_W, 0};
+    LS_TRY(launch_tokens<float>(ta, s));
+  } else if (g && scaled) {
+    LS_TRY(launch_tokens<__half>(ta, s));
+  }
   if (g) {
+    int *tgt = reinterpret_cast<int*>(ws + p.o_tgt), *exp_g = reinterpret_cast<int*>(ws + p.o_exp);
     const int64_t b = (c.tokens + 255) / 256;
     count_launch();
     LS_TRY(launch_dependent(loss_rows_kernel, dim3((unsigned)(b < 592 ? b : 592)), 256, 0, s, a.targets, g->dloss,
-                            g->dlse, c.tokens, c.vocab_size, c.ignore_index, (const unsigned*)(f32 ? top : nullptr),
-                            reinterpret_cast<float2*>(ws + p.o_coef), tgt, amax + AMAX_G, amax + AMAX_H,
+                            g->dlse, c.tokens, c.vocab_size, c.ignore_index, (const unsigned*)(scaled ? top : nullptr),
+                            reinterpret_cast<float2*>(ws + p.o_coef), tgt, exp_g, amax + PEAK,
                             reinterpret_cast<int*>(ws + O_ERR)));
-    if (f32) {
+    if (scaled) {
       char *hi = ws + p.o_h2, *lo = hi + c.tokens * p.ld * 2;
       o->h2[0] = hi;
       o->h2[1] = lo;
-      B.m[2] = {a.h, c.tokens, c.d_model, a.h_stride, hi, lo, p.ld, amax + AMAX_H, tgt, 0};
+      o->ldh2 = p.ld;
+      B.m[2] = {a.h, c.tokens, c.d_model, a.h_stride, hi, lo, p.ld, nullptr, tgt, exp_g, amax + PEAK};
     }
   }
   return launch_pieces(B, c.dtype, s);
@@ -1183,7 +1198,8 @@ cudaError_t launch_loss_backward(const memlayer_loss_config& c, const memlayer_l
   const bool f32 = c.dtype == MEMLAYER_F32;
   const int bf16 = c.dtype == MEMLAYER_BF16;
   const unsigned *top = f32 ? reinterpret_cast<unsigned*>(ws + p.o_top) : nullptr, *aw = f32 ? words + AMAX_W : nullptr,
-                 *ah = f32 ? words + AMAX_H : nullptr, *ag = bf16 ? nullptr : words + AMAX_G;
+                 *peak = bf16 ? nullptr : words + PEAK;
+  const int* exp_g = bf16 ? nullptr : reinterpret_cast<int*>(ws + p.o_exp);
   const float2* coef = reinterpret_cast<float2*>(ws + p.o_coef);
   const int* tgt = reinterpret_cast<int*>(ws + p.o_tgt);
   uint16_t *gh = reinterpret_cast<uint16_t*>(ws + p.o_g), *gl = reinterpret_cast<uint16_t*>(ws + p.o_g2);
@@ -1208,7 +1224,7 @@ cudaError_t launch_loss_backward(const memlayer_loss_config& c, const memlayer_l
     S.BN = p.BN;
     S.bf16 = bf16;
     g16::distribute(&S, sms, 0);
-    GradArgs ga{T, v0, vc, top, aw, ag, g.lse, coef, tgt, {}};
+    GradArgs ga{T, v0, vc, top, aw, exp_g, g.lse, coef, tgt, {}};
     LS_TRY(g16::make_store(&ga.out[0], gh, T, p.vc, p.vc, f32 ? MEMLAYER_F16 : c.dtype));
     if (p.PZ == 2) LS_TRY(g16::make_store(&ga.out[1], gl, T, p.vc, p.vc, f32 ? MEMLAYER_F16 : c.dtype));
     S.seg = LOGIT_SEG;
@@ -1240,7 +1256,7 @@ cudaError_t launch_loss_backward(const memlayer_loss_config& c, const memlayer_l
     const int sw = S2.prod[qw].splits, sh = S2.prod[qh].splits;
     char* dwp = (char*)g.dweight + (size_t)v0 * d * esize;
     OutArgs ea{};
-    auto out = [&](OutOne& O, int64_t M, void* q, int type, bool add, int slices, const unsigned* ub) {
+    auto out = [&](OutOne& O, int64_t M, void* q, int type, bool add, int slices, bool is_dh) {
       O.M = M;
       O.N = (int)d;
       O.ld = d;
@@ -1249,18 +1265,19 @@ cudaError_t launch_loss_backward(const memlayer_loss_config& c, const memlayer_l
       O.type = type;
       O.add = add;
       O.tma = al16(q) && (d * (type == MEMLAYER_F32 ? 4 : 2)) % 16 == 0;
-      O.amax_a = ag;
-      O.amax_b = ub;
+      O.exp_g = is_dh ? exp_g : nullptr;
+      O.peak = is_dh ? nullptr : peak;
+      O.amax_w = is_dh ? aw : nullptr;
       return O.tma ? g16::make_store(&O.map, q, M, d, d, type, slices, M * d) : cudaSuccess;
     };
     if (sw > 1)
-      LS_TRY(out(ea.o[qw], vc, ws + p.o_dw, MEMLAYER_F32, false, sw, ah));
+      LS_TRY(out(ea.o[qw], vc, ws + p.o_dw, MEMLAYER_F32, false, sw, false));
     else
-      LS_TRY(out(ea.o[qw], vc, dwp, c.dtype, false, 1, ah));
+      LS_TRY(out(ea.o[qw], vc, dwp, c.dtype, false, 1, false));
     if (direct_h)
-      LS_TRY(out(ea.o[qh], T, g.dh, c.dtype, i > 0, 1, aw));
+      LS_TRY(out(ea.o[qh], T, g.dh, c.dtype, i > 0, 1, true));
     else   // a shorter last piece may have fewer slices: the others keep what they hold
-      LS_TRY(out(ea.o[qh], T, acc_h, MEMLAYER_F32, i > 0, sh, aw));
+      LS_TRY(out(ea.o[qh], T, acc_h, MEMLAYER_F32, i > 0, sh, true));
     if (f32)
       LS_TRY((launch<EpiOut<true>, 2, 2>(p.cg, m2, S2, ea, err, s)));
     else

@@ -78,13 +78,17 @@ struct PiecesMat {
   int64_t rows, cols, pitch;
   void *hi, *lo;               // rows x ld (ld a multiple of 8); lo: float32 sources only
   int64_t ld;
-  // float32 sources: x times a power of two, from the matrix's largest
-  // magnitude, or (row_tgt) from the largest of the rows that count
-  const unsigned* amax;
-  const int* row_tgt;          // PIECE_SKIP: the row is left out (zeros)
+  const unsigned* amax;        // float32 sources: the largest magnitude, for a scale of the matrix; or
+  const int* row_tgt;          // by row: PIECE_SKIP leaves it out (zeros),
+  const int* row_exp;          // else it goes by piece_exp(*peak) - row_exp (float32 and f16; null: unscaled)
+  const unsigned* peak;
   int blocks;
 };
 constexpr int PIECE_SKIP = -2;
+// The largest exponent of a row less its row_exp, as a word for atomicMax (0:
+// no row), and the power of two that brings it to 2^14.
+__device__ __forceinline__ unsigned piece_peak(int e) { return (unsigned)(e + 1024); }
+__device__ __forceinline__ int piece_exp(unsigned peak) { return peak ? 14 - ((int)peak - 1024) : 0; }
 struct PiecesArgs { PiecesMat m[3]; };
 
 // Pieces (float32) or padded copies (16-bit) of up to three matrices.

@@ -178,3 +178,28 @@ def test_loss_of_tokens_beside_tiny_ones():
         within(dh[at], ref.dh, ref.dh_tol, "dh")
     ref = LossRef(h, w, y, dl)
     within(dw, ref.dw, ref.dw_tol, "dw")
+
+
+# loss weights over many orders of magnitude: every token's dh has its own digits
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("T,d,V", [(60, 40, 700), (128, 64, 5000), (200, 64, 700), (700, 128, 3001)])
+def test_loss_gradient_of_light_tokens(T, d, V, t):
+    h, w, y, _ = loss_case(T, d, V, t, seed=T + V)
+    # f16 results hold 2^-24 and more: its weights stay above that
+    kinds = [2.0 ** 9, 2.0 ** -1, 2.0 ** -9] if t == F16 else [1.0, 1e-4, 1e-9, 1e-15]
+    dl = torch.tensor(kinds, device="cuda")[torch.arange(T, device="cuda") % len(kinds)]
+    dl = dl * (0.5 + torch.rand(T, device="cuda", generator=gen(1)))
+    dlse = dl * torch.randn(T, device="cuda", generator=gen(2))
+    loss, lse, dh, dw = run_loss(h, w, y, dl, dlse, check=True)
+    for i in range(len(kinds)):
+        at = torch.arange(i, T, len(kinds), device="cuda")
+        ref = LossRef(h[at], w, y[at], dl[at], dlse[at])
+        # part of the tokens stands for all of them: where more than 128 are
+        # given, an entry of dz is rounded once to the type
+        mag = dl[at].double() + dlse[at].double().abs()
+        p = (h[at].double() @ w.double().T - ref.lse[:, None]).exp() * mag[:, None]
+        p.scatter_add_(1, y[at].long()[:, None], dl[at].double()[:, None])
+        extra = half_step(t) * (p @ w.double().abs()) if T > 128 and t != F32 else 0
+        within(dh[at], ref.dh, ref.dh_tol + extra, f"dh of weight {kinds[i]}")
+    ref = LossRef(h, w, y, dl, dlse)
+    ref.check(loss, lse, dh, dw)
