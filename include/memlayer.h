@@ -705,8 +705,8 @@ int32_t memlayer_cross_entropy(const memlayer_loss_config* cfg, const memlayer_l
  * forward (loss and lse there are not used).  A token's dh keeps its
  * digits whatever the other tokens weigh; dweight sums over tokens, and there
  * float32 and float16 calls hold each term to 2^-39 of the largest
- * (|dloss| + |dlse|) |h| of a token, or better.  h must be finite at ignored
- * tokens too: their zero gradient multiplies it in dweight. */
+ * (|dloss| + |dlse|) |h| of a token, or better.  A token without a gradient
+ * (ignored, say, and no dlse) adds nothing, whatever its h holds. */
 int32_t memlayer_cross_entropy_backward(const memlayer_loss_config* cfg, const memlayer_loss_args* args,
                                         const memlayer_loss_grads* grads, void* workspace, size_t workspace_bytes,
                                         void* stream);

@@ -77,8 +77,9 @@ __device__ __forceinline__ float logit_unscale(const unsigned* top_h, int64_t ro
 // each of them adds has to carry the same power of two: there h is converted
 // once more, a token's rows times the inverse of its dz scale, all of them
 // such that the largest h / scale comes to 2^14 (a token's share of dW is that
-// size times p); tokens without a gradient are left out.  The first blocks
-// look for the weight's largest magnitude meanwhile.
+// size times p).  That copy of h leaves out the tokens without a gradient, bf16
+// too: their rows may hold anything, and zeros times a NaN would be in all of
+// dW.  The first blocks look for the weight's largest magnitude meanwhile.
 struct TokenArgs {
   AmaxMat w;
   const void* h;
@@ -638,9 +639,10 @@ __global__ void __launch_bounds__(FEWB_T, TM <= 4 ? 2 : 1) loss_few_backward_ker
     l[t] = t < A.T ? A.lse[t] : 0.f;
     tg[t] = in ? v : -1;
   }
+  __syncthreads();
   for (int e = t; e < TM * d; e += FEWB_T) {
-    const int m = e / d;
-    hs[e] = m < A.T ? to_f32(h[m * A.ldh + (e - m * d)]) : 0.f;
+    const int m = e / d;               // a token without a gradient: nothing, whatever its row holds
+    hs[e] = m < A.T && !(q[m] == 0.f && g[m] == 0.f) ? to_f32(h[m * A.ldh + (e - m * d)]) : 0.f;
   }
   __syncthreads();
   const int groups = few_groups(d), width = groups > 1 ? (d + 31) / 32 * 32 : FEWB_T;
@@ -1041,8 +1043,8 @@ bool plan(const memlayer_loss_config& c, bool backward, Plan* out) {
 }
 
 struct Operands {
-  const void *h[2], *w[2], *h2[2];     // h2: dW's
-  int64_t ldh, ldw, ldh2;
+  const void *h[2], *w[2], *h2[2];     // h2: dW's, a row every p.ld
+  int64_t ldh, ldw;
 };
 
 #define LS_TRY(x)                             \
@@ -1058,9 +1060,9 @@ cudaError_t prepare(const memlayer_loss_config& c, const memlayer_loss_args& a, 
   unsigned* amax = reinterpret_cast<unsigned*>(ws + O_AMAX);
   unsigned* top = reinterpret_cast<unsigned*>(ws + p.o_top);
   const bool f32 = c.dtype == MEMLAYER_F32;
-  o->h[0] = o->h2[0] = a.h;
+  o->h[0] = a.h;
   o->w[0] = a.weight;
-  o->ldh = o->ldh2 = a.h_stride;
+  o->ldh = a.h_stride;
   o->ldw = a.weight_stride;
   PiecesArgs B{};
   if (f32 || !tma_rows(a.weight, a.weight_stride)) {
@@ -1070,9 +1072,9 @@ cudaError_t prepare(const memlayer_loss_config& c, const memlayer_loss_args& a, 
     B.m[0] = {a.weight, c.vocab_size, c.d_model, a.weight_stride, ws + p.o_wh, ws + p.o_wl, p.ld, amax + AMAX_W};
   }
   if (f32 || !tma_rows(a.h, a.h_stride)) {
-    o->h[0] = o->h2[0] = ws + p.o_hh;
+    o->h[0] = ws + p.o_hh;
     o->h[1] = ws + p.o_hl;
-    o->ldh = o->ldh2 = p.ld;
+    o->ldh = p.ld;
     if (!f32) B.m[1] = {a.h, c.tokens, c.d_model, a.h_stride, ws + p.o_hh, nullptr, p.ld};
   }
   const bool scaled = c.dtype != MEMLAYER_BF16;        // dz carries scales
@@ -1091,13 +1093,11 @@ cudaError_t prepare(const memlayer_loss_config& c, const memlayer_loss_args& a, 
                             g->dlse, c.tokens, c.vocab_size, c.ignore_index, (const unsigned*)(scaled ? top : nullptr),
                             reinterpret_cast<float2*>(ws + p.o_coef), tgt, exp_g, amax + PEAK,
                             reinterpret_cast<int*>(ws + O_ERR)));
-    if (scaled) {
-      char *hi = ws + p.o_h2, *lo = hi + c.tokens * p.ld * 2;
-      o->h2[0] = hi;
-      o->h2[1] = lo;
-      o->ldh2 = p.ld;
-      B.m[2] = {a.h, c.tokens, c.d_model, a.h_stride, hi, lo, p.ld, nullptr, tgt, exp_g, amax + PEAK};
-    }
+    char *hi = ws + p.o_h2, *lo = hi + c.tokens * p.ld * 2;
+    o->h2[0] = hi;
+    o->h2[1] = lo;
+    B.m[2] = {a.h, c.tokens, c.d_model, a.h_stride, hi, lo, p.ld, nullptr, tgt, scaled ? exp_g : nullptr,
+              scaled ? amax + PEAK : nullptr};
   }
   return launch_pieces(B, c.dtype, s);
 }
@@ -1250,7 +1250,7 @@ cudaError_t launch_loss_backward(const memlayer_loss_config& c, const memlayer_l
       LS_TRY(g16::make_operand(&m2.a[qh][q], gz[q], T, vc, p.vc, false, 128, bf16));
     }
     for (int q = 0; q < p.P; ++q) {
-      LS_TRY(g16::make_operand(&m2.b[qw][q], o.h2[q], d, T, o.ldh2, true, 0, bf16));
+      LS_TRY(g16::make_operand(&m2.b[qw][q], o.h2[q], d, T, p.ld, true, 0, bf16));
       LS_TRY(g16::make_operand(&m2.b[qh][q], (const char*)o.w[q] + woff, d, vc, o.ldw, true, 0, bf16));
     }
     const int sw = S2.prod[qw].splits, sh = S2.prod[qh].splits;

@@ -203,3 +203,27 @@ def test_loss_gradient_of_light_tokens(T, d, V, t):
         within(dh[at], ref.dh, ref.dh_tol + extra, f"dh of weight {kinds[i]}")
     ref = LossRef(h, w, y, dl, dlse)
     ref.check(loss, lse, dh, dw)
+
+
+# padding with anything in it: an ignored token's h reaches nothing but its own lse
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("fill", [float("nan"), float("inf"), -float("inf"), "largest"])
+@pytest.mark.parametrize("T,d,V", [(3, 40, 200), (9, 513, 300), (16, 1024, 129), (30, 64, 500), (100, 72, 257), (300, 100, 700), (280, 33, 400)])
+def test_loss_padding_may_hold_anything(T, d, V, fill, t):
+    h, w, y, dl = loss_case(T, d, V, t, seed=T + d)
+    pad = torch.arange(T, device="cuda") % 3 == 1
+    y[pad] = -100
+    clean = h.clone()
+    clean[pad] = 0
+    h[pad] = torch.finfo(t).max if fill == "largest" else fill
+    dl[pad] = float("nan")                                        # not read
+    want, got = run_loss(clean, w, y, dl, check=True), run_loss(h, w, y, dl, check=True)
+    keep = ~pad
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1][keep], want[1][keep])
+    assert torch.equal(got[2], want[2]) and torch.equal(got[3], want[3])
+    assert not got[2][pad].any()
+    LossRef(clean, w, y, dl).check(got[0], torch.where(pad, want[1], got[1]), got[2], got[3])
+    # the same of a target that is no id
+    y[1] = V + 3
+    want, got = run_loss(clean, w, y, dl), run_loss(h, w, y, dl)
+    assert torch.equal(got[2], want[2]) and torch.equal(got[3], want[3])
