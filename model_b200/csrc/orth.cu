@@ -475,20 +475,37 @@ bool orth_workspace(const memlayer_orth_config& c, size_t* bytes) {
   return true;
 }
 
-bool orth_coefficients_ok(const memlayer_orth_config& c) {
-  // singular values start in [0, 1] and go through x (a + b x^2 + c x^4);
-  // every matrix of a step is bounded by its largest singular value
-  const double a = c.a, b = c.b, d = c.c;
-  for (int i = 0; i <= 256; ++i) {
-    double x = i / 256.0;
-    for (int k = 0; k < c.steps; ++k) {
-      const double p = x * x, r = b + d * p, q = a + r * p;
-      if (!(p <= BOUND * 0.5) || !(fabs(r) <= BOUND * 0.8) || !(fabs(q) <= BOUND * 0.8)) return false;
-      x = fabs(x * q);
+bool orth_coefficients_ok(const memlayer_orth_config& cfg) {
+  // Singular values start in [0, 1] and go through f(x) = x (a + b x^2 + c x^4);
+  // every matrix of a step is bounded by its largest singular value.  f is
+  // continuous and f(0) = 0, so a step takes [0, hi] to [0, max |f|] exactly,
+  // and the maxima are at the ends or where a derivative is zero: no value in
+  // between is missed (samples of [0, 1] missed some that grow without bound).
+  const double a = cfg.a, b = cfg.b, c = cfg.c;
+  double hi = 1.0;
+  for (int k = 0; k < cfg.steps; ++k) {
+    const double u = hi * hi;                              // u = x^2 in [0, u]
+    const double r = fmax(fabs(b), fabs(b + c * u));
+    auto q_at = [&](double v) { return a + (b + c * v) * v; };
+    double q = fmax(fabs(a), fabs(q_at(u))), top = fabs(hi * q_at(u));
+    if (c != 0.0 && -b / (2 * c) > 0.0 && -b / (2 * c) < u) q = fmax(q, fabs(q_at(-b / (2 * c))));
+    double root[2] = {-1.0, -1.0};                         // of a + 3 b v + 5 c v^2
+    if (c != 0.0) {
+      const double d = 9 * b * b - 20 * a * c;
+      if (d >= 0.0) {
+        root[0] = (-3 * b + sqrt(d)) / (10 * c);
+        root[1] = (-3 * b - sqrt(d)) / (10 * c);
+      }
+    } else if (b != 0.0) {
+      root[0] = -a / (3 * b);
     }
-    if (!(x <= BOUND * 0.2)) return false;
+    for (double v : root)
+      if (v > 0.0 && v < u) top = fmax(top, sqrt(v) * fabs(q_at(v)));
+    // (a NaN among the coefficients fails the comparisons: fmax drops it, the sum keeps it)
+    if (!(u <= BOUND * 0.5) || !(r <= BOUND * 0.8) || !(q <= BOUND * 0.8) || !(a + b + c == a + b + c)) return false;
+    hi = top;
   }
-  return true;
+  return hi <= BOUND * 0.2;
 }
 
 cudaError_t launch_orthogonalize(const memlayer_orth_config& c, const void* update, void* out, char* ws,

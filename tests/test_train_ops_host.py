@@ -302,3 +302,47 @@ def test_head_gradients_pass_check_to_every_call(monkeypatch, check):
     seen.clear()
     prep.loss(tokens, tokens, check=check)
     assert seen == {"hidden": check, "loss": check}
+
+
+# ---- the range of the update's iteration ---------------------------------------------------
+def leaves_range(a, b, c, steps):
+    """Whether some singular value in [0, 1] leaves the documented range (by a grid finer than any that the library needs)."""
+    import numpy as np
+    x = np.linspace(0, 1, 400001)
+    for _ in range(steps):
+        p = x * x
+        r = b + c * p
+        q = a + r * p
+        if max(p.max() / 7.5, abs(r).max() / 12, abs(q).max() / 12) > 1:
+            return True
+        x = abs(x * q)
+    return x.max() > 3
+
+
+def orth_accepts(a, b, c, steps):
+    n, cfg = C.c_size_t(), orth_cfg(a=a, b=b, c=c, steps=steps)
+    return L.lib().memlayer_orthogonalize_workspace_size(C.byref(cfg), C.byref(n)) == L.OK
+
+
+@pytest.mark.parametrize("a,b,c,steps", [(-1.3941725320194571, 3.485549324717482, -1.0893582225835132, 11),
+                                         (0.9655603461302071, -8.625747304512245, 7.939453129480508, 3)])
+def test_orth_iterations_that_few_singular_values_leave_refused(a, b, c, steps):
+    # most values stay below 1.5, those of a narrow band grow to 1e290 (first case) or past 3
+    assert leaves_range(a, b, c, steps) and not orth_accepts(a, b, c, steps)
+
+
+def test_orth_iterations_inside_their_range_accepted():
+    import numpy as np
+    rng = np.random.default_rng(5)
+    taken = 0
+    for _ in range(300):
+        a, b, c = (float(np.float32(v)) for v in (rng.uniform(-5, 5), rng.uniform(-10, 10), rng.uniform(-6, 6)))
+        steps = int(rng.integers(1, 6))
+        ok = orth_accepts(a, b, c, steps)
+        taken += ok
+        if ok:
+            assert not leaves_range(a, b, c, steps), (a, b, c, steps)
+    assert taken > 30
+    for coef in ((3.4445, -4.7750, 2.0315), (1.5, -0.5, 0.0), (1.875, -1.25, 0.375), (2.0, -1.5, 0.5)):
+        for steps in (1, 5, 64):
+            assert orth_accepts(*coef, steps) == (not leaves_range(*coef, steps))
