@@ -5,7 +5,9 @@ Every ``csrc/*.cu`` file is compiled for sm_100a only
 library that exports the C ABI of ``include/memlayer.h``.  nvcc
 cross-compiles without a GPU, so this runs on any machine with CUDA 12.9.
 ``csrc/fast_calls.cpp``, the training operators' calls from torch tensors, is
-compiled beside it against this interpreter and its torch.
+compiled beside it against this interpreter and its torch, again whenever one
+of them or the command changes.  Without it (no host compiler, no headers) the
+operators go over ctypes, so a failure there is a warning.
 """
 
 from __future__ import annotations
@@ -24,6 +26,7 @@ INCLUDE = os.path.join(ROOT, "include")
 BUILD = os.path.join(ROOT, "_build")
 LIB = os.path.join(PKG, "libmemlayer.so")
 FAST = os.path.join(PKG, "_fast" + sysconfig.get_config_var("EXT_SUFFIX"))
+FAST_STAMP = os.path.join(BUILD, "fast_calls.stamp")   # what FAST was built with
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -45,12 +48,40 @@ def _fast_command():
     tinc, cuda = os.path.join(tdir, "include"), os.path.dirname(os.path.dirname(NVCC))
     src = os.path.join(CSRC, "fast_calls.cpp")
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", src, "-o", FAST, "-I", INCLUDE,
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f'-DMEMLAYER_TORCH_VERSION="{torch.__version__}"', src, "-o", FAST, "-I", INCLUDE,
            "-I", tinc, "-I", os.path.join(tinc, "torch", "csrc", "api", "include"),
            "-I", os.path.join(cuda, "include"), "-I", sysconfig.get_paths()["include"],
-           "-L", PKG, "-l:" + os.path.basename(LIB), "-L", os.path.join(tdir, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python",
-           "-Wl,-rpath,$ORIGIN"]
+           "-L", PKG, "-l:" + os.path.basename(LIB), "-L", os.path.join(tdir, "lib"), "-lc10", "-lc10_cuda",
+           "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
     return cmd, [src, os.path.join(INCLUDE, "memlayer.h")]
+
+
+def build_fast() -> bool:
+    """The extension module, where it is not what this torch, source and command give; False: not built."""
+    cmd, deps = _fast_command()
+    stamp = "\n".join([sys.version, *cmd])           # the command names torch's version and folder
+    try:
+        with open(FAST_STAMP) as f:
+            same = f.read() == stamp
+    except OSError:
+        same = False
+    if same and not _stale(FAST, deps):
+        return True
+    if os.path.exists(FAST):
+        os.remove(FAST)                              # one of another torch must not be loaded
+    try:
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        failed = None if r.returncode == 0 else f"{r.stdout}\n{r.stderr}"
+    except OSError as e:
+        failed = str(e)
+    if failed is not None:
+        print(f"warning: {os.path.basename(FAST)} is not built, the training operators' calls go over ctypes "
+              f"({' '.join(cmd)}):\n{failed}", file=sys.stderr)
+        return False
+    with open(FAST_STAMP, "w") as f:
+        f.write(stamp)
+    return True
 
 
 def build(verbose: bool = False, ptxas_verbose: bool = False) -> str:
@@ -80,9 +111,7 @@ def build(verbose: bool = False, ptxas_verbose: bool = False) -> str:
     if jobs or not os.path.exists(LIB):
         run([NVCC, *ARCH, "-shared", "-o", LIB, *objs, "-lcudart_static", "-Xlinker",
              "-rpath=/usr/local/cuda/lib64", "-lrt", "-ldl", "-lpthread"])
-    cmd, deps = _fast_command()
-    if _stale(FAST, deps):
-        run(cmd)
+    build_fast()
     # the XLA FFI handlers of the JAX binding, where JAX is installed
     from model_b200 import jax_ffi
     jax_ffi.build(verbose=verbose)

@@ -250,4 +250,16 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_fast", nullptr, -1, methods, null
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__fast() { return PyModule_Create(&module); }
+// train_ops.py uses the module with the torch it was compiled against only.
+PyMODINIT_FUNC PyInit__fast() {
+  if (memlayer_abi_version() != MEMLAYER_ABI_VERSION) {
+    PyErr_SetString(PyExc_ImportError, "_fast was built for another version of libmemlayer.so's interface");
+    return nullptr;
+  }
+  PyObject* m = PyModule_Create(&module);
+  if (m && PyModule_AddStringConstant(m, "torch_version", MEMLAYER_TORCH_VERSION) < 0) {
+    Py_DECREF(m);
+    return nullptr;
+  }
+  return m;
+}

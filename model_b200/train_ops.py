@@ -32,10 +32,16 @@ import torch
 from . import _lib as L
 from .memory import _DTYPES, _workspace
 
+def _usable(module):
+    """The extension module if it was built for this torch (another's layouts differ), else None."""
+    return module if getattr(module, "torch_version", None) == torch.__version__ else None
+
+
 try:
     from . import _fast
 except ImportError:          # not built for this interpreter: every call takes the general way
     _fast = None
+_fast = _usable(_fast)
 
 
 def _on_tensor_device(fn):

@@ -346,3 +346,51 @@ def test_orth_iterations_inside_their_range_accepted():
     for coef in ((3.4445, -4.7750, 2.0315), (1.5, -0.5, 0.0), (1.875, -1.25, 0.375), (2.0, -1.5, 0.5)):
         for steps in (1, 5, 64):
             assert orth_accepts(*coef, steps) == (not leaves_range(*coef, steps))
+
+
+# ---- the extension module's build -----------------------------------------------------------
+@pytest.fixture
+def elsewhere(monkeypatch, tmp_path):
+    from model_b200 import build as B
+    monkeypatch.setattr(B, "FAST", str(tmp_path / "_fast.so"))
+    monkeypatch.setattr(B, "FAST_STAMP", str(tmp_path / "stamp"))
+    runs = []
+
+    def compiler(fails):
+        def run(cmd, **kw):
+            runs.append(cmd)
+            if fails == "missing":
+                raise FileNotFoundError(cmd[0])
+            if not fails:
+                (tmp_path / "_fast.so").write_text("built")
+            return type("R", (), {"returncode": int(bool(fails)), "stdout": "", "stderr": "no such header"})()
+        monkeypatch.setattr(B.subprocess, "run", run)
+    return B, compiler, runs
+
+
+@pytest.mark.parametrize("fails", [True, "missing"])
+def test_extension_that_does_not_compile_is_a_warning(elsewhere, capsys, fails):
+    B, compiler, runs = elsewhere
+    with open(B.FAST, "w") as f:                     # one of another torch
+        f.write("old")
+    compiler(fails)
+    assert B.build_fast() is False and "go over ctypes" in capsys.readouterr().err
+    import os
+    assert not os.path.exists(B.FAST) and not os.path.exists(B.FAST_STAMP)
+
+
+def test_extension_is_built_again_for_another_torch(elsewhere, monkeypatch):
+    B, compiler, runs = elsewhere
+    compiler(False)
+    assert B.build_fast() and B.build_fast() and len(runs) == 1
+    monkeypatch.setattr(torch, "__version__", "0.0+other")
+    assert B.build_fast() and B.build_fast() and len(runs) == 2
+
+
+def test_extension_of_another_torch_is_not_used(monkeypatch):
+    from model_b200 import train_ops
+    fast = train_ops._fast
+    assert fast is not None and fast.torch_version == torch.__version__ and train_ops._usable(fast) is fast
+    assert train_ops._usable(None) is None
+    monkeypatch.setattr(torch, "__version__", "0.0+other")
+    assert train_ops._usable(fast) is None
