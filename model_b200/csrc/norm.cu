@@ -30,8 +30,9 @@
 //
 // The parameter gradients: dscale / dbias of the columns stay in registers over
 // all of a block's rows; it adds its row groups in shared memory and writes one
-// partial row; a second kernel adds the partials in block order,
-// so the result does not depend on timing (no atomics).
+// partial row; a second kernel adds the partials, 32 groups of blocks in block
+// order and the groups in a fixed tree, so the result does not depend on timing
+// (no atomics).
 //
 // Launches are dependent ones: a kernel's start hides behind the end of the
 // one before it (8192 x 256 float32, forward and gradient: 22.3 us for 24.6).
@@ -614,42 +615,38 @@ __global__ void __launch_bounds__(MAXT, MINB) layer_norm_wide_kernel(NormArgs A)
   }
 }
 
-// R rows of a block's batch, as loaded.
-template <typename E, int R, int NV, bool SHIFT>
-struct Batch {
+// A block's row, as loaded.
+template <typename E, int NV, bool SHIFT>
+struct WideRow {
   static constexpr int V = 16 / sizeof(E);
-  Vec16<E, V> p[R][NV], q[R][NV], e[R][NV];
-  __device__ __forceinline__ void load(const NormArgs& A, int64_t base, int o) {
+  Vec16<E, V> p[NV], q[NV], e[NV];
+  __device__ __forceinline__ void load(const NormArgs& A, int64_t row, int o) {
+    if (row >= A.rows) return;
     const int t = threadIdx.x, nt = blockDim.x;
+    const bool last = row + 1 == A.rows;
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int64_t row = base + r;
-      if (row >= A.rows) break;
-      const bool last = row + 1 == A.rows;
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int j = (i * nt + t) * V - o;
-        if (j >= A.d) continue;
-        p[r][i] = load_part<E, V, SHIFT>(reinterpret_cast<const E*>(A.x) + row * A.ldx, j, A.d, last);
-        q[r][i] = load_part<E, V, SHIFT>(reinterpret_cast<const E*>(A.dy) + row * A.lddy, j, A.d, last);
-        if (A.dr) e[r][i] = load_part<E, V, SHIFT>(reinterpret_cast<const E*>(A.dr) + row * A.lddr, j, A.d, last);
-      }
+    for (int i = 0; i < NV; ++i) {
+      const int j = (i * nt + t) * V - o;
+      if (j >= A.d) continue;
+      p[i] = load_part<E, V, SHIFT>(reinterpret_cast<const E*>(A.x) + row * A.ldx, j, A.d, last);
+      q[i] = load_part<E, V, SHIFT>(reinterpret_cast<const E*>(A.dy) + row * A.lddy, j, A.d, last);
+      if (A.dr) e[i] = load_part<E, V, SHIFT>(reinterpret_cast<const E*>(A.dr) + row * A.lddr, j, A.d, last);
     }
   }
 };
 
-// AHEAD: the next batch's loads are issued before this one's sums, so HBM is
+// AHEAD: the next row's loads are issued before this one's sums, so HBM is
 // busy during the barriers (where the registers allow it: shifted 16-bit rows
 // would spill, 155 us for 130 at 9557 x 2498).
-template <typename E, int R, int NV, int MAXT, int MINB, bool AHEAD, bool SHIFT>
+template <typename E, int NV, int MAXT, int MINB, bool AHEAD, bool SHIFT>
 __global__ void __launch_bounds__(MAXT, MINB) layer_norm_wide_backward_kernel(NormArgs A) {
   constexpr int V = 16 / sizeof(E), H = V / 2;
   using Vec = Vec16<E, V>;
   allow_next();
   wait_previous();
-  __shared__ alignas(16) float red[2][3 * R * 32];
+  __shared__ alignas(16) float red[2][3 * 32];
   const int d = A.d, t = threadIdx.x, nt = blockDim.x, o = block_shift<V, SHIFT>(d);
-  for (int i = t; i < 2 * 3 * R * 32; i += nt) (&red[0][0])[i] = 0.f;   // slots without a warp
+  for (int i = t; i < 2 * 3 * 32; i += nt) (&red[0][0])[i] = 0.f;       // slots without a warp
   __syncthreads();
   if (blockIdx.x == 0 && threadIdx.x == 0) *A.err = 0;
   F2 ag[NV][H], ab[NV][H], sc[NV][H];
@@ -666,46 +663,43 @@ __global__ void __launch_bounds__(MAXT, MINB) layer_norm_wide_backward_kernel(No
       sc[i][k] = f2(f[2 * k], f[2 * k + 1]);
     }
   }
-  const int64_t step = (int64_t)gridDim.x * R;
-  Batch<E, R, NV, SHIFT> next;
-  if constexpr (AHEAD) next.load(A, (int64_t)blockIdx.x * R, o);
-  for (int64_t base = (int64_t)blockIdx.x * R; base < A.rows; base += step) {
-    Batch<E, R, NV, SHIFT> b;
+  WideRow<E, NV, SHIFT> next;
+  if constexpr (AHEAD) next.load(A, blockIdx.x, o);
+  for (int64_t row = blockIdx.x; row < A.rows; row += gridDim.x) {
+    WideRow<E, NV, SHIFT> b;
     if constexpr (AHEAD) {
       b = next;
-      next.load(A, base + step, o);
+      next.load(A, row + gridDim.x, o);
     } else {
-      b.load(A, base, o);
+      b.load(A, row, o);
     }
-    float s[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
+    float s[1];
+    {
       F2 acc = f2(0.f);
 #pragma unroll
       for (int i = 0; i < NV; ++i)
         if (const int j = (i * nt + t) * V - o; j < d) {
           F2 a[H];
-          unpack2(b.p[r][i], a);
+          unpack2(b.p[i], a);
           keep_row<V, SHIFT>(a, j, d, 0.f);
 #pragma unroll
           for (int k = 0; k < H; ++k) acc = acc + a[k];
         }
-      s[r] = sum(acc);
+      s[0] = sum(acc);
     }
     block_sums(s, red[0]);
     // around the mean: sum c^2, sum gy, sum gy c (c2 = rstd times it)
-    float m[3 * R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const float mean_f = s[r] * A.inv_d;
-      const F2 mean = f2(-mean_f);
+    const float mean_f = s[0] * A.inv_d;
+    const F2 mean = f2(-mean_f);
+    float m[3];
+    {
       F2 s2 = f2(0.f), sg = f2(0.f), sgc = f2(0.f);
 #pragma unroll
       for (int i = 0; i < NV; ++i)
         if (const int j = (i * nt + t) * V - o; j < d) {
           F2 a[H], g[H];
-          unpack2(b.p[r][i], a);
-          unpack2(b.q[r][i], g);
+          unpack2(b.p[i], a);
+          unpack2(b.q[i], g);
           keep_row<V, SHIFT>(a, j, d, mean_f);
           keep_row<V, SHIFT>(g, j, d, 0.f);
 #pragma unroll
@@ -716,43 +710,38 @@ __global__ void __launch_bounds__(MAXT, MINB) layer_norm_wide_backward_kernel(No
             sgc = fma2(gy, c, sgc);
           }
         }
-      m[3 * r] = sum(s2);
-      m[3 * r + 1] = sum(sg);
-      m[3 * r + 2] = sum(sgc);
+      m[0] = sum(s2);
+      m[1] = sum(sg);
+      m[2] = sum(sgc);
     }
     block_sums(m, red[1]);
+    const float rstd_f = rsqrtf(m[0] * A.inv_d + A.eps);
+    const F2 rstd = f2(rstd_f), c1 = f2(-(m[1] * A.inv_d)), c2 = f2(-(m[2] * rstd_f * A.inv_d));
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      if (base + r >= A.rows) break;
-      const float rstd_f = rsqrtf(m[3 * r] * A.inv_d + A.eps);
-      const F2 mean = f2(-(s[r] * A.inv_d)), rstd = f2(rstd_f), c1 = f2(-(m[3 * r + 1] * A.inv_d)),
-               c2 = f2(-(m[3 * r + 2] * rstd_f * A.inv_d));
+    for (int i = 0; i < NV; ++i) {
+      const int j = (i * nt + t) * V - o;
+      if (j >= d) continue;
+      F2 a[H], g[H];
+      float x[V];
+      unpack2(b.p[i], a);
+      unpack2(b.q[i], g);
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int j = (i * nt + t) * V - o;
-        if (j >= d) continue;
-        F2 a[H], g[H];
-        float x[V];
-        unpack2(b.p[r][i], a);
-        unpack2(b.q[r][i], g);
-#pragma unroll
-        for (int k = 0; k < H; ++k) {
-          const F2 xh = (a[k] + mean) * rstd;
-          ag[i][k] = fma2(g[k], xh, ag[i][k]);
-          ab[i][k] = ab[i][k] + g[k];
-          a[k] = rstd * fma2(xh, c2, g[k] * sc[i][k] + c1);
-        }
-        if (A.dr) {
-          unpack2(b.e[r][i], g);
-#pragma unroll
-          for (int k = 0; k < H; ++k) a[k] = a[k] + g[k];
-        }
-#pragma unroll
-        for (int k = 0; k < H; ++k) split(a[k], x[2 * k], x[2 * k + 1]);
-        Vec v;
-        pack(v, x);
-        store_part<E, V, SHIFT>(reinterpret_cast<E*>(A.dx) + (base + r) * (int64_t)d, j, d, v);
+      for (int k = 0; k < H; ++k) {
+        const F2 xh = (a[k] + mean) * rstd;
+        ag[i][k] = fma2(g[k], xh, ag[i][k]);
+        ab[i][k] = ab[i][k] + g[k];
+        a[k] = rstd * fma2(xh, c2, g[k] * sc[i][k] + c1);
       }
+      if (A.dr) {
+        unpack2(b.e[i], g);
+#pragma unroll
+        for (int k = 0; k < H; ++k) a[k] = a[k] + g[k];
+      }
+#pragma unroll
+      for (int k = 0; k < H; ++k) split(a[k], x[2 * k], x[2 * k + 1]);
+      Vec v;
+      pack(v, x);
+      store_part<E, V, SHIFT>(reinterpret_cast<E*>(A.dx) + row * (int64_t)d, j, d, v);
     }
   }
   float* out = A.part + (int64_t)blockIdx.x * 2 * d;
@@ -927,8 +916,8 @@ __global__ void __launch_bounds__(MAXW * 32, 1) layer_norm_ring_backward_kernel(
   }
 }
 
-// dscale | dbias = the blocks' partial rows added in block order: 32 groups of
-// blocks per column, then the groups in order.
+// dscale | dbias = the blocks' partial rows: 32 groups of blocks a column, each
+// added in block order, then the groups in a fixed tree.
 __global__ void __launch_bounds__(1024) layer_norm_params_kernel(const float* __restrict__ part, int blocks, int d,
                                                                  float* __restrict__ dscale,
                                                                  float* __restrict__ dbias, int* err) {
@@ -1043,22 +1032,21 @@ cudaError_t norm_forward_t(NormArgs& A, Access how, cudaStream_t s) {
     if (V == 8 && w.nv == 2 && w.nt <= 256) w = {(int)ceil_div(A.d + V - 1, V * 32) * 32, 1};
     const int most = w.nt > 256 ? 1024 / w.nt : w.per_sm(w.nv * V > 8 ? 3 : 4);
     const int grid = shifted_grid(A.rows, A.d, V, (int64_t)most * g16::device_sms());
-    if (w.nt > 256 && w.nv == 1)
-      launch_dependent(layer_norm_wide_kernel<E, 1, 1024, 1, true>, dim3(grid), w.nt, 0, s, A);
-    else if (w.nt > 256 && w.nv == 2)
-      launch_dependent(layer_norm_wide_kernel<E, 2, 1024, 1, true>, dim3(grid), w.nt, 0, s, A);
-    else if (w.nt > 256)
-      launch_dependent(layer_norm_wide_kernel<E, 4, 1024, 1, true>, dim3(grid), w.nt, 0, s, A);
-    else if (w.nv == 1)
-      launch_dependent(layer_norm_wide_kernel<E, 1, 256, 4, true>, dim3(grid), w.nt, 0, s, A);
-    else if constexpr (V == 4) {
-      if (w.nv == 2)
-        launch_dependent(layer_norm_wide_kernel<E, 2, 256, 4, true>, dim3(grid), w.nt, 0, s, A);
-      else
-        launch_dependent(layer_norm_wide_kernel<E, 4, 256, 3, true>, dim3(grid), w.nt, 0, s, A);
-    }
     count_launch();
-    return cudaGetLastError();
+    if (w.nt > 256) {
+      if constexpr (V == 8)
+        if (w.nv == 1)
+          return launch_dependent(layer_norm_wide_kernel<E, 1, 1024, 1, true>, dim3(grid), w.nt, 0, s, A);
+      if (w.nv == 2) return launch_dependent(layer_norm_wide_kernel<E, 2, 1024, 1, true>, dim3(grid), w.nt, 0, s, A);
+      if (w.nv == 4) return launch_dependent(layer_norm_wide_kernel<E, 4, 1024, 1, true>, dim3(grid), w.nt, 0, s, A);
+    } else {
+      if (w.nv == 1) return launch_dependent(layer_norm_wide_kernel<E, 1, 256, 4, true>, dim3(grid), w.nt, 0, s, A);
+      if constexpr (V == 4) {
+        if (w.nv == 2) return launch_dependent(layer_norm_wide_kernel<E, 2, 256, 4, true>, dim3(grid), w.nt, 0, s, A);
+        if (w.nv == 4) return launch_dependent(layer_norm_wide_kernel<E, 4, 256, 3, true>, dim3(grid), w.nt, 0, s, A);
+      }
+    }
+    return cudaErrorInvalidConfiguration;                 // no such width
   }
   const bool warp = A.d > 32 * VALS && (vec ? vecs <= 512 : A.d <= 2048);
   if (warp) {
@@ -1077,12 +1065,13 @@ cudaError_t norm_forward_t(NormArgs& A, Access how, cudaStream_t s) {
   } else if (vec && vecs > 512) {
     const Wide w = wide_for(A.d, V);
     const int grid = (int)(A.rows < MOST ? A.rows : MOST);
-    if (w.nv == 1)
-      launch_dependent(layer_norm_wide_kernel<E, 1, 1024, 1, false>, dim3(grid), w.nt, 0, s, A);
-    else if (w.nv == 2)
-      launch_dependent(layer_norm_wide_kernel<E, 2, 1024, 1, false>, dim3(grid), w.nt, 0, s, A);
-    else if constexpr (sizeof(E) == 4)   // 16-bit rows end at two vectors
-      launch_dependent(layer_norm_wide_kernel<E, 4, 1024, 1, false>, dim3(grid), w.nt, 0, s, A);
+    count_launch();
+    if constexpr (V == 8)                // float32 rows begin at two vectors, 16-bit ones end there
+      if (w.nv == 1) return launch_dependent(layer_norm_wide_kernel<E, 1, 1024, 1, false>, dim3(grid), w.nt, 0, s, A);
+    if (w.nv == 2) return launch_dependent(layer_norm_wide_kernel<E, 2, 1024, 1, false>, dim3(grid), w.nt, 0, s, A);
+    if constexpr (V == 4)
+      if (w.nv == 4) return launch_dependent(layer_norm_wide_kernel<E, 4, 1024, 1, false>, dim3(grid), w.nt, 0, s, A);
+    return cudaErrorInvalidConfiguration;                 // no such width
   } else {
     const bool wide = A.tpr > 32;
     const int nt = wide ? A.tpr : NT;
@@ -1112,23 +1101,36 @@ cudaError_t launch_ring(const NormArgs& A, const Ring& r, int grid, cudaStream_t
 // Blocks of 256 threads an SM holds with the gradient's registers: by columns a thread.
 int backward_resident(int cols) { return cols <= 4 ? 4 : cols <= 8 ? 3 : 2; }
 
+// Aligned rows come here from 2049 columns on and shifted ones from 513 on,
+// so a type has some of the shapes only.
 template <typename E, bool SHIFT>
-void launch_wide_backward(const NormArgs& A, const Wide& w, int grid, cudaStream_t s) {
+cudaError_t launch_wide_backward(const NormArgs& A, const Wide& w, int grid, cudaStream_t s) {
   constexpr int V = 16 / sizeof(E);
-  if (w.nt > 256 && w.nv == 1)
-    launch_dependent(layer_norm_wide_backward_kernel<E, 1, 1, 1024, 1, false, SHIFT>, dim3(grid), w.nt, 0, s, A);
-  else if (w.nt > 256 && w.nv == 2)
-    launch_dependent(layer_norm_wide_backward_kernel<E, 1, 2, 1024, 1, false, SHIFT>, dim3(grid), w.nt, 0, s, A);
-  else if (w.nt > 256)
-    launch_dependent(layer_norm_wide_backward_kernel<E, 1, 4, 1024, 1, false, SHIFT>, dim3(grid), w.nt, 0, s, A);
-  else if (w.nv == 1)
-    launch_dependent(layer_norm_wide_backward_kernel<E, 1, 1, 256, V == 4 ? 4 : 3, V == 4 || !SHIFT, SHIFT>,
-                     dim3(grid), w.nt, 0, s, A);
-  else if (w.nv == 2)
-    launch_dependent(layer_norm_wide_backward_kernel<E, 1, 2, 256, V == 4 ? 3 : 2, V == 4 || !SHIFT, SHIFT>,
-                     dim3(grid), w.nt, 0, s, A);
-  else if constexpr (V == 4)
-    launch_dependent(layer_norm_wide_backward_kernel<E, 1, 4, 256, 2, false, SHIFT>, dim3(grid), w.nt, 0, s, A);
+  constexpr bool F = V == 4;           // float32
+  if (w.nt > 256) {
+    if constexpr (!F)
+      if (w.nv == 1)
+        return launch_dependent(layer_norm_wide_backward_kernel<E, 1, 1024, 1, false, SHIFT>, dim3(grid), w.nt, 0, s, A);
+    if (w.nv == 2)
+      return launch_dependent(layer_norm_wide_backward_kernel<E, 2, 1024, 1, false, SHIFT>, dim3(grid), w.nt, 0, s, A);
+    if constexpr (F || SHIFT)
+      if (w.nv == 4)
+        return launch_dependent(layer_norm_wide_backward_kernel<E, 4, 1024, 1, false, SHIFT>, dim3(grid), w.nt, 0, s, A);
+  } else {
+    constexpr bool AHEAD = F || !SHIFT;
+    if constexpr (SHIFT)
+      if (w.nv == 1)
+        return launch_dependent(layer_norm_wide_backward_kernel<E, 1, 256, F ? 4 : 3, AHEAD, SHIFT>, dim3(grid), w.nt, 0,
+                                s, A);
+    if constexpr (!F || SHIFT)
+      if (w.nv == 2)
+        return launch_dependent(layer_norm_wide_backward_kernel<E, 2, 256, F ? 3 : 2, AHEAD, SHIFT>, dim3(grid), w.nt, 0,
+                                s, A);
+    if constexpr (F)
+      if (w.nv == 4)
+        return launch_dependent(layer_norm_wide_backward_kernel<E, 4, 256, 2, false, SHIFT>, dim3(grid), w.nt, 0, s, A);
+  }
+  return cudaErrorInvalidConfiguration;                   // no such width
 }
 
 template <typename E>
@@ -1136,8 +1138,10 @@ cudaError_t norm_backward_t(NormArgs& A, Access how, int grid, cudaStream_t s) {
   constexpr int V = 16 / sizeof(E);
   const bool vec = how == VECTORS;
   if (how == SHIFTED) {
-    launch_wide_backward<E, true>(A, wide_for(A.d + V - 1, V), grid, s);
-  } else if (vec && ring_rows(A.d, V)) {
+    count_launch();
+    return launch_wide_backward<E, true>(A, wide_for(A.d + V - 1, V), grid, s);
+  }
+  if (vec && ring_rows(A.d, V)) {
     const Ring r = ring_for(A.d, sizeof(E));
     cudaError_t e;
     if (A.d <= 1024)
@@ -1146,7 +1150,8 @@ cudaError_t norm_backward_t(NormArgs& A, Access how, int grid, cudaStream_t s) {
       e = launch_ring<E, 64 / V, 8>(A, r, grid, s);
     if (e != cudaSuccess) return e;
   } else if (vec && wide_rows(A.d, V)) {
-    launch_wide_backward<E, false>(A, wide_for(A.d, V), grid, s);
+    count_launch();
+    return launch_wide_backward<E, false>(A, wide_for(A.d, V), grid, s);
   } else {
     const bool wide = A.tpr > 32;
     const int nt = wide ? A.tpr : NT;

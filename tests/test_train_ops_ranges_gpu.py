@@ -10,7 +10,8 @@ import torch
 
 import model_b200 as mb
 from model_b200 import _lib as L
-from test_train_ops_gpu import BF16, F16, F32, TYPES, U, LossRef, gen, half_step, loss_case, run_loss, tiny, within
+from test_train_ops_gpu import (BF16, F16, F32, TYPES, U, LossRef, check_norm_backward, gen, half_step, loss_case,
+                                norm_case, norm_ref, run_loss, tiny, within)
 
 pytestmark = pytest.mark.gpu
 
@@ -227,3 +228,19 @@ def test_loss_padding_may_hold_anything(T, d, V, fill, t):
     y[1] = V + 3
     want, got = run_loss(clean, w, y, dl), run_loss(h, w, y, dl)
     assert torch.equal(got[2], want[2]) and torch.equal(got[3], want[3])
+
+
+# ---- norm: the first and last widths of each layout --------------------------------------
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("d", [512, 516, 1022, 2042, 2046, 2048, 2052, 2056, 4090, 4094, 4096, 4100, 4104, 8186, 8190, 8192,
+                               8196, 8200, 16378, 16380, 16384])
+def test_norm_at_the_borders_of_the_layouts(d, t):
+    x, r, scale, bias, dy, dr = norm_case(5, d, t, seed=d)
+    params = torch.empty(2, d + 4, device="cuda")
+    params[0, 1:d + 1], params[1, 1:d + 1] = scale, bias
+    for sc, bi in ((scale, bias), (params[0, 1:d + 1], params[1, 1:d + 1])):      # parameters beside a 16-byte boundary, too
+        y, s = mb.layer_norm(x, sc, bi, residual=r)
+        want, tol, *_ = norm_ref(s, scale, bias, 1e-6)
+        within(y, want, tol + half_step(t) * want.abs() + tiny(t), "y")
+        dx, dp = mb.layer_norm_backward(dy, s, sc, dresidual=dr, check=True)
+        check_norm_backward(dx, dp, dy, s, scale, dr, 1e-6, t)
