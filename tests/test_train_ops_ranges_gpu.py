@@ -244,3 +244,27 @@ def test_norm_at_the_borders_of_the_layouts(d, t):
         within(y, want, tol + half_step(t) * want.abs() + tiny(t), "y")
         dx, dp = mb.layer_norm_backward(dy, s, sc, dresidual=dr, check=True)
         check_norm_backward(dx, dp, dy, s, scale, dr, 1e-6, t)
+
+
+# ---- loss: sums cut into slices -----------------------------------------------------------
+# few tiles and many tokens: dW's sum over tokens is cut (s_w 2 to 5), joined by vectors or entry by entry;
+# (5003, 65, 501): rows that TMA cannot address, an odd number of entries
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("T,d,V", [(4096, 128, 1000), (5003, 65, 501), (3000, 72, 777), (2500, 200, 640)])
+def test_loss_sliced_dweight(T, d, V, t):
+    h, w, y, dl = loss_case(T, d, V, t, seed=T + d, gap=5)
+    dlse = 0.1 * dl * torch.randn(T, device="cuda", generator=gen(3))
+    got = run_loss(h, w, y, dl, dlse, check=True)
+    LossRef(h, w, y, dl, dlse).check(*got)
+    assert all(torch.equal(a, b) for a, b in zip(got, run_loss(h, w, y, dl, dlse)))
+
+
+@pytest.mark.parametrize("T,d,V", [(3000, 64, 60000), (2600, 65, 56001), (4200, 520, 40001)])
+def test_loss_several_vocabulary_pieces_f16(T, d, V):
+    h, w, y, dl = loss_case(T, d, V, F16, seed=15, gap=9)
+    dl = dl * 1000                                    # its results are above f16's subnormals
+    loss, lse, dh, dw = run_loss(h, w, y, dl, check=True)
+    again = run_loss(h, w, y, dl)
+    assert all(torch.equal(a, b) for a, b in zip((loss, lse, dh, dw), again))
+    ref = LossRef(h, w, y, dl)
+    ref.check(loss, lse, dh, dw)
