@@ -11,6 +11,10 @@
 // in registers, so the variance is the centred one -- E[x^2] - E[x]^2 loses
 // the variance of a row whose mean is large -- and the gradient recomputes
 // mean and rstd from the row it reads anyway instead of reading them back.
+// A float32 mean is off by some units of its last place, which is the whole of
+// a centred value where the row is (nearly) constant: its xhat came to 1
+// instead of 0 at values of 1e4.  So the centred values are summed beside their
+// squares; their mean is what the first one was off by, and is taken out.
 // Statistics and sums are float32 whatever the storage type.  Three layouts:
 //
 //   group   a row in a power of two of threads, 16 values each; up to a warp
@@ -111,6 +115,11 @@ __device__ __forceinline__ float row_sum(float x, int tpr, float* red) {
   }
 }
 
+// The variance from the mean square around a mean that is `off` from the row's.
+__device__ __forceinline__ float variance(float mean_square, float off) {
+  return fmaxf(fmaf(-off, off, mean_square), 0.f);
+}
+
 struct NormArgs {
   int64_t rows;
   int d, tpr;
@@ -154,18 +163,20 @@ __global__ void __launch_bounds__(MAXT ? MAXT : NT, MAXT ? 1 : 2) layer_norm_ker
     for (int k = 0; k < VALS; ++k)
       if (col_of<VEC>(k, t, tpr) < d) s += p.get(k);
     const float mean = row_sum<WIDE>(s, tpr, red) * A.inv_d;
-    float s2 = 0.f;
+    float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int k = 0; k < VALS; ++k)
       if (col_of<VEC>(k, t, tpr) < d) {
         const float c = p.get(k) - mean;
+        s1 += c;
         s2 = fmaf(c, c, s2);
       }
-    const float rstd = 1.0f / sqrtf(row_sum<WIDE>(s2, tpr, red) * A.inv_d + A.eps);
+    const float off = row_sum<WIDE>(s1, tpr, red) * A.inv_d;
+    const float rstd = 1.0f / sqrtf(variance(row_sum<WIDE>(s2, tpr, red) * A.inv_d, off) + A.eps);
 #pragma unroll
     for (int k = 0; k < VALS; ++k) {
       const int j = col_of<VEC>(k, t, tpr);
-      if (j < d) p.set(k, fmaf((p.get(k) - mean) * rstd, A.scale[j], A.bias[j]));
+      if (j < d) p.set(k, fmaf((p.get(k) - mean - off) * rstd, A.scale[j], A.bias[j]));
     }
     if (on) p.store(reinterpret_cast<E*>(A.y) + row * (int64_t)d, t, tpr, d);
   }
@@ -199,20 +210,22 @@ __global__ void __launch_bounds__(MAXT ? MAXT : NT, MAXT ? 1 : 2) layer_norm_bac
     for (int k = 0; k < VALS; ++k)
       if (col_of<VEC>(k, t, tpr) < d) s += p.get(k);
     const float mean = row_sum<WIDE>(s, tpr, red) * A.inv_d;
-    float s2 = 0.f;
+    float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int k = 0; k < VALS; ++k)
       if (col_of<VEC>(k, t, tpr) < d) {
         const float c = p.get(k) - mean;
+        s1 += c;
         s2 = fmaf(c, c, s2);
       }
-    const float rstd = 1.0f / sqrtf(row_sum<WIDE>(s2, tpr, red) * A.inv_d + A.eps);
+    const float off = row_sum<WIDE>(s1, tpr, red) * A.inv_d;
+    const float rstd = 1.0f / sqrtf(variance(row_sum<WIDE>(s2, tpr, red) * A.inv_d, off) + A.eps);
     float c1 = 0.f, c2 = 0.f;
 #pragma unroll
     for (int k = 0; k < VALS; ++k) {
       const int j = col_of<VEC>(k, t, tpr);
       if (j < d) {
-        const float xh = (p.get(k) - mean) * rstd, dy = q.get(k), gy = __fmul_rn(dy, A.scale[j]);
+        const float xh = (p.get(k) - mean - off) * rstd, dy = q.get(k), gy = __fmul_rn(dy, A.scale[j]);
         c1 += gy;
         c2 = fmaf(gy, xh, c2);
         if (on) {
@@ -227,7 +240,7 @@ __global__ void __launch_bounds__(MAXT ? MAXT : NT, MAXT ? 1 : 2) layer_norm_bac
     for (int k = 0; k < VALS; ++k) {
       const int j = col_of<VEC>(k, t, tpr);
       if (j < d) {
-        const float xh = (p.get(k) - mean) * rstd;
+        const float xh = (p.get(k) - mean - off) * rstd;
         // the same rounded product as in c1: a constant row cancels exactly
         float x = rstd * (__fmul_rn(q.get(k), A.scale[j]) - c1 - xh * c2);
         if (A.dr) x += r.get(k);
@@ -431,7 +444,7 @@ __global__ void __launch_bounds__(128) layer_norm_warp_kernel(NormArgs A) {
       for (int k = 0; k < V; ++k) s += a[k];
     }
   const float mean = warp_sum(s) * A.inv_d;
-  float s2 = 0.f;
+  float s1 = 0.f, s2 = 0.f;
 #pragma unroll
   for (int i = 0; i < NV; ++i)
     if ((i * 32 + lane) * V < d) {
@@ -440,10 +453,12 @@ __global__ void __launch_bounds__(128) layer_norm_warp_kernel(NormArgs A) {
 #pragma unroll
       for (int k = 0; k < V; ++k) {
         const float c = a[k] - mean;
+        s1 += c;
         s2 = fmaf(c, c, s2);
       }
     }
-  const float rstd = 1.0f / sqrtf(warp_sum(s2) * A.inv_d + A.eps);
+  const float off = warp_sum(s1) * A.inv_d;
+  const float rstd = 1.0f / sqrtf(variance(warp_sum(s2) * A.inv_d, off) + A.eps);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int j = (i * 32 + lane) * V;
@@ -453,7 +468,7 @@ __global__ void __launch_bounds__(128) layer_norm_warp_kernel(NormArgs A) {
     load_f32(A.scale + j, sc);
     load_f32(A.bias + j, bi);
 #pragma unroll
-    for (int k = 0; k < V; ++k) a[k] = fmaf((a[k] - mean) * rstd, sc[k], bi[k]);
+    for (int k = 0; k < V; ++k) a[k] = fmaf((a[k] - mean - off) * rstd, sc[k], bi[k]);
     pack(p[i], a);
     *reinterpret_cast<Vec*>(reinterpret_cast<E*>(A.y) + row * (int64_t)d + j) = p[i];
   }
@@ -528,11 +543,11 @@ template <typename E, int NV, int MAXT, int MINB, bool SHIFT>
 __global__ void __launch_bounds__(MAXT, MINB) layer_norm_wide_kernel(NormArgs A) {
   constexpr int V = 16 / sizeof(E);
   using Vec = Vec16<E, V>;
-  __shared__ alignas(16) float red[2][32];
+  __shared__ alignas(16) float red[2][2 * 32];
   const int d = A.d, t = threadIdx.x, nt = blockDim.x, o = block_shift<V, SHIFT>(d);
   allow_next();
   wait_previous();
-  if (t < 64) (&red[0][0])[t] = 0.f;     // slots without a warp
+  for (int i = t; i < 2 * 2 * 32; i += nt) (&red[0][0])[i] = 0.f;       // slots without a warp
   __syncthreads();
   float scale[NV][V], bias[NV][V];       // SHIFT: kept over the block's rows
   if constexpr (SHIFT) {
@@ -547,7 +562,7 @@ __global__ void __launch_bounds__(MAXT, MINB) layer_norm_wide_kernel(NormArgs A)
   for (int64_t row = blockIdx.x; row < A.rows; row += gridDim.x) {
     const bool last = row + 1 == A.rows;
     Vec p[NV], q[NV];
-    float s[1] = {0.f}, s2[1] = {0.f};
+    float s[1] = {0.f}, s2[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int j = (i * nt + t) * V - o;
@@ -587,10 +602,12 @@ __global__ void __launch_bounds__(MAXT, MINB) layer_norm_wide_kernel(NormArgs A)
       for (int k = 0; k < V; ++k) {
         const float c = a[k] - mean;
         s2[0] = fmaf(c, c, s2[0]);
+        s2[1] += c;
       }
     }
     block_sums(s2, red[1]);
-    const float rstd = 1.0f / sqrtf(s2[0] * A.inv_d + A.eps);
+    const float off = s2[1] * A.inv_d;
+    const float rstd = 1.0f / sqrtf(variance(s2[0] * A.inv_d, off) + A.eps);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int j = (i * nt + t) * V - o;
@@ -608,7 +625,7 @@ __global__ void __launch_bounds__(MAXT, MINB) layer_norm_wide_kernel(NormArgs A)
         load_f32(A.bias + j, bi);
       }
 #pragma unroll
-      for (int k = 0; k < V; ++k) a[k] = fmaf((a[k] - mean) * rstd, sc[k], bi[k]);
+      for (int k = 0; k < V; ++k) a[k] = fmaf((a[k] - mean - off) * rstd, sc[k], bi[k]);
       pack(p[i], a);
       store_part<E, V, SHIFT>(reinterpret_cast<E*>(A.y) + row * (int64_t)d, j, d, p[i]);
     }
@@ -644,9 +661,9 @@ __global__ void __launch_bounds__(MAXT, MINB) layer_norm_wide_backward_kernel(No
   using Vec = Vec16<E, V>;
   allow_next();
   wait_previous();
-  __shared__ alignas(16) float red[2][3 * 32];
+  __shared__ alignas(16) float red[2][4 * 32];
   const int d = A.d, t = threadIdx.x, nt = blockDim.x, o = block_shift<V, SHIFT>(d);
-  for (int i = t; i < 2 * 3 * 32; i += nt) (&red[0][0])[i] = 0.f;       // slots without a warp
+  for (int i = t; i < 2 * 4 * 32; i += nt) (&red[0][0])[i] = 0.f;       // slots without a warp
   __syncthreads();
   if (blockIdx.x == 0 && threadIdx.x == 0) *A.err = 0;
   F2 ag[NV][H], ab[NV][H], sc[NV][H];
@@ -688,12 +705,12 @@ __global__ void __launch_bounds__(MAXT, MINB) layer_norm_wide_backward_kernel(No
       s[0] = sum(acc);
     }
     block_sums(s, red[0]);
-    // around the mean: sum c^2, sum gy, sum gy c (c2 = rstd times it)
+    // around the mean: sum c^2, sum gy, sum gy c (c2 = rstd times it), sum c
     const float mean_f = s[0] * A.inv_d;
     const F2 mean = f2(-mean_f);
-    float m[3];
+    float m[4];
     {
-      F2 s2 = f2(0.f), sg = f2(0.f), sgc = f2(0.f);
+      F2 s1 = f2(0.f), s2 = f2(0.f), sg = f2(0.f), sgc = f2(0.f);
 #pragma unroll
       for (int i = 0; i < NV; ++i)
         if (const int j = (i * nt + t) * V - o; j < d) {
@@ -705,6 +722,7 @@ __global__ void __launch_bounds__(MAXT, MINB) layer_norm_wide_backward_kernel(No
 #pragma unroll
           for (int k = 0; k < H; ++k) {
             const F2 c = a[k] + mean, gy = g[k] * sc[i][k];
+            s1 = s1 + c;
             s2 = fma2(c, c, s2);
             sg = sg + gy;
             sgc = fma2(gy, c, sgc);
@@ -713,10 +731,12 @@ __global__ void __launch_bounds__(MAXT, MINB) layer_norm_wide_backward_kernel(No
       m[0] = sum(s2);
       m[1] = sum(sg);
       m[2] = sum(sgc);
+      m[3] = sum(s1);
     }
     block_sums(m, red[1]);
-    const float rstd_f = rsqrtf(m[0] * A.inv_d + A.eps);
-    const F2 rstd = f2(rstd_f), c1 = f2(-(m[1] * A.inv_d)), c2 = f2(-(m[2] * rstd_f * A.inv_d));
+    const float off = m[3] * A.inv_d, rstd_f = rsqrtf(variance(m[0] * A.inv_d, off) + A.eps);
+    const F2 rstd = f2(rstd_f), c1 = f2(-(m[1] * A.inv_d)), c2 = f2(-(fmaf(-off, m[1], m[2]) * rstd_f * A.inv_d)),
+             noff = f2(-off);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int j = (i * nt + t) * V - o;
@@ -727,7 +747,7 @@ __global__ void __launch_bounds__(MAXT, MINB) layer_norm_wide_backward_kernel(No
       unpack2(b.q[i], g);
 #pragma unroll
       for (int k = 0; k < H; ++k) {
-        const F2 xh = (a[k] + mean) * rstd;
+        const F2 xh = (a[k] + mean + noff) * rstd;
         ag[i][k] = fma2(g[k], xh, ag[i][k]);
         ab[i][k] = ab[i][k] + g[k];
         a[k] = rstd * fma2(xh, c2, g[k] * sc[i][k] + c1);
@@ -765,7 +785,7 @@ __global__ void __launch_bounds__(MAXT, MINB) layer_norm_wide_backward_kernel(No
 // The gradient of rows that a warp holds: a warp per row, without a barrier.
 // Each warp streams its rows of x and dy through a ring of its own in shared
 // memory (bulk copies, signalled by mbarriers) and reads them from there: the
-// mean, the three sums around it, dx.  The columns' parameter sums stay in its
+// mean, the four sums around it, dx.  The columns' parameter sums stay in its
 // registers over all of its rows; the block adds its warps' at the end.
 template <typename E, int NV, int MAXW>
 __global__ void __launch_bounds__(MAXW * 32, 1) layer_norm_ring_backward_kernel(NormArgs A, int stages) {
@@ -841,7 +861,7 @@ __global__ void __launch_bounds__(MAXW * 32, 1) layer_norm_ring_backward_kernel(
         for (int k = 0; k < H; ++k) acc = acc + a[k];
       }
     const F2 mean = f2(-(warp_sum(sum(acc)) * A.inv_d));
-    F2 s2 = f2(0.f), sg = f2(0.f), sgc = f2(0.f);
+    F2 s1 = f2(0.f), s2 = f2(0.f), sg = f2(0.f), sgc = f2(0.f);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
       if ((i * 32 + lane) * V < d) {
@@ -852,14 +872,16 @@ __global__ void __launch_bounds__(MAXW * 32, 1) layer_norm_ring_backward_kernel(
 #pragma unroll
         for (int k = 0; k < H; ++k) {
           const F2 c = a[k] + mean, gy = g[k] * sc[k];
+          s1 = s1 + c;
           s2 = fma2(c, c, s2);
           sg = sg + gy;
           sgc = fma2(gy, c, sgc);
         }
       }
-    const float rstd_f = rsqrtf(warp_sum(sum(s2)) * A.inv_d + A.eps);
-    const F2 rstd = f2(rstd_f), c1 = f2(-(warp_sum(sum(sg)) * A.inv_d)),
-             c2 = f2(-(warp_sum(sum(sgc)) * rstd_f * A.inv_d));
+    const float off = warp_sum(sum(s1)) * A.inv_d, gsum = warp_sum(sum(sg));
+    const float rstd_f = rsqrtf(variance(warp_sum(sum(s2)) * A.inv_d, off) + A.eps);
+    const F2 rstd = f2(rstd_f), c1 = f2(-(gsum * A.inv_d)),
+             c2 = f2(-(fmaf(-off, gsum, warp_sum(sum(sgc))) * rstd_f * A.inv_d)), noff = f2(-off);
     Vec* out = reinterpret_cast<Vec*>(reinterpret_cast<E*>(A.dx) + row * (int64_t)d);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
@@ -871,7 +893,7 @@ __global__ void __launch_bounds__(MAXW * 32, 1) layer_norm_ring_backward_kernel(
         const F2* sc = reinterpret_cast<const F2*>(scale_s + (i * 32 + lane) * V);
 #pragma unroll
         for (int k = 0; k < H; ++k) {
-          const F2 xh = (a[k] + mean) * rstd;
+          const F2 xh = (a[k] + mean + noff) * rstd;
           ag[i][k] = fma2(g[k], xh, ag[i][k]);
           ab[i][k] = ab[i][k] + g[k];
           a[k] = rstd * fma2(xh, c2, g[k] * sc[k] + c1);

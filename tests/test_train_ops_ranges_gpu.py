@@ -268,3 +268,38 @@ def test_loss_several_vocabulary_pieces_f16(T, d, V):
     assert all(torch.equal(a, b) for a, b in zip((loss, lse, dh, dw), again))
     ref = LossRef(h, w, y, dl)
     ref.check(loss, lse, dh, dw)
+
+
+# ---- norm: rows whose mean is far larger than their spread --------------------------------
+# The mean as first summed is off by at most m0 = 32 u mean|x|; the centred values (exact beside such a mean, else u of
+# themselves) are summed again, which leaves 32 u (spread + m0) of it, and 64 u m0^2 of the variance.
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("value,spread", [(1e4, 0.0), (-773.3, 0.0), (1e4, 0.05), (3e5, 1.0), (0.3, 1e-6), (1e-3, 0.0)])
+@pytest.mark.parametrize("d", [7, 33, 256, 300, 768, 1003, 1500, 2048, 2498, 5000, 8200, 12288, 16384])
+def test_norm_of_nearly_constant_rows(d, value, spread, t):
+    if t == F16:
+        value = max(-6e4, min(6e4, value))
+    g = gen(d)
+    x = (value * (1 + torch.rand(37, 1, device="cuda", generator=g) * 0.1)
+         + spread * torch.randn(37, d, device="cuda", generator=g)).to(t)
+    _, _, scale, bias, dy, _ = norm_case(37, d, t, seed=d)
+    v = x.double()
+    mean, sd = v.mean(-1, keepdim=True), v.std(-1, unbiased=False, keepdim=True)
+    rstd = (sd ** 2 + 1e-6).rsqrt()
+    xhat = (v - mean) * rstd
+    m0 = 32 * U * v.abs().mean(-1, keepdim=True)
+    e_rstd = 32 * U + 64 * U * (m0 * rstd) ** 2                       # relative
+    e = 32 * U * (sd + m0) * rstd + (8 * U + e_rstd) * xhat.abs()
+    want = xhat * scale.double() + bias.double()
+    within(mb.layer_norm(x, scale, bias), want, scale.double().abs() * e + (4 * U + half_step(t)) * (want.abs() + bias.double().abs())
+           + tiny(t), "y")
+    dx, dp = mb.layer_norm_backward(dy, x, scale)
+    gy = dy.double() * scale.double()
+    c1, c2, mg = gy.mean(-1, keepdim=True), (gy * xhat).mean(-1, keepdim=True), gy.abs().mean(-1, keepdim=True)
+    want = rstd * (gy - c1 - xhat * c2)
+    mag = rstd * (gy.abs() + mg + xhat.abs() * (gy * xhat).abs().mean(-1, keepdim=True))
+    # c2 from the first centred values less off times sum gy: 32 u of both, and the means' error once more
+    e2 = (gy.abs() * e).mean(-1, keepdim=True) + 64 * U * m0 * rstd * mg
+    tol = (64 * U + e_rstd) * mag + rstd * (e * c2.abs() + xhat.abs() * e2)
+    within(dx, want, tol + half_step(t) * want.abs() + tiny(t), "dx")
+    within(dp["scale"], (dy.double() * xhat).sum(0), (dy.double().abs() * (e + 96 * U * xhat.abs())).sum(0) + 1e-30, "dscale")
