@@ -158,6 +158,15 @@ cudaError_t launch_tokens(TokenArgs A, cudaStream_t s) {
                           0, s, A);
 }
 
+// log p of a logit whose forward may have been added in another order (the
+// kernels of few tokens and the tiles differ, and lse may come from elsewhere):
+// rounding of large logits does not make p more than 1.  A NaN stays.
+__device__ __forceinline__ float at_most_0(float x) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(0.f));
+  return r;
+}
+
 __device__ __forceinline__ unsigned long long pair(float a, float b) {
   unsigned long long r;
   asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
@@ -533,7 +542,7 @@ struct EpiGrad {
       float x[32];
 #pragma unroll
       for (int j = 0; j < 32; ++j)
-        x[j] = g16::exp2_fast(fmaf(__uint_as_float(v[j]), un, -l) * LOG2E) * q;
+        x[j] = g16::exp2_fast(at_most_0(fmaf(__uint_as_float(v[j]), un, -l)) * LOG2E) * q;
       const unsigned at = (unsigned)(tg - (col0 + cc));
       if (at < 32u) {
 #pragma unroll
@@ -685,9 +694,7 @@ __global__ void __launch_bounds__(FEWB_T, TM <= 4 ? 2 : 1) loss_few_backward_ker
     __syncthreads();
     for (int e = t; e < rows * TM; e += FEWB_T) {
       const int m = e % TM, v = v0 + e / TM;
-      const float lp = dz[e] - l[m];
-      // p <= 1, though the forward added these logits in another order (a NaN stays)
-      float x = g16::exp2_fast(lp > 0.f ? 0.f : lp * LOG2E) * q[m];
+      float x = g16::exp2_fast(at_most_0(dz[e] - l[m]) * LOG2E) * q[m];
       if (tg[m] == v) x -= g[m];
       dz[e] = q[m] == 0.f && g[m] == 0.f ? 0.f : x;     // an ignored token: nothing, whatever its logits are
     }

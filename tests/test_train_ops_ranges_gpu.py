@@ -303,3 +303,19 @@ def test_norm_of_nearly_constant_rows(d, value, spread, t):
     tol = (64 * U + e_rstd) * mag + rstd * (e * c2.abs() + xhat.abs() * e2)
     within(dx, want, tol + half_step(t) * want.abs() + tiny(t), "dx")
     within(dp["scale"], (dy.double() * xhat).sum(0), (dy.double().abs() * (e + 96 * U * xhat.abs())).sum(0) + 1e-30, "dscale")
+
+
+# the forward and the gradient of 17 to 24 float32 tokens add their logits in different orders: p stays at most 1
+@pytest.mark.parametrize("T", [16, 17, 20, 24, 25])
+@pytest.mark.parametrize("size", [1e5, 1e7, 1e9, 1e11])
+def test_loss_gradient_of_large_logits_is_bounded(T, size):
+    for seed in range(12):
+        h, w, y, dl = loss_case(T, 36 + 4 * seed, 500, F32, seed=seed + T)
+        y[::2] = (h.double() @ w.double().T).argmax(1)[::2].int()
+        a = (size / 3) ** 0.5
+        h, w = h * a, w * a
+        _, _, dh, dw = run_loss(h, w, y, dl, check=True)
+        # |dz| <= dl and the sum of p is 1 but for roundings of large logits, which leave each p below 1
+        assert torch.isfinite(dh).all() and torch.isfinite(dw).all()
+        near = ((h.double() @ w.double().T) > (h.double() @ w.double().T).max(1, keepdim=True).values - size * 1e-5 - 50).sum(1)
+        assert (dh.abs() <= (near + 2)[:, None] * dl[:, None] * w.abs().max()).all()
