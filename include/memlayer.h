@@ -689,6 +689,11 @@ typedef struct {
   void* dweight;                 /* [V, d_model] */
 } memlayer_loss_grads;
 
+/* Beside its own sums the size holds 16-bit forms of h and the weight, 2 bytes
+ * an entry (float32: 4), since it does not know the call's addresses: a
+ * 16-bit call whose rows are 16 bytes apart and aligned leaves them untouched
+ * (1 GB for a weight of 128,256 x 4096).  The backward has one more of h and up
+ * to 256 MB of logit gradients. */
 int32_t memlayer_cross_entropy_workspace_size(const memlayer_loss_config* cfg, int32_t backward, size_t* bytes);
 
 /* The integer-label softmax cross entropy of the tied logits
@@ -705,14 +710,17 @@ int32_t memlayer_cross_entropy(const memlayer_loss_config* cfg, const memlayer_l
  * forward (loss and lse there are not used).  A token's dh keeps its
  * digits whatever the other tokens weigh; dweight sums over tokens, and there
  * float32 and float16 calls hold each term to 2^-39 of the largest
- * (|dloss| + |dlse|) |h| of a token, or better.  A token without a gradient
+ * (|dloss| + |dlse|) |h| of a token, or better.  16-bit calls of more than
+ * 128 tokens round the gradient of a logit once to their type before the two
+ * products (half a step of each term: 2^-9 for bfloat16, 2^-12 for float16, on
+ * top of the rounding of the results).  A token without a gradient
  * (ignored, say, and no dlse) adds nothing, whatever its h holds. */
 int32_t memlayer_cross_entropy_backward(const memlayer_loss_config* cfg, const memlayer_loss_args* args,
                                         const memlayer_loss_grads* grads, void* workspace, size_t workspace_bytes,
                                         void* stream);
 
 typedef struct {
-  int64_t batch;                 /* matrices */
+  int64_t batch;                 /* matrices, at most 65535 */
   int32_t rows, cols;            /* of each, 1 .. 32768 */
   int32_t dtype;                 /* memlayer_dtype of update and out */
   int32_t steps;                 /* 1 .. 64 */

@@ -17,8 +17,12 @@
 // both ways, dW of the piece and its part of dh.
 //
 // float32 operands run as two f16 pieces each (22 bits, see gemm16.cuh; h with
-// a scale a token), dz too; 16-bit operands as they are, dz rounded once to their type (its
-// relative error, 2^-9 or 2^-12, averages out over the sums it enters).
+// a scale a token), dz too; 16-bit operands as they are.  dz of a 16-bit call
+// has two pieces up to 128 tokens and is rounded once to the type beyond, half
+// a step of each term.  It shows where one term is most of a sum, as a
+// target's is: 8192 x 1024 over 32,768 bf16 is 2.4e-3 from the gradients in 64
+// bits, 1999 x 512 over 30,011 f16 4.3e-4; two pieces leave the rounding of
+// the results, 1.7e-3 and 3.9e-4, and take 2935 us for 1876 and 401 for 276.
 // Statistics, exponentials and sums are float32.
 #include "loss.cuh"
 

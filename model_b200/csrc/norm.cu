@@ -734,6 +734,7 @@ __global__ void __launch_bounds__(MAXT, MINB) layer_norm_wide_backward_kernel(No
       m[3] = sum(s1);
     }
     block_sums(m, red[1]);
+    // rsqrtf: within 2 units of the last place
     const float off = m[3] * A.inv_d, rstd_f = rsqrtf(variance(m[0] * A.inv_d, off) + A.eps);
     const F2 rstd = f2(rstd_f), c1 = f2(-(m[1] * A.inv_d)), c2 = f2(-(fmaf(-off, m[1], m[2]) * rstd_f * A.inv_d)),
              noff = f2(-off);

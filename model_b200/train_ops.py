@@ -5,8 +5,8 @@ blocks with the residual add before it (memory_pool_model/model.py:87,96,124),
 ``linear_cross_entropy`` / ``linear_cross_entropy_backward`` the integer-label
 cross entropy of the tied logits (model.py:125 under the trainer's loss)
 without the ``[tokens, vocab]`` logits, ``orthogonalize`` an update for the
-Dense kernels (the value table has its row-wise Adagrad in ``sparse``).  Like ``MemoryLayer.backward`` they
-are explicit functions, not autograd nodes.
+Dense kernels (the value table has its row-wise Adagrad in ``sparse``).  Like
+``MemoryLayer.backward`` they are explicit functions, not autograd nodes.
 
 Activations are float32, float16 or bfloat16 CUDA tensors and results have
 their type; parameters of the norm, losses and statistics are float32.  Input
@@ -243,9 +243,10 @@ def linear_cross_entropy(h: torch.Tensor, weight: torch.Tensor, targets: torch.T
                          ) -> Tuple[torch.Tensor, torch.Tensor]:
     """Softmax cross entropy of the logits ``h @ weight.T`` against integer
     ``targets``, without storing them: ``(loss, lse)``, float32 of the shape
-    of ``targets``, ``lse`` being log sum exp of the logits.  A token whose
-    target is ``ignore_index`` has loss 0; any other target outside the
-    vocabulary gives NaN, and raises with ``check=True``."""
+    of ``targets`` (any integer type but uint64), ``lse`` being log sum exp of
+    the logits.  A token whose target is ``ignore_index`` has loss 0; any
+    other target outside the vocabulary gives NaN, and raises with
+    ``check=True``."""
     if _fast is not None and stream is None and not check:
         out = _fast.linear_cross_entropy(h, weight, targets, ignore_index)
         if out is not None:
@@ -275,7 +276,9 @@ def linear_cross_entropy_backward(h: torch.Tensor, weight: torch.Tensor, targets
     """``(dh, dweight)`` of ``sum(dloss * loss) + sum(dlse * lse)`` for the
     forward on the same ``h``, ``weight`` and ``targets`` that gave ``lse``
     (a mean over n tokens: ``dloss`` filled with 1 / n).  ``dloss`` is not
-    read at ignored tokens, and ``h`` may hold anything there."""
+    read at ignored tokens, and ``h`` may hold anything there.  Above 128
+    tokens of a 16-bit type the logits' gradient is rounded once to that type
+    before it is multiplied with ``weight`` and ``h``."""
     if _fast is not None and stream is None and not check:
         out = _fast.linear_cross_entropy_backward(h, weight, targets, lse, dloss, dlse, ignore_index)
         if out is not None:
