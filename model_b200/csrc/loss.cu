@@ -28,6 +28,8 @@
 
 #include <float.h>
 
+#include <type_traits>
+
 #include "gemm16.cuh"
 #include "pieces16.cuh"
 
@@ -63,11 +65,11 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f32(float x) { return 
 
 __device__ __forceinline__ int exp_of(const unsigned* amax) { return amax ? g16::scale_exp(*amax) : 0; }
 
-// Factor that turns an accumulator of a token's logits back: a normal float
-// (beyond that range logits are zero or infinite for every purpose).  top_h:
-// the tokens' largest magnitudes (float32 operands, else null).
-__device__ __forceinline__ float logit_unscale(const unsigned* top_h, int64_t row, bool on, const unsigned* amax_w) {
-  return g16::pow2(max(-100, min(126, -(on && top_h ? g16::scale_exp(top_h[row]) : 0) - exp_of(amax_w))));
+// Factor that turns an accumulator of a token's logits back, from the scales'
+// exponents: a normal float (beyond that range logits are zero or infinite for
+// every purpose).
+__device__ __forceinline__ float logit_unscale(int exp_h, int exp_w) {
+  return g16::pow2(max(-100, min(126, -exp_h - exp_w)));
 }
 
 // ---- a scale for each token ----------------------------------------------------------
@@ -90,20 +92,40 @@ struct TokenArgs {
   int64_t T, ldh, ld;
   int d, tpr;                          // tpr: threads a token, 32 or all
   __half *hi, *lo;                     // [T][ld] (float32)
-  unsigned* top;                       // [T] bits of the largest finite magnitude
+  int* exp_h;                          // [T] exponent of h's scale (float32 forward)
+  // the gradient's part (token null: none): a token's record, its target (-1:
+  // none; PIECE_SKIP: no gradient at all) and exponent of dz's scale,
+  // |p q - [target] g| <= 2 max(|q|, |g|) < 2^15; the largest exponent of
+  // h / scale over the tokens that have a gradient
+  const int* targets;
+  const float *dloss, *dlse;
+  int V, ignore;
+  float4* token;
+  int *tgt, *exp_g;
+  unsigned* peak;
+  int* err;
 };
+
+// What the epilogue of dz needs of a token, in one load: the factors of p and
+// of the one-hot target, scaled; the target; the exponent of h's scale.
+__device__ __forceinline__ float4 token_record(float q, float g, int target, int exp_h) {
+  return make_float4(q, g, __int_as_float(target), __int_as_float(exp_h));
+}
 
 template <typename E>
 __global__ void __launch_bounds__(PIECE_THREADS) loss_tokens_kernel(TokenArgs A) {
   constexpr int V = 16 / sizeof(E);
+  constexpr bool F32 = sizeof(E) == 4, SCALED = !std::is_same<E, __nv_bfloat16>::value;
   struct alignas(16) Vec { E e[V]; };
-  __shared__ unsigned red[PIECE_THREADS / 32];
+  __shared__ unsigned red[PIECE_THREADS / 32], top_peak;
   allow_next();
   wait_previous();
   if ((int)blockIdx.x < A.w.blocks) {
     amax_block(A.w, blockIdx.x);
     return;
   }
+  if (threadIdx.x == 0) top_peak = 0;
+  __syncthreads();
   const int t = threadIdx.x & (A.tpr - 1), groups = PIECE_THREADS / A.tpr, d = A.d;
   const bool vec = A.ldh % V == 0 && d % V == 0 && (reinterpret_cast<uintptr_t>(A.h) & 15) == 0;
   const int64_t step = (int64_t)(gridDim.x - A.w.blocks) * groups;
@@ -112,7 +134,8 @@ __global__ void __launch_bounds__(PIECE_THREADS) loss_tokens_kernel(TokenArgs A)
     const bool on = row < A.T;
     const E* x = reinterpret_cast<const E*>(A.h) + (on ? row : 0) * A.ldh;
     unsigned mx = 0;
-    if (vec) {
+    if (!SCALED) {
+    } else if (vec) {
 #pragma unroll 2
       for (int c = t * V; c < d; c += A.tpr * V) {
         const Vec v = *reinterpret_cast<const Vec*>(x + c);
@@ -130,9 +153,26 @@ __global__ void __launch_bounds__(PIECE_THREADS) loss_tokens_kernel(TokenArgs A)
       for (int w = 0; w < PIECE_THREADS / 32; ++w) mx = max(mx, red[w]);
     }
     if (!on) continue;
-    if (t == 0) A.top[row] = mx;
-    if constexpr (sizeof(E) == 2) continue;
-    const float sc = g16::pow2(g16::scale_exp(mx));
+    const int eh = F32 ? g16::scale_exp(mx) : 0;
+    if (t == 0 && A.token) {
+      const int v = A.targets[row];
+      const bool in = v >= 0 && v < A.V && v != A.ignore;
+      if (!in && v != A.ignore) atomicCAS(A.err, 0, STATUS_TARGET);
+      const float g = in ? A.dloss[row] : 0.f, q = g + (A.dlse ? A.dlse[row] : 0.f);
+      const bool none = g == 0.f && q == 0.f;
+      const int target = none ? PIECE_SKIP : in ? v : -1;
+      const int f = SCALED ? g16::scale_exp(max(finite_bits(g), finite_bits(q))) - 1 : 0;
+      const float sg = g16::pow2(f);
+      A.token[row] = token_record(q * sg, g * sg, target, eh);
+      A.tgt[row] = target;
+      if constexpr (SCALED) {
+        A.exp_g[row] = f;
+        if (!none && mx) atomicMax(&top_peak, piece_peak((int)(mx >> 23) - 127 - f));
+      }
+    }
+    if constexpr (!F32) continue;
+    if (t == 0 && A.exp_h) A.exp_h[row] = eh;
+    const float sc = g16::pow2(eh);
     for (int c = t * 8; c < (int)A.ld; c += A.tpr * 8) {
       float v[8];
       if (vec && c + 8 <= d) {
@@ -150,6 +190,8 @@ __global__ void __launch_bounds__(PIECE_THREADS) loss_tokens_kernel(TokenArgs A)
       *reinterpret_cast<uint4*>(A.lo + row * A.ld + c) = *reinterpret_cast<uint4*>(l);
     }
   }
+  __syncthreads();
+  if (threadIdx.x == 0 && top_peak) atomicMax(A.peak, top_peak);   // a maximum: the order does not matter
 }
 
 template <typename E>
@@ -198,7 +240,8 @@ struct FromSums {
 struct StatsArgs {
   int64_t T;
   int V;
-  const unsigned *top_h, *amax_w;    // float32 operands: largest magnitudes, a token's and the weight's (else null)
+  const int* exp_h;                  // float32 operands: scales of the tokens and the weight (else null)
+  const unsigned* amax_w;
   const int* targets;
   float2* part;                      // [slot][half][T] (maximum, sum of exp(z - maximum))
   float* zt;                         // [T] target logit
@@ -235,7 +278,7 @@ struct EpiStats {
       s = 0.f;
       any = true;
       target = row < A.T ? A.targets[row] : -1;
-      un = logit_unscale(A.top_h, row, row < A.T, A.amax_w);
+      un = logit_unscale(A.exp_h && row < A.T ? A.exp_h[row] : 0, exp_of(A.amax_w));
       c = un * LOG2E;
     }
     const int hw = S.BN >> 1;
@@ -462,46 +505,12 @@ bool few_tokens(const memlayer_loss_config& c, const memlayer_loss_args& a) {
 }
 
 // ---- backward ---------------------------------------------------------------------
-// Per token: the factor of p, the factor of the one-hot target and the target
-// (-1: none; PIECE_SKIP: no gradient at all); where dz carries scales (top_h)
-// the token's, |p q - [target] g| <= 2 max(|q|, |g|) < 2^15, and the largest
-// exponent of h / scale over the tokens that have a gradient.
-__global__ void __launch_bounds__(256) loss_rows_kernel(const int* __restrict__ targets,
-                                                        const float* __restrict__ dloss,
-                                                        const float* __restrict__ dlse, int64_t T, int V, int ignore,
-                                                        const unsigned* __restrict__ top_h,
-                                                        float2* __restrict__ coef, int* __restrict__ tgt,
-                                                        int* __restrict__ exp_g, unsigned* __restrict__ peak,
-                                                        int* __restrict__ err) {
-  allow_next();
-  wait_previous();
-  unsigned mx = 0;
-  for (int64_t t = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; t < T; t += (int64_t)gridDim.x * blockDim.x) {
-    const int v = targets[t];
-    const bool in = v >= 0 && v < V && v != ignore;
-    if (!in && v != ignore) atomicCAS(err, 0, STATUS_TARGET);
-    const float g = in ? dloss[t] : 0.f, q = g + (dlse ? dlse[t] : 0.f);
-    coef[t] = make_float2(q, g);
-    const bool none = g == 0.f && q == 0.f;
-    tgt[t] = none ? PIECE_SKIP : in ? v : -1;
-    if (top_h) {
-      const int f = g16::scale_exp(max(finite_bits(g), finite_bits(q))) - 1;
-      exp_g[t] = f;
-      if (!none && top_h[t]) mx = max(mx, piece_peak((int)(top_h[t] >> 23) - 127 - f));
-    }
-  }
-  mx = __reduce_max_sync(FULL, mx);
-  if ((threadIdx.x & 31) == 0 && mx) atomicMax(peak, mx);
-}
-
 struct GradArgs {
   int64_t T;
   int v0, vc;                          // the piece: columns [v0, v0 + vc)
-  const unsigned *top_h, *amax_w;
-  const int* exp_g;                    // the tokens' scales of dz (null: none)
+  const unsigned* amax_w;
   const float* lse;
-  const float2* coef;
-  const int* tgt;
+  const float4* token;                 // token_record
   CUtensorMap out[2];                  // dz: hi, lo
 };
 
@@ -512,10 +521,12 @@ struct EpiGrad {
   float sum[128];
   using Args = GradArgs;
   uint32_t buf;
+  int exp_w;
   StagingTurn turn;
   __device__ __forceinline__ void begin(const Args& A, const Sched&, int, uint8_t* staging) {
     buf = tc::smem_u32(staging);
     turn = StagingTurn{};
+    exp_w = exp_of(A.amax_w);
   }
   template <class Get>
   __device__ __forceinline__ void blocks(const Args& A, const Sched& S, const Tile& t, int64_t row, int half,
@@ -523,18 +534,14 @@ struct EpiGrad {
     // a warp whose 32 rows are past the last token has nothing to store, and
     // stages nothing: what it staged last may still be on its way
     if (row - (threadIdx.x & 31) >= A.T) return;
-    const bool on = row < A.T;
-    const float un = logit_unscale(A.top_h, row, on, A.amax_w);
-    float l = 0.f, q = 0.f, g = 0.f;
-    int tg = -1;
-    if (on) {
-      const float2 c = A.coef[row];
-      const float sg = A.exp_g ? g16::pow2(A.exp_g[row]) : 1.f;
+    float l = 0.f;
+    float4 k = token_record(0.f, 0.f, -1, 0);
+    if (row < A.T) {
+      k = A.token[row];
       l = A.lse[row];
-      q = c.x * sg;
-      g = c.y * sg;
-      tg = A.tgt[row] - A.v0;
     }
+    const float q = k.x, g = k.y, un = logit_unscale(__float_as_int(k.w), exp_w);
+    const int tg = __float_as_int(k.z) - A.v0;
     const int hw = S.BN >> 1;
     const int col0 = t.nt * S.BN + half * hw;
 #pragma unroll
@@ -543,10 +550,21 @@ struct EpiGrad {
       uint32_t v[32];
       __syncwarp();
       get(cc, v);
-      float x[32];
+      float x[32];                     // p q, two columns an instruction where there is one
+      const unsigned long long un2 = pair(un, un), nl2 = pair(-l, -l), log2e2 = pair(LOG2E, LOG2E), q2 = pair(q, q);
 #pragma unroll
-      for (int j = 0; j < 32; ++j)
-        x[j] = g16::exp2_fast(at_most_0(fmaf(__uint_as_float(v[j]), un, -l)) * LOG2E) * q;
+      for (int j = 0; j < 32; j += 2) {
+        unsigned long long y = pair(__uint_as_float(v[j]), __uint_as_float(v[j + 1]));
+        float a, b;
+        asm("fma.rn.f32x2 %0, %0, %1, %2;" : "+l"(y) : "l"(un2), "l"(nl2));
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(y));
+        y = pair(at_most_0(a), at_most_0(b));
+        asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(y) : "l"(log2e2));
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(y));
+        y = pair(g16::exp2_fast(a), g16::exp2_fast(b));
+        asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(y) : "l"(q2));
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(x[j]), "=f"(x[j + 1]) : "l"(y));
+      }
       const unsigned at = (unsigned)(tg - (col0 + cc));
       if (at < 32u) {
 #pragma unroll
@@ -935,7 +953,7 @@ struct Plan {
   int vc;                              // columns of a vocabulary piece = row pitch of its dz
   int oBN, oNB;                        // columns per tile of the gradient products, tiles at once
   int s_h, s_w;                        // k slices of dh and of dW
-  size_t o_hh, o_hl, o_top, o_h2, o_wh, o_wl, o_part, o_zt, o_coef, o_tgt, o_exp, o_g, o_g2, o_dh, o_dw, bytes;
+  size_t o_hh, o_hl, o_eh, o_h2, o_wh, o_wl, o_part, o_zt, o_token, o_tgt, o_exp, o_g, o_g2, o_dh, o_dw, bytes;
 };
 
 constexpr size_t O_ERR = 256, O_AMAX = 512, HEAD = 1024;
@@ -1025,16 +1043,15 @@ bool plan(const memlayer_loss_config& c, bool backward, Plan* out) {
   if (f32) {
     p.o_hl = take(T * p.ld * 2);
     p.o_wl = take(V * p.ld * 2);
-    if (!backward) p.o_top = take(T * 4);
+    if (!backward) p.o_eh = take(T * 4);
   }
   if (!backward) {
     const int64_t few = f32 && T <= FEW ? up(V, FEW_V) / FEW_V * T * 8 : 0, part = (int64_t)p.slots * 2 * T * 8;
     p.o_part = take(few > part ? few : part);
     p.o_zt = take(T * 4);
   } else {
-    p.o_coef = take(T * 8);
+    p.o_token = take(T * 16);
     p.o_tgt = take(T * 4);
-    p.o_top = take(T * 4);
     p.o_exp = take(T * 4);
     p.o_h2 = take(p.P * T * p.ld * 2);   // hi, lo
     p.oBN = d > 128 ? 256 : 128;
@@ -1069,7 +1086,6 @@ struct Operands {
 cudaError_t prepare(const memlayer_loss_config& c, const memlayer_loss_args& a, const memlayer_loss_grads* g,
                     const Plan& p, char* ws, Operands* o, cudaStream_t s) {
   unsigned* amax = reinterpret_cast<unsigned*>(ws + O_AMAX);
-  unsigned* top = reinterpret_cast<unsigned*>(ws + p.o_top);
   const bool f32 = c.dtype == MEMLAYER_F32;
   o->h[0] = a.h;
   o->w[0] = a.weight;
@@ -1089,21 +1105,28 @@ cudaError_t prepare(const memlayer_loss_config& c, const memlayer_loss_args& a, 
     if (!f32) B.m[1] = {a.h, c.tokens, c.d_model, a.h_stride, ws + p.o_hh, nullptr, p.ld};
   }
   const bool scaled = c.dtype != MEMLAYER_BF16;        // dz carries scales
-  TokenArgs ta{{}, a.h, c.tokens, a.h_stride, p.ld, c.d_model, 0, (__half*)(ws + p.o_hh), (__half*)(ws + p.o_hl), top};
-  if (f32) {
-    ta.w = {(const float*)a.weight, c.vocab_size, c.d_model, a.weight_stride, amax + AMAX_W, 0};
-    LS_TRY(launch_tokens<float>(ta, s));
-  } else if (g && scaled) {
-    LS_TRY(launch_tokens<__half>(ta, s));
-  }
+  TokenArgs ta{{}, a.h, c.tokens, a.h_stride, p.ld, c.d_model, 0, (__half*)(ws + p.o_hh), (__half*)(ws + p.o_hl)};
+  int *tgt = reinterpret_cast<int*>(ws + p.o_tgt), *exp_g = reinterpret_cast<int*>(ws + p.o_exp);
+  if (f32) ta.w = {(const float*)a.weight, c.vocab_size, c.d_model, a.weight_stride, amax + AMAX_W, 0};
   if (g) {
-    int *tgt = reinterpret_cast<int*>(ws + p.o_tgt), *exp_g = reinterpret_cast<int*>(ws + p.o_exp);
-    const int64_t b = (c.tokens + 255) / 256;
-    count_launch();
-    LS_TRY(launch_dependent(loss_rows_kernel, dim3((unsigned)(b < 592 ? b : 592)), 256, 0, s, a.targets, g->dloss,
-                            g->dlse, c.tokens, c.vocab_size, c.ignore_index, (const unsigned*)(scaled ? top : nullptr),
-                            reinterpret_cast<float2*>(ws + p.o_coef), tgt, exp_g, amax + PEAK,
-                            reinterpret_cast<int*>(ws + O_ERR)));
+    ta.targets = a.targets;
+    ta.dloss = g->dloss;
+    ta.dlse = g->dlse;
+    ta.V = c.vocab_size;
+    ta.ignore = c.ignore_index;
+    ta.token = reinterpret_cast<float4*>(ws + p.o_token);
+    ta.tgt = tgt;
+    ta.exp_g = exp_g;
+    ta.peak = amax + PEAK;
+    ta.err = reinterpret_cast<int*>(ws + O_ERR);
+  } else {
+    ta.exp_h = reinterpret_cast<int*>(ws + p.o_eh);
+  }
+  if (f32)
+    LS_TRY(launch_tokens<float>(ta, s));
+  else if (g)
+    LS_TRY(scaled ? launch_tokens<__half>(ta, s) : launch_tokens<__nv_bfloat16>(ta, s));
+  if (g) {
     char *hi = ws + p.o_h2, *lo = hi + c.tokens * p.ld * 2;
     o->h2[0] = hi;
     o->h2[1] = lo;
@@ -1167,7 +1190,7 @@ cudaError_t launch_loss_forward(const memlayer_loss_config& c, const memlayer_lo
   StatsArgs ea{};
   ea.T = c.tokens;
   ea.V = c.vocab_size;
-  ea.top_h = f32 ? reinterpret_cast<unsigned*>(ws + p.o_top) : nullptr;
+  ea.exp_h = f32 ? reinterpret_cast<int*>(ws + p.o_eh) : nullptr;
   ea.amax_w = f32 ? reinterpret_cast<unsigned*>(ws + O_AMAX) + AMAX_W : nullptr;
   ea.targets = a.targets;
   ea.part = reinterpret_cast<float2*>(ws + p.o_part);
@@ -1208,11 +1231,9 @@ cudaError_t launch_loss_backward(const memlayer_loss_config& c, const memlayer_l
   unsigned* words = reinterpret_cast<unsigned*>(ws + O_AMAX);
   const bool f32 = c.dtype == MEMLAYER_F32;
   const int bf16 = c.dtype == MEMLAYER_BF16;
-  const unsigned *top = f32 ? reinterpret_cast<unsigned*>(ws + p.o_top) : nullptr, *aw = f32 ? words + AMAX_W : nullptr,
-                 *peak = bf16 ? nullptr : words + PEAK;
+  const unsigned *aw = f32 ? words + AMAX_W : nullptr, *peak = bf16 ? nullptr : words + PEAK;
   const int* exp_g = bf16 ? nullptr : reinterpret_cast<int*>(ws + p.o_exp);
-  const float2* coef = reinterpret_cast<float2*>(ws + p.o_coef);
-  const int* tgt = reinterpret_cast<int*>(ws + p.o_tgt);
+  const float4* token = reinterpret_cast<float4*>(ws + p.o_token);
   uint16_t *gh = reinterpret_cast<uint16_t*>(ws + p.o_g), *gl = reinterpret_cast<uint16_t*>(ws + p.o_g2);
   float* acc_h = reinterpret_cast<float*>(ws + p.o_dh);
   const int sms = g16::device_sms() / p.cg;
@@ -1235,7 +1256,7 @@ cudaError_t launch_loss_backward(const memlayer_loss_config& c, const memlayer_l
     S.BN = p.BN;
     S.bf16 = bf16;
     g16::distribute(&S, sms, 0);
-    GradArgs ga{T, v0, vc, top, aw, exp_g, g.lse, coef, tgt, {}};
+    GradArgs ga{T, v0, vc, aw, g.lse, token, {}};
     LS_TRY(g16::make_store(&ga.out[0], gh, T, p.vc, p.vc, f32 ? MEMLAYER_F16 : c.dtype));
     if (p.PZ == 2) LS_TRY(g16::make_store(&ga.out[1], gl, T, p.vc, p.vc, f32 ? MEMLAYER_F16 : c.dtype));
     S.seg = LOGIT_SEG;
