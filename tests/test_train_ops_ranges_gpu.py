@@ -319,3 +319,67 @@ def test_loss_gradient_of_large_logits_is_bounded(T, size):
         assert torch.isfinite(dh).all() and torch.isfinite(dw).all()
         near = ((h.double() @ w.double().T) > (h.double() @ w.double().T).max(1, keepdim=True).values - size * 1e-5 - 50).sum(1)
         assert (dh.abs() <= (near + 2)[:, None] * dl[:, None] * w.abs().max()).all()
+
+
+def test_model_head_on_a_stream_and_captured():
+    from model_b200 import MemoryPoolLM, ModelConfig
+    cfg = ModelConfig(vocab_size=300, max_len=32, d_model=64, n_layers=2, n_heads=2, ffn_mult=2, memory_layers=(1,),
+                      n_sub_keys=16, pool_heads=2, d_key=32, d_value=64, top_k=4)
+    m = MemoryPoolLM(cfg)
+    prep = m.prepare(m.init(2))
+    tok = torch.randint(0, 300, (3, 32), device="cuda", generator=gen(60))
+    tgt = torch.randint(0, 300, (3, 32), device="cuda", generator=gen(61))
+    tgt[:, -3:] = -100
+
+    def flat(out):
+        loss, g = out
+        return [loss, g["hidden"], g["ln_final"]["scale"], g["ln_final"]["bias"], g["embed"]["embedding"]]
+    want = flat(m.loss_and_head_grads(prep, tok, tgt, check=True))
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    got = flat(m.loss_and_head_grads(prep, tok, tgt, stream=s, check=True))
+    alone, _ = m.loss(prep, tok, tgt, stream=s)
+    s.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.equal(alone, want[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = flat(m.loss_and_head_grads(prep, tok, tgt))
+    for shift in (0, 1):
+        tok.copy_((tok + shift) % 300)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = flat(m.loss_and_head_grads(prep, tok, tgt))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# two threads on streams of their own, one of them through the general way
+def test_calls_from_two_threads():
+    import threading
+    h, w, y, dl = loss_case(200, 128, 3000, BF16, seed=70, gap=5)
+    x, r, scale, bias, dy, dr = norm_case(300, 1003, F16, seed=71)
+    u = torch.randn(3, 100, 200, device="cuda", generator=gen(72))
+
+    def run(it):
+        n, s = mb.layer_norm(x, scale, bias, residual=r)
+        dx, dp = mb.layer_norm_backward(dy, s, scale, dresidual=dr)
+        return [n, dx, dp["scale"], mb.orthogonalize(u), *run_loss(h, w, y.to(it), dl)]
+    want = run(torch.int32)
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(it):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got = run(it)
+                    torch.cuda.current_stream().synchronize()
+                    if not all(torch.equal(a, b) for a, b in zip(got, want)):
+                        failed.append(it)
+        except Exception as e:                       # reported by the test, not lost in the thread
+            failed.append(e)
+    threads = [threading.Thread(target=work, args=(it,)) for it in (torch.int32, torch.int64)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
