@@ -276,9 +276,10 @@ def linear_cross_entropy_backward(h: torch.Tensor, weight: torch.Tensor, targets
     """``(dh, dweight)`` of ``sum(dloss * loss) + sum(dlse * lse)`` for the
     forward on the same ``h``, ``weight`` and ``targets`` that gave ``lse``
     (a mean over n tokens: ``dloss`` filled with 1 / n).  ``dloss`` is not
-    read at ignored tokens, and ``h`` may hold anything there.  Above 128
-    tokens of a 16-bit type the logits' gradient is rounded once to that type
-    before it is multiplied with ``weight`` and ``h``."""
+    read at ignored tokens, and ``h`` may hold anything there unless ``dlse``
+    gives them a gradient.  Above 128 tokens of a 16-bit type the logits'
+    gradient is rounded once to that type before it is multiplied with
+    ``weight`` and ``h``."""
     if _fast is not None and stream is None and not check:
         out = _fast.linear_cross_entropy_backward(h, weight, targets, lse, dloss, dlse, ignore_index)
         if out is not None:
